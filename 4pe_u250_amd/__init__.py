@@ -43,6 +43,12 @@ TOKEN_BYTES = 288          # algorithmic bytes per cached token-head: 2 x 128 co
 
 OK, EINVAL, ERANGE, EHIP, ENOMEM, ESTATE = 0, -1, -2, -3, -4, -5
 DIST_NORMAL, DIST_STUDENT_T3 = 0, 1
+F32, BF16, F16 = 0, 1, 2                                # element types of the rotary and block entries
+ROPE_LINEAR, ROPE_THETA, ROPE_BANDS = 1, 2, 3           # RopeScaling.kind
+BLOCK_TOKENS = 16
+BLOCK_MAX_SEQ = 131072
+BLOCK_WEIGHT_QUERIES = 8
+ROTARY_MAX_POSITIONS = 1048576
 KERNEL_APPEND, KERNEL_STEP, KERNEL_EXACT = 0, 1, 2
 KERNEL_KINDS = 3
 _STATUS_NAMES = {EINVAL: "EINVAL", ERANGE: "ERANGE", EHIP: "EHIP", ENOMEM: "ENOMEM", ESTATE: "ESTATE"}
@@ -56,6 +62,7 @@ class SwiftKVError(RuntimeError):
 
 _vp = C.c_void_p
 _i32 = C.c_int32
+_i64 = C.c_int64
 _sz = C.c_size_t
 
 # name -> (restype, argtypes); every declaration of include/swiftkv.h.
@@ -95,6 +102,19 @@ _SIGNATURES = {
     "swiftkv_fill_synthetic_f32": (C.c_int, [_vp, _vp, _sz, C.c_uint64, C.c_uint64, C.c_uint64, _i32, _i32]),
     "swiftkv_kv_cache_fill_synthetic": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, C.c_uint64,
                                                   _i32, _i32]),
+    "swiftkv_rope_lut_generate_scaled": (C.c_int, [_vp, _i32, C.c_double, _vp, C.POINTER(_vp)]),
+    "swiftkv_rotary_create": (C.c_int, [_vp, _i32, _i32, C.c_double, _vp, C.POINTER(_vp)]),
+    "swiftkv_rotary_destroy": (C.c_int, [_vp]),
+    "swiftkv_rotary": (C.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32]),
+    "swiftkv_block_cache_create": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_vp)]),
+    "swiftkv_block_cache_destroy": (C.c_int, [_vp]),
+    "swiftkv_block_cache_bytes": (_sz, [_vp]),
+    "swiftkv_block_cache_blocks": (_i32, [_vp]),
+    "swiftkv_block_append": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _vp, _i32, _i32]),
+    "swiftkv_block_values": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "swiftkv_block_attention": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _vp, _i32, _i32,
+                                          C.c_float, _vp, _vp, _i64]),
+    "swiftkv_block_evict": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "swiftkv_device_alloc": (C.c_int, [_vp, _sz, C.POINTER(_vp)]),
     "swiftkv_device_free": (C.c_int, [_vp, _vp]),
     "swiftkv_memcpy_h2d": (C.c_int, [_vp, _vp, _vp, _sz]),
@@ -367,6 +387,15 @@ class RopeLut:
         _check(lib().swiftkv_rope_lut_generate(ctx.handle, positions, theta, C.byref(h)))
         return cls(ctx, h.value)
 
+    @classmethod
+    def generate_scaled(cls, ctx: Context, scaling: Optional["RopeScaling"], positions: int = REFERENCE_MAX_SEQ,
+                        theta: float = 10000.0) -> "RopeLut":
+        """The closed form with frequencies scaled for contexts beyond the trained one."""
+        h = C.c_void_p()
+        _check(lib().swiftkv_rope_lut_generate_scaled(ctx.handle, positions, theta,
+                                                      C.byref(scaling) if scaling is not None else None, C.byref(h)))
+        return cls(ctx, h.value)
+
     @property
     def positions(self) -> int:
         return int(lib().swiftkv_rope_lut_positions(self.handle))
@@ -440,6 +469,72 @@ class KVCache:
         if self.handle:
             h, self.handle = self.handle, None
             _check(lib().swiftkv_kv_cache_destroy(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class RopeScaling(C.Structure):
+    """How rotary frequencies change for long contexts (swiftkv_rope_scaling)."""
+    _fields_ = [("kind", C.c_int32), ("original_positions", C.c_int32), ("factor", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("magnitude", C.c_double)]
+
+    def __init__(self, kind: int = 0, factor: float = 1.0, original_positions: int = 0, low: float = 0.0,
+                 high: float = 0.0, magnitude: float = 1.0):
+        super().__init__(kind, original_positions, factor, low, high, magnitude)
+
+
+class RotaryTable:
+    """FP32 cos and sin of positions [0, positions) for `rotary_dim` channels of a head."""
+
+    def __init__(self, ctx: Context, rotary_dim: int, positions: int, theta: float = 10000.0,
+                 scaling: Optional[RopeScaling] = None):
+        h = C.c_void_p()
+        _check(lib().swiftkv_rotary_create(ctx.handle, rotary_dim, positions, theta,
+                                           C.byref(scaling) if scaling is not None else None, C.byref(h)))
+        self.ctx, self.handle = ctx, h.value
+        self.rotary_dim, self.positions = rotary_dim, positions
+
+    def close(self) -> None:
+        if self.handle:
+            h, self.handle = self.handle, None
+            _check(lib().swiftkv_rotary_destroy(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class BlockCache:
+    """GPU-resident INT8 cache with one K and one V scale per 16 tokens and key/value head."""
+
+    def __init__(self, ctx: Context, layers: int, max_batch: int, heads: int, kv_heads: int, head_dim: int,
+                 max_seq_len: int):
+        h = C.c_void_p()
+        _check(lib().swiftkv_block_cache_create(ctx.handle, layers, max_batch, heads, kv_heads, head_dim, max_seq_len,
+                                                C.byref(h)))
+        self.ctx, self.handle = ctx, h.value
+        self.layers, self.max_batch, self.max_seq_len = layers, max_batch, max_seq_len
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().swiftkv_block_cache_bytes(self.handle))
+
+    @property
+    def blocks(self) -> int:
+        """Blocks of one (sequence, layer, key/value head)."""
+        return int(lib().swiftkv_block_cache_blocks(self.handle))
+
+    def close(self) -> None:
+        if self.handle:
+            h, self.handle = self.handle, None
+            _check(lib().swiftkv_block_cache_destroy(h))
 
     def __del__(self):
         try:
@@ -606,6 +701,80 @@ def swiftkv_append_tokens(ctx: Context, k, v, kv_cache: KVCache, rope_lut: RopeL
     _check(lib().swiftkv_append_tokens(ctx.handle, _io_ptr(ctx, k, it), _io_ptr(ctx, v, it), 1 if q17 else 0,
                                        kv_cache.handle, rope_lut.handle, int(layer_index), int(seq), int(pos0),
                                        int(n)))
+
+
+def swiftkv_rotary(ctx: Context, table: RotaryTable, x, out, position, heads: int, head_dim: int, n: int = 1,
+                   dtype: int = BF16, halves: bool = True, inverse: bool = False, x_stride: Optional[int] = None,
+                   out_stride: Optional[int] = None) -> None:
+    """Rotate `heads` heads of n tokens of each sequence, token i of sequence b at
+    position[b] + i.  x, out: device [batch * n] rows x_stride and out_stride
+    elements apart (default heads * head_dim); x may be out.  halves: channels
+    j and j + rotary_dim / 2 make a pair, else 2j and 2j + 1.  inverse: by the
+    negative angle, which is the gradient too.
+    Asynchronous on the context stream, as the calls below are.
+    """
+    pos, batch, _keep = _positions(ctx, position)
+    row = heads * head_dim
+    _check(lib().swiftkv_rotary(ctx.handle, table.handle, _ptr(x), row if x_stride is None else x_stride, _ptr(out),
+                                row if out_stride is None else out_stride, dtype, 1 if halves else 0,
+                                1 if inverse else 0, pos, batch, n, heads, head_dim))
+
+
+def swiftkv_block_append(ctx: Context, k, v, cache: BlockCache, layer_index: int, position, n: int = 1,
+                         dtype: int = BF16, seq0: int = 0, k_stride: Optional[int] = None,
+                         v_stride: Optional[int] = None) -> None:
+    """Append n tokens to each of sequences seq0, seq0 + 1, ... at cached tokens
+    [position[b], position[b] + n); a negative position skips its sequence.
+    k, v: device [batch * n][kv_heads * head_dim], rows k_stride and v_stride
+    elements apart (default dense)."""
+    pos, batch, _keep = _positions(ctx, position)
+    row = cache.kv_heads * cache.head_dim
+    _check(lib().swiftkv_block_append(ctx.handle, _ptr(k), row if k_stride is None else k_stride, _ptr(v),
+                                      row if v_stride is None else v_stride, dtype, cache.handle, layer_index, seq0,
+                                      pos, batch, n))
+
+
+def swiftkv_block_values(ctx: Context, cache: BlockCache, layer_index: int, position, k, v, n: int = 1,
+                         dtype: int = BF16, seq0: int = 0) -> None:
+    """The values that cached tokens [position[b], position[b] + n) stand for, to
+    device k and v, [batch * n][kv_heads * head_dim] each."""
+    pos, batch, _keep = _positions(ctx, position)
+    _check(lib().swiftkv_block_values(ctx.handle, cache.handle, layer_index, seq0, pos, batch, n, dtype, _ptr(k),
+                                      _ptr(v)))
+
+
+def swiftkv_block_attention(ctx: Context, q, k, v, cache: BlockCache, layer_index: int, position, out, n: int = 1,
+                            dtype: int = BF16, scale: float = 0.0, weights=None, seq0: int = 0,
+                            q_stride: Optional[int] = None, k_stride: Optional[int] = None,
+                            v_stride: Optional[int] = None, out_stride: Optional[int] = None) -> None:
+    """Append n tokens to each sequence (unless k and v are None) and attend: query
+    i of sequence b sees cached tokens [0, position[b] + i]; a sequence with a
+    negative position takes no part and its rows of out are zero.
+    q, out: device [batch * n][heads * head_dim].  weights: device FP32
+    [batch][kv_heads][cache.blocks] to which each block's softmax weight is
+    added (n <= BLOCK_WEIGHT_QUERIES), or None."""
+    pos, batch, _keep = _positions(ctx, position)
+    row, kv_row = cache.heads * cache.head_dim, cache.kv_heads * cache.head_dim
+    _check(lib().swiftkv_block_attention(ctx.handle, _ptr(q), row if q_stride is None else q_stride, _ptr(k),
+                                         kv_row if k_stride is None else k_stride, _ptr(v),
+                                         kv_row if v_stride is None else v_stride, dtype, cache.handle, layer_index,
+                                         seq0, pos, batch, n, scale, _ptr(weights), _ptr(out),
+                                         row if out_stride is None else out_stride))
+
+
+def swiftkv_block_evict(ctx: Context, cache: BlockCache, layer0: int, layers: int, position, keep: int, weights,
+                        kept=None, sinks: int = 0, recent: int = 1, seq0: int = 0) -> list:
+    """Keep `keep` blocks of each (layer, sequence, key/value head) that holds
+    more: the first `sinks`, the last `recent`, and those of the largest weight.
+    position: cached tokens of each sequence.  weights: device FP32 [layers]
+    [batch][kv_heads][cache.blocks], moved along; kept: device int32 [layers]
+    [batch][kv_heads][keep] for the former block indices, or None.  Returns the
+    numbers of tokens then cached."""
+    pos, batch, _keep = _positions(ctx, position)
+    left = (C.c_int32 * batch)()
+    _check(lib().swiftkv_block_evict(ctx.handle, cache.handle, layer0, layers, seq0, pos, batch, keep, sinks, recent,
+                                     _ptr(weights), _ptr(kept), left))
+    return list(left)
 
 
 def a14_unpack(words: np.ndarray) -> np.ndarray:

@@ -1,0 +1,778 @@
+// swiftkv_block.hip -- kernels of the block cache: append, values, attention,
+// eviction.  Layout and numerics: swiftkv_block.hpp, include/swiftkv.h.
+#include "swiftkv_block.hpp"
+#include "swiftkv_device.hpp"
+
+namespace swiftkv {
+namespace {
+
+using namespace dev;
+
+constexpr float kFloatMax = 3.402823466e+38f;
+// Larger rows are taken as infinite: a code 64 of scale 2^122 would stand for 2^128.
+constexpr float kRowMax = 0x1.fcp+126f;          // 127 * 2^120
+
+template <typename T>
+struct alignas(16) Vec8 {
+    T v[8];
+};
+
+template <typename F>
+void with_type(ElementType t, F&& f) {
+    if (t == kF32) f(float{});
+    else if (t == kBF16) f(__bf16{});
+    else f(_Float16{});
+}
+
+// ---------------------------------------------------------------- codes
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+
+// The smallest power of two s = 2^e, e >= -100, with amax <= 127 * s.  With
+// amax = 1.f * 2^x that is e = x - 6, and one more where 1.f > 127 / 64.
+__device__ __forceinline__ float code_scale(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23) - 133 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return __uint_as_float(static_cast<uint32_t>(max(e, -100) + 127) << 23);
+}
+
+// 1 / s of a power of two within 2^-126 .. 2^126, exactly.
+__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+__device__ __forceinline__ uint32_t code_byte(float x) {
+    return static_cast<uint32_t>(static_cast<int32_t>(__builtin_rintf(x))) & 0xffu;
+}
+
+__device__ __forceinline__ float byte_value(uint32_t word, int i) {
+    return static_cast<float>(static_cast<int8_t>(static_cast<uint8_t>(word >> (8 * i))));
+}
+
+// One block's scale after rows with largest magnitude amax join it: the wave
+// gives its lanes' amax and whether any value is not finite.
+__device__ __forceinline__ float joined_scale(float amax, bool bad, bool held, float old) {
+    amax = wave_max(amax);
+    const bool any_bad = __ballot(bad) != 0;
+    float s = code_scale(amax);
+    if (held) s = old >= s || old != old ? old : s;
+    return any_bad ? __builtin_nanf("") : s;
+}
+
+// Workgroup (key/value head, touched block, sequence): wave 0 appends the
+// block's K rows, wave 1 its V rows.  Reading and writing bound it; a row is
+// read once, and a block that keeps its scale writes K codes of the new rows
+// only.  A V channel's 16 tokens are one lane's 16 bytes, so one wave owns the
+// whole record half and merges new bytes into it without a race.
+template <typename T, int HD>
+__global__ __launch_bounds__(128) void block_append_kernel(const BlockRowsArgs a) {
+    constexpr int NC = HD / 64;
+    const int kh = blockIdx.x, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int p = a.positions[b];
+    if (p < 0) return;
+    const int blk = p / kBlockRows + static_cast<int>(blockIdx.y);
+    const int tok0 = blk * kBlockRows, end = p + a.n;
+    if (tok0 >= end) return;
+    const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
+    int8_t* const base = a.view.base + page * a.view.page_bytes;
+    const int rec = a.view.table[page * a.view.blocks + blk];
+    int8_t* const record = base + static_cast<int64_t>(rec) * (2 * kBlockRows * HD) + wave * (kBlockRows * HD);
+    float* const scale = reinterpret_cast<float*>(base + static_cast<int64_t>(a.view.blocks) * (2 * kBlockRows * HD)) +
+                         2 * rec + wave;
+    const bool held = tok0 < p;                  // the block keeps rows of earlier calls
+    const float old = held ? *scale : 0.0f;
+    const int64_t row0 = static_cast<int64_t>(b) * a.n - p;   // row of token 0
+    float s;
+    if (wave == 0) {
+        // lane = (token, 16-channel chunks c and c + 4)
+        const int t = lane >> 2, c = lane & 3, tok = tok0 + t;
+        const bool fresh = tok >= p && tok < end;
+        float x[NC][16];
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+            if (fresh) {
+                const T* src = static_cast<const T*>(a.k) + (row0 + tok) * a.k_stride + kh * HD + (c + 4 * i) * 16;
+                const Vec8<T> lo = *reinterpret_cast<const Vec8<T>*>(src);
+                const Vec8<T> hi = *reinterpret_cast<const Vec8<T>*>(src + 8);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[i][j] = static_cast<float>(lo.v[j]);
+                    x[i][8 + j] = static_cast<float>(hi.v[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                amax = fmaxf(amax, fabsf(x[i][j]));
+                bad |= !(fabsf(x[i][j]) <= kRowMax);
+            }
+        }
+        s = joined_scale(amax, bad, held, old);
+        const bool poisoned = s != s;
+        const float inv = poisoned ? 0.0f : pow2_inverse(s);
+        const float ratio = old * inv;
+        const bool requantize = held && !poisoned && old != s;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            int8_t* const dst = record + (c + 4 * i) * (kBlockRows * 16) + t * 16;
+            v4i w = {0, 0, 0, 0};
+            if (fresh && !poisoned) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j >> 2] |= static_cast<int32_t>(code_byte(x[i][j] * inv) << (8 * (j & 3)));
+            }
+            if (requantize && !fresh) {
+                const v4i o = *reinterpret_cast<const v4i*>(dst);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    w[j >> 2] |= static_cast<int32_t>(code_byte(byte_value(static_cast<uint32_t>(o[j >> 2]), j & 3) * ratio)
+                                                      << (8 * (j & 3)));
+            }
+            if (fresh || !held || requantize) *reinterpret_cast<v4i*>(dst) = w;
+        }
+    } else {
+        // lane = channels NC * lane ..; its NC runs of 16 tokens
+        const T* src = static_cast<const T*>(a.v) + kh * HD + lane * NC;
+        float x[kBlockRows][NC];
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < kBlockRows; ++t) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) x[t][i] = 0.0f;
+            const int tok = tok0 + t;
+            if (tok >= p && tok < end) {
+                struct alignas(sizeof(T) * NC) Pack { T v[NC]; };
+                const Pack w = *reinterpret_cast<const Pack*>(src + (row0 + tok) * a.v_stride);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) x[t][i] = static_cast<float>(w.v[i]);
+            }
+        }
+        v4i o[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            o[i] = v4i{0, 0, 0, 0};
+            if (held) o[i] = *reinterpret_cast<const v4i*>(record + (lane * NC + i) * kBlockRows);
+        }
+#pragma unroll
+        for (int t = 0; t < kBlockRows; ++t)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                amax = fmaxf(amax, fabsf(x[t][i]));
+                bad |= !(fabsf(x[t][i]) <= kRowMax);
+            }
+        s = joined_scale(amax, bad, held, old);
+        const bool poisoned = s != s;
+        const float inv = poisoned ? 0.0f : pow2_inverse(s);
+        const float ratio = old == s || poisoned ? 1.0f : old * inv;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            v4i w = {0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < kBlockRows; ++t) {
+                const int tok = tok0 + t;
+                const bool fresh = tok >= p && tok < end;
+                const float kept = byte_value(static_cast<uint32_t>(o[i][t >> 2]), t & 3) * ratio;
+                const float v = fresh ? (poisoned ? 0.0f : x[t][i] * inv) : kept;
+                w[t >> 2] |= static_cast<int32_t>(code_byte(v) << (8 * (t & 3)));
+            }
+            *reinterpret_cast<v4i*>(record + (lane * NC + i) * kBlockRows) = w;
+        }
+    }
+    if (lane == 0 && !(held && old == s)) *scale = s;
+}
+
+// The reverse, with the same lanes: values of cached rows, rounded once.
+template <typename T, int HD>
+__global__ __launch_bounds__(128) void block_values_kernel(const BlockRowsArgs a) {
+    constexpr int NC = HD / 64;
+    const int kh = blockIdx.x, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int p = a.positions[b];
+    if (p < 0) return;
+    const int blk = p / kBlockRows + static_cast<int>(blockIdx.y);
+    const int tok0 = blk * kBlockRows, end = p + a.n;
+    if (tok0 >= end) return;
+    const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
+    const int8_t* const base = a.view.base + page * a.view.page_bytes;
+    const int rec = a.view.table[page * a.view.blocks + blk];
+    const int8_t* const record = base + static_cast<int64_t>(rec) * (2 * kBlockRows * HD) + wave * (kBlockRows * HD);
+    const float s = reinterpret_cast<const float*>(base + static_cast<int64_t>(a.view.blocks) * (2 * kBlockRows * HD))[
+        2 * rec + wave];
+    const int64_t row0 = static_cast<int64_t>(b) * a.n - p;
+    const int64_t stride = static_cast<int64_t>(a.view.kv_heads) * HD;
+    if (wave == 0) {
+        const int t = lane >> 2, c = lane & 3, tok = tok0 + t;
+        if (tok < p || tok >= end) return;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const v4i o = *reinterpret_cast<const v4i*>(record + (c + 4 * i) * (kBlockRows * 16) + t * 16);
+            T* dst = static_cast<T*>(a.k_out) + (row0 + tok) * stride + kh * HD + (c + 4 * i) * 16;
+            Vec8<T> w[2];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                w[j >> 3].v[j & 7] = static_cast<T>(byte_value(static_cast<uint32_t>(o[j >> 2]), j & 3) * s);
+            *reinterpret_cast<Vec8<T>*>(dst) = w[0];
+            *reinterpret_cast<Vec8<T>*>(dst + 8) = w[1];
+        }
+    } else {
+        v4i o[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) o[i] = *reinterpret_cast<const v4i*>(record + (lane * NC + i) * kBlockRows);
+        T* dst = static_cast<T*>(a.v_out) + kh * HD + lane * NC;
+#pragma unroll
+        for (int t = 0; t < kBlockRows; ++t) {
+            const int tok = tok0 + t;
+            if (tok < p || tok >= end) continue;
+            struct alignas(sizeof(T) * NC) Pack { T v[NC]; } w;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                w.v[i] = static_cast<T>(byte_value(static_cast<uint32_t>(o[i][t >> 2]), t & 3) * s);
+            *reinterpret_cast<Pack*>(dst + (row0 + tok) * stride) = w;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64_t n, int blocks) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step)
+        table[i] = static_cast<uint16_t>(i % blocks);
+}
+
+// ---------------------------------------------------------------- attention
+
+// softmax(scale q k^T) v of the rows of one chunk -- query tokens times the
+// query heads that share a key/value head, 4, 8 or 16 of them -- over the
+// tiles of one split.  Both products run on the 8-bit matrix instructions
+// straight from the codes (D[16][16] += A[16][64] B[64][16]):
+//
+//   scores  A: the queries as integers q = m 2^E (E for a row, |m| <= 2^30), the
+//           four signed bytes of m as four rows, so a 16-row A holds 4 queries;
+//           B: the K codes as they lie.  The byte sums are exact; one lane has the
+//           four of a (row, token) and joins them into m.k.
+//   output  A: p 2^27 as four 7-bit digits, p = 2^(score - the tile's largest), each
+//           times its block's V scale over the tile's largest (a power of two);
+//           B: the V codes as they lie, 64 tokens of 16 channels at a time.
+//
+// So a code is never converted, the operator is bound by reading the codes
+// (2 * head_dim + 0.5 bytes a token), and what a product rounds is 2^-30 of a
+// row's largest query value and 2^-28 of a tile's largest weight: less than
+// FP32 products would.
+//
+// Wave w takes tiles w, w + 4, ... of the split, each with its own running
+// (max, sum, output); the waves meet in LDS, the splits in block_merge_kernel.
+constexpr int kAttendThreads = 256;
+constexpr int kAttendWaves4 = 4;
+constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
+constexpr int kDigitBits = 7;
+constexpr float kDigitOne = 134217728.0f;        // 2^27
+
+#define SWIFTKV_CONSTANT __attribute__((address_space(4)))
+
+template <int HD, int RT>
+struct AttendShared {
+    static constexpr int kQueryBytes = RT * (HD / 64) * 1024;
+    static constexpr int kDigitBytes = kAttendWaves4 * RT * 16 * kDigitStride;
+    static constexpr int kRows = RT * kRowTile;
+    static constexpr int kMergeBytes = kAttendWaves4 * kRows * (HD + 2) * 4;
+    static constexpr int kScanBytes = kQueryBytes + kDigitBytes;
+    static constexpr int kBytes = kScanBytes > kMergeBytes ? kScanBytes : kMergeBytes;
+};
+
+// The queries of a chunk as A operands: [row tile][64-channel step][lane][16
+// bytes], lane = (chunk g of the step) * 16 + (row * 4 + byte); scales in q_scale.
+template <typename T, int HD, int RT>
+__device__ __forceinline__ void stage_queries(const BlockAttendArgs& a, int b, int kh, int row_first, int rows,
+                                              uint8_t* lds, float* q_scale) {
+    constexpr int kPieces = HD / 8;              // lanes of a row, 8 channels each
+    constexpr int kRows = RT * kRowTile;
+    for (int i = threadIdx.x; i < kRows * kPieces; i += kAttendThreads) {
+        const int row = i / kPieces, piece = i % kPieces;
+        float x[8] = {};
+        if (row < rows) {
+            const int r = row_first + row;
+            const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
+            const T* src = static_cast<const T*>(a.q) + token * a.q_stride +
+                           static_cast<int64_t>(kh * a.group + r % a.group) * HD + piece * 8;
+            const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(src);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(w.v[j]);
+        }
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            amax = fmaxf(amax, fabsf(x[j]));
+            bad |= !(fabsf(x[j]) <= kFloatMax);
+        }
+        int poison = bad ? 1 : 0;
+#pragma unroll
+        for (int d = 1; d < kPieces; d <<= 1) {
+            amax = fmaxf(amax, __shfl_xor(amax, d));
+            poison |= __shfl_xor(poison, d);
+        }
+        int e = 0;
+        (void)frexpf(amax, &e);                  // amax < 2^e
+        e = poison ? 0 : max(e, -90);
+        if (piece == 0) q_scale[row] = poison ? __builtin_nanf("") : ldexpf(a.scale, e - 30);
+        uint64_t limb[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            int32_t m = poison ? 0 : static_cast<int32_t>(__builtin_rintf(ldexpf(x[j], 30 - e)));   // |m| <= 2^30
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int32_t l = static_cast<int8_t>(static_cast<uint8_t>(m));
+                limb[k] |= static_cast<uint64_t>(static_cast<uint8_t>(l)) << (8 * j);
+                m = (m - l) >> 8;
+            }
+        }
+        // 8 channels: half (piece & 1) of chunk piece / 2 = 4 * step + g
+        const int chunk = piece >> 1, step = chunk >> 2, g = chunk & 3;
+        uint8_t* dst = lds + (((row >> 2) * (HD / 64) + step) * 64 + g * 16 + (row & 3) * 4) * 16 + (piece & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint64_t*>(dst + k * 16) = limb[k];
+    }
+}
+
+__device__ __forceinline__ float row16_max_f(float x) {
+    x = fmaxf(x, dpp_f<kDppQuadXor1>(x));
+    x = fmaxf(x, dpp_f<kDppQuadXor2>(x));
+    x = fmaxf(x, dpp_f<kDppHalfMirror>(x));
+    return fmaxf(x, dpp_f<kDppRowRor8>(x));
+}
+__device__ __forceinline__ float row16_sum_f(float x) {
+    x += dpp_f<kDppQuadXor1>(x);
+    x += dpp_f<kDppQuadXor2>(x);
+    x += dpp_f<kDppHalfMirror>(x);
+    return x + dpp_f<kDppRowRor8>(x);
+}
+
+template <typename T, int HD, int RT, bool LSE>
+__global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const BlockAttendArgs a) {
+    using S = AttendShared<HD, RT>;
+    constexpr int NS = HD / 64;                  // 64-channel steps of a score
+    constexpr int ND = HD / 16;                  // 16-channel tiles of an output
+    constexpr int kRows = S::kRows;
+    __shared__ __align__(16) uint8_t lds[S::kBytes];
+    __shared__ float q_scale[kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n16 = lane & 15;
+    const int b = blockIdx.y;
+    int id = blockIdx.x;
+    const int kh = id % a.view.kv_heads;         // heads fastest: a head's workgroups share an XCD's L2
+    id /= a.view.kv_heads;
+    const int split = id % a.splits, chunk = id / a.splits;
+    const int all_rows = a.group * a.n;
+    const int row_first = chunk * kRows, rows = min(kRows, all_rows - row_first);
+    const int p = a.positions[b];
+    // tokens that the chunk's last row sees
+    const int most = p < 0 ? 0 : p + (row_first + rows - 1) / a.group + 1;
+    const int tiles = (most + kTileTokens - 1) / kTileTokens;
+    const int my_splits = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
+    if (split >= my_splits) return;
+    const int tile_end = min(tiles, (split + 1) * a.split_tiles);
+
+    stage_queries<T, HD, RT>(a, b, kh, row_first, rows, lds, q_scale);
+    __syncthreads();
+
+    const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
+    int8_t* const base = a.view.base + page * a.view.page_bytes;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        base, static_cast<short>(0), static_cast<int32_t>(a.view.page_bytes), kBufferWord3);
+    const auto* table = (const SWIFTKV_CONSTANT uint64_t*)(a.view.table + page * a.view.blocks);
+    const auto* scales = (const SWIFTKV_CONSTANT uint64_t*)(base + static_cast<int64_t>(a.view.blocks) * (2 * kBlockRows * HD));
+
+    v4i qa[RT][NS];
+    float qs[RT], m_run[RT], l_run[RT];
+    float acc[RT][ND];
+    int limit[RT];                               // tokens that row (rt, g) sees
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qa[rt][s] = *reinterpret_cast<const v4i*>(lds + ((rt * NS + s) * 64 + lane) * 16);
+        const int row = rt * kRowTile + g;
+        qs[rt] = q_scale[row];
+        limit[rt] = row < rows && p >= 0 ? p + (row_first + row) / a.group + 1 : 0;
+        m_run[rt] = -INFINITY;
+        l_run[rt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[rt][i] = 0.0f;
+    }
+    uint8_t* const digits = lds + S::kQueryBytes + wave * (RT * 16 * kDigitStride);
+
+    for (int tile = split * a.split_tiles + wave; tile < tile_end; tile += kAttendWaves4) {
+        const uint64_t entry = table[tile];
+        int rec[kTileBlocks];
+        float ks[kTileBlocks], vs[kTileBlocks];
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) {
+            rec[j] = static_cast<int>((entry >> (16 * j)) & 0xffffu);
+            const uint64_t w = scales[rec[j]];
+            ks[j] = __uint_as_float(static_cast<uint32_t>(w));
+            vs[j] = __uint_as_float(static_cast<uint32_t>(w >> 32));
+        }
+        v4i kb[kTileBlocks][NS], vb[ND];
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j)
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, rec[j] * (2 * kBlockRows * HD) + s * 1024, 0);
+        const int mine = g & 2 ? (g & 1 ? rec[3] : rec[2]) : (g & 1 ? rec[1] : rec[0]);
+        const int v_lane = mine * (2 * kBlockRows * HD) + kBlockRows * HD + n16 * 16;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, v_lane, i * 256, 0);
+
+        // V scales over the tile's largest; a scale that is not a number poisons
+        // the rows that see its block.
+        float v_top = 0x1p-100f;
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) v_top = fmaxf(v_top, vs[j]);
+        const float v_inv = pow2_inverse(v_top);
+        const int tok0 = tile * kTileTokens;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float s[kTileBlocks];
+            float top = -INFINITY;
+            bool poison = false;
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) {
+                v4i c = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < NS; ++k) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][k], kb[j][k], c, 0, 0, 0);
+                const float low = static_cast<float>(c[0] + c[1] * 256);       // below 2^30
+                const float high = static_cast<float>(c[2] + c[3] * 256);
+                s[j] = __builtin_fmaf(high, 65536.0f, low) * (qs[rt] * ks[j]);
+                if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[j] = -INFINITY;
+                if (vs[j] != vs[j] && tok0 + kBlockRows * j < limit[rt]) poison = true;
+                top = fmaxf(top, s[j]);
+            }
+            top = row16_max_f(top);
+            const float top_safe = top == -INFINITY ? 0.0f : top;    // a row that sees nothing here
+            float sum = 0.0f;
+            float each[kTileBlocks];
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) {
+                const float w = fast_exp2(s[j] - top_safe);
+                each[j] = w;
+                sum += w;
+                const uint32_t d = static_cast<uint32_t>(__builtin_rintf(w * (vs[j] * v_inv) * kDigitOne));
+                uint8_t* dst = digits + (rt * 16 + g * 4) * kDigitStride + j * kBlockRows + n16;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dst[k * kDigitStride] = static_cast<uint8_t>((d >> (kDigitBits * k)) & 127u);
+            }
+            if (LSE) {
+                // log2 of each block's sum, by the lane n16 == j
+                float mine_sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kTileBlocks; ++j) {
+                    const float t = row16_sum_f(each[j]);
+                    if (n16 == j) mine_sum = t;
+                }
+                const int row = rt * kRowTile + g;
+                if (n16 < kTileBlocks && row < rows) {
+                    const int64_t at = ((static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + row_first + row) *
+                                           a.view.blocks + tile * kTileBlocks + n16;
+                    a.block_lse[at] = top_safe + __log2f(mine_sum);
+                }
+            }
+            const float m_new = fmaxf(m_run[rt], top);
+            const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = fast_exp2(m_run[rt] - m_safe), beta = fast_exp2(top - m_safe);
+            m_run[rt] = m_new;
+            l_run[rt] = l_run[rt] * alpha + sum * beta;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const v4i pa = *reinterpret_cast<const v4i*>(digits + (rt * 16 + n16) * kDigitStride + g * 16);
+            const float v_mul = poison ? __builtin_nanf("") : beta * v_top * (1.0f / kDigitOne);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                v4i c = {0, 0, 0, 0};
+                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, vb[i], c, 0, 0, 0);
+                const float low = static_cast<float>(c[0] + c[1] * 128);       // below 2^28
+                const float high = static_cast<float>(c[2] + c[3] * 128);
+                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(high, 16384.0f, low), v_mul, acc[rt][i] * alpha);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+    // The waves' partials meet in LDS.
+    __syncthreads();
+    float* const merge = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float* dst = merge + (wave * kRows + rt * kRowTile + g) * (HD + 2);
+        const float l = row16_sum_f(l_run[rt]);
+        if (n16 == 0) {
+            dst[0] = m_run[rt];
+            dst[1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < ND; ++i) dst[2 + i * 16 + n16] = acc[rt][i];
+    }
+    __syncthreads();
+    const int64_t pair = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.chunks + chunk;
+    for (int i = threadIdx.x; i < kRows * HD; i += kAttendThreads) {
+        const int row = i / HD, d = i % HD;
+        if (row >= rows) break;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttendWaves4; ++w) m = fmaxf(m, merge[(w * kRows + row) * (HD + 2)]);
+        const float m_safe = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttendWaves4; ++w) {
+            const float* src = merge + (w * kRows + row) * (HD + 2);
+            const float f = fast_exp2(src[0] - m_safe);
+            l = __builtin_fmaf(src[1], f, l);
+            o = __builtin_fmaf(src[2 + d], f, o);
+        }
+        if (my_splits > 1) {
+            float* dst = a.partials + ((pair * a.splits + split) * kRows + row) * (HD + 2);
+            if (d == 0) {
+                dst[0] = m;
+                dst[1] = l;
+            }
+            dst[2 + d] = o;
+            continue;
+        }
+        const int r = row_first + row;
+        const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
+        static_cast<T*>(a.out)[token * a.out_stride + static_cast<int64_t>(kh * a.group + r % a.group) * HD + d] =
+            static_cast<T>(l == 0.0f ? 0.0f : o / l);
+        if (LSE && d == 0)
+            a.row_lse[(static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + r] = m_safe + __log2f(l);
+    }
+}
+
+// Joins the splits of a row, in split order: workgroup (kv head and chunk, sequence).
+template <typename T, int HD, bool LSE>
+__global__ __launch_bounds__(HD) void block_merge_kernel(const BlockAttendArgs a, int chunk_rows) {
+    const int kh = blockIdx.x % a.view.kv_heads, chunk = blockIdx.x / a.view.kv_heads, b = blockIdx.y;
+    const int all_rows = a.group * a.n, row_first = chunk * chunk_rows;
+    const int rows = min(chunk_rows, all_rows - row_first);
+    const int p = a.positions[b];
+    const int most = p < 0 ? 0 : p + (row_first + rows - 1) / a.group + 1;
+    const int tiles = (most + kTileTokens - 1) / kTileTokens;
+    const int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
+    if (splits <= 1) return;
+    const int64_t pair = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.chunks + chunk;
+    const int row = blockIdx.z, d = threadIdx.x;
+    if (row >= rows) return;
+    const float* src = a.partials + (pair * a.splits * chunk_rows + row) * (HD + 2);
+    const int64_t step = static_cast<int64_t>(chunk_rows) * (HD + 2);
+    float m = -INFINITY;
+    for (int j = 0; j < splits; ++j) m = fmaxf(m, src[j * step]);
+    const float m_safe = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o = 0.0f;
+    for (int j = 0; j < splits; ++j) {
+        const float f = fast_exp2(src[j * step] - m_safe);
+        l = __builtin_fmaf(src[j * step + 1], f, l);
+        o = __builtin_fmaf(src[j * step + 2 + d], f, o);
+    }
+    const int r = row_first + row;
+    const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
+    static_cast<T*>(a.out)[token * a.out_stride + static_cast<int64_t>(kh * a.group + r % a.group) * HD + d] =
+        static_cast<T>(l == 0.0f ? 0.0f : o / l);
+    if (LSE && d == 0)
+        a.row_lse[(static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + r] = m_safe + __log2f(l);
+}
+
+// weights[block] += sum over rows of 2^(the block's log-sum - the row's): rows in
+// order, so a block's sum has one order whatever ran first.
+__global__ __launch_bounds__(256) void block_weights_kernel(const BlockAttendArgs a) {
+    const int blk = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    const int p = a.positions[b], rows = a.group * a.n;
+    if (p < 0 || blk * kBlockRows >= p + a.n) return;
+    const int64_t head = static_cast<int64_t>(b) * a.view.kv_heads + kh;
+    float sum = 0.0f;
+    for (int r = 0; r < rows; ++r)
+        if (blk * kBlockRows <= p + r / a.group)
+            sum += fast_exp2(a.block_lse[(head * rows + r) * a.view.blocks + blk] - a.row_lse[head * rows + r]);
+    a.weights[head * a.view.blocks + blk] += sum;
+}
+
+// ---------------------------------------------------------------- eviction
+
+// Workgroup (kv head, sequence, layer).  The threshold is found by four passes
+// over the weights' bits in LDS, from the top 8 down (non-negative floats order
+// as their bits); then one pass in order gives each block its new place.  What
+// is read and written is a few KiB a workgroup: latency bounds it.
+__global__ __launch_bounds__(256) void block_evict_kernel(const BlockEvictArgs a) {
+    extern __shared__ __align__(16) uint8_t evict_lds[];
+    __shared__ uint32_t bins[256];
+    __shared__ uint32_t found[2];                // the digit's bin, and how many lie above it
+    __shared__ uint32_t wave_eq[4], wave_keep[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int kh = blockIdx.x, b = blockIdx.y, blocks = a.view.blocks;
+    const int nb = (a.positions[b] + kBlockRows - 1) / kBlockRows;
+    const int64_t row = (static_cast<int64_t>(blockIdx.z) * a.batch + a.b0 + b) * a.view.kv_heads + kh;
+    float* const weights = a.weights + row * blocks;
+    int32_t* const kept = a.kept ? a.kept + row * a.keep : nullptr;
+    if (a.positions[b] < 0) return;
+    if (nb <= a.keep) {
+        for (int i = nb + tid; i < blocks; i += 256) weights[i] = 0.0f;
+        if (kept)
+            for (int i = tid; i < a.keep; i += 256) kept[i] = i < nb ? i : -1;
+        return;
+    }
+    uint16_t* const table = a.view.table + block_page(a.view, a.slot0 + a.b0 + b, a.layer0 + blockIdx.z, kh) * blocks;
+    float* const w = reinterpret_cast<float*>(evict_lds);
+    uint16_t* const old = reinterpret_cast<uint16_t*>(evict_lds + 4 * static_cast<size_t>(blocks));
+    for (int i = tid; i < nb; i += 256) {
+        w[i] = weights[i];
+        old[i] = table[i];
+    }
+    const int lo = a.sinks, hi = nb - a.recent;
+    auto key = [&](int i) { return w[i] > 0.0f ? __float_as_uint(w[i]) : 0u; };
+    uint32_t want = a.keep - a.sinks - a.recent;     // of [lo, hi), which holds more
+    uint32_t prefix = 0, threshold = 0xffffffffu;
+    __syncthreads();
+    if (want > 0) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            bins[tid] = 0;
+            __syncthreads();
+            for (int i = lo + tid; i < hi; i += 256) {
+                const uint32_t k = key(i);
+                if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&bins[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            // wave 0: lane l holds bins 4l .. 4l + 3; how many keys lie in higher lanes' bins
+            if (wave == 0) {
+                uint32_t c[4], mine = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine += c[j] = bins[4 * lane + j];
+                uint32_t above = mine;           // inclusive sum from the top lane down
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t t = __shfl_down(above, d);
+                    if (lane + d < 64) above += t;
+                }
+                above -= mine;
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                    if (above < want && above + c[j] >= want) {
+                        found[0] = 4 * lane + j;
+                        found[1] = above;
+                    }
+                    above += c[j];
+                }
+            }
+            __syncthreads();
+            prefix = (prefix << 8) | found[0];
+            want -= found[1];
+            __syncthreads();
+        }
+        threshold = prefix;
+    }
+    // In order: keys above the threshold stay, and the first `want` that equal it.
+    uint32_t eq_before = 0, keep_before = 0;
+    for (int i0 = 0; i0 < nb; i0 += 256) {
+        const int i = i0 + tid;
+        const bool inside = i < nb, middle = inside && i >= lo && i < hi;
+        const uint32_t k = middle ? key(i) : 0u;
+        const bool eq = middle && want > 0 && k == threshold;
+        const uint64_t eqs = __ballot(eq);
+        if (lane == 0) wave_eq[wave] = __popcll(eqs);
+        __syncthreads();
+        uint32_t e = eq_before + __popcll(eqs & ((1ull << lane) - 1));
+        for (int v = 0; v < wave; ++v) e += wave_eq[v];
+        const bool stays = inside && (!middle || k > threshold || (eq && e < want));
+        const uint64_t keeps = __ballot(stays);
+        if (lane == 0) wave_keep[wave] = __popcll(keeps);
+        __syncthreads();
+        uint32_t at = keep_before + __popcll(keeps & ((1ull << lane) - 1));
+        for (int v = 0; v < wave; ++v) at += wave_keep[v];
+        if (inside) {
+            if (stays) {
+                weights[at] = w[i];
+                if (kept) kept[at] = i;
+            }
+            table[stays ? at : a.keep + (i - at)] = old[i];
+        }
+        for (int v = 0; v < 4; ++v) {
+            eq_before += wave_eq[v];
+            keep_before += wave_keep[v];
+        }
+        __syncthreads();
+    }
+    for (int i = a.keep + tid; i < blocks; i += 256) weights[i] = 0.0f;
+}
+
+}  // namespace
+
+hipError_t launch_block_table(const BlockView& v, int64_t pages, hipStream_t s) {
+    block_table_kernel<<<1024, 256, 0, s>>>(v.table, pages * v.blocks, v.blocks);
+    return hipGetLastError();
+}
+
+namespace {
+template <typename T, int HD>
+void append_or_values(const BlockRowsArgs& a, int batch, bool values, hipStream_t s) {
+    const dim3 grid(a.view.kv_heads, (a.n + 2 * kBlockRows - 2) / kBlockRows, batch);
+    if (values) block_values_kernel<T, HD><<<grid, 128, 0, s>>>(a);
+    else block_append_kernel<T, HD><<<grid, 128, 0, s>>>(a);
+}
+hipError_t launch_rows(const BlockRowsArgs& a, int batch, ElementType t, bool values, hipStream_t s) {
+    with_type(t, [&](auto tag) {
+        using T = decltype(tag);
+        if (a.view.head_dim == 64) append_or_values<T, 64>(a, batch, values, s);
+        else append_or_values<T, 128>(a, batch, values, s);
+    });
+    return hipGetLastError();
+}
+
+template <typename T, int HD, int RT, bool LSE>
+void attend(const BlockAttendArgs& a, int batch, hipStream_t s) {
+    block_attend_kernel<T, HD, RT, LSE>
+        <<<dim3(a.view.kv_heads * a.splits * a.chunks, batch), kAttendThreads, 0, s>>>(a);
+    if (a.splits > 1)
+        block_merge_kernel<T, HD, LSE>
+            <<<dim3(a.view.kv_heads * a.chunks, batch, RT * kRowTile), HD, 0, s>>>(a, RT * kRowTile);
+    if (LSE) {
+        int most = 0;
+        for (int b = 0; b < batch; ++b) most = a.positions[b] + a.n > most ? a.positions[b] + a.n : most;
+        const int blocks = (most + kBlockRows - 1) / kBlockRows;
+        if (blocks > 0)
+            block_weights_kernel<<<dim3((blocks + 255) / 256, a.view.kv_heads, batch), 256, 0, s>>>(a);
+    }
+}
+}  // namespace
+
+hipError_t launch_block_append(const BlockRowsArgs& a, int batch, ElementType t, hipStream_t s) {
+    return launch_rows(a, batch, t, false, s);
+}
+hipError_t launch_block_values(const BlockRowsArgs& a, int batch, ElementType t, hipStream_t s) {
+    return launch_rows(a, batch, t, true, s);
+}
+
+hipError_t launch_block_attend(const BlockAttendArgs& a, int batch, int row_tiles, ElementType t, hipStream_t s) {
+    with_type(t, [&](auto tag) {
+        using T = decltype(tag);
+        auto shaped = [&](auto hd, auto rt) {
+            if (a.weights) attend<T, decltype(hd)::value, decltype(rt)::value, true>(a, batch, s);
+            else attend<T, decltype(hd)::value, decltype(rt)::value, false>(a, batch, s);
+        };
+        auto tiled = [&](auto hd) {
+            if (row_tiles == 1) shaped(hd, std::integral_constant<int, 1>{});
+            else if (row_tiles == 2) shaped(hd, std::integral_constant<int, 2>{});
+            else shaped(hd, std::integral_constant<int, 4>{});
+        };
+        if (a.view.head_dim == 64) tiled(std::integral_constant<int, 64>{});
+        else tiled(std::integral_constant<int, 128>{});
+    });
+    return hipGetLastError();
+}
+
+hipError_t launch_block_evict(const BlockEvictArgs& a, int layers, int batch, hipStream_t s) {
+    block_evict_kernel<<<dim3(a.view.kv_heads, batch, layers), 256, 6 * static_cast<size_t>(a.view.blocks), s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace swiftkv

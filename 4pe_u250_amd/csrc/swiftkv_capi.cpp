@@ -7,30 +7,21 @@
 // swiftkv_exact.hip (the integer-compatibility step) and swiftkv_synth.hip
 // (synthetic inputs); this file only validates, sizes and enqueues.  No exception crosses the C boundary: every entry point converts
 // failures to a negative status and a thread-local message.
-#include "../../include/swiftkv.h"
-
-#include <hip/hip_runtime.h>
+#include "swiftkv_internal.hpp"
 
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <cstring>
 #include <memory>
 #include <mutex>
 #include <new>
 #include <string>
-#include <unordered_map>
-#include <unordered_set>
 #include <vector>
-
-#include "swiftkv_common.hpp"
 
 namespace {
 
 using namespace swiftkv;
 
-constexpr int kTimerSlots = 64;
 constexpr int kProfilePairs = 8192;
 constexpr size_t kRopeEntryBytes = sizeof(int2);
 constexpr int kMaxSplitTokens = SWIFTKV_MAX_SEQ;
@@ -40,36 +31,6 @@ static_assert(SWIFTKV_ROPE_LUT_BYTES_PER_POSITION == 512, "RoPE LUT image: 8 x 6
 static_assert(SWIFTKV_RECORD_BYTES == 5 * 64, "record is [meta, K0, K1, V0, V1]");
 static_assert(SWIFTKV_NOALLOC_WORKSPACE_BYTES == kNoAllocScratchBytes, "allocation-free workspace size");
 static_assert(SWIFTKV_A14_WORD_BYTES == kA14WordBytes, "A14 word: 32 x 14 bits");
-
-// A fixed buffer, so that reporting an error never allocates.
-thread_local char g_last_error[512];
-
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    std::vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-int ok() {
-    g_last_error[0] = '\0';
-    return SWIFTKV_OK;
-}
-
-#define SKV_HIP(expr)                                                                          \
-    do {                                                                                       \
-        hipError_t e_ = (expr);                                                                \
-        if (e_ != hipSuccess)                                                                  \
-            return fail(SWIFTKV_EHIP, "%s: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, \
-                        __LINE__);                                                             \
-    } while (0)
-
-struct ProfilePair {
-    hipEvent_t begin;
-    hipEvent_t end;
-    int kind;
-};
 
 // Device address of the allocation-free entry's workspace, per device,
 // resolved and zeroed once (by the first context created on the device).
@@ -87,108 +48,6 @@ hipError_t scratch_for_device(int device, int count, hipStream_t s, void** out) 
     }
     *out = g_scratch[device];
     return hipSuccess;
-}
-
-}  // namespace
-
-struct swiftkv_context {
-    int device = 0;
-    int cus = 256;              // compute units of the device
-    int step_per_cu = 3;        // 4-wave step workgroups one CU holds at once
-    hipStream_t stream = nullptr;
-    int32_t split_tokens = 0;   // 0: heuristic
-    StepShape forced_shape{0, 0};   // testing aid: waves 0 = the launch plan's shape
-    // split-context workspace: [partial_rows][32] arrival words (kArrivalStride
-    // apart), then [partial_rows][32][partial_slots][kSlotWords] tagged words,
-    // zero-filled when allocated (generation 0; tag 0 is never current)
-    uint64_t* partials = nullptr;
-    int32_t partial_rows = 0;
-    int32_t partial_slots = 0;
-    // Graphs record the workspace pointer in their kernel nodes.  Each graph
-    // names the buffer it recorded (if any), with a count of live graphs per
-    // buffer here; a buffer the workspace outgrows is freed at once unless a
-    // live graph recorded it, and is then kept in `retired` until the last
-    // such graph is destroyed.
-    std::unordered_map<void*, int64_t> graph_refs;
-    std::vector<void*> retired;
-    bool capture_uses_workspace = false;   // a split launch of the capture in progress used `partials`
-    // [kMaxBatchPerLaunch][32] arrival words (kArrivalStride apart), zero, for
-    // launches that split no head: the step reads its arrival word on every
-    // path but only a split head's merge writes one
-    uint64_t* arrivals = nullptr;
-    // workspace of the integer-compatibility step: the exp2 table, then the
-    // split exchange (kExactWorkspaceWords; fixed, so a graph may record it at
-    // any time)
-    uint64_t* exact_workspace = nullptr;
-    uint8_t* scratch = nullptr;     // this device's allocation-free workspace (arrival words, then partials)
-    // Fault word of the split merges: pinned host memory that a step kernel
-    // writes (system scope) when a merge gives up on a partial, read without
-    // a device round trip by swiftkv_synchronize, the step entries and graph
-    // launches, which report it once and clear it.
-    uint32_t* fault_host = nullptr;
-    uint32_t* fault_dev = nullptr;
-    bool merge_fault_test = false;  // testing aid: merges wait for a tag no word carries
-    // timing
-    hipEvent_t timers[kTimerSlots] = {};
-    bool profiling = false;
-    std::vector<ProfilePair> profile_pool;
-    size_t profile_used = 0;
-    bool capturing = false;     // the stream is being recorded into a graph
-    // host-memory I/O mode: step inputs/outputs are host pointers staged here
-    bool host_io = false;
-    uint8_t* io_stage = nullptr;
-    size_t io_bytes = 0;
-    // Objects created from the context (caches, tables, graphs, device
-    // buffers) may outlive swiftkv_context_destroy: the context is only
-    // marked released then, and freed when the last of them is destroyed.
-    int64_t children = 0;
-    bool released = false;
-    std::unordered_set<void*> buffers;   // swiftkv_device_alloc allocations not yet freed
-};
-
-struct swiftkv_graph {
-    swiftkv_context* ctx = nullptr;
-    hipGraph_t graph = nullptr;
-    hipGraphExec_t exec = nullptr;
-    void* workspace = nullptr;   // the split workspace buffer its launches recorded, if any
-};
-
-struct swiftkv_rope_lut {
-    swiftkv_context* ctx = nullptr;
-    int32_t positions = 0;
-    int2* table = nullptr;              // device [positions][64] (cos, sin)
-    std::vector<int2> host;             // host copy for export
-};
-
-struct swiftkv_kv_cache {
-    swiftkv_context* ctx = nullptr;
-    int32_t layers = 0;
-    int32_t max_batch = 0;
-    int32_t seq_cap = 0;
-    int64_t page_bytes = 0;
-    size_t bytes = 0;
-    int8_t* base = nullptr;
-};
-
-namespace {
-
-int set_device(const swiftkv_context* ctx) {
-    if (ctx->released) return fail(SWIFTKV_ESTATE, "the context has been destroyed");
-    SKV_HIP(hipSetDevice(ctx->device));
-    return SWIFTKV_OK;
-}
-
-void free_context(swiftkv_context* ctx);
-
-// One object created from `ctx` has been destroyed.
-void release_child(swiftkv_context* ctx) {
-    if (--ctx->children == 0 && ctx->released) free_context(ctx);
-}
-
-// Entry points that synchronize, copy, allocate or memset cannot be recorded.
-int not_capturing(const swiftkv_context* ctx, const char* what) {
-    if (ctx && ctx->capturing) return fail(SWIFTKV_ESTATE, "%s is not allowed during graph capture", what);
-    return SWIFTKV_OK;
 }
 
 // A split merge that gave up waiting for another split's partial (its head's
@@ -789,14 +648,17 @@ const uint32_t* exp2_table() {
     return table.data();
 }
 
+}  // namespace
+
 // Releases everything the context owns (after its last object is gone).
-void free_context(swiftkv_context* ctx) {
+void swiftkv::free_context(swiftkv_context* ctx) {
     (void)hipSetDevice(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->partials) (void)hipFree(ctx->partials);
     for (void* p : ctx->retired) (void)hipFree(p);
     if (ctx->arrivals) (void)hipFree(ctx->arrivals);
     if (ctx->exact_workspace) (void)hipFree(ctx->exact_workspace);
+    if (ctx->block_partials) (void)hipFree(ctx->block_partials);
     if (ctx->io_stage) (void)hipFree(ctx->io_stage);
     if (ctx->fault_host) (void)hipHostFree(ctx->fault_host);
     for (auto& t : ctx->timers)
@@ -808,8 +670,6 @@ void free_context(swiftkv_context* ctx) {
     if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
 }
-
-}  // namespace
 
 extern "C" {
 
@@ -1045,20 +905,28 @@ int swiftkv_rope_lut_load(swiftkv_context* ctx, const void* image, size_t image_
 }
 
 int swiftkv_rope_lut_generate(swiftkv_context* ctx, int32_t positions, double theta, swiftkv_rope_lut** out) {
+    return swiftkv_rope_lut_generate_scaled(ctx, positions, theta, nullptr, out);
+}
+
+int swiftkv_rope_lut_generate_scaled(swiftkv_context* ctx, int32_t positions, double theta,
+                                     const swiftkv_rope_scaling* scaling, swiftkv_rope_lut** out) {
     if (!ctx || !out) return fail(SWIFTKV_EINVAL, "null argument");
     *out = nullptr;
     if (int rc0 = not_capturing(ctx, "swiftkv_rope_lut_generate")) return rc0;
     if (positions < 1 || positions > SWIFTKV_MAX_SEQ)
         return fail(SWIFTKV_ERANGE, "positions %d outside [1, %d]", positions, SWIFTKV_MAX_SEQ);
-    if (!(theta > 1.0) || !std::isfinite(theta)) return fail(SWIFTKV_EINVAL, "theta must be finite and > 1");
-    int rc = set_device(ctx);
+    double freq[kRopePairs], magnitude = 1.0;
+    int rc = rope_frequencies(kHeadDim, theta, scaling, freq, &magnitude);
     if (rc) return rc;
+    if (!(std::fabs(magnitude) < 2.0))
+        return fail(SWIFTKV_EINVAL, "RoPE scaling: a Q1.17 table holds magnitudes below 2");
+    if ((rc = set_device(ctx))) return rc;
     std::vector<int2> host(static_cast<size_t>(positions) * kRopePairs);
     for (int32_t p = 0; p < positions; ++p)
         for (int j = 0; j < kRopePairs; ++j) {
-            const double freq = 1.0 / std::pow(theta, static_cast<double>(j) / kRopePairs);
-            const double ang = static_cast<double>(p) * freq;
-            host[static_cast<size_t>(p) * kRopePairs + j] = make_int2(q17_19bit(std::cos(ang)), q17_19bit(std::sin(ang)));
+            const double ang = static_cast<double>(p) * freq[j];
+            host[static_cast<size_t>(p) * kRopePairs + j] =
+                make_int2(q17_19bit(magnitude * std::cos(ang)), q17_19bit(magnitude * std::sin(ang)));
         }
     return upload_lut(ctx, std::move(host), positions, out);
 }

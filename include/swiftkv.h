@@ -354,6 +354,150 @@ int swiftkv_kv_cache_fill_synthetic(swiftkv_context* ctx, swiftkv_kv_cache* kv,
                                     int32_t distribution, int32_t k_outliers);
 
 /* --------------------------------------------------------------------------
+ * Rotary positions and the block cache.  They have no counterpart in the
+ * reference, whose stage fixes 32 heads of 128, one query token and INT8 codes
+ * with a scale per token and 32 channels: these operators serve models with
+ * other heads (grouped ones among them), other rotations, 16-bit tensors,
+ * several query tokens at a time, and sequences longer than their cache.
+ * A program calls them in this order: swiftkv_rotary on the projection's query
+ * and key heads, swiftkv_block_attention (which appends the new K/V rows), and,
+ * where a sequence nears its capacity, swiftkv_block_evict.
+ *
+ * Tensors are device pointers, 16-byte aligned, of one element type; a stride
+ * is the distance, in elements, between two consecutive tokens of a tensor (a
+ * multiple of 16 bytes, so a tensor may be a part of a fused projection's
+ * rows).  Token i of sequence b is row b * n + i.  `positions` are host
+ * arrays.  Host-memory I/O mode is refused (SWIFTKV_ESTATE).
+ * ------------------------------------------------------------------------ */
+#define SWIFTKV_F32 0
+#define SWIFTKV_BF16 1
+#define SWIFTKV_F16 2
+
+/* How the frequencies f_j = theta^(-2j / rotary_dim) are changed for contexts
+ * longer than the model was trained on. */
+#define SWIFTKV_ROPE_LINEAR 1 /* f / factor */
+#define SWIFTKV_ROPE_THETA 2  /* theta * factor^(rotary_dim / (rotary_dim - 2)) in the place of theta */
+#define SWIFTKV_ROPE_BANDS 3  /* by the turns t = original_positions * f / (2 pi) that a pair makes within the
+                               * original context: f where t >= high, f / factor where t <= low, and linearly
+                               * in t between the two */
+typedef struct swiftkv_rope_scaling {
+    int32_t kind;               /* one of the above, or 0: none */
+    int32_t original_positions; /* BANDS only, >= 1 */
+    double factor;              /* >= 1 (kinds 1 to 3) */
+    double low, high;           /* BANDS only, 0 < low < high */
+    double magnitude;           /* multiplies cos and sin; 0 stands for 1 */
+} swiftkv_rope_scaling;
+
+/* swiftkv_rope_lut_generate with scaled frequencies (rotary_dim 128), for the
+ * step entries above; |magnitude| < 2, the Q1.17 range.  scaling may be NULL. */
+int swiftkv_rope_lut_generate_scaled(swiftkv_context* ctx, int32_t positions, double theta,
+                                     const swiftkv_rope_scaling* scaling, swiftkv_rope_lut** out);
+
+/* FP32 cos and sin of positions [0, positions), computed in 64 bits and
+ * rounded once.  rotary_dim: the channels of a head that rotate, even, 2 to
+ * 256 (4 or more for THETA); positions: 1 to SWIFTKV_ROTARY_MAX_POSITIONS. */
+#define SWIFTKV_ROTARY_MAX_POSITIONS 1048576
+typedef struct swiftkv_rotary_table swiftkv_rotary_table;
+int swiftkv_rotary_create(swiftkv_context* ctx, int32_t rotary_dim, int32_t positions, double theta,
+                          const swiftkv_rope_scaling* scaling, swiftkv_rotary_table** out);
+int swiftkv_rotary_destroy(swiftkv_rotary_table* table);
+
+/* Rotate `heads` heads of batch x n tokens: token i of sequence b stands at
+ * positions[b] + i.  Pair j of a head is channels (2j, 2j + 1), or with
+ * `halves` (j, j + rotary_dim / 2); (a, b) becomes (a c - b s, a s + b c), or
+ * with `inverse` (a c + b s, b c - a s), which is also the gradient of the
+ * rotation; channels past rotary_dim are copied.  Computed in FP32, rounded
+ * once.  x and out may be the same tensor (with one stride); otherwise they
+ * must not overlap.
+ *   head_dim   rotary_dim <= head_dim <= 1024
+ *   x_stride, out_stride   >= heads * head_dim
+ * Of the rules above only the element's own alignment holds here; with 16-byte
+ * aligned tensors, strides and head_dim in multiples of 8 and rotary_dim of 16
+ * the fast form runs. */
+int swiftkv_rotary(swiftkv_context* ctx, const swiftkv_rotary_table* table, const void* x, int64_t x_stride,
+                   void* out, int64_t out_stride, int32_t dtype, int32_t halves, int32_t inverse,
+                   const int32_t* positions, int32_t batch, int32_t n, int32_t heads, int32_t head_dim);
+
+/* The block cache: INT8 codes with one scale for the K codes and one for the V
+ * codes of each block of SWIFTKV_BLOCK_TOKENS tokens and key/value head.  A
+ * scale is 2^e, e the smallest integer >= -100 with max|x| <= 127 * 2^e; a code
+ * is x / 2^e, rounded half-even.  A NaN or a magnitude above 127 * 2^120 among a
+ * block's rows makes its scale NaN, and with it every output that attends to the
+ * block.
+ *   heads     query heads, a multiple of kv_heads; heads / kv_heads consecutive
+ *             query heads share a key/value head (<= 64)
+ *   head_dim  64 or 128
+ *   max_seq_len   <= SWIFTKV_BLOCK_MAX_SEQ; the capacity is the next multiple of
+ *             64 tokens
+ * Blocks of a (sequence, layer, key/value head) have an order of their own,
+ * which eviction changes without moving a code; appending rows at position 0
+ * starts a sequence anew. */
+#define SWIFTKV_BLOCK_TOKENS 16
+#define SWIFTKV_BLOCK_MAX_SEQ 131072
+typedef struct swiftkv_block_cache swiftkv_block_cache;
+int swiftkv_block_cache_create(swiftkv_context* ctx, int32_t layers, int32_t max_batch, int32_t heads,
+                               int32_t kv_heads, int32_t head_dim, int32_t max_seq_len,
+                               swiftkv_block_cache** out);
+int swiftkv_block_cache_destroy(swiftkv_block_cache* cache);
+size_t swiftkv_block_cache_bytes(const swiftkv_block_cache* cache);
+/* Blocks of one (sequence, layer, key/value head): capacity / 16. */
+int32_t swiftkv_block_cache_blocks(const swiftkv_block_cache* cache);
+
+/* Append n tokens to each of the sequences seq0 .. seq0 + batch - 1 of one
+ * layer, at cached tokens [positions[b], positions[b] + n); a negative position
+ * skips the sequence.  k, v: [batch * n][kv_heads * head_dim], rows k_stride and
+ * v_stride apart.  A block that holds earlier rows keeps its scale unless the
+ * new rows need a larger one; its codes are then rounded to that one. */
+int swiftkv_block_append(swiftkv_context* ctx, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                         int32_t dtype, swiftkv_block_cache* cache, int32_t layer_index, int32_t seq0,
+                         const int32_t* positions, int32_t batch, int32_t n);
+
+/* The values that cached tokens [positions[b], positions[b] + n) stand for, to
+ * k and v: device [batch * n][kv_heads * head_dim], dense.  A negative position
+ * leaves its sequence's rows as they are. */
+int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache, int32_t layer_index, int32_t seq0,
+                         const int32_t* positions, int32_t batch, int32_t n, int32_t dtype, void* k, void* v);
+
+/* Attention of n query tokens of each sequence over one layer's cache.  With k
+ * and v (both, or neither) it first appends their rows as swiftkv_block_append
+ * does; without, the rows have to be there.  Query i of sequence b attends to
+ * cached tokens [0, positions[b] + i]; a sequence with a negative position takes
+ * no part, and its output rows are zero.
+ *   q, out    [batch * n][heads * head_dim], q_stride and out_stride apart; out
+ *             has q's type and must not overlap the inputs
+ *   scale     multiplies q.k; 0 stands for 1 / sqrt(head_dim)
+ *   weights   NULL, or device FP32 [batch][kv_heads][blocks of the cache], in the
+ *             blocks' present order: the softmax weight that the n queries of the
+ *             key/value head's query heads give the tokens of each block is added
+ *             (n <= SWIFTKV_BLOCK_WEIGHT_QUERIES).  The first call with weights,
+ *             and the first with a larger n, allocates; run it once before a
+ *             capture.
+ * Scores, softmax sums and outputs are held in FP32; results do not depend on
+ * which workgroup ends first. */
+#define SWIFTKV_BLOCK_WEIGHT_QUERIES 8
+int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                            const void* v, int64_t v_stride, int32_t dtype, swiftkv_block_cache* cache,
+                            int32_t layer_index, int32_t seq0, const int32_t* positions, int32_t batch, int32_t n,
+                            float scale, float* weights, void* out, int64_t out_stride);
+
+/* Drop all but `keep` blocks of each (layer, sequence, key/value head) of layers
+ * layer0 .. layer0 + layers - 1 and sequences seq0 .. seq0 + batch - 1 that holds
+ * more; positions[b] is the number of cached tokens.  The first `sinks` and the
+ * last `recent` blocks stay (recent >= 1: the block that is being filled stays
+ * last; sinks + recent <= keep); of the others those of the largest weight, ties
+ * to the lower index.  A weight that is negative or NaN counts as 0.  The blocks that stay keep their
+ * order, the weights move with them, and the rest of the weights is set to 0.
+ *   weights   device FP32 [layers][batch][kv_heads][blocks of the cache]
+ *   kept      NULL, or device int32 [layers][batch][kv_heads][keep]: the former
+ *             index of each block that stayed, then -1
+ *   out_positions   NULL, or host [batch]: the number of tokens then cached
+ * Rotated keys keep their rotation: later rows are rotated by their own
+ * position, not by their place in the cache. */
+int swiftkv_block_evict(swiftkv_context* ctx, swiftkv_block_cache* cache, int32_t layer0, int32_t layers,
+                        int32_t seq0, const int32_t* positions, int32_t batch, int32_t keep, int32_t sinks,
+                        int32_t recent, float* weights, int32_t* kept, int32_t* out_positions);
+
+/* --------------------------------------------------------------------------
  * Device-memory helpers for FFI callers without a GPU framework (ctypes).
  * swiftkv_device_free takes only pointers from swiftkv_device_alloc on the
  * same context (anything else, or a second free: SWIFTKV_EINVAL); it waits
