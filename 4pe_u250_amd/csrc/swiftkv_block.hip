@@ -61,130 +61,161 @@ __device__ __forceinline__ float joined_scale(float amax, bool bad, bool held, f
     return any_bad ? __builtin_nanf("") : s;
 }
 
+// What a wave needs to append rows to one block: where its tokens and rows lie.
+template <typename T>
+struct BlockRows {
+    int tok0;             // the block's first token
+    int p, end;           // tokens [p, end) are new
+    const T* rows;        // the new rows of this key/value head: token p's
+    int64_t stride;
+    bool held;            // the block keeps rows of earlier calls
+    float old;            // its scale then
+};
+
+// One wave appends a block's K rows: lane = (token, 16-channel chunks c and
+// c + 4).  A block that keeps its scale has only the new rows written; with
+// COPY the whole block also goes to `copy` (LDS).  Returns the scale.
+template <typename T, int HD, bool COPY>
+__device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record, int8_t* copy, int lane) {
+    constexpr int NC = HD / 64;
+    const int t = lane >> 2, c = lane & 3, tok = r.tok0 + t;
+    const bool fresh = tok >= r.p && tok < r.end;
+    float x[NC][16];
+    v4i o[NC];
+    float amax = 0.0f;
+    bool bad = false;
+    // Every lane loads a row, the nearest new one where its own is not new: no
+    // branch that the loads would wait at.
+    const T* src = r.rows + (min(max(tok, r.p), r.end - 1) - r.p) * r.stride + c * 16;
+    Vec8<T> lo[NC], hi[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        lo[i] = *reinterpret_cast<const Vec8<T>*>(src + i * 64);
+        hi[i] = *reinterpret_cast<const Vec8<T>*>(src + i * 64 + 8);
+        o[i] = v4i{0, 0, 0, 0};
+        if (COPY && r.held && !fresh) o[i] = *reinterpret_cast<const v4i*>(record + (c + 4 * i) * (kBlockRows * 16) + t * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[i][j] = fresh ? static_cast<float>(lo[i].v[j]) : 0.0f;
+            x[i][8 + j] = fresh ? static_cast<float>(hi[i].v[j]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            amax = fmaxf(amax, fabsf(x[i][j]));
+            bad |= !(fabsf(x[i][j]) <= kRowMax);
+        }
+    const float s = joined_scale(amax, bad, r.held, r.old);
+    const bool poisoned = s != s;
+    const float inv = poisoned ? 0.0f : pow2_inverse(s);
+    const float ratio = r.old * inv;
+    const bool requantize = r.held && !poisoned && r.old != s;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int at = (c + 4 * i) * (kBlockRows * 16) + t * 16;
+        v4i w = COPY ? o[i] : v4i{0, 0, 0, 0};
+        if (fresh && !poisoned) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j >> 2] |= static_cast<int32_t>(code_byte(x[i][j] * inv) << (8 * (j & 3)));
+        }
+        if (requantize && !fresh) {
+            if (!COPY) o[i] = *reinterpret_cast<const v4i*>(record + at);
+            w = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                w[j >> 2] |= static_cast<int32_t>(code_byte(byte_value(static_cast<uint32_t>(o[i][j >> 2]), j & 3) * ratio)
+                                                  << (8 * (j & 3)));
+        }
+        if (fresh || !r.held || requantize) *reinterpret_cast<v4i*>(record + at) = w;
+        if (COPY) *reinterpret_cast<v4i*>(copy + at) = w;
+    }
+    return s;
+}
+
+// The same for V: lane = channels NC * lane .., each a run of 16 tokens that the
+// lane alone holds, so new bytes merge into it without a race.
+template <typename T, int HD, bool COPY>
+__device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record, int8_t* copy, int lane) {
+    constexpr int NC = HD / 64;
+    struct alignas(sizeof(T) * NC) Pack { T v[NC]; };
+    const T* src = r.rows + lane * NC;
+    v4i o[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        o[i] = v4i{0, 0, 0, 0};
+        if (r.held) o[i] = *reinterpret_cast<const v4i*>(record + (lane * NC + i) * kBlockRows);
+    }
+    float x[kBlockRows][NC];
+    float amax = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < kBlockRows; ++t) {
+        const int tok = r.tok0 + t;
+        const Pack w = *reinterpret_cast<const Pack*>(src + (min(max(tok, r.p), r.end - 1) - r.p) * r.stride);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) x[t][i] = tok >= r.p && tok < r.end ? static_cast<float>(w.v[i]) : 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < kBlockRows; ++t)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            amax = fmaxf(amax, fabsf(x[t][i]));
+            bad |= !(fabsf(x[t][i]) <= kRowMax);
+        }
+    const float s = joined_scale(amax, bad, r.held, r.old);
+    const bool poisoned = s != s;
+    const float inv = poisoned ? 0.0f : pow2_inverse(s);
+    const float ratio = r.old == s || poisoned ? 1.0f : r.old * inv;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        v4i w = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < kBlockRows; ++t) {
+            const int tok = r.tok0 + t;
+            const bool fresh = tok >= r.p && tok < r.end;
+            const float kept = byte_value(static_cast<uint32_t>(o[i][t >> 2]), t & 3) * ratio;
+            const float v = fresh ? (poisoned ? 0.0f : x[t][i] * inv) : kept;
+            w[t >> 2] |= static_cast<int32_t>(code_byte(v) << (8 * (t & 3)));
+        }
+        *reinterpret_cast<v4i*>(record + (lane * NC + i) * kBlockRows) = w;
+        if (COPY) *reinterpret_cast<v4i*>(copy + (lane * NC + i) * kBlockRows) = w;
+    }
+    return s;
+}
+
 // Workgroup (key/value head, touched block, sequence): wave 0 appends the
-// block's K rows, wave 1 its V rows.  Reading and writing bound it; a row is
-// read once, and a block that keeps its scale writes K codes of the new rows
-// only.  A V channel's 16 tokens are one lane's 16 bytes, so one wave owns the
-// whole record half and merges new bytes into it without a race.
+// block's K rows, wave 1 its V rows.  Reading the rows and writing the codes
+// bound it.
 template <typename T, int HD>
 __global__ __launch_bounds__(128) void block_append_kernel(const BlockRowsArgs a) {
-    constexpr int NC = HD / 64;
     const int kh = blockIdx.x, b = blockIdx.z;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int p = a.positions[b];
     if (p < 0) return;
     const int blk = p / kBlockRows + static_cast<int>(blockIdx.y);
-    const int tok0 = blk * kBlockRows, end = p + a.n;
-    if (tok0 >= end) return;
+    BlockRows<T> r;
+    r.tok0 = blk * kBlockRows;
+    r.p = p;
+    r.end = p + a.n;
+    if (r.tok0 >= r.end) return;
     const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
     int8_t* const base = a.view.base + page * a.view.page_bytes;
     const int rec = a.view.table[page * a.view.blocks + blk];
     int8_t* const record = base + static_cast<int64_t>(rec) * (2 * kBlockRows * HD) + wave * (kBlockRows * HD);
     float* const scale = reinterpret_cast<float*>(base + static_cast<int64_t>(a.view.blocks) * (2 * kBlockRows * HD)) +
                          2 * rec + wave;
-    const bool held = tok0 < p;                  // the block keeps rows of earlier calls
-    const float old = held ? *scale : 0.0f;
-    const int64_t row0 = static_cast<int64_t>(b) * a.n - p;   // row of token 0
-    float s;
-    if (wave == 0) {
-        // lane = (token, 16-channel chunks c and c + 4)
-        const int t = lane >> 2, c = lane & 3, tok = tok0 + t;
-        const bool fresh = tok >= p && tok < end;
-        float x[NC][16];
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
-            if (fresh) {
-                const T* src = static_cast<const T*>(a.k) + (row0 + tok) * a.k_stride + kh * HD + (c + 4 * i) * 16;
-                const Vec8<T> lo = *reinterpret_cast<const Vec8<T>*>(src);
-                const Vec8<T> hi = *reinterpret_cast<const Vec8<T>*>(src + 8);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[i][j] = static_cast<float>(lo.v[j]);
-                    x[i][8 + j] = static_cast<float>(hi.v[j]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                amax = fmaxf(amax, fabsf(x[i][j]));
-                bad |= !(fabsf(x[i][j]) <= kRowMax);
-            }
-        }
-        s = joined_scale(amax, bad, held, old);
-        const bool poisoned = s != s;
-        const float inv = poisoned ? 0.0f : pow2_inverse(s);
-        const float ratio = old * inv;
-        const bool requantize = held && !poisoned && old != s;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            int8_t* const dst = record + (c + 4 * i) * (kBlockRows * 16) + t * 16;
-            v4i w = {0, 0, 0, 0};
-            if (fresh && !poisoned) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) w[j >> 2] |= static_cast<int32_t>(code_byte(x[i][j] * inv) << (8 * (j & 3)));
-            }
-            if (requantize && !fresh) {
-                const v4i o = *reinterpret_cast<const v4i*>(dst);
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    w[j >> 2] |= static_cast<int32_t>(code_byte(byte_value(static_cast<uint32_t>(o[j >> 2]), j & 3) * ratio)
-                                                      << (8 * (j & 3)));
-            }
-            if (fresh || !held || requantize) *reinterpret_cast<v4i*>(dst) = w;
-        }
-    } else {
-        // lane = channels NC * lane ..; its NC runs of 16 tokens
-        const T* src = static_cast<const T*>(a.v) + kh * HD + lane * NC;
-        float x[kBlockRows][NC];
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int t = 0; t < kBlockRows; ++t) {
-#pragma unroll
-            for (int i = 0; i < NC; ++i) x[t][i] = 0.0f;
-            const int tok = tok0 + t;
-            if (tok >= p && tok < end) {
-                struct alignas(sizeof(T) * NC) Pack { T v[NC]; };
-                const Pack w = *reinterpret_cast<const Pack*>(src + (row0 + tok) * a.v_stride);
-#pragma unroll
-                for (int i = 0; i < NC; ++i) x[t][i] = static_cast<float>(w.v[i]);
-            }
-        }
-        v4i o[NC];
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            o[i] = v4i{0, 0, 0, 0};
-            if (held) o[i] = *reinterpret_cast<const v4i*>(record + (lane * NC + i) * kBlockRows);
-        }
-#pragma unroll
-        for (int t = 0; t < kBlockRows; ++t)
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                amax = fmaxf(amax, fabsf(x[t][i]));
-                bad |= !(fabsf(x[t][i]) <= kRowMax);
-            }
-        s = joined_scale(amax, bad, held, old);
-        const bool poisoned = s != s;
-        const float inv = poisoned ? 0.0f : pow2_inverse(s);
-        const float ratio = old == s || poisoned ? 1.0f : old * inv;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            v4i w = {0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < kBlockRows; ++t) {
-                const int tok = tok0 + t;
-                const bool fresh = tok >= p && tok < end;
-                const float kept = byte_value(static_cast<uint32_t>(o[i][t >> 2]), t & 3) * ratio;
-                const float v = fresh ? (poisoned ? 0.0f : x[t][i] * inv) : kept;
-                w[t >> 2] |= static_cast<int32_t>(code_byte(v) << (8 * (t & 3)));
-            }
-            *reinterpret_cast<v4i*>(record + (lane * NC + i) * kBlockRows) = w;
-        }
-    }
-    if (lane == 0 && !(held && old == s)) *scale = s;
+    r.stride = wave == 0 ? a.k_stride : a.v_stride;
+    r.rows = static_cast<const T*>(wave == 0 ? a.k : a.v) + static_cast<int64_t>(b) * a.n * r.stride + kh * HD;
+    r.held = r.tok0 < p;
+    r.old = r.held ? *scale : 0.0f;
+    const float s = wave == 0 ? append_k<T, HD, false>(r, record, nullptr, lane)
+                              : append_v<T, HD, false>(r, record, nullptr, lane);
+    if (lane == 0 && !(r.held && r.old == s)) *scale = s;
 }
 
 // The reverse, with the same lanes: values of cached rows, rounded once.
@@ -265,14 +296,25 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 // FP32 products would.
 //
 // Wave w takes tiles w, w + 4, ... of the split, each with its own running
-// (max, sum, output); the waves meet in LDS, the splits in block_merge_kernel.
+// (max, sum, output); the waves meet in LDS.  A wave always has a tile's loads
+// in flight: the next tile's K codes are asked for once the scores are done
+// with this one's, its V codes once the output is.
+//
+// ONCE (one row chunk, so each page is read once): the codes are read past the
+// caches (nontemporal; 64 sequences of 4096 tokens, 8 key/value heads, 82 us
+// against 100.6), and the call's new rows are appended here: each workgroup
+// appends to the blocks of its own range, at most two (n <= 16), writes them to
+// the cache and keeps them in LDS, from where the wave that scans their tile
+// takes them.
+//
+// A sequence's splits publish (m, l, acc) with write-through stores and count
+// themselves; the last to arrive joins them in split order, so the result does
+// not depend on who that is.
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves4 = 4;
 constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
 constexpr int kDigitBits = 7;
 constexpr float kDigitOne = 134217728.0f;        // 2^27
-
-#define SWIFTKV_CONSTANT __attribute__((address_space(4)))
 
 template <int HD, int RT>
 struct AttendShared {
@@ -352,17 +394,64 @@ __device__ __forceinline__ float row16_sum_f(float x) {
     return x + dpp_f<kDppRowRor8>(x);
 }
 
+__device__ __forceinline__ void publish(float* p, float v) {
+    __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float fetch(const float* p) {
+    return __uint_as_float(__hip_atomic_load(const_cast<uint32_t*>(reinterpret_cast<const uint32_t*>(p)),
+                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// A tile's scales, uniform over the wave.
+struct TileHead {
+    float ks[kTileBlocks], vs[kTileBlocks];
+};
+
+// The table entries and scales of 64 of a wave's tiles, a tile in each lane,
+// so that the scan's loads wait for no other: read one tile at a time (scalar
+// loads, which share a counter with LDS accesses) they took two trips to memory
+// a tile, and 64 sequences of 4096 tokens 128 us.
+struct TileHeads {
+    uint64_t entry;
+    uint64_t scale[kTileBlocks];
+
+    __device__ __forceinline__ void load_entries(const uint64_t* table, int tile, int last) {
+        entry = table[min(tile, last)];
+    }
+    __device__ __forceinline__ void load_scales(const int8_t* scales) {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j)
+            scale[j] = *reinterpret_cast<const uint64_t*>(scales + 8 * ((entry >> (16 * j)) & 0xffffu));
+    }
+    // Records 0 and 1 of a tile, then 2 and 3.
+    __device__ __forceinline__ uint32_t low(int lane) const {
+        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry), lane);
+    }
+    __device__ __forceinline__ uint32_t high(int lane) const {
+        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry >> 32), lane);
+    }
+    __device__ __forceinline__ void scales_of(int lane, TileHead& h) const {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) {
+            h.ks[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j]), lane));
+            h.vs[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j] >> 32), lane));
+        }
+    }
+};
+
 template <typename T, int HD, int RT, bool LSE, bool ONCE>
-__global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const BlockAttendArgs a) {
+__global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_kernel(const BlockAttendArgs a) {
     using S = AttendShared<HD, RT>;
     constexpr int NS = HD / 64;                  // 64-channel steps of a score
     constexpr int ND = HD / 16;                  // 16-channel tiles of an output
-    // ONCE: each page is read by one row chunk, past the caches (nontemporal): 64
-    // sequences of 4096 tokens, 8 key/value heads, 82 us against 100.6.
-    constexpr int kPolicy = ONCE ? 2 : 0;
+    constexpr int kPolicy = ONCE ? 2 : 0;        // nontemporal
+    constexpr int kRecord = 2 * kBlockRows * HD;
     constexpr int kRows = S::kRows;
     __shared__ __align__(16) uint8_t lds[S::kBytes];
+    __shared__ __align__(16) int8_t tail[ONCE ? 2 * kRecord : 16];   // the blocks that this call appends to
+    __shared__ float tail_scale[4];
     __shared__ float q_scale[kRows];
+    __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n16 = lane & 15;
     const int b = blockIdx.y;
@@ -378,17 +467,78 @@ __global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const Bloc
     const int tiles = (most + kTileTokens - 1) / kTileTokens;
     const int my_splits = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
     if (split >= my_splits) return;
-    const int tile_end = min(tiles, (split + 1) * a.split_tiles);
-
-    stage_queries<T, HD, RT>(a, b, kh, row_first, rows, lds, q_scale);
-    __syncthreads();
+    const int tile_begin = split * a.split_tiles, tile_end = min(tiles, tile_begin + a.split_tiles);
 
     const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
     int8_t* const base = a.view.base + page * a.view.page_bytes;
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
         base, static_cast<short>(0), static_cast<int32_t>(a.view.page_bytes), kBufferWord3);
-    const auto* table = (const SWIFTKV_CONSTANT uint64_t*)(a.view.table + page * a.view.blocks);
-    const auto* scales = (const SWIFTKV_CONSTANT uint64_t*)(base + static_cast<int64_t>(a.view.blocks) * (2 * kBlockRows * HD));
+    const uint64_t* table = reinterpret_cast<const uint64_t*>(a.view.table + page * a.view.blocks);
+    int8_t* const scale_base = base + static_cast<int64_t>(a.view.blocks) * kRecord;
+
+    v4i kb[kTileBlocks][NS], vb[ND];
+    auto load_k = [&](uint32_t low, uint32_t high) {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) {
+            const int at = static_cast<int>(((j & 2 ? high : low) >> (16 * (j & 1))) & 0xffffu) * kRecord;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, at + s * 1024, kPolicy);
+        }
+    };
+    auto load_v = [&](uint32_t low, uint32_t high) {
+        const uint32_t mine = ((g & 2 ? high : low) >> (16 * (g & 1))) & 0xffffu;
+        const int at = static_cast<int>(mine) * kRecord + kBlockRows * HD + n16 * 16;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, i * 256, kPolicy);
+    };
+
+    // The first tile's loads go out before any math; a wave without a tile asks
+    // for the split's last again and drops it.
+    const int last_tile = max(tile_begin, tile_end - 1);
+    int tile0 = tile_begin + wave;               // first of the 64 tiles whose heads the wave holds
+    TileHeads heads;
+    uint32_t low = 0, high = 0;                  // the next tile's table entry
+    auto start = [&]() {
+        heads.load_entries(table, tile0 + lane * kAttendWaves4, last_tile);
+        low = heads.low(0);
+        high = heads.high(0);
+        load_k(low, high);
+        load_v(low, high);
+        heads.load_scales(scale_base);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    start();
+
+    stage_queries<T, HD, RT>(a, b, kh, row_first, rows, lds, q_scale);
+
+    // Blocks of this range that new rows go to: wave pairs take one each, K and V.
+    int touch_begin = 0, touch_end = 0;
+    if (ONCE && a.k != nullptr && p >= 0) {
+        touch_begin = max(p / kBlockRows, tile_begin * kTileBlocks);
+        touch_end = min((p + a.n - 1) / kBlockRows + 1, tile_end * kTileBlocks);
+        const int blk = touch_begin + (wave >> 1), is_v = wave & 1;
+        if (blk < touch_end) {
+            const int mine = static_cast<int>((table[blk / kTileBlocks] >> (16 * (blk % kTileBlocks))) & 0xffffu);
+            int8_t* const record = base + static_cast<int64_t>(mine) * kRecord + is_v * (kBlockRows * HD);
+            int8_t* const copy = tail + (wave >> 1) * kRecord + is_v * (kBlockRows * HD);
+            float* const scale = reinterpret_cast<float*>(scale_base) + 2 * mine + is_v;
+            BlockRows<T> r;
+            r.tok0 = blk * kBlockRows;
+            r.p = p;
+            r.end = p + a.n;
+            r.stride = is_v ? a.v_stride : a.k_stride;
+            r.rows = static_cast<const T*>(is_v ? a.v : a.k) + static_cast<int64_t>(b) * a.n * r.stride + kh * HD;
+            r.held = r.tok0 < p;
+            r.old = r.held ? *scale : 0.0f;
+            const float s = is_v ? append_v<T, HD, true>(r, record, copy, lane) : append_k<T, HD, true>(r, record, copy, lane);
+            if (lane == 0) {
+                tail_scale[wave] = s;
+                if (!(r.held && r.old == s)) *scale = s;
+            }
+        }
+    }
+    __syncthreads();
 
     v4i qa[RT][NS];
     float qs[RT], m_run[RT], l_run[RT];
@@ -407,63 +557,80 @@ __global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const Bloc
         for (int i = 0; i < ND; ++i) acc[rt][i] = 0.0f;
     }
     uint8_t* const digits = lds + S::kQueryBytes + wave * (RT * 16 * kDigitStride);
+    const int64_t head_row = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + row_first;
 
-    for (int tile = split * a.split_tiles + wave; tile < tile_end; tile += kAttendWaves4) {
-        const uint64_t entry = table[tile];
-        int rec[kTileBlocks];
-        float ks[kTileBlocks], vs[kTileBlocks];
+    for (; tile0 < tile_end;) {
+    const int held_tiles = min(64, (tile_end - tile0 + kAttendWaves4 - 1) / kAttendWaves4);
+    for (int at = 0; at < held_tiles; ++at) {
+        const int tile = tile0 + at * kAttendWaves4;
+        const bool more = at + 1 < held_tiles;
+        TileHead head;
+        heads.scales_of(at, head);
+        if (ONCE && tile >= touch_begin / kTileBlocks && tile * kTileBlocks < touch_end) {
+            // blocks appended to by this call: from LDS, over what was loaded
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            rec[j] = static_cast<int>((entry >> (16 * j)) & 0xffffu);
-            const uint64_t w = scales[rec[j]];
-            ks[j] = __uint_as_float(static_cast<uint32_t>(w));
-            vs[j] = __uint_as_float(static_cast<uint32_t>(w >> 32));
+            for (int j = 0; j < kTileBlocks; ++j) {
+                const int t = tile * kTileBlocks + j - touch_begin;
+                if (t < 0 || t >= touch_end - touch_begin) continue;
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    kb[j][s] = *reinterpret_cast<const v4i*>(tail + t * kRecord + s * 1024 + lane * 16);
+                if (g == j) {
+#pragma unroll
+                    for (int i = 0; i < ND; ++i)
+                        vb[i] = *reinterpret_cast<const v4i*>(tail + t * kRecord + kBlockRows * HD + i * 256 + n16 * 16);
+                }
+                head.ks[j] = tail_scale[2 * t];
+                head.vs[j] = tail_scale[2 * t + 1];
+            }
         }
-        v4i kb[kTileBlocks][NS], vb[ND];
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j)
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, rec[j] * (2 * kBlockRows * HD) + s * 1024, kPolicy);
-        const int mine = g & 2 ? (g & 1 ? rec[3] : rec[2]) : (g & 1 ? rec[1] : rec[0]);
-        const int v_lane = mine * (2 * kBlockRows * HD) + kBlockRows * HD + n16 * 16;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) vb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, v_lane, i * 256, kPolicy);
-
-        // V scales over the tile's largest; a scale that is not a number poisons
-        // the rows that see its block.
-        float v_top = 0x1p-100f;
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) v_top = fmaxf(v_top, vs[j]);
-        const float v_inv = pow2_inverse(v_top);
+        if (more) {
+            low = heads.low(at + 1);
+            high = heads.high(at + 1);
+        }
         const int tok0 = tile * kTileTokens;
+
+        float s[RT][kTileBlocks];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float s[kTileBlocks];
-            float top = -INFINITY;
-            bool poison = false;
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
                 v4i c = {0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < NS; ++k) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][k], kb[j][k], c, 0, 0, 0);
-                const float low = static_cast<float>(c[0] + c[1] * 256);       // below 2^30
-                const float high = static_cast<float>(c[2] + c[3] * 256);
-                s[j] = __builtin_fmaf(high, 65536.0f, low) * (qs[rt] * ks[j]);
-                if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[j] = -INFINITY;
-                if (vs[j] != vs[j] && tok0 + kBlockRows * j < limit[rt]) poison = true;
-                top = fmaxf(top, s[j]);
+                const float lower = static_cast<float>(c[0] + c[1] * 256);     // below 2^30
+                const float upper = static_cast<float>(c[2] + c[3] * 256);
+                s[rt][j] = __builtin_fmaf(upper, 65536.0f, lower) * (qs[rt] * head.ks[j]);
+                if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[rt][j] = -INFINITY;
+            }
+        if (more) load_k(low, high);
+
+        // V scales over the tile's largest; a scale that is not a number poisons
+        // the rows that see its block.
+        float v_top = 0x1p-100f;
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) v_top = fmaxf(v_top, head.vs[j]);
+        const float v_inv = pow2_inverse(v_top);
+        v4i pa[RT];
+        float alpha[RT], v_mul[RT], block_sum[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float top = -INFINITY;
+            bool poison = false;
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) {
+                if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit[rt]) poison = true;
+                top = fmaxf(top, s[rt][j]);
             }
             top = row16_max_f(top);
             const float top_safe = top == -INFINITY ? 0.0f : top;    // a row that sees nothing here
             float sum = 0.0f;
-            float each[kTileBlocks];
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
-                const float w = fast_exp2(s[j] - top_safe);
-                each[j] = w;
+                const float w = fast_exp2(s[rt][j] - top_safe);
+                s[rt][j] = w;
                 sum += w;
-                const uint32_t d = static_cast<uint32_t>(__builtin_rintf(w * (vs[j] * v_inv) * kDigitOne));
+                const uint32_t d = static_cast<uint32_t>(__builtin_rintf(w * (head.vs[j] * v_inv) * kDigitOne));
                 uint8_t* dst = digits + (rt * 16 + g * 4) * kDigitStride + j * kBlockRows + n16;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) dst[k * kDigitStride] = static_cast<uint8_t>((d >> (kDigitBits * k)) & 127u);
@@ -473,36 +640,55 @@ __global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const Bloc
                 float mine_sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < kTileBlocks; ++j) {
-                    const float t = row16_sum_f(each[j]);
+                    const float t = row16_sum_f(s[rt][j]);
                     if (n16 == j) mine_sum = t;
                 }
-                const int row = rt * kRowTile + g;
-                if (n16 < kTileBlocks && row < rows) {
-                    const int64_t at = ((static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + row_first + row) *
-                                           a.view.blocks + tile * kTileBlocks + n16;
-                    a.block_lse[at] = top_safe + __log2f(mine_sum);
-                }
+                block_sum[rt] = top_safe + __log2f(mine_sum);
             }
             const float m_new = fmaxf(m_run[rt], top);
             const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = fast_exp2(m_run[rt] - m_safe), beta = fast_exp2(top - m_safe);
+            alpha[rt] = fast_exp2(m_run[rt] - m_safe);
+            const float beta = fast_exp2(top - m_safe);
             m_run[rt] = m_new;
-            l_run[rt] = l_run[rt] * alpha + sum * beta;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const v4i pa = *reinterpret_cast<const v4i*>(digits + (rt * 16 + n16) * kDigitStride + g * 16);
-            const float v_mul = poison ? __builtin_nanf("") : beta * v_top * (1.0f / kDigitOne);
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                v4i c = {0, 0, 0, 0};
-                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, vb[i], c, 0, 0, 0);
-                const float low = static_cast<float>(c[0] + c[1] * 128);       // below 2^28
-                const float high = static_cast<float>(c[2] + c[3] * 128);
-                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(high, 16384.0f, low), v_mul, acc[rt][i] * alpha);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            l_run[rt] = l_run[rt] * alpha[rt] + sum * beta;
+            v_mul[rt] = poison ? __builtin_nanf("") : beta * v_top * (1.0f / kDigitOne);
         }
+        // The digits were written by other lanes of this wave, whose LDS accesses
+        // stay in order; the fences keep the compiler to it.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            pa[rt] = *reinterpret_cast<const v4i*>(digits + (rt * 16 + n16) * kDigitStride + g * 16);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                v4i c = {0, 0, 0, 0};
+                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[rt], vb[i], c, 0, 0, 0);
+                const float lower = static_cast<float>(c[0] + c[1] * 128);     // below 2^28
+                const float upper = static_cast<float>(c[2] + c[3] * 128);
+                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 16384.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
+            }
+        if (more) load_v(low, high);
+        if (LSE) {
+            // The lane n16 == j < 4 has block j's.  After the loads, which would
+            // otherwise wait for these stores.
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int row = rt * kRowTile + g;
+                if (n16 < kTileBlocks && row < rows) {
+                    float* dst = a.block_lse + (head_row + row) * a.view.blocks + tile * kTileBlocks + n16;
+                    if (my_splits > 1) publish(dst, block_sum[rt]);
+                    else *dst = block_sum[rt];
+                }
+            }
+        }
+    }
+    tile0 += 64 * kAttendWaves4;
+    if (tile0 < tile_end) start();
     }
 
     // The waves' partials meet in LDS.
@@ -520,10 +706,13 @@ __global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const Bloc
         for (int i = 0; i < ND; ++i) dst[2 + i * 16 + n16] = acc[rt][i];
     }
     __syncthreads();
+    constexpr int kItems = kRows * HD / kAttendThreads;      // outputs of a thread
     const int64_t pair = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.chunks + chunk;
-    for (int i = threadIdx.x; i < kRows * HD; i += kAttendThreads) {
-        const int row = i / HD, d = i % HD;
-        if (row >= rows) break;
+    float* const partial = a.partials + pair * a.splits * kRows * (HD + 2);
+    float m_all[kItems], l_all[kItems], o_all[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kAttendWaves4; ++w) m = fmaxf(m, merge[(w * kRows + row) * (HD + 2)]);
@@ -536,55 +725,78 @@ __global__ __launch_bounds__(kAttendThreads) void block_attend_kernel(const Bloc
             l = __builtin_fmaf(src[1], f, l);
             o = __builtin_fmaf(src[2 + d], f, o);
         }
+        m_all[k] = m;
+        l_all[k] = l;
+        o_all[k] = o;
         if (my_splits > 1) {
-            float* dst = a.partials + ((pair * a.splits + split) * kRows + row) * (HD + 2);
+            float* dst = partial + (static_cast<int64_t>(split) * kRows + row) * (HD + 2);
             if (d == 0) {
-                dst[0] = m;
-                dst[1] = l;
+                publish(dst, m);
+                publish(dst + 1, l);
             }
-            dst[2 + d] = o;
-            continue;
+            publish(dst + 2 + d, o);
         }
+    }
+    if (my_splits > 1 || LSE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what was published has arrived
+    __syncthreads();
+    if (my_splits > 1) {
+        uint32_t* const counter = a.counters + pair * kCounterStride;
+        if (threadIdx.x == 0)
+            arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (static_cast<int>(arrived) != my_splits - 1) return;
+        // The last split: everybody's partials, in split order.  The counter is
+        // zero again for the next launch.
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
+            float m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll 8
+            for (int j = 0; j < my_splits; ++j) {
+                const float* src = partial + (static_cast<int64_t>(j) * kRows + row) * (HD + 2);
+                const float mj = fetch(src), lj = fetch(src + 1), oj = fetch(src + 2 + d);
+                const float m_new = fmaxf(m, mj), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+                const float f = fast_exp2(m - m_safe), fj = fast_exp2(mj - m_safe);
+                l = l * f + lj * fj;
+                o = o * f + oj * fj;
+                m = m_new;
+            }
+            m_all[k] = m;
+            l_all[k] = l;
+            o_all[k] = o;
+        }
+    }
+    float* const lse = merge;                    // log2 of each row's sum
+    if (LSE) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
+        if (row >= rows) break;
         const int r = row_first + row;
         const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
         static_cast<T*>(a.out)[token * a.out_stride + static_cast<int64_t>(kh * a.group + r % a.group) * HD + d] =
-            static_cast<T>(l == 0.0f ? 0.0f : o / l);
-        if (LSE && d == 0)
-            a.row_lse[(static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + r] = m_safe + __log2f(l);
+            static_cast<T>(l_all[k] == 0.0f ? 0.0f : o_all[k] / l_all[k]);
+        if (LSE && d == 0) {
+            const float v = (m_all[k] == -INFINITY ? 0.0f : m_all[k]) + __log2f(l_all[k]);
+            if (ONCE) lse[row] = v;
+            else a.row_lse[head_row + row] = v;
+        }
     }
-}
-
-// Joins the splits of a row, in split order: workgroup (kv head and chunk, sequence).
-template <typename T, int HD, bool LSE>
-__global__ __launch_bounds__(HD) void block_merge_kernel(const BlockAttendArgs a, int chunk_rows) {
-    const int kh = blockIdx.x % a.view.kv_heads, chunk = blockIdx.x / a.view.kv_heads, b = blockIdx.y;
-    const int all_rows = a.group * a.n, row_first = chunk * chunk_rows;
-    const int rows = min(chunk_rows, all_rows - row_first);
-    const int p = a.positions[b];
-    const int most = p < 0 ? 0 : p + (row_first + rows - 1) / a.group + 1;
-    const int tiles = (most + kTileTokens - 1) / kTileTokens;
-    const int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
-    if (splits <= 1) return;
-    const int64_t pair = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.chunks + chunk;
-    const int row = blockIdx.z, d = threadIdx.x;
-    if (row >= rows) return;
-    const float* src = a.partials + (pair * a.splits * chunk_rows + row) * (HD + 2);
-    const int64_t step = static_cast<int64_t>(chunk_rows) * (HD + 2);
-    float m = -INFINITY;
-    for (int j = 0; j < splits; ++j) m = fmaxf(m, src[j * step]);
-    const float m_safe = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o = 0.0f;
-    for (int j = 0; j < splits; ++j) {
-        const float f = fast_exp2(src[j * step] - m_safe);
-        l = __builtin_fmaf(src[j * step + 1], f, l);
-        o = __builtin_fmaf(src[j * step + 2 + d], f, o);
+    if (LSE && ONCE) {
+        // All rows are here: weights[block] += sum over rows of 2^(the block's
+        // log-sum - the row's), rows in order.
+        __syncthreads();
+        if (p < 0) return;
+        float* const weights = a.weights + (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.view.blocks;
+        for (int blk = threadIdx.x; blk * kBlockRows < p + a.n; blk += kAttendThreads) {
+            float sum = 0.0f;
+            for (int r = 0; r < rows; ++r)
+                if (blk * kBlockRows <= p + r / a.group)
+                    sum += fast_exp2(fetch(a.block_lse + (head_row + r) * a.view.blocks + blk) - lse[r]);
+            weights[blk] += sum;
+        }
     }
-    const int r = row_first + row;
-    const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
-    static_cast<T*>(a.out)[token * a.out_stride + static_cast<int64_t>(kh * a.group + r % a.group) * HD + d] =
-        static_cast<T>(l == 0.0f ? 0.0f : o / l);
-    if (LSE && d == 0)
-        a.row_lse[(static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + r] = m_safe + __log2f(l);
 }
 
 // weights[block] += sum over rows of 2^(the block's log-sum - the row's): rows in
@@ -734,17 +946,19 @@ hipError_t launch_rows(const BlockRowsArgs& a, int batch, ElementType t, bool va
 template <typename T, int HD, int RT, bool LSE>
 void attend(const BlockAttendArgs& a, int batch, hipStream_t s) {
     const dim3 grid(a.view.kv_heads * a.splits * a.chunks, batch);
-    if (a.chunks == 1) block_attend_kernel<T, HD, RT, LSE, true><<<grid, kAttendThreads, 0, s>>>(a);
-    else if constexpr (RT == kMaxRowTiles) block_attend_kernel<T, HD, RT, LSE, false><<<grid, kAttendThreads, 0, s>>>(a);
-    if (a.splits > 1)
-        block_merge_kernel<T, HD, LSE>
-            <<<dim3(a.view.kv_heads * a.chunks, batch, RT * kRowTile), HD, 0, s>>>(a, RT * kRowTile);
-    if (LSE) {
-        int most = 0;
-        for (int b = 0; b < batch; ++b) most = a.positions[b] + a.n > most ? a.positions[b] + a.n : most;
-        const int blocks = (most + kBlockRows - 1) / kBlockRows;
-        if (blocks > 0)
-            block_weights_kernel<<<dim3((blocks + 255) / 256, a.view.kv_heads, batch), 256, 0, s>>>(a);
+    if (a.chunks == 1) {
+        block_attend_kernel<T, HD, RT, LSE, true><<<grid, kAttendThreads, 0, s>>>(a);
+        return;
+    }
+    if constexpr (RT == kMaxRowTiles) {
+        block_attend_kernel<T, HD, RT, LSE, false><<<grid, kAttendThreads, 0, s>>>(a);
+        if (LSE) {
+            int most = 0;
+            for (int b = 0; b < batch; ++b) most = a.positions[b] + a.n > most ? a.positions[b] + a.n : most;
+            const int blocks = (most + kBlockRows - 1) / kBlockRows;
+            if (blocks > 0)
+                block_weights_kernel<<<dim3((blocks + 255) / 256, a.view.kv_heads, batch), 256, 0, s>>>(a);
+        }
     }
 }
 }  // namespace

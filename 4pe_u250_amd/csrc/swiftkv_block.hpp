@@ -57,8 +57,12 @@ struct BlockAttendArgs {
     BlockView view;
     const void* q;
     void* out;
+    const void* k;        // new rows, appended by the same launch (chunks == 1 only); null: none
+    const void* v;
     int64_t q_stride;
     int64_t out_stride;
+    int64_t k_stride;
+    int64_t v_stride;
     float scale;          // log2(e) times the caller's
     int32_t group;        // query heads per key/value head
     int32_t n;
@@ -68,6 +72,7 @@ struct BlockAttendArgs {
     int32_t splits;       // of the longest sequence
     int32_t split_tiles;  // tiles per split
     float* partials;      // [pair][split][rows of a chunk][2 + head_dim]: m, l, acc
+    uint32_t* counters;   // [pair] arrived splits, kCounterStride apart, zero between launches
     float* block_lse;     // null, or [sequence][kv head][row][blocks]: log2 of each block's sum of 2^score
     float* row_lse;       // [sequence][kv head][row]: the same of the whole row
     float* weights;       // [sequence][kv head][blocks]
@@ -104,6 +109,8 @@ struct RotaryArgs {
 // Rows (query tokens times grouped heads) that one attention workgroup holds.
 constexpr int kRowTile = 4;          // rows of one matrix instruction, four limbs each
 constexpr int kMaxRowTiles = 4;
+// Words between the arrival counts of two pairs: a 128-byte line each.
+constexpr int kCounterStride = 32;
 
 hipError_t launch_block_table(const BlockView& v, int64_t pages, hipStream_t s);
 hipError_t launch_block_append(const BlockRowsArgs& a, int batch, ElementType t, hipStream_t s);

@@ -270,11 +270,17 @@ int swiftkv_block_cache_create(swiftkv_context* ctx, int32_t layers, int32_t max
         return fail(SWIFTKV_EINVAL, "max_seq_len %d outside [1, %d]", max_seq_len, kBlockMaxSeq);
     int rc = set_device(ctx);
     if (rc) return rc;
-    if (!ctx->block_partials) {
+    if (!ctx->block_workspace) {
         void* p = nullptr;
-        if (hipMalloc(&p, kPartialFloats * sizeof(float)) != hipSuccess)
-            return fail(SWIFTKV_ENOMEM, "hipMalloc of %zu bytes failed", kPartialFloats * sizeof(float));
-        ctx->block_partials = static_cast<float*>(p);
+        const size_t counters = kMaxSplitGroups * kCounterStride * sizeof(uint32_t);
+        const size_t bytes = counters + kPartialFloats * sizeof(float);
+        if (hipMalloc(&p, bytes) != hipSuccess) return fail(SWIFTKV_ENOMEM, "hipMalloc of %zu bytes failed", bytes);
+        const hipError_t e = hipMemsetAsync(p, 0, counters, ctx->stream);
+        if (e != hipSuccess) {
+            (void)hipFree(p);
+            return fail(SWIFTKV_EHIP, "split counters: %s", hipGetErrorString(e));
+        }
+        ctx->block_workspace = static_cast<uint32_t*>(p);
     }
     swiftkv_block_cache* c = new (std::nothrow) swiftkv_block_cache();
     if (!c) return fail(SWIFTKV_ENOMEM, "out of host memory");
@@ -403,7 +409,8 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.group = cache->heads / view.kv_heads;
     a.n = n;
     a.layer = layer_index;
-    a.partials = ctx->block_partials;
+    a.counters = ctx->block_workspace;
+    a.partials = reinterpret_cast<float*>(ctx->block_workspace + kMaxSplitGroups * kCounterStride);
     if (weights) {
         const size_t rows = static_cast<size_t>(std::min(cache->max_batch, kMaxBatchPerLaunch)) * cache->heads * n;
         const size_t need = rows * (static_cast<size_t>(view.blocks) + 1);
@@ -423,7 +430,12 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         a.row_lse = cache->log_sums;
         a.block_lse = cache->log_sums + rows;
     }
-    if (k && (rc = append_rows(ctx, k, k_stride, v, v_stride, dtype, cache, layer_index, seq0, positions, batch, n)))
+    // One row chunk: the attention's own launch appends.
+    const bool fused = a.group * n <= kMaxRowTiles * kRowTile;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    if (k && !fused &&
+        (rc = append_rows(ctx, k, k_stride, v, v_stride, dtype, cache, layer_index, seq0, positions, batch, n)))
         return rc;
     const int64_t size = static_cast<int64_t>(element_bytes(dtype));
     for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
@@ -432,6 +444,10 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.q = static_cast<const char*>(q) + first * q_stride * size;
         a.out = static_cast<char*>(out) + first * out_stride * size;
+        if (k && fused) {
+            a.k = static_cast<const char*>(k) + first * k_stride * size;
+            a.v = static_cast<const char*>(v) + first * v_stride * size;
+        }
         a.weights = weights ? weights + static_cast<int64_t>(b0) * view.kv_heads * view.blocks : nullptr;
         a.slot0 = seq0 + b0;
         a.chunks = plan.chunks;

@@ -658,7 +658,7 @@ void swiftkv::free_context(swiftkv_context* ctx) {
     for (void* p : ctx->retired) (void)hipFree(p);
     if (ctx->arrivals) (void)hipFree(ctx->arrivals);
     if (ctx->exact_workspace) (void)hipFree(ctx->exact_workspace);
-    if (ctx->block_partials) (void)hipFree(ctx->block_partials);
+    if (ctx->block_workspace) (void)hipFree(ctx->block_workspace);
     if (ctx->io_stage) (void)hipFree(ctx->io_stage);
     if (ctx->fault_host) (void)hipHostFree(ctx->fault_host);
     for (auto& t : ctx->timers)

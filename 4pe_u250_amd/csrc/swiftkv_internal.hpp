@@ -105,9 +105,10 @@ struct swiftkv_context {
     int64_t children = 0;
     bool released = false;
     std::unordered_set<void*> buffers;   // swiftkv_device_alloc allocations not yet freed
-    // Split partials of the block cache's attention, of a fixed size (a graph
-    // may record it at any time): allocated with the first block cache.
-    float* block_partials = nullptr;
+    // Arrival counts and split partials of the block cache's attention, of a
+    // fixed size (a graph may record them at any time): allocated with the first
+    // block cache.
+    uint32_t* block_workspace = nullptr;
 };
 
 struct swiftkv_graph {
