@@ -1,5 +1,7 @@
 // swiftkv_block.hip -- kernels of the block cache: append, values, attention,
 // eviction.  Layout and numerics: swiftkv_block.hpp, include/swiftkv.h.
+#include <type_traits>
+
 #include "swiftkv_block.hpp"
 #include "swiftkv_device.hpp"
 
@@ -423,6 +425,11 @@ struct TileHeads {
         for (int j = 0; j < kTileBlocks; ++j)
             scale[j] = *reinterpret_cast<const uint64_t*>(scales + 8 * ((entry >> (16 * j)) & 0xffffu));
     }
+    // Waits for the scales here, and not in each turn of the loop that uses them.
+    __device__ __forceinline__ void arrive() const {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) asm volatile("" ::"v"(scale[j]));
+    }
     // Records 0 and 1 of a tile, then 2 and 3.
     __device__ __forceinline__ uint32_t low(int lane) const {
         return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry), lane);
@@ -477,18 +484,18 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     int8_t* const scale_base = base + static_cast<int64_t>(a.view.blocks) * kRecord;
 
     v4i kb[kTileBlocks][NS], vb[ND];
-    auto load_k = [&](uint32_t low, uint32_t high) {
+    auto load_k = [&](uint32_t low, uint32_t high, int past) {
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
             const int at = static_cast<int>(((j & 2 ? high : low) >> (16 * (j & 1))) & 0xffffu) * kRecord;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
-                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, at + s * 1024, kPolicy);
+                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16 + past, at + s * 1024, kPolicy);
         }
     };
-    auto load_v = [&](uint32_t low, uint32_t high) {
+    auto load_v = [&](uint32_t low, uint32_t high, int past) {
         const uint32_t mine = ((g & 2 ? high : low) >> (16 * (g & 1))) & 0xffffu;
-        const int at = static_cast<int>(mine) * kRecord + kBlockRows * HD + n16 * 16;
+        const int at = static_cast<int>(mine) * kRecord + kBlockRows * HD + n16 * 16 + past;
 #pragma unroll
         for (int i = 0; i < ND; ++i) vb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, i * 256, kPolicy);
     };
@@ -503,9 +510,11 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
         heads.load_entries(table, tile0 + lane * kAttendWaves4, last_tile);
         low = heads.low(0);
         high = heads.high(0);
-        load_k(low, high);
-        load_v(low, high);
         heads.load_scales(scale_base);
+        __builtin_amdgcn_sched_barrier(0);       // in this order, as the scan waits for them
+        load_k(low, high, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(low, high, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
     start();
@@ -559,15 +568,12 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     uint8_t* const digits = lds + S::kQueryBytes + wave * (RT * 16 * kDigitStride);
     const int64_t head_row = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + row_first;
 
-    for (; tile0 < tile_end;) {
-    const int held_tiles = min(64, (tile_end - tile0 + kAttendWaves4 - 1) / kAttendWaves4);
-    for (int at = 0; at < held_tiles; ++at) {
-        const int tile = tile0 + at * kAttendWaves4;
-        const bool more = at + 1 < held_tiles;
+    // One tile.  FROM_LDS: it has blocks that this call appends to, which come
+    // from LDS over what was loaded; such a tile is its wave's last.
+    auto scan = [&](auto from_lds, int tile, int at, bool more) {
         TileHead head;
         heads.scales_of(at, head);
-        if (ONCE && tile >= touch_begin / kTileBlocks && tile * kTileBlocks < touch_end) {
-            // blocks appended to by this call: from LDS, over what was loaded
+        if constexpr (decltype(from_lds)::value) {
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
                 const int t = tile * kTileBlocks + j - touch_begin;
@@ -584,10 +590,11 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 head.vs[j] = tail_scale[2 * t + 1];
             }
         }
-        if (more) {
-            low = heads.low(at + 1);
-            high = heads.high(at + 1);
-        }
+        // A wave's last tile asks past the page's end, which fetches nothing: a
+        // branch around the loads would make every turn wait for both kinds.
+        const int past = more ? 0 : static_cast<int>(a.view.page_bytes);
+        low = heads.low(min(at + 1, 63));
+        high = heads.high(min(at + 1, 63));
         const int tok0 = tile * kTileTokens;
 
         float s[RT][kTileBlocks];
@@ -603,7 +610,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 s[rt][j] = __builtin_fmaf(upper, 65536.0f, lower) * (qs[rt] * head.ks[j]);
                 if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[rt][j] = -INFINITY;
             }
-        if (more) load_k(low, high);
+        load_k(low, high, past);
 
         // V scales over the tile's largest; a scale that is not a number poisons
         // the rows that see its block.
@@ -672,7 +679,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 const float upper = static_cast<float>(c[2] + c[3] * 128);
                 acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 16384.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
             }
-        if (more) load_v(low, high);
+        load_v(low, high, past);
         if (LSE) {
             // The lane n16 == j < 4 has block j's.  After the loads, which would
             // otherwise wait for these stores.
@@ -686,9 +693,18 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 }
             }
         }
-    }
-    tile0 += 64 * kAttendWaves4;
-    if (tile0 < tile_end) start();
+    };
+    // Tiles without appended blocks end here.
+    const int plain_end = touch_begin < touch_end ? touch_begin / kTileBlocks : tile_end;
+    while (tile0 < tile_end) {
+        heads.arrive();
+        const int end = min(tile_end, tile0 + 64 * kAttendWaves4);
+        int tile = tile0, at = 0;
+        for (; tile < min(end, plain_end); tile += kAttendWaves4, ++at)
+            scan(std::false_type{}, tile, at, tile + kAttendWaves4 < end);
+        if (ONCE && tile < end) scan(std::true_type{}, tile, at, false);
+        tile0 = end == tile_end ? tile_end : tile0 + 64 * kAttendWaves4;
+        if (tile0 < tile_end) start();
     }
 
     // The waves' partials meet in LDS.
