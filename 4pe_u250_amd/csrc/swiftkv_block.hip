@@ -53,14 +53,24 @@ __device__ __forceinline__ float byte_value(uint32_t word, int i) {
     return static_cast<float>(static_cast<int8_t>(static_cast<uint8_t>(word >> (8 * i))));
 }
 
-// One block's scale after rows with largest magnitude amax join it: the wave
-// gives its lanes' amax and whether any value is not finite.
-__device__ __forceinline__ float joined_scale(float amax, bool bad, bool held, float old) {
-    amax = wave_max(amax);
-    const bool any_bad = __ballot(bad) != 0;
+// 16 codes under a larger scale.
+__device__ __forceinline__ v4i rescaled(v4i o, float ratio) {
+    v4i w = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        w[j >> 2] |= static_cast<int32_t>(code_byte(byte_value(static_cast<uint32_t>(o[j >> 2]), j & 3) * ratio)
+                                          << (8 * (j & 3)));
+    return w;
+}
+
+// A row value's magnitude, infinite for all that a scale cannot cover (NaN too).
+__device__ __forceinline__ float row_magnitude(float x) { return fabsf(x) <= kRowMax ? fabsf(x) : INFINITY; }
+
+// A block's scale after rows of largest magnitude amax join it.
+__device__ __forceinline__ float joined_scale(float amax, bool held, float old) {
     float s = code_scale(amax);
     if (held) s = old >= s || old != old ? old : s;
-    return any_bad ? __builtin_nanf("") : s;
+    return amax == INFINITY ? __builtin_nanf("") : s;
 }
 
 // What a wave needs to append rows to one block: where its tokens and rows lie.
@@ -75,17 +85,15 @@ struct BlockRows {
 };
 
 // One wave appends a block's K rows: lane = (token, 16-channel chunks c and
-// c + 4).  A block that keeps its scale has only the new rows written; with
-// COPY the whole block also goes to `copy` (LDS).  Returns the scale.
-template <typename T, int HD, bool COPY>
-__device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record, int8_t* copy, int lane) {
+// c + 4).  A block that keeps its scale has only the new rows written.  Returns
+// the scale.
+template <typename T, int HD>
+__device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record, int lane) {
     constexpr int NC = HD / 64;
     const int t = lane >> 2, c = lane & 3, tok = r.tok0 + t;
     const bool fresh = tok >= r.p && tok < r.end;
     float x[NC][16];
-    v4i o[NC];
     float amax = 0.0f;
-    bool bad = false;
     // Every lane loads a row, the nearest new one where its own is not new: no
     // branch that the loads would wait at.
     const T* src = r.rows + (min(max(tok, r.p), r.end - 1) - r.p) * r.stride + c * 16;
@@ -94,8 +102,6 @@ __device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record,
     for (int i = 0; i < NC; ++i) {
         lo[i] = *reinterpret_cast<const Vec8<T>*>(src + i * 64);
         hi[i] = *reinterpret_cast<const Vec8<T>*>(src + i * 64 + 8);
-        o[i] = v4i{0, 0, 0, 0};
-        if (COPY && r.held && !fresh) o[i] = *reinterpret_cast<const v4i*>(record + (c + 4 * i) * (kBlockRows * 16) + t * 16);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -109,10 +115,9 @@ __device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record,
     for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            amax = fmaxf(amax, fabsf(x[i][j]));
-            bad |= !(fabsf(x[i][j]) <= kRowMax);
+            amax = fmaxf(amax, row_magnitude(x[i][j]));
         }
-    const float s = joined_scale(amax, bad, r.held, r.old);
+    const float s = joined_scale(wave_max(amax), r.held, r.old);
     const bool poisoned = s != s;
     const float inv = poisoned ? 0.0f : pow2_inverse(s);
     const float ratio = r.old * inv;
@@ -120,29 +125,23 @@ __device__ __forceinline__ float append_k(const BlockRows<T>& r, int8_t* record,
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         const int at = (c + 4 * i) * (kBlockRows * 16) + t * 16;
-        v4i w = COPY ? o[i] : v4i{0, 0, 0, 0};
+        v4i w = {0, 0, 0, 0};
         if (fresh && !poisoned) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j >> 2] |= static_cast<int32_t>(code_byte(x[i][j] * inv) << (8 * (j & 3)));
         }
         if (requantize && !fresh) {
-            if (!COPY) o[i] = *reinterpret_cast<const v4i*>(record + at);
-            w = v4i{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                w[j >> 2] |= static_cast<int32_t>(code_byte(byte_value(static_cast<uint32_t>(o[i][j >> 2]), j & 3) * ratio)
-                                                  << (8 * (j & 3)));
+            w = rescaled(*reinterpret_cast<const v4i*>(record + at), ratio);
         }
         if (fresh || !r.held || requantize) *reinterpret_cast<v4i*>(record + at) = w;
-        if (COPY) *reinterpret_cast<v4i*>(copy + at) = w;
     }
     return s;
 }
 
 // The same for V: lane = channels NC * lane .., each a run of 16 tokens that the
 // lane alone holds, so new bytes merge into it without a race.
-template <typename T, int HD, bool COPY>
-__device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record, int8_t* copy, int lane) {
+template <typename T, int HD>
+__device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record, int lane) {
     constexpr int NC = HD / 64;
     struct alignas(sizeof(T) * NC) Pack { T v[NC]; };
     const T* src = r.rows + lane * NC;
@@ -154,7 +153,6 @@ __device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record,
     }
     float x[kBlockRows][NC];
     float amax = 0.0f;
-    bool bad = false;
 #pragma unroll
     for (int t = 0; t < kBlockRows; ++t) {
         const int tok = r.tok0 + t;
@@ -166,10 +164,9 @@ __device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record,
     for (int t = 0; t < kBlockRows; ++t)
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            amax = fmaxf(amax, fabsf(x[t][i]));
-            bad |= !(fabsf(x[t][i]) <= kRowMax);
+            amax = fmaxf(amax, row_magnitude(x[t][i]));
         }
-    const float s = joined_scale(amax, bad, r.held, r.old);
+    const float s = joined_scale(wave_max(amax), r.held, r.old);
     const bool poisoned = s != s;
     const float inv = poisoned ? 0.0f : pow2_inverse(s);
     const float ratio = r.old == s || poisoned ? 1.0f : r.old * inv;
@@ -185,7 +182,6 @@ __device__ __forceinline__ float append_v(const BlockRows<T>& r, int8_t* record,
             w[t >> 2] |= static_cast<int32_t>(code_byte(v) << (8 * (t & 3)));
         }
         *reinterpret_cast<v4i*>(record + (lane * NC + i) * kBlockRows) = w;
-        if (COPY) *reinterpret_cast<v4i*>(copy + (lane * NC + i) * kBlockRows) = w;
     }
     return s;
 }
@@ -215,8 +211,7 @@ __global__ __launch_bounds__(128) void block_append_kernel(const BlockRowsArgs a
     r.rows = static_cast<const T*>(wave == 0 ? a.k : a.v) + static_cast<int64_t>(b) * a.n * r.stride + kh * HD;
     r.held = r.tok0 < p;
     r.old = r.held ? *scale : 0.0f;
-    const float s = wave == 0 ? append_k<T, HD, false>(r, record, nullptr, lane)
-                              : append_v<T, HD, false>(r, record, nullptr, lane);
+    const float s = wave == 0 ? append_k<T, HD>(r, record, lane) : append_v<T, HD>(r, record, lane);
     if (lane == 0 && !(r.held && r.old == s)) *scale = s;
 }
 
@@ -288,23 +283,24 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 //           four signed bytes of m as four rows, so a 16-row A holds 4 queries;
 //           B: the K codes as they lie.  The byte sums are exact; one lane has the
 //           four of a (row, token) and joins them into m.k.
-//   output  A: p 2^27 as four 7-bit digits, p = 2^(score - the tile's largest), each
+//   output  A: p 2^30 as its four signed bytes, p = 2^(score - the tile's largest), each
 //           times its block's V scale over the tile's largest (a power of two);
 //           B: the V codes as they lie, 64 tokens of 16 channels at a time.
 //
 // So a code is never converted, the operator is bound by reading the codes
 // (2 * head_dim + 0.5 bytes a token), and what a product rounds is 2^-30 of a
-// row's largest query value and 2^-28 of a tile's largest weight: less than
+// row's largest query value and 2^-31 of a tile's largest weight: less than
 // FP32 products would.
 //
 // Wave w takes tiles w, w + 4, ... of the split, each with its own running
-// (max, sum, output); the waves meet in LDS.  A wave always has a tile's loads
-// in flight: the next tile's K codes are asked for once the scores are done
-// with this one's, its V codes once the output is.
+// (max, sum, output); the waves meet in LDS.  A tile's loads all go out together
+// and four workgroups fill a CU (128 registers), so that others' loads fly while
+// one computes: 64 sequences x 32 heads of 4096 tokens 308 us, 7.0 TB/s.  Asking
+// for the next tile's codes ahead took 154 registers and 328 us.
 //
 // ONCE (one row chunk, so each page is read once): the codes are read past the
 // caches (nontemporal; 64 sequences of 4096 tokens, 8 key/value heads, 82 us
-// against 100.6), and the call's new rows are appended here: each workgroup
+// against 100.6), and the call's new rows may be appended here: each workgroup
 // appends to the blocks of its own range, at most two (n <= 16), writes them to
 // the cache and keeps them in LDS, from where the wave that scans their tile
 // takes them.
@@ -315,8 +311,7 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves4 = 4;
 constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
-constexpr int kDigitBits = 7;
-constexpr float kDigitOne = 134217728.0f;        // 2^27
+constexpr float kDigitOne = 1073741824.0f;       // 2^30
 
 template <int HD, int RT>
 struct AttendShared {
@@ -330,57 +325,59 @@ struct AttendShared {
 
 // The queries of a chunk as A operands: [row tile][64-channel step][lane][16
 // bytes], lane = (chunk g of the step) * 16 + (row * 4 + byte); scales in q_scale.
+//
+// With b = 0x00808080 the bytes of (m + b) ^ b are the signed digits of m: adding
+// b carries exactly where a byte's digit is negative.
+constexpr uint32_t kDigitBias = 0x00808080u;
+__device__ __forceinline__ uint32_t signed_digits(int32_t m) {
+    return (static_cast<uint32_t>(m) + kDigitBias) ^ kDigitBias;
+}
+
+// Bytes k of four words, as one word.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int k) {
+    const uint32_t low = __builtin_amdgcn_perm(w1, w0, 0x0c0c0400u + 0x0101u * k);
+    const uint32_t high = __builtin_amdgcn_perm(w3, w2, 0x04000c0cu + 0x01010000u * k);
+    return low | high;
+}
+
+// r / group and the query token of a row, without a division.
+__device__ __forceinline__ int row_token(const BlockAttendArgs& a, int r) {
+    return a.group_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_magic));
+}
+
 template <typename T, int HD, int RT>
 __device__ __forceinline__ void stage_queries(const BlockAttendArgs& a, int b, int kh, int row_first, int rows,
                                               uint8_t* lds, float* q_scale) {
     constexpr int kPieces = HD / 8;              // lanes of a row, 8 channels each
-    constexpr int kRows = RT * kRowTile;
-    for (int i = threadIdx.x; i < kRows * kPieces; i += kAttendThreads) {
-        const int row = i / kPieces, piece = i % kPieces;
-        float x[8] = {};
-        if (row < rows) {
-            const int r = row_first + row;
-            const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
-            const T* src = static_cast<const T*>(a.q) + token * a.q_stride +
-                           static_cast<int64_t>(kh * a.group + r % a.group) * HD + piece * 8;
-            const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(src);
+    static_assert(RT * kRowTile * kPieces <= kAttendThreads, "a row's piece for each thread");
+    const int row = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+    if (row >= RT * kRowTile) return;
+    const int r = row_first + min(row, rows - 1), i = row_token(a, r);
+    const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(
+        static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride +
+        (kh * a.group + r - i * a.group) * HD + piece * 8);
+    float x[8];
+    float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(w.v[j]);
-        }
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            amax = fmaxf(amax, fabsf(x[j]));
-            bad |= !(fabsf(x[j]) <= kFloatMax);
-        }
-        int poison = bad ? 1 : 0;
-#pragma unroll
-        for (int d = 1; d < kPieces; d <<= 1) {
-            amax = fmaxf(amax, __shfl_xor(amax, d));
-            poison |= __shfl_xor(poison, d);
-        }
-        int e = 0;
-        (void)frexpf(amax, &e);                  // amax < 2^e
-        e = poison ? 0 : max(e, -90);
-        if (piece == 0) q_scale[row] = poison ? __builtin_nanf("") : ldexpf(a.scale, e - 30);
-        uint64_t limb[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            int32_t m = poison ? 0 : static_cast<int32_t>(__builtin_rintf(ldexpf(x[j], 30 - e)));   // |m| <= 2^30
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int32_t l = static_cast<int8_t>(static_cast<uint8_t>(m));
-                limb[k] |= static_cast<uint64_t>(static_cast<uint8_t>(l)) << (8 * j);
-                m = (m - l) >> 8;
-            }
-        }
-        // 8 channels: half (piece & 1) of chunk piece / 2 = 4 * step + g
-        const int chunk = piece >> 1, step = chunk >> 2, g = chunk & 3;
-        uint8_t* dst = lds + (((row >> 2) * (HD / 64) + step) * 64 + g * 16 + (row & 3) * 4) * 16 + (piece & 1) * 8;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint64_t*>(dst + k * 16) = limb[k];
+    for (int j = 0; j < 8; ++j) {
+        x[j] = row < rows ? static_cast<float>(w.v[j]) : 0.0f;
+        amax = fmaxf(amax, fabsf(x[j]) <= kFloatMax ? fabsf(x[j]) : INFINITY);
     }
+#pragma unroll
+    for (int d = 1; d < kPieces; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+    const bool poison = amax == INFINITY;
+    const int e = poison ? 0 : max(static_cast<int>(__float_as_uint(amax) >> 23) - 126, -90);   // amax < 2^e
+    if (piece == 0) q_scale[row] = poison ? __builtin_nanf("") : ldexpf(a.scale, e - 30);
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)                  // |m| <= 2^30
+        u[j] = signed_digits(poison ? 0 : static_cast<int32_t>(__builtin_rintf(ldexpf(x[j], 30 - e))));
+    // 8 channels: half (piece & 1) of chunk piece / 2 = 4 * step + g
+    const int chunk = piece >> 1, step = chunk >> 2, g = chunk & 3;
+    uint8_t* dst = lds + (((row >> 2) * (HD / 64) + step) * 64 + g * 16 + (row & 3) * 4) * 16 + (piece & 1) * 8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<v2u*>(dst + k * 16) = v2u{bytes_of(u[0], u[1], u[2], u[3], k), bytes_of(u[4], u[5], u[6], u[7], k)};
 }
 
 __device__ __forceinline__ float row16_max_f(float x) {
@@ -446,8 +443,81 @@ struct TileHeads {
     }
 };
 
+// A workgroup appends the call's rows to the (at most two) blocks `first` ..
+// of its range: to the cache and to `tail`, whose copies the scan reads.  Small
+// code, for it runs once a workgroup: its rows are few.
+template <typename T, int HD>
+__device__ __forceinline__ void append_here(const BlockAttendArgs& a, int b, int kh, int p, int first, int touched,
+                                            int64_t page, int8_t* base, int8_t* scale_base, int8_t* tail,
+                                            uint32_t* tail_max, float* tail_scale) {
+    constexpr int NC = HD / 64, kRecord = 2 * kBlockRows * HD, kPieces = kRecord / 16;
+    struct alignas(sizeof(T) * NC) Pack { T v[NC]; };
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int piece = min(tid, kPieces - 1), is_v = piece >= kPieces / 2;       // a thread's 16 bytes of a record
+    int rec[2];
+    v4i o[2];
+    float old[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        rec[t] = a.view.table[page * a.view.blocks + min(first + t, first + touched - 1)];
+        o[t] = *reinterpret_cast<const v4i*>(base + static_cast<int64_t>(rec[t]) * kRecord + piece * 16);
+        old[t] = reinterpret_cast<const float*>(scale_base)[2 * rec[t] + is_v];
+    }
+    if (tid < 4) tail_max[tid] = 0;
+    __syncthreads();
+    // A wave takes the K or the V part of one row after another.
+    auto rows = [&](auto&& f) {
+        for (int i = wave; i < 2 * a.n; i += kAttendWaves4) {
+            const int tok = p + (i >> 1), t = tok / kBlockRows - first;
+            if (t < 0 || t >= touched) continue;
+            const T* src = static_cast<const T*>(i & 1 ? a.v : a.k) +
+                           (static_cast<int64_t>(b) * a.n + (i >> 1)) * (i & 1 ? a.v_stride : a.k_stride) + kh * HD;
+            const Pack w = *reinterpret_cast<const Pack*>(src + lane * NC);
+            f(w, i & 1, t, tok % kBlockRows);
+        }
+    };
+    rows([&](const Pack& w, int v, int t, int) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) amax = fmaxf(amax, row_magnitude(static_cast<float>(w.v[i])));
+        amax = wave_max(amax);
+        if (lane == 0) atomicMax(&tail_max[2 * t + v], __float_as_uint(amax));
+    });
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (t >= touched || tid >= kPieces) continue;
+        const bool held = (first + t) * kBlockRows < p;
+        const float s = joined_scale(__uint_as_float(tail_max[2 * t + is_v]), held, old[t]);
+        if (!held) o[t] = v4i{0, 0, 0, 0};
+        else if (s > old[t]) o[t] = rescaled(o[t], old[t] * pow2_inverse(s));
+        *reinterpret_cast<v4i*>(tail + t * kRecord + piece * 16) = o[t];
+        if (piece % (kPieces / 2) == 0) {
+            tail_scale[2 * t + is_v] = s;
+            reinterpret_cast<float*>(scale_base)[2 * rec[t] + is_v] = s;
+        }
+    }
+    __syncthreads();
+    rows([&](const Pack& w, int v, int t, int slot) {
+        const float s = tail_scale[2 * t + v], inv = s != s ? 0.0f : pow2_inverse(s);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int c = lane * NC + i;
+            const float x = s != s ? 0.0f : static_cast<float>(w.v[i]) * inv;
+            tail[t * kRecord + (v ? kBlockRows * HD + c * kBlockRows + slot : (c >> 4) * (kBlockRows * 16) + slot * 16 + (c & 15))] =
+                static_cast<int8_t>(code_byte(x));
+        }
+    });
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        if (t < touched && tid < kPieces)
+            *reinterpret_cast<v4i*>(base + static_cast<int64_t>(rec[t]) * kRecord + piece * 16) =
+                *reinterpret_cast<const v4i*>(tail + t * kRecord + piece * 16);
+}
+
 template <typename T, int HD, int RT, bool LSE, bool ONCE>
-__global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_kernel(const BlockAttendArgs a) {
+__global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void block_attend_kernel(const BlockAttendArgs a) {
     using S = AttendShared<HD, RT>;
     constexpr int NS = HD / 64;                  // 64-channel steps of a score
     constexpr int ND = HD / 16;                  // 16-channel tiles of an output
@@ -456,6 +526,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     constexpr int kRows = S::kRows;
     __shared__ __align__(16) uint8_t lds[S::kBytes];
     __shared__ __align__(16) int8_t tail[ONCE ? 2 * kRecord : 16];   // the blocks that this call appends to
+    __shared__ uint32_t tail_max[4];
     __shared__ float tail_scale[4];
     __shared__ float q_scale[kRows];
     __shared__ uint32_t arrived;
@@ -470,7 +541,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     const int row_first = chunk * kRows, rows = min(kRows, all_rows - row_first);
     const int p = a.positions[b];
     // tokens that the chunk's last row sees
-    const int most = p < 0 ? 0 : p + (row_first + rows - 1) / a.group + 1;
+    const int most = p < 0 ? 0 : p + row_token(a, row_first + rows - 1) + 1;
     const int tiles = (most + kTileTokens - 1) / kTileTokens;
     const int my_splits = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
     if (split >= my_splits) return;
@@ -505,48 +576,21 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     const int last_tile = max(tile_begin, tile_end - 1);
     int tile0 = tile_begin + wave;               // first of the 64 tiles whose heads the wave holds
     TileHeads heads;
-    uint32_t low = 0, high = 0;                  // the next tile's table entry
     auto start = [&]() {
         heads.load_entries(table, tile0 + lane * kAttendWaves4, last_tile);
-        low = heads.low(0);
-        high = heads.high(0);
         heads.load_scales(scale_base);
-        __builtin_amdgcn_sched_barrier(0);       // in this order, as the scan waits for them
-        load_k(low, high, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_v(low, high, 0);
-        __builtin_amdgcn_sched_barrier(0);
     };
     start();
 
     stage_queries<T, HD, RT>(a, b, kh, row_first, rows, lds, q_scale);
-
-    // Blocks of this range that new rows go to: wave pairs take one each, K and V.
-    int touch_begin = 0, touch_end = 0;
+    // Blocks of this range that new rows go to.
+    int touch_begin = tile_end * kTileBlocks, touched = 0;
     if (ONCE && a.k != nullptr && p >= 0) {
         touch_begin = max(p / kBlockRows, tile_begin * kTileBlocks);
-        touch_end = min((p + a.n - 1) / kBlockRows + 1, tile_end * kTileBlocks);
-        const int blk = touch_begin + (wave >> 1), is_v = wave & 1;
-        if (blk < touch_end) {
-            const int mine = static_cast<int>((table[blk / kTileBlocks] >> (16 * (blk % kTileBlocks))) & 0xffffu);
-            int8_t* const record = base + static_cast<int64_t>(mine) * kRecord + is_v * (kBlockRows * HD);
-            int8_t* const copy = tail + (wave >> 1) * kRecord + is_v * (kBlockRows * HD);
-            float* const scale = reinterpret_cast<float*>(scale_base) + 2 * mine + is_v;
-            BlockRows<T> r;
-            r.tok0 = blk * kBlockRows;
-            r.p = p;
-            r.end = p + a.n;
-            r.stride = is_v ? a.v_stride : a.k_stride;
-            r.rows = static_cast<const T*>(is_v ? a.v : a.k) + static_cast<int64_t>(b) * a.n * r.stride + kh * HD;
-            r.held = r.tok0 < p;
-            r.old = r.held ? *scale : 0.0f;
-            const float s = is_v ? append_v<T, HD, true>(r, record, copy, lane) : append_k<T, HD, true>(r, record, copy, lane);
-            if (lane == 0) {
-                tail_scale[wave] = s;
-                if (!(r.held && r.old == s)) *scale = s;
-            }
-        }
+        touched = min((p + a.n - 1) / kBlockRows + 1, tile_end * kTileBlocks) - touch_begin;
     }
+
+    if (touched > 0) append_here<T, HD>(a, b, kh, p, touch_begin, touched, page, base, scale_base, tail, tail_max, tail_scale);
     __syncthreads();
 
     v4i qa[RT][NS];
@@ -559,25 +603,38 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
         for (int s = 0; s < NS; ++s) qa[rt][s] = *reinterpret_cast<const v4i*>(lds + ((rt * NS + s) * 64 + lane) * 16);
         const int row = rt * kRowTile + g;
         qs[rt] = q_scale[row];
-        limit[rt] = row < rows && p >= 0 ? p + (row_first + row) / a.group + 1 : 0;
+        limit[rt] = row < rows && p >= 0 ? p + row_token(a, row_first + row) + 1 : 0;
         m_run[rt] = -INFINITY;
         l_run[rt] = 0.0f;
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[rt][i] = 0.0f;
     }
+    // Which bytes a lane k of a quad takes: of its own word and its neighbours' (k ^ 1,
+    // then k ^ 2 and k ^ 3), byte k of token i to place i.
+    const int k4 = n16 & 3;
+    auto at_place = [](int byte, int place) { return static_cast<uint32_t>(byte) << (8 * place); };
+    const uint32_t turn_a = (0x0c0c0c0cu & ~(at_place(0xff, k4) | at_place(0xff, k4 ^ 1))) | at_place(k4, k4) |
+                            at_place(4 + k4, k4 ^ 1);
+    const uint32_t turn_b = (0x0c0c0c0cu & ~(at_place(0xff, k4 ^ 2) | at_place(0xff, k4 ^ 3))) | at_place(k4, k4 ^ 2) |
+                            at_place(4 + k4, k4 ^ 3);
     uint8_t* const digits = lds + S::kQueryBytes + wave * (RT * 16 * kDigitStride);
     const int64_t head_row = (static_cast<int64_t>(b) * a.view.kv_heads + kh) * all_rows + row_first;
 
     // One tile.  FROM_LDS: it has blocks that this call appends to, which come
-    // from LDS over what was loaded; such a tile is its wave's last.
+    // from LDS over what was loaded; such a tile is its wave's last.  (A second
+    // body, not a branch in one: the loop would wait for all loads at its join.)
     auto scan = [&](auto from_lds, int tile, int at, bool more) {
         TileHead head;
+        const uint32_t low = heads.low(at), high = heads.high(at);
+        load_k(low, high, 0);
+        load_v(low, high, 0);
+        __builtin_amdgcn_sched_barrier(0);
         heads.scales_of(at, head);
         if constexpr (decltype(from_lds)::value) {
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
                 const int t = tile * kTileBlocks + j - touch_begin;
-                if (t < 0 || t >= touch_end - touch_begin) continue;
+                if (t < 0 || t >= touched) continue;
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
                     kb[j][s] = *reinterpret_cast<const v4i*>(tail + t * kRecord + s * 1024 + lane * 16);
@@ -590,11 +647,6 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 head.vs[j] = tail_scale[2 * t + 1];
             }
         }
-        // A wave's last tile asks past the page's end, which fetches nothing: a
-        // branch around the loads would make every turn wait for both kinds.
-        const int past = more ? 0 : static_cast<int>(a.view.page_bytes);
-        low = heads.low(min(at + 1, 63));
-        high = heads.high(min(at + 1, 63));
         const int tok0 = tile * kTileTokens;
 
         float s[RT][kTileBlocks];
@@ -610,7 +662,6 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 s[rt][j] = __builtin_fmaf(upper, 65536.0f, lower) * (qs[rt] * head.ks[j]);
                 if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[rt][j] = -INFINITY;
             }
-        load_k(low, high, past);
 
         // V scales over the tile's largest; a scale that is not a number poisons
         // the rows that see its block.
@@ -637,10 +688,13 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
                 const float w = fast_exp2(s[rt][j] - top_safe);
                 s[rt][j] = w;
                 sum += w;
-                const uint32_t d = static_cast<uint32_t>(__builtin_rintf(w * (head.vs[j] * v_inv) * kDigitOne));
-                uint8_t* dst = digits + (rt * 16 + g * 4) * kDigitStride + j * kBlockRows + n16;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) dst[k * kDigitStride] = static_cast<uint8_t>((d >> (kDigitBits * k)) & 127u);
+                const uint32_t u = signed_digits(static_cast<int32_t>(__builtin_rintf(w * (head.vs[j] * v_inv) * kDigitOne)));
+                // The four lanes of a quad turn their words (a token's digits) into
+                // digit n16 & 3 of the quad's four tokens.
+                const uint32_t x1 = dpp_u<kDppQuadXor1>(u), x2 = dpp_u<kDppQuadXor2>(u), x3 = dpp_u<kDppQuadXor1>(x2);
+                const uint32_t turned = __builtin_amdgcn_perm(x1, u, turn_a) | __builtin_amdgcn_perm(x3, x2, turn_b);
+                *reinterpret_cast<uint32_t*>(digits + (rt * 16 + g * 4 + (n16 & 3)) * kDigitStride + j * kBlockRows +
+                                             (n16 & ~3)) = turned;
             }
             if (LSE) {
                 // log2 of each block's sum, by the lane n16 == j
@@ -675,11 +729,10 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
             for (int rt = 0; rt < RT; ++rt) {
                 v4i c = {0, 0, 0, 0};
                 c = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[rt], vb[i], c, 0, 0, 0);
-                const float lower = static_cast<float>(c[0] + c[1] * 128);     // below 2^28
-                const float upper = static_cast<float>(c[2] + c[3] * 128);
-                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 16384.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
+                const float lower = static_cast<float>(c[0] + c[1] * 256);     // below 2^29
+                const float upper = static_cast<float>(c[2] + c[3] * 256);
+                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 65536.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
             }
-        load_v(low, high, past);
         if (LSE) {
             // The lane n16 == j < 4 has block j's.  After the loads, which would
             // otherwise wait for these stores.
@@ -694,8 +747,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
             }
         }
     };
-    // Tiles without appended blocks end here.
-    const int plain_end = touch_begin < touch_end ? touch_begin / kTileBlocks : tile_end;
+    const int plain_end = min(tile_end, touch_begin / kTileBlocks);     // tiles without appended blocks end here
     while (tile0 < tile_end) {
         heads.arrive();
         const int end = min(tile_end, tile0 + 64 * kAttendWaves4);
@@ -703,7 +755,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
         for (; tile < min(end, plain_end); tile += kAttendWaves4, ++at)
             scan(std::false_type{}, tile, at, tile + kAttendWaves4 < end);
         if (ONCE && tile < end) scan(std::true_type{}, tile, at, false);
-        tile0 = end == tile_end ? tile_end : tile0 + 64 * kAttendWaves4;
+        tile0 += 64 * kAttendWaves4;
         if (tile0 < tile_end) start();
     }
 
@@ -768,7 +820,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
         for (int k = 0; k < kItems; ++k) {
             const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
             float m = -INFINITY, l = 0.0f, o = 0.0f;
-#pragma unroll 8
+#pragma unroll 4
             for (int j = 0; j < my_splits; ++j) {
                 const float* src = partial + (static_cast<int64_t>(j) * kRows + row) * (HD + 2);
                 const float mj = fetch(src), lj = fetch(src + 1), oj = fetch(src + 2 + d);
@@ -789,9 +841,9 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
     for (int k = 0; k < kItems; ++k) {
         const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
         if (row >= rows) break;
-        const int r = row_first + row;
-        const int64_t token = static_cast<int64_t>(b) * a.n + r / a.group;
-        static_cast<T*>(a.out)[token * a.out_stride + static_cast<int64_t>(kh * a.group + r % a.group) * HD + d] =
+        const int r = row_first + row, i_q = row_token(a, r);
+        const int64_t token = static_cast<int64_t>(b) * a.n + i_q;
+        static_cast<T*>(a.out)[token * a.out_stride + (kh * a.group + r - i_q * a.group) * HD + d] =
             static_cast<T>(l_all[k] == 0.0f ? 0.0f : o_all[k] / l_all[k]);
         if (LSE && d == 0) {
             const float v = (m_all[k] == -INFINITY ? 0.0f : m_all[k]) + __log2f(l_all[k]);
@@ -808,7 +860,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : 2) void block_attend_
         for (int blk = threadIdx.x; blk * kBlockRows < p + a.n; blk += kAttendThreads) {
             float sum = 0.0f;
             for (int r = 0; r < rows; ++r)
-                if (blk * kBlockRows <= p + r / a.group)
+                if (blk * kBlockRows <= p + row_token(a, r))
                     sum += fast_exp2(fetch(a.block_lse + (head_row + r) * a.view.blocks + blk) - lse[r]);
             weights[blk] += sum;
         }

@@ -65,6 +65,7 @@ struct BlockAttendArgs {
     int64_t v_stride;
     float scale;          // log2(e) times the caller's
     int32_t group;        // query heads per key/value head
+    uint32_t group_magic; // ceil(2^32 / group), 0 for 1: r / group is its product with r, shifted (r < 2^26)
     int32_t n;
     int32_t layer;
     int32_t slot0;

@@ -119,8 +119,19 @@ int append_rows(const swiftkv_context* ctx, const void* k, int64_t k_stride, con
 // Tokens per split, in tiles.  Splits fill the chip where the (sequence,
 // key/value head, row chunk) triples alone do not; a workgroup's four waves
 // take a tile each at least.
+//
+// One row chunk may append the call's rows in the attention's own launch, which
+// costs each sequence's last workgroup five trips to memory, or leave them to a
+// launch before it.  us of a step, own launch against one before: batch 1 / 8 /
+// 32 at 4096 tokens and 8 key/value heads 11.9 / 18.3 / 49.4 against 15.0 / 21.8 /
+// 51.8, batch 64 at 128 tokens 9.1 against 12.8; but batch 64 at 4096 tokens 89.4
+// against 85.7, with 32 heads 343 against 316, and those at 1024 tokens 96.6
+// against 92.1.  So: before it where no sequence is split and pairs times tokens
+// reach kAppendBefore.
+constexpr int64_t kAppendBefore = int64_t(1) << 21;
 struct AttendPlan {
     int32_t row_tiles, chunks, splits, split_tiles;
+    bool appends;
 };
 AttendPlan attend_plan(const swiftkv_context* ctx, const BlockView& view, int32_t group, int32_t n,
                        const int32_t* positions, int32_t batch) {
@@ -140,6 +151,7 @@ AttendPlan attend_plan(const swiftkv_context* ctx, const BlockView& view, int32_
     else per = std::max(per, (tiles + most - 1) / most);
     p.split_tiles = static_cast<int32_t>(per);
     p.splits = static_cast<int32_t>((tiles + per - 1) / per);
+    p.appends = p.chunks == 1 && (p.splits > 1 || pairs * longest < kAppendBefore);
     return p;
 }
 
@@ -407,6 +419,7 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.out_stride = out_stride;
     a.scale = (scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(view.head_dim)) : scale) * kLog2E;
     a.group = cache->heads / view.kv_heads;
+    a.group_magic = a.group == 1 ? 0u : static_cast<uint32_t>(((uint64_t(1) << 32) + a.group - 1) / a.group);
     a.n = n;
     a.layer = layer_index;
     a.counters = ctx->block_workspace;
@@ -430,13 +443,8 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         a.row_lse = cache->log_sums;
         a.block_lse = cache->log_sums + rows;
     }
-    // One row chunk: the attention's own launch appends.
-    const bool fused = a.group * n <= kMaxRowTiles * kRowTile;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    if (k && !fused &&
-        (rc = append_rows(ctx, k, k_stride, v, v_stride, dtype, cache, layer_index, seq0, positions, batch, n)))
-        return rc;
     const int64_t size = static_cast<int64_t>(element_bytes(dtype));
     for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
         const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
@@ -444,9 +452,17 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.q = static_cast<const char*>(q) + first * q_stride * size;
         a.out = static_cast<char*>(out) + first * out_stride * size;
-        if (k && fused) {
-            a.k = static_cast<const char*>(k) + first * k_stride * size;
-            a.v = static_cast<const char*>(v) + first * v_stride * size;
+        a.k = a.v = nullptr;
+        if (k) {
+            const char* kb = static_cast<const char*>(k) + first * k_stride * size;
+            const char* vb = static_cast<const char*>(v) + first * v_stride * size;
+            if (plan.appends) {
+                a.k = kb;
+                a.v = vb;
+            } else if ((rc = append_rows(ctx, kb, k_stride, vb, v_stride, dtype, cache, layer_index, seq0 + b0,
+                                         positions + b0, nb, n))) {
+                return rc;
+            }
         }
         a.weights = weights ? weights + static_cast<int64_t>(b0) * view.kv_heads * view.blocks : nullptr;
         a.slot0 = seq0 + b0;
