@@ -17,6 +17,7 @@ without the built library raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 import re
@@ -183,6 +184,12 @@ def _positions(ctx: "Context", position):
         buf = ctx._one_position
         buf[0] = int(position)
         return C.addressof(buf), 1, buf
+    if type(position) is list and position:
+        try:    # as quick for a list: an array of C ints refuses what does not fit one
+            pos = array.array("i", position)
+            return (*pos.buffer_info(), pos)
+        except TypeError:
+            pass
     pos = np.ascontiguousarray(np.atleast_1d(np.asarray(position, dtype=np.int32)))
     return pos.ctypes.data, int(pos.size), pos
 
@@ -544,8 +551,8 @@ class BlockCache:
 
 
 def _ptr(x) -> Optional[int]:
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DeviceBuffer):
         return x.ptr
     if isinstance(x, np.ndarray):

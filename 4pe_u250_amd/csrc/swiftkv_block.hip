@@ -883,109 +883,150 @@ __global__ __launch_bounds__(256) void block_weights_kernel(const BlockAttendArg
 
 // ---------------------------------------------------------------- eviction
 
-// Workgroup (kv head, sequence, layer).  The threshold is found by four passes
-// over the weights' bits in LDS, from the top 8 down (non-negative floats order
-// as their bits); then one pass in order gives each block its new place.  What
-// is read and written is a few KiB a workgroup: latency bounds it.
-__global__ __launch_bounds__(256) void block_evict_kernel(const BlockEvictArgs a) {
-    extern __shared__ __align__(16) uint8_t evict_lds[];
-    __shared__ uint32_t bins[256];
-    __shared__ uint32_t found[2];                // the digit's bin, and how many lie above it
-    __shared__ uint32_t wave_eq[4], wave_keep[4];
+// Workgroup (kv head, sequence, layer); a thread has blocks tid, tid + 256, ...
+// (PER of them) in registers.  The smallest weight that stays is found by three
+// passes over the weights' bits, 11 from the top, 11 and 9 (non-negative floats
+// order as their bits): a histogram in LDS, then the bin where the count from the
+// top reaches what is wanted.  (8-bit passes put the few exponents of real weights
+// into few bins, whose atomics wait for each other: 32 layers x 8 sequences x 8
+// heads of 2032 blocks took 32.8 us.)  Ballots and one prefix over (turn, wave)
+// give each block its place.  A few KiB are read and written a workgroup: latency
+// bounds it.
+constexpr int kEvictThreads = 256;
+constexpr int kEvictBins = 2048;
+
+// counts[0 .. n) -> exclusive prefix, by one wave; n <= 128.
+__device__ __forceinline__ void prefix_counts(uint32_t* counts, int n, int lane) {
+    const uint32_t c0 = 2 * lane < n ? counts[2 * lane] : 0, c1 = 2 * lane + 1 < n ? counts[2 * lane + 1] : 0;
+    uint32_t sum = c0 + c1;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t t = __shfl_up(sum, d);
+        if (lane >= d) sum += t;
+    }
+    sum -= c0 + c1;
+    if (2 * lane < n) counts[2 * lane] = sum;
+    if (2 * lane + 1 < n) counts[2 * lane + 1] = sum + c0;
+}
+
+template <int PER>
+__global__ __launch_bounds__(kEvictThreads) void block_evict_kernel(const BlockEvictArgs a) {
+    __shared__ __align__(16) uint32_t bins[kEvictBins];
+    __shared__ uint32_t found[2];                // the bin, and how many keys lie above it
+    __shared__ uint32_t wave_sum[4];
+    __shared__ uint32_t counts[2][4 * PER];      // of each (turn, wave): equal to the threshold; staying
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int kh = blockIdx.x, b = blockIdx.y, blocks = a.view.blocks;
-    const int nb = (a.positions[b] + kBlockRows - 1) / kBlockRows;
+    const int p = a.positions[b];
+    if (p < 0) return;
+    const int nb = (p + kBlockRows - 1) / kBlockRows;
     const int64_t row = (static_cast<int64_t>(blockIdx.z) * a.batch + a.b0 + b) * a.view.kv_heads + kh;
     float* const weights = a.weights + row * blocks;
     int32_t* const kept = a.kept ? a.kept + row * a.keep : nullptr;
-    if (a.positions[b] < 0) return;
     if (nb <= a.keep) {
-        for (int i = nb + tid; i < blocks; i += 256) weights[i] = 0.0f;
+        for (int i = nb + tid; i < blocks; i += kEvictThreads) weights[i] = 0.0f;
         if (kept)
-            for (int i = tid; i < a.keep; i += 256) kept[i] = i < nb ? i : -1;
+            for (int i = tid; i < a.keep; i += kEvictThreads) kept[i] = i < nb ? i : -1;
         return;
     }
     uint16_t* const table = a.view.table + block_page(a.view, a.slot0 + a.b0 + b, a.layer0 + blockIdx.z, kh) * blocks;
-    float* const w = reinterpret_cast<float*>(evict_lds);
-    uint16_t* const old = reinterpret_cast<uint16_t*>(evict_lds + 4 * static_cast<size_t>(blocks));
-    for (int i = tid; i < nb; i += 256) {
-        w[i] = weights[i];
-        old[i] = table[i];
+    float w[PER];
+    uint16_t old[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = min(k * kEvictThreads + tid, nb - 1);
+        w[k] = weights[i];
+        old[k] = table[i];
     }
     const int lo = a.sinks, hi = nb - a.recent;
-    auto key = [&](int i) { return w[i] > 0.0f ? __float_as_uint(w[i]) : 0u; };
     uint32_t want = a.keep - a.sinks - a.recent;     // of [lo, hi), which holds more
-    uint32_t prefix = 0, threshold = 0xffffffffu;
-    __syncthreads();
+    uint32_t key[PER];                           // plus 1; 0 outside [lo, hi)
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * kEvictThreads + tid;
+        key[k] = i >= lo && i < hi ? (w[k] > 0.0f ? __float_as_uint(w[k]) : 0u) + 1u : 0u;
+    }
+    uint32_t threshold = 0xffffffffu, prefix = 0;
     if (want > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            bins[tid] = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 20 : pass == 1 ? 9 : 0, above_bits = pass == 1 ? 11 : 9;
+            uint4* const mine = reinterpret_cast<uint4*>(bins) + 2 * tid;
+            mine[0] = mine[1] = make_uint4(0, 0, 0, 0);
             __syncthreads();
-            for (int i = lo + tid; i < hi; i += 256) {
-                const uint32_t k = key(i);
-                if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&bins[(k >> shift) & 255u], 1u);
+            uint32_t zeros = 0;                  // blocks nobody attended to: many, counted by the wave
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                const uint32_t v = key[k] - 1;
+                zeros += __popcll(__ballot(v == 0));
+                if (key[k] > 1 && (pass == 0 || v >> (shift + above_bits) == prefix))
+                    atomicAdd(&bins[(v >> shift) & (pass == 2 ? 511u : 2047u)], 1u);
+            }
+            if (lane == 0 && prefix == 0) atomicAdd(&bins[0], zeros);
+            __syncthreads();
+            const uint4 c0 = mine[0], c1 = mine[1];
+            const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            uint32_t sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += c[j];
+            uint32_t above = sum;                // from the top lane down to this one
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t t = __shfl_down(above, d);
+                if (lane + d < 64) above += t;
+            }
+            if (lane == 0) wave_sum[wave] = above;
+            __syncthreads();
+            above -= sum;
+            for (int v = wave + 1; v < 4; ++v) above += wave_sum[v];
+#pragma unroll
+            for (int j = 7; j >= 0; --j) {
+                if (above < want && above + c[j] >= want) {
+                    found[0] = 8 * tid + j;
+                    found[1] = above;
+                }
+                above += c[j];
             }
             __syncthreads();
-            // wave 0: lane l holds bins 4l .. 4l + 3; how many keys lie in higher lanes' bins
-            if (wave == 0) {
-                uint32_t c[4], mine = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mine += c[j] = bins[4 * lane + j];
-                uint32_t above = mine;           // inclusive sum from the top lane down
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const uint32_t t = __shfl_down(above, d);
-                    if (lane + d < 64) above += t;
-                }
-                above -= mine;
-#pragma unroll
-                for (int j = 3; j >= 0; --j) {
-                    if (above < want && above + c[j] >= want) {
-                        found[0] = 4 * lane + j;
-                        found[1] = above;
-                    }
-                    above += c[j];
-                }
-            }
-            __syncthreads();
-            prefix = (prefix << 8) | found[0];
+            prefix = (prefix << (pass == 0 ? 0 : pass == 1 ? 11 : 9)) | found[0];
             want -= found[1];
-            __syncthreads();
         }
-        threshold = prefix;
+        threshold = prefix + 1;
     }
-    // In order: keys above the threshold stay, and the first `want` that equal it.
-    uint32_t eq_before = 0, keep_before = 0;
-    for (int i0 = 0; i0 < nb; i0 += 256) {
-        const int i = i0 + tid;
-        const bool inside = i < nb, middle = inside && i >= lo && i < hi;
-        const uint32_t k = middle ? key(i) : 0u;
-        const bool eq = middle && want > 0 && k == threshold;
-        const uint64_t eqs = __ballot(eq);
-        if (lane == 0) wave_eq[wave] = __popcll(eqs);
-        __syncthreads();
-        uint32_t e = eq_before + __popcll(eqs & ((1ull << lane) - 1));
-        for (int v = 0; v < wave; ++v) e += wave_eq[v];
-        const bool stays = inside && (!middle || k > threshold || (eq && e < want));
-        const uint64_t keeps = __ballot(stays);
-        if (lane == 0) wave_keep[wave] = __popcll(keeps);
-        __syncthreads();
-        uint32_t at = keep_before + __popcll(keeps & ((1ull << lane) - 1));
-        for (int v = 0; v < wave; ++v) at += wave_keep[v];
-        if (inside) {
-            if (stays) {
-                weights[at] = w[i];
-                if (kept) kept[at] = i;
-            }
-            table[stays ? at : a.keep + (i - at)] = old[i];
-        }
-        for (int v = 0; v < 4; ++v) {
-            eq_before += wave_eq[v];
-            keep_before += wave_keep[v];
-        }
-        __syncthreads();
+    // Keys above the threshold stay, and the first `want` that equal it.
+    uint64_t equal[PER], stays[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        equal[k] = __ballot(key[k] == threshold);
+        if (lane == 0) counts[0][4 * k + wave] = __popcll(equal[k]);
     }
-    for (int i = a.keep + tid; i < blocks; i += 256) weights[i] = 0.0f;
+    __syncthreads();
+    if (wave == 0) prefix_counts(counts[0], 4 * PER, lane);
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * kEvictThreads + tid;
+        const bool first = key[k] == threshold && counts[0][4 * k + wave] + __popcll(equal[k] & below) < want;
+        stays[k] = __ballot(i < nb && (key[k] == 0 || (key[k] > threshold) || first));
+        if (lane == 0) counts[1][4 * k + wave] = __popcll(stays[k]);
+    }
+    __syncthreads();
+    if (wave == 0) prefix_counts(counts[1], 4 * PER, lane);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * kEvictThreads + tid;
+        if (i >= nb) continue;
+        const int at = counts[1][4 * k + wave] + __popcll(stays[k] & below);
+        if ((stays[k] >> lane) & 1) {
+            weights[at] = w[k];
+            table[at] = old[k];
+            if (kept) kept[at] = i;
+        } else {
+            table[a.keep + i - at] = old[k];
+        }
+    }
+    for (int i = a.keep + tid; i < blocks; i += kEvictThreads) weights[i] = 0.0f;
 }
 
 }  // namespace
@@ -1057,7 +1098,16 @@ hipError_t launch_block_attend(const BlockAttendArgs& a, int batch, int row_tile
 }
 
 hipError_t launch_block_evict(const BlockEvictArgs& a, int layers, int batch, hipStream_t s) {
-    block_evict_kernel<<<dim3(a.view.kv_heads, batch, layers), 256, 6 * static_cast<size_t>(a.view.blocks), s>>>(a);
+    int most = 0;
+    for (int b = 0; b < batch; ++b) most = a.positions[b] > most ? a.positions[b] : most;
+    const int per = ((most + kBlockRows - 1) / kBlockRows + kEvictThreads - 1) / kEvictThreads;
+    const dim3 grid(a.view.kv_heads, batch, layers);
+    if (per <= 1) block_evict_kernel<1><<<grid, kEvictThreads, 0, s>>>(a);
+    else if (per <= 2) block_evict_kernel<2><<<grid, kEvictThreads, 0, s>>>(a);
+    else if (per <= 4) block_evict_kernel<4><<<grid, kEvictThreads, 0, s>>>(a);
+    else if (per <= 8) block_evict_kernel<8><<<grid, kEvictThreads, 0, s>>>(a);
+    else if (per <= 16) block_evict_kernel<16><<<grid, kEvictThreads, 0, s>>>(a);
+    else block_evict_kernel<32><<<grid, kEvictThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 
