@@ -43,7 +43,7 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=8",
 ]
 SOURCES = ["swiftkv_kernels.hip", "swiftkv_synth.hip", "swiftkv_exact.hip", "swiftkv_exact_short.hip",
-           "swiftkv_block.hip", "swiftkv_rotary.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp"]
+           "swiftkv_block.hip", "swiftkv_block_prompt.hip", "swiftkv_rotary.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp"]
 HOST_SRC = os.path.join(PKG_DIR, "host", "swiftkv_host.cpp")
 HOST_BIN = os.path.join(PKG_DIR, "swiftkv_host")
 

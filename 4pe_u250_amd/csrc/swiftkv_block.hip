@@ -1,30 +1,14 @@
 // swiftkv_block.hip -- kernels of the block cache: append, values, attention,
 // eviction.  Layout and numerics: swiftkv_block.hpp, include/swiftkv.h.
-#include <type_traits>
-
-#include "swiftkv_block.hpp"
-#include "swiftkv_device.hpp"
+#include "swiftkv_block_device.hpp"
 
 namespace swiftkv {
 namespace {
 
 using namespace dev;
 
-constexpr float kFloatMax = 3.402823466e+38f;
 // Larger rows are taken as infinite: a code 64 of scale 2^122 would stand for 2^128.
 constexpr float kRowMax = 0x1.fcp+126f;          // 127 * 2^120
-
-template <typename T>
-struct alignas(16) Vec8 {
-    T v[8];
-};
-
-template <typename F>
-void with_type(ElementType t, F&& f) {
-    if (t == kF32) f(float{});
-    else if (t == kBF16) f(__bf16{});
-    else f(_Float16{});
-}
 
 // ---------------------------------------------------------------- codes
 
@@ -41,9 +25,6 @@ __device__ __forceinline__ float code_scale(float amax) {
     const int e = static_cast<int>(u >> 23) - 133 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
     return __uint_as_float(static_cast<uint32_t>(max(e, -100) + 127) << 23);
 }
-
-// 1 / s of a power of two within 2^-126 .. 2^126, exactly.
-__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 __device__ __forceinline__ uint32_t code_byte(float x) {
     return static_cast<uint32_t>(static_cast<int32_t>(__builtin_rintf(x))) & 0xffu;
@@ -340,11 +321,6 @@ __device__ __forceinline__ uint32_t bytes_of(uint32_t w0, uint32_t w1, uint32_t 
     return low | high;
 }
 
-// r / group and the query token of a row, without a division.
-__device__ __forceinline__ int row_token(const BlockAttendArgs& a, int r) {
-    return a.group_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_magic));
-}
-
 template <typename T, int HD, int RT>
 __device__ __forceinline__ void stage_queries(const BlockAttendArgs& a, int b, int kh, int row_first, int rows,
                                               uint8_t* lds, float* q_scale) {
@@ -392,56 +368,6 @@ __device__ __forceinline__ float row16_sum_f(float x) {
     x += dpp_f<kDppHalfMirror>(x);
     return x + dpp_f<kDppRowRor8>(x);
 }
-
-__device__ __forceinline__ void publish(float* p, float v) {
-    __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float fetch(const float* p) {
-    return __uint_as_float(__hip_atomic_load(const_cast<uint32_t*>(reinterpret_cast<const uint32_t*>(p)),
-                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-
-// A tile's scales, uniform over the wave.
-struct TileHead {
-    float ks[kTileBlocks], vs[kTileBlocks];
-};
-
-// The table entries and scales of 64 of a wave's tiles, a tile in each lane,
-// so that the scan's loads wait for no other: read one tile at a time (scalar
-// loads, which share a counter with LDS accesses) they took two trips to memory
-// a tile, and 64 sequences of 4096 tokens 128 us.
-struct TileHeads {
-    uint64_t entry;
-    uint64_t scale[kTileBlocks];
-
-    __device__ __forceinline__ void load_entries(const uint64_t* table, int tile, int last) {
-        entry = table[min(tile, last)];
-    }
-    __device__ __forceinline__ void load_scales(const int8_t* scales) {
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j)
-            scale[j] = *reinterpret_cast<const uint64_t*>(scales + 8 * ((entry >> (16 * j)) & 0xffffu));
-    }
-    // Waits for the scales here, and not in each turn of the loop that uses them.
-    __device__ __forceinline__ void arrive() const {
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) asm volatile("" ::"v"(scale[j]));
-    }
-    // Records 0 and 1 of a tile, then 2 and 3.
-    __device__ __forceinline__ uint32_t low(int lane) const {
-        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry), lane);
-    }
-    __device__ __forceinline__ uint32_t high(int lane) const {
-        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry >> 32), lane);
-    }
-    __device__ __forceinline__ void scales_of(int lane, TileHead& h) const {
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            h.ks[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j]), lane));
-            h.vs[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j] >> 32), lane));
-        }
-    }
-};
 
 // A workgroup appends the call's rows to the (at most two) blocks `first` ..
 // of its range: to the cache and to `tail`, whose copies the scan reads.  Small

@@ -110,6 +110,8 @@ struct RotaryArgs {
 // Rows (query tokens times grouped heads) that one attention workgroup holds.
 constexpr int kRowTile = 4;          // rows of one matrix instruction, four limbs each
 constexpr int kMaxRowTiles = 4;
+// Rows of a workgroup of the prompt kernel, for calls with more rows than that.
+constexpr int kPromptRows = 64;
 // Words between the arrival counts of two pairs: a 128-byte line each.
 constexpr int kCounterStride = 32;
 
@@ -118,6 +120,8 @@ hipError_t launch_block_append(const BlockRowsArgs& a, int batch, ElementType t,
 hipError_t launch_block_values(const BlockRowsArgs& a, int batch, ElementType t, hipStream_t s);
 // row_tiles: 1, 2 or 4
 hipError_t launch_block_attend(const BlockAttendArgs& a, int batch, int row_tiles, ElementType t, hipStream_t s);
+// a.chunks of kPromptRows rows; a.k, a.weights null
+hipError_t launch_block_prompt(const BlockAttendArgs& a, int batch, ElementType t, hipStream_t s);
 hipError_t launch_block_evict(const BlockEvictArgs& a, int layers, int batch, hipStream_t s);
 hipError_t launch_rotary(const RotaryArgs& a, int batch, ElementType t, bool halves, bool inverse, hipStream_t s);
 

@@ -130,28 +130,32 @@ int append_rows(const swiftkv_context* ctx, const void* k, int64_t k_stride, con
 // reach kAppendBefore.
 constexpr int64_t kAppendBefore = int64_t(1) << 21;
 struct AttendPlan {
-    int32_t row_tiles, chunks, splits, split_tiles;
+    int32_t row_tiles;   // 0: the prompt kernel
+    int32_t chunks, splits, split_tiles;
     bool appends;
 };
 AttendPlan attend_plan(const swiftkv_context* ctx, const BlockView& view, int32_t group, int32_t n,
-                       const int32_t* positions, int32_t batch) {
+                       const int32_t* positions, int32_t batch, bool weights) {
     AttendPlan p{};
     const int64_t rows = static_cast<int64_t>(group) * n;
-    p.row_tiles = rows <= kRowTile ? 1 : rows <= 2 * kRowTile ? 2 : kMaxRowTiles;
-    p.chunks = static_cast<int32_t>((rows + p.row_tiles * kRowTile - 1) / (p.row_tiles * kRowTile));
+    const bool prompt = rows > kMaxRowTiles * kRowTile && !weights;
+    p.row_tiles = prompt ? 0 : rows <= kRowTile ? 1 : rows <= 2 * kRowTile ? 2 : kMaxRowTiles;
+    const int32_t chunk = prompt ? kPromptRows : p.row_tiles * kRowTile;
+    p.chunks = static_cast<int32_t>((rows + chunk - 1) / chunk);
     const int64_t pairs = static_cast<int64_t>(batch) * view.kv_heads * p.chunks;
     int32_t longest = 0;
     for (int32_t b = 0; b < batch; ++b) longest = std::max(longest, positions[b] < 0 ? 0 : positions[b] + n);
     const int64_t tiles = std::max(1, (longest + kTileTokens - 1) / kTileTokens);
-    int64_t splits = std::max<int64_t>(1, 2 * ctx->cus / pairs);
+    int64_t splits = std::max<int64_t>(1, (prompt ? 1 : 2) * ctx->cus / pairs);
     int64_t per = std::max<int64_t>(4, (tiles + splits - 1) / splits);
     if (ctx->split_tokens > 0) per = ctx->split_tokens / kTileTokens;
-    const int64_t most = kMaxSplitGroups / pairs;      // what the workspace holds
+    // what the workspace holds
+    const int64_t most = kMaxSplitGroups * kMaxRowTiles * kRowTile / std::max(chunk, kMaxRowTiles * kRowTile) / pairs;
     if (most <= 1) per = tiles;
     else per = std::max(per, (tiles + most - 1) / most);
     p.split_tiles = static_cast<int32_t>(per);
     p.splits = static_cast<int32_t>((tiles + per - 1) / per);
-    p.appends = p.chunks == 1 && (p.splits > 1 || pairs * longest < kAppendBefore);
+    p.appends = !prompt && p.chunks == 1 && (p.splits > 1 || pairs * longest < kAppendBefore);
     return p;
 }
 
@@ -448,7 +452,7 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     const int64_t size = static_cast<int64_t>(element_bytes(dtype));
     for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
         const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
-        const AttendPlan plan = attend_plan(ctx, view, a.group, n, positions + b0, nb);
+        const AttendPlan plan = attend_plan(ctx, view, a.group, n, positions + b0, nb, weights != nullptr);
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.q = static_cast<const char*>(q) + first * q_stride * size;
         a.out = static_cast<char*>(out) + first * out_stride * size;
@@ -470,7 +474,9 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         a.splits = plan.splits;
         a.split_tiles = plan.split_tiles;
         set_positions(a, positions + b0, nb);
-        SKV_HIP(launch_block_attend(a, nb, plan.row_tiles, static_cast<ElementType>(dtype), ctx->stream));
+        const ElementType type = static_cast<ElementType>(dtype);
+        SKV_HIP(plan.row_tiles == 0 ? launch_block_prompt(a, nb, type, ctx->stream)
+                                    : launch_block_attend(a, nb, plan.row_tiles, type, ctx->stream));
     }
     return ok();
 }

@@ -1,0 +1,87 @@
+// swiftkv_block_device.hpp -- device code that the block cache's kernel files
+// share.
+#pragma once
+
+#include <type_traits>
+
+#include "swiftkv_block.hpp"
+#include "swiftkv_device.hpp"
+
+namespace swiftkv {
+namespace dev {
+
+constexpr float kFloatMax = 3.402823466e+38f;
+
+template <typename T>
+struct alignas(16) Vec8 {
+    T v[8];
+};
+
+template <typename F>
+void with_type(ElementType t, F&& f) {
+    if (t == kF32) f(float{});
+    else if (t == kBF16) f(__bf16{});
+    else f(_Float16{});
+}
+
+// 1 / s of a power of two within 2^-126 .. 2^126, exactly.
+__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+// r / group and the query token of a row, without a division.
+__device__ __forceinline__ int row_token(const BlockAttendArgs& a, int r) {
+    return a.group_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_magic));
+}
+
+// What one workgroup tells another: write-through stores, loads past the caches.
+__device__ __forceinline__ void publish(float* p, float v) {
+    __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float fetch(const float* p) {
+    return __uint_as_float(__hip_atomic_load(const_cast<uint32_t*>(reinterpret_cast<const uint32_t*>(p)),
+                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// A tile's scales, uniform over the wave.
+struct TileHead {
+    float ks[kTileBlocks], vs[kTileBlocks];
+};
+
+// The table entries and scales of 64 of a wave's tiles, a tile in each lane,
+// so that the scan's loads wait for no other: read one tile at a time (scalar
+// loads, which share a counter with LDS accesses) they took two trips to memory
+// a tile, and 64 sequences of 4096 tokens 128 us.
+struct TileHeads {
+    uint64_t entry;
+    uint64_t scale[kTileBlocks];
+
+    __device__ __forceinline__ void load_entries(const uint64_t* table, int tile, int last) {
+        entry = table[min(tile, last)];
+    }
+    __device__ __forceinline__ void load_scales(const int8_t* scales) {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j)
+            scale[j] = *reinterpret_cast<const uint64_t*>(scales + 8 * ((entry >> (16 * j)) & 0xffffu));
+    }
+    // Waits for the scales here, and not in each turn of the loop that uses them.
+    __device__ __forceinline__ void arrive() const {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) asm volatile("" ::"v"(scale[j]));
+    }
+    // Records 0 and 1 of a tile, then 2 and 3.
+    __device__ __forceinline__ uint32_t low(int lane) const {
+        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry), lane);
+    }
+    __device__ __forceinline__ uint32_t high(int lane) const {
+        return __builtin_amdgcn_readlane(static_cast<uint32_t>(entry >> 32), lane);
+    }
+    __device__ __forceinline__ void scales_of(int lane, TileHead& h) const {
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) {
+            h.ks[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j]), lane));
+            h.vs[j] = __uint_as_float(__builtin_amdgcn_readlane(static_cast<uint32_t>(scale[j] >> 32), lane));
+        }
+    }
+};
+
+}  // namespace dev
+}  // namespace swiftkv

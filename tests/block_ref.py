@@ -63,11 +63,11 @@ class Page:
 
 
 def attention(page, q, at, scale):
-    """q [rows of one query head: n][dim] over tokens [0, at + i]: out [n][dim], block weights, and S, the largest
-    sum of |q k| scale log2(e), which the scores' rounding goes by."""
+    """q [rows of one query head: n][dim] over tokens [0, at + i]: out [n][dim], block weights, S, the largest sum of
+    |q k| scale log2(e), which the scores' rounding goes by, and the same with the largest |q| for each."""
     n, dim = q.shape
     k, v = page.values(at + n)
-    out, s_max = np.zeros((n, dim)), 0.0
+    out, s_max, q_max = np.zeros((n, dim)), 0.0, 0.0
     weights = np.zeros(len(page.scales[0]))
     for i in range(n):
         t = at + i + 1
@@ -78,7 +78,8 @@ def attention(page, q, at, scale):
         out[i] = p @ v[:t]
         weights += np.add.reduceat(np.pad(p, (0, len(weights) * BLOCK - t)), np.arange(0, len(weights) * BLOCK, BLOCK))
         s_max = max(s_max, np.nanmax(np.abs(k[:t]) @ np.abs(q[i])) * abs(scale) * np.log2(np.e))
-    return out, weights, s_max
+        q_max = max(q_max, np.abs(q[i]).max() * np.nanmax(np.abs(k[:t]).sum(1)) * abs(scale) * np.log2(np.e))
+    return out, weights, s_max, q_max
 
 
 def relative_bound(s_max, tokens):
@@ -87,6 +88,15 @@ def relative_bound(s_max, tokens):
     times ln 2 in the weight); exp2 and the factors that join tiles, waves and splits are good for 16 * 2^-24; and
     a sum of T weights takes T / 64 + 24 additions along one path."""
     return (np.log(2) * 6 * s_max + tokens / 64 + 40) * 2.0 ** -24
+
+
+def prompt_bound(s_max, q_max, tokens, t):
+    """The same where a call has more than 16 rows and no weights, and (half floats' rounding of a weight).  Products
+    of half floats and codes are exact in FP32; a score is a sum of 128 in an order of the instruction's (127
+    roundings by 2^-24 of S at most) times scales (3); a query's half floats leave 2^-24 of its largest value.  Sums
+    over T tokens round T + 64 times at most.  A weight is one half float, 2^-12 of it, or for FP32 two, 2^-22."""
+    rel = (np.log(2) * (130 * s_max + q_max) + tokens + 64) * 2.0 ** -24
+    return rel, 2.0 ** -22 if t == "f32" else 2.0 ** -12
 
 
 def evict(weights, held, keep, sinks, recent):

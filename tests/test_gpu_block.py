@@ -85,9 +85,11 @@ class Rig:
                 v_max = np.abs(page.values(p + n)[1]).max()
                 each, off = np.zeros(self.cache.blocks), 0.0
                 for g in range(group):
-                    want, w, s = R.attention(page, q[b, :, h * group + g], p, scale)
-                    rel = R.relative_bound(s, p + n)
-                    bound = 2 * rel * v_max + R.HALF_STEP[self.t] * np.abs(want) * (1 + 2 * rel) + 2.0 ** -24 * (self.t == "f16")
+                    want, w, s, s_q = R.attention(page, q[b, :, h * group + g], p, scale)
+                    rel, step = R.relative_bound(s, p + n), 0.0
+                    if group * n > 16 and after is None:
+                        rel, step = R.prompt_bound(s, s_q, p + n, self.t)
+                    bound = (2 * rel + step) * v_max + R.HALF_STEP[self.t] * np.abs(want) * (1 + 2 * rel) + 2.0 ** -24 * (self.t == "f16")
                     err = np.abs(out[b, :, h * group + g] - want)
                     assert (err <= bound).all(), f"sequence {b} head {h * group + g}: {(err / bound).max():.3g} of the bound"
                     each += w
@@ -156,18 +158,18 @@ def test_attention(skv, ctx, t, heads, kv_heads, dim, at, n):
     rig.check_attention(rng, at, n, weights=n <= 8)
 
 
-@pytest.mark.parametrize("split", [256, 512])
-def test_forced_splits(skv, ctx, split):
+@pytest.mark.parametrize("split,n", [(256, 3), (512, 3), (256, 5), (256, 37), (512, 70)])
+def test_forced_splits(skv, ctx, split, n):
     """Splits of a few tiles, some sequences with one split, some with many, one absent."""
     rng = np.random.default_rng(split)
-    at, n = [1023, 200, -1, 777], 3
+    at = [1023, 200, -1, 777]
     rig = Rig(skv, ctx, "f32", 4, 8, 2, 64, 1100)
     for b, p in enumerate(at):
         if p > 0:
             rig.append(rng, [0], p, seq0=b)
     ctx.set_split_tokens(split)
     try:
-        rig.check_attention(rng, at, n, weights=True)
+        rig.check_attention(rng, at, n, weights=n <= 8)
     finally:
         ctx.set_split_tokens(0)
 
@@ -180,6 +182,39 @@ def test_long_context(skv, ctx, n):
     rig.check_attention(rng, [20011], n, weights=n <= 8)
     if n == 1:
         rig.check_attention(rng, [20011], n, append=False, scale=0.5)     # a peaked softmax, nothing appended
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 64), (8, 1, 128), (10, 2, 128)])
+@pytest.mark.parametrize("at,n", [(0, 130), (100, 17), (64, 64), (8300, 20), (5, 300)])
+def test_prompt_chunks(skv, ctx, t, heads, kv_heads, dim, at, n):
+    """Chunks that end inside a row tile, a workgroup's rows and a block; more than 64 tiles; heavy channels."""
+    rng = np.random.default_rng(at + n)
+    rig = Rig(skv, ctx, t, 1, heads, kv_heads, dim, at + n)
+    if at:
+        rig.append(rng, [0], at, spread=20.0)
+    rig.check_attention(rng, [at], n, spread=20.0)
+
+
+def test_not_a_number_in_a_chunk(skv, ctx):
+    """Within a chunk: a poisoned block reaches the queries that see it and no others."""
+    rng = np.random.default_rng(15)
+    rig = Rig(skv, ctx, "f32", 2, 2, 1, 64, 128)
+    (kr, k), (vr, v) = (rig.rows(rng, 2, 100, 1) for _ in "kv")
+    k[0, 70], v[1, 37, 0, 7] = np.nan, np.inf
+    dk, dv = (ctx.to_device(R.typed(x, "f32")[0]) for x in (k, v))
+    qr, q = rig.rows(rng, 2, 100, 2)
+    q[:, 5, 1, 3] = np.nan
+    qr, _ = R.typed(q, "f32")
+    dq, dout = ctx.to_device(qr), ctx.alloc(qr.size)
+    skv.swiftkv_block_attention(ctx, dq, dk, dv, rig.cache, 0, [0, 0], dout, n=100, dtype=skv.F32)
+    ctx.synchronize()
+    out = dout.download(np.float32, (2, 100, 2, 64))
+    for b, first in enumerate((64, 32)):        # the first token of the poisoned block
+        assert np.isnan(out[b, first:]).all()
+        assert np.isnan(out[b, 5, 1]).all()
+        out[b, 5, 1] = 0
+        assert np.isfinite(out[b, :first]).all()
 
 
 def test_layers_and_slots_are_apart(skv, ctx):
