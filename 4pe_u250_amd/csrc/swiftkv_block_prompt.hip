@@ -25,10 +25,8 @@ using namespace dev;
 //           maximum.  P = 2^15 p (scale over the largest seen), rounded to a half
 //           float: 2^-12 of each weight, below the output's own rounding in
 //           bfloat16 and at it in float16; FP32 outputs take two, 22 bits.
-constexpr int kPromptWaves = 8;
-constexpr int kPromptThreads = kPromptWaves * 64;
-constexpr int kPromptHalves = 2;
-constexpr int kHalfThreads = kPromptThreads / kPromptHalves;
+constexpr int kTeamWaves = 4;                     // 16 rows each
+constexpr int kTeamThreads = kTeamWaves * 64;
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -56,21 +54,21 @@ __device__ __forceinline__ float across_groups_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-template <typename T, int HD>
-__global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const BlockAttendArgs a) {
+template <typename T, int HD, int TEAMS>
+__global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(const BlockAttendArgs a) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;    // half floats of a query value, and of a weight
     constexpr int NS = HD / 32, ND = HD / 16, kRecord = 2 * kBlockRows * HD;
     constexpr int kTileBytes = kTileTokens * HD * 2;         // of K, and of V
-    constexpr int NL = kTileBlocks * kRecord / 16 / kHalfThreads;    // a thread's 16-byte pieces of a tile
+    constexpr int NL = kTileBlocks * kRecord / 16 / kTeamThreads;    // a thread's 16-byte pieces of a tile
     constexpr int kPieces = kRecord / 16;
     constexpr int kMergeFloats = kPromptRows * (HD + 2);
-    constexpr int kLdsBytes = kPromptHalves * 2 * kTileBytes > kMergeFloats * 4 ? kPromptHalves * 2 * kTileBytes : kMergeFloats * 4;
+    constexpr int kLdsBytes = TEAMS * 2 * kTileBytes > (TEAMS - 1) * kMergeFloats * 4 ? TEAMS * 2 * kTileBytes : (TEAMS - 1) * kMergeFloats * 4;
     __shared__ __align__(16) uint8_t lds[kLdsBytes];
     __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n16 = lane & 15;
-    const int half = wave / (kPromptWaves / kPromptHalves), part = wave % (kPromptWaves / kPromptHalves);
-    const int tid = threadIdx.x % kHalfThreads;
+    const int team = wave / kTeamWaves, part = wave % kTeamWaves;
+    const int tid = threadIdx.x % kTeamThreads;
     const int b = blockIdx.y;
     int id = blockIdx.x;
     const int kh = id % a.view.kv_heads;         // heads fastest: a head's workgroups share an XCD's L2
@@ -128,13 +126,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
             }
     }
 
-    uint8_t* const k_lds = lds + half * 2 * kTileBytes;      // [block][32-channel step][lane][16 bytes]
+    uint8_t* const k_lds = lds + team * 2 * kTileBytes;      // [block][32-channel step][lane][16 bytes]
     uint8_t* const v_lds = k_lds + kTileBytes;               // [16 channels][32 tokens][lane][16 bytes]
     TileHeads heads;
     v4i piece[NL];
     // Piece i of the thread: unit `unit` of block blk(i).
     const int unit = tid % kPieces;
-    auto blk = [&](int i) { return (i * kHalfThreads + part * 64) / kPieces; };
+    auto blk = [&](int i) { return (i * kTeamThreads + part * 64) / kPieces; };
     auto load_tile = [&](int at) {
         const uint32_t low = heads.low(at), high = heads.high(at);
 #pragma unroll
@@ -170,13 +168,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
     for (int i = 0; i < ND; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -INFINITY, l_run = 0.0f, unit_scale = 0x1p-100f;   // acc counts in unit_scale * 2^-15
     bool poison = false;
-    const int my_first = tile_begin + half;
-    const int turns = (tile_end - tile_begin + kPromptHalves - 1) / kPromptHalves;   // both halves'
+    const int my_first = tile_begin + team;
+    const int turns = (tile_end - tile_begin + TEAMS - 1) / TEAMS;   // every team's
     const int last_tile = max(tile_begin, tile_end - 1);
     for (int turn = 0; turn < turns; ++turn) {
-        const int at = turn & 63, tile = my_first + turn * kPromptHalves;
+        const int at = turn & 63, tile = my_first + turn * TEAMS;
         if (at == 0) {
-            heads.load_entries(table, tile + lane * kPromptHalves, last_tile);
+            heads.load_entries(table, tile + lane * TEAMS, last_tile);
             heads.load_scales(scale_base);
             load_tile(0);
         }
@@ -268,7 +266,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
             }
     }
 
-    // Join the halves in LDS: the second one's (m, l, acc) per row.
+    // Join the teams in LDS: (m, l, acc) per row of all but the first.
     float l = across_groups_sum(l_run);
     if (poison) l = __builtin_nanf("");
     const float to_values = unit_scale * (1.0f / 32768.0f);
@@ -276,8 +274,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
     for (int i = 0; i < ND; ++i) acc[i] *= to_values;
     __syncthreads();
     float* const merge = reinterpret_cast<float*>(lds);
-    float* const mine = merge + row * (HD + 2);
-    if (half == 1) {
+    if (team > 0) {
+        float* const mine = merge + (team - 1) * kMergeFloats + row * (HD + 2);
         if (g == 0) {
             mine[0] = m_run;
             mine[1] = l;
@@ -291,11 +289,20 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
     float* const partial = a.partials + pair * a.splits * kMergeFloats;
     const int64_t token = static_cast<int64_t>(b) * a.n + i_q;
     T* const out = static_cast<T*>(a.out) + token * a.out_stride + (kh * a.group + r - i_q * a.group) * HD;
-    if (half == 0) {
-        const float m2 = mine[0], l2 = mine[1];
-        const float m = fmaxf(m_run, m2), m_safe = m == -INFINITY ? 0.0f : m;
-        const float f1 = fast_exp2(m_run - m_safe), f2 = fast_exp2(m2 - m_safe);
-        l = l * f1 + l2 * f2;
+    if (team == 0) {
+        const float* const others = merge + row * (HD + 2);
+        float m = m_run;
+#pragma unroll
+        for (int t = 0; t < TEAMS - 1; ++t) m = fmaxf(m, others[t * kMergeFloats]);
+        const float m_safe = m == -INFINITY ? 0.0f : m;
+        const float f1 = fast_exp2(m_run - m_safe);
+        float f2[TEAMS - 1];
+        l *= f1;
+#pragma unroll
+        for (int t = 0; t < TEAMS - 1; ++t) {
+            f2[t] = fast_exp2(others[t * kMergeFloats] - m_safe);
+            l += others[t * kMergeFloats + 1] * f2[t];
+        }
         float* const dst = partial + static_cast<int64_t>(split) * kMergeFloats + row * (HD + 2);
         if (my_splits > 1 && g == 0) {
             publish(dst, m);
@@ -306,7 +313,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
             struct alignas(sizeof(T) * 4) Four { T v[4]; } t;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float o = acc[i][k] * f1 + mine[2 + i * 16 + g * 4 + k] * f2;
+                float o = acc[i][k] * f1;
+#pragma unroll
+                for (int u = 0; u < TEAMS - 1; ++u) o += others[u * kMergeFloats + 2 + i * 16 + g * 4 + k] * f2[u];
                 if (my_splits > 1) publish(dst + 2 + i * 16 + g * 4 + k, o);
                 else t.v[k] = static_cast<T>(l == 0.0f ? 0.0f : o / l);
             }
@@ -322,7 +331,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void block_prompt_kernel(const B
     if (static_cast<int>(arrived) != my_splits - 1) return;
     // The last split joins everybody's, in split order; the counter is zero again.
     if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = threadIdx.x; i < rows * HD; i += kPromptThreads) {
+    for (int i = threadIdx.x; i < rows * HD; i += TEAMS * kTeamThreads) {
         const int jr = i / HD, d = i % HD, rr = row_first + jr, ii = row_token(a, rr);
         float m = -INFINITY, ls = 0.0f, o = 0.0f;
 #pragma unroll 4
@@ -346,8 +355,9 @@ hipError_t launch_block_prompt(const BlockAttendArgs& a, int batch, ElementType 
     const dim3 grid(a.view.kv_heads * a.splits * a.chunks, batch);
     with_type(t, [&](auto tag) {
         using T = decltype(tag);
-        if (a.view.head_dim == 64) block_prompt_kernel<T, 64><<<grid, kPromptThreads, 0, s>>>(a);
-        else block_prompt_kernel<T, 128><<<grid, kPromptThreads, 0, s>>>(a);
+        constexpr int TEAMS = sizeof(T) == 4 ? 2 : 4;
+        if (a.view.head_dim == 64) block_prompt_kernel<T, 64, TEAMS><<<grid, TEAMS * kTeamThreads, 0, s>>>(a);
+        else block_prompt_kernel<T, 128, TEAMS><<<grid, TEAMS * kTeamThreads, 0, s>>>(a);
     });
     return hipGetLastError();
 }
