@@ -180,10 +180,10 @@ def _positions(ctx: "Context", position):
     batch-1 step) goes through the context's one-element buffer: building a
     numpy array and its ctypes view cost several microseconds per call, more
     than a short step takes on the GPU."""
-    if isinstance(position, (int, np.integer)) and _INT32_MIN <= position <= _INT32_MAX:
+    if (type(position) is int or isinstance(position, np.integer)) and _INT32_MIN <= position <= _INT32_MAX:
         buf = ctx._one_position
         buf[0] = int(position)
-        return C.addressof(buf), 1, buf
+        return ctx._one_address, 1, buf
     if type(position) is list and position:
         try:    # as quick for a list: an array of C ints refuses what does not fit one
             pos = array.array("i", position)
@@ -253,6 +253,7 @@ class Context:
         self.device = device
         self.host_io = False
         self._one_position = (C.c_int32 * 1)()
+        self._one_address = C.addressof(self._one_position)
 
     def close(self) -> None:
         if self.handle:

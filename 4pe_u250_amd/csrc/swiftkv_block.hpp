@@ -13,6 +13,10 @@ constexpr int kTileTokens = kBlockRows * kTileBlocks;
 constexpr int kBlockMaxSeq = 131072;
 constexpr int kBlockWeightQueries = 8;
 
+// Sequences per launch: positions travel by value in the kernel arguments, and
+// 256 of them made every launch 0.9 us longer on the host (4.1 us against 3.2).
+constexpr int kBlockBatch = 64;
+
 // Element types of the tensors.
 enum ElementType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 inline size_t element_bytes(int t) { return t == kF32 ? 4 : 2; }
@@ -50,7 +54,7 @@ struct BlockRowsArgs {
     int32_t layer;
     int32_t slot0;
     int32_t n;
-    int32_t positions[kMaxBatchPerLaunch];   // negative: the sequence is skipped
+    int32_t positions[kBlockBatch];   // negative: the sequence is skipped
 };
 
 struct BlockAttendArgs {
@@ -77,7 +81,7 @@ struct BlockAttendArgs {
     float* block_lse;     // null, or [sequence][kv head][row][blocks]: log2 of each block's sum of 2^score
     float* row_lse;       // [sequence][kv head][row]: the same of the whole row
     float* weights;       // [sequence][kv head][blocks]
-    int32_t positions[kMaxBatchPerLaunch];
+    int32_t positions[kBlockBatch];
 };
 
 struct BlockEvictArgs {
@@ -91,7 +95,7 @@ struct BlockEvictArgs {
     int32_t keep;
     int32_t sinks;
     int32_t recent;
-    int32_t positions[kMaxBatchPerLaunch];
+    int32_t positions[kBlockBatch];
 };
 
 struct RotaryArgs {
@@ -104,7 +108,7 @@ struct RotaryArgs {
     int32_t head_dim;
     int32_t rotary_dim;
     int32_t n;
-    int32_t positions[kMaxBatchPerLaunch];
+    int32_t positions[kBlockBatch];
 };
 
 // Rows (query tokens times grouped heads) that one attention workgroup holds.

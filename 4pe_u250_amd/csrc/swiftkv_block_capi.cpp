@@ -104,8 +104,8 @@ int append_rows(const swiftkv_context* ctx, const void* k, int64_t k_stride, con
     a.v_stride = v_stride;
     a.layer = layer;
     a.n = n;
-    for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
-        const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
+    for (int32_t b0 = 0; b0 < batch; b0 += kBlockBatch) {
+        const int32_t nb = std::min<int32_t>(kBlockBatch, batch - b0);
         const int64_t row = static_cast<int64_t>(b0) * n;
         a.k = static_cast<const char*>(k) + row * k_stride * static_cast<int64_t>(size);
         a.v = static_cast<const char*>(v) + row * v_stride * static_cast<int64_t>(size);
@@ -257,8 +257,8 @@ int swiftkv_rotary(swiftkv_context* ctx, const swiftkv_rotary_table* table, cons
     a.head_dim = head_dim;
     a.rotary_dim = table->rotary_dim;
     a.n = n;
-    for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
-        const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
+    for (int32_t b0 = 0; b0 < batch; b0 += kBlockBatch) {
+        const int32_t nb = std::min<int32_t>(kBlockBatch, batch - b0);
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.x = static_cast<const char*>(x) + first * x_stride * static_cast<int64_t>(size);
         a.out = static_cast<char*>(out) + first * out_stride * static_cast<int64_t>(size);
@@ -383,8 +383,8 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
     a.view = cache->view;
     a.layer = layer_index;
     a.n = n;
-    for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
-        const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
+    for (int32_t b0 = 0; b0 < batch; b0 += kBlockBatch) {
+        const int32_t nb = std::min<int32_t>(kBlockBatch, batch - b0);
         const int64_t first = static_cast<int64_t>(b0) * n * row * static_cast<int64_t>(element_bytes(dtype));
         a.k_out = static_cast<char*>(k) + first;
         a.v_out = static_cast<char*>(v) + first;
@@ -429,7 +429,7 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.counters = ctx->block_workspace;
     a.partials = reinterpret_cast<float*>(ctx->block_workspace + kMaxSplitGroups * kCounterStride);
     if (weights) {
-        const size_t rows = static_cast<size_t>(std::min(cache->max_batch, kMaxBatchPerLaunch)) * cache->heads * n;
+        const size_t rows = static_cast<size_t>(std::min(cache->max_batch, kBlockBatch)) * cache->heads * n;
         const size_t need = rows * (static_cast<size_t>(view.blocks) + 1);
         if (need > cache->log_sum_floats) {
             if ((rc = not_capturing(ctx, "the first attention with weights (or with more queries)"))) return rc;
@@ -450,8 +450,8 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     const int64_t size = static_cast<int64_t>(element_bytes(dtype));
-    for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
-        const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
+    for (int32_t b0 = 0; b0 < batch; b0 += kBlockBatch) {
+        const int32_t nb = std::min<int32_t>(kBlockBatch, batch - b0);
         const AttendPlan plan = attend_plan(ctx, view, a.group, n, positions + b0, nb, weights != nullptr);
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.q = static_cast<const char*>(q) + first * q_stride * size;
@@ -503,8 +503,8 @@ int swiftkv_block_evict(swiftkv_context* ctx, swiftkv_block_cache* cache, int32_
     a.keep = keep;
     a.sinks = sinks;
     a.recent = recent;
-    for (int32_t b0 = 0; b0 < batch; b0 += kMaxBatchPerLaunch) {
-        const int32_t nb = std::min<int32_t>(kMaxBatchPerLaunch, batch - b0);
+    for (int32_t b0 = 0; b0 < batch; b0 += kBlockBatch) {
+        const int32_t nb = std::min<int32_t>(kBlockBatch, batch - b0);
         a.b0 = b0;
         set_positions(a, positions + b0, nb);
         SKV_HIP(launch_block_evict(a, layers, nb, ctx->stream));
