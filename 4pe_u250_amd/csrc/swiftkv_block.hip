@@ -458,7 +458,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
     __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n16 = lane & 15;
-    const int b = blockIdx.y;
+    const int b = a.order[blockIdx.y];
     int id = blockIdx.x;
     const int kh = id % a.view.kv_heads;         // heads fastest: a head's workgroups share an XCD's L2
     id /= a.view.kv_heads;
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
     const int tiles = (most + kTileTokens - 1) / kTileTokens;
     const int my_splits = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
     if (split >= my_splits) return;
-    const int tile_begin = split * a.split_tiles, tile_end = min(tiles, tile_begin + a.split_tiles);
+    const int per = split_length(tiles, my_splits), tile_begin = split * per, tile_end = min(tiles, tile_begin + per);
 
     const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
     int8_t* const base = a.view.base + page * a.view.page_bytes;
@@ -685,8 +685,23 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         if (tile0 < tile_end) start();
     }
 
+    // With weights: the block that the thread adds first, its weight until now and
+    // its log-sums of each row, asked for before the joins that they wait for.
+    float* const weights = LSE && ONCE ? a.weights + (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.view.blocks : nullptr;
+    const int first_blk = min(static_cast<int>(threadIdx.x), a.view.blocks - 1);
+    float first_weight = 0.0f, first_sums[LSE && ONCE ? kRows : 1];
+    auto ask_sums = [&]() {
+        if constexpr (LSE && ONCE) {
+            first_weight = weights[first_blk];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                first_sums[r] = fetch(a.block_lse + (head_row + min(r, rows - 1)) * a.view.blocks + first_blk);
+        }
+    };
     // The waves' partials meet in LDS.
+    if (LSE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the block sums have arrived
     __syncthreads();
+    if (my_splits == 1) ask_sums();
     float* const merge = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -731,7 +746,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             publish(dst + 2 + d, o);
         }
     }
-    if (my_splits > 1 || LSE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what was published has arrived
+    if (my_splits > 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // what was published has arrived
     __syncthreads();
     if (my_splits > 1) {
         uint32_t* const counter = a.counters + pair * kCounterStride;
@@ -742,23 +757,11 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         // The last split: everybody's partials, in split order.  The counter is
         // zero again for the next launch.
         if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        ask_sums();
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
             const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
-            float m = -INFINITY, l = 0.0f, o = 0.0f;
-#pragma unroll 4
-            for (int j = 0; j < my_splits; ++j) {
-                const float* src = partial + (static_cast<int64_t>(j) * kRows + row) * (HD + 2);
-                const float mj = fetch(src), lj = fetch(src + 1), oj = fetch(src + 2 + d);
-                const float m_new = fmaxf(m, mj), m_safe = m_new == -INFINITY ? 0.0f : m_new;
-                const float f = fast_exp2(m - m_safe), fj = fast_exp2(mj - m_safe);
-                l = l * f + lj * fj;
-                o = o * f + oj * fj;
-                m = m_new;
-            }
-            m_all[k] = m;
-            l_all[k] = l;
-            o_all[k] = o;
+            join_splits(partial + row * (HD + 2), kRows * (HD + 2), my_splits, d, m_all[k], l_all[k], o_all[k]);
         }
     }
     float* const lse = merge;                    // log2 of each row's sum
@@ -782,8 +785,15 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         // log-sum - the row's), rows in order.
         __syncthreads();
         if (p < 0) return;
-        float* const weights = a.weights + (static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.view.blocks;
-        for (int blk = threadIdx.x; blk * kBlockRows < p + a.n; blk += kAttendThreads) {
+        const int held = (p + a.n - 1) / kBlockRows + 1;
+        if (static_cast<int>(threadIdx.x) < held) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (r < rows && first_blk * kBlockRows <= p + row_token(a, r)) sum += fast_exp2(first_sums[r] - lse[r]);
+            weights[first_blk] = first_weight + sum;
+        }
+        for (int blk = threadIdx.x + kAttendThreads; blk < held; blk += kAttendThreads) {
             float sum = 0.0f;
             for (int r = 0; r < rows; ++r)
                 if (blk * kBlockRows <= p + row_token(a, r))

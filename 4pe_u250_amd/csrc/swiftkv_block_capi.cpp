@@ -116,9 +116,16 @@ int append_rows(const swiftkv_context* ctx, const void* k, int64_t k_stride, con
     return SWIFTKV_OK;
 }
 
-// Tokens per split, in tiles.  Splits fill the chip where the (sequence,
-// key/value head, row chunk) triples alone do not; a workgroup's four waves
-// take a tile each at least.
+// Tokens per split, in tiles.  Splits make a workgroup for each CU where the
+// (sequence, key/value head, row chunk) triples alone do not, and no more than the
+// square root of a sequence's tiles, or 16, since the last of them joins all: us
+// of a step with this rule's tokens against others, 8 key/value heads: batch 1 at
+// 4096 512 (8 splits) 11.1; 256 11.7, 1024 12.4; at 16000 1024 (16) 15.6; 512 17.6,
+// 2048 18.3; at 32000 2048 (16) 21.0; 1024 22.0, 4096 27.8; batch 4 at 4096 512 (8)
+// 12.7; 256 15.6, 1024 14.0; batch 8 1024 (4) 16.8; 512 18.0, 2048 20.1; batch 16
+// 2048 (2) 27.0; 1024 27.5; batch 4 at 32000 4096 (8) 44.9; 2048 48.6, 8192 52.1.
+// Sequences of different lengths take a quarter more workgroups: 16 of 2000 to
+// 32511 tokens 105.8 with 8192 tokens, 116.9 with the 9700 of one for each CU.
 //
 // One row chunk may append the call's rows in the attention's own launch, which
 // costs each sequence's last workgroup five trips to memory, or leave them to a
@@ -144,15 +151,23 @@ AttendPlan attend_plan(const swiftkv_context* ctx, const BlockView& view, int32_
     p.chunks = static_cast<int32_t>((rows + chunk - 1) / chunk);
     const int64_t pairs = static_cast<int64_t>(batch) * view.kv_heads * p.chunks;
     int32_t longest = 0;
-    for (int32_t b = 0; b < batch; ++b) longest = std::max(longest, positions[b] < 0 ? 0 : positions[b] + n);
+    int64_t total = 0;
+    for (int32_t b = 0; b < batch; ++b) {
+        const int32_t len = positions[b] < 0 ? 0 : positions[b] + n;
+        longest = std::max(longest, len);
+        total += (len + kTileTokens - 1) / kTileTokens;
+    }
     const int64_t tiles = std::max(1, (longest + kTileTokens - 1) / kTileTokens);
-    int64_t splits = std::max<int64_t>(1, (prompt ? 1 : 2) * ctx->cus / pairs);
-    int64_t per = std::max<int64_t>(4, (tiles + splits - 1) / splits);
+    total *= view.kv_heads * p.chunks;
+    const int64_t most_splits = std::min<int64_t>(16, std::ceil(std::sqrt(static_cast<double>(tiles))));
+    const int64_t groups = total * 5 < pairs * tiles * 4 ? ctx->cus * 5 / 4 : ctx->cus;
+    int64_t per = std::max<int64_t>((total + groups - 1) / groups, (tiles + most_splits - 1) / most_splits);
     if (ctx->split_tokens > 0) per = ctx->split_tokens / kTileTokens;
     // what the workspace holds
     const int64_t most = kMaxSplitGroups * kMaxRowTiles * kRowTile / std::max(chunk, kMaxRowTiles * kRowTile) / pairs;
     if (most <= 1) per = tiles;
     else per = std::max(per, (tiles + most - 1) / most);
+    per = (per + 3) / 4 * 4;
     p.split_tiles = static_cast<int32_t>(per);
     p.splits = static_cast<int32_t>((tiles + per - 1) / per);
     p.appends = !prompt && p.chunks == 1 && (p.splits > 1 || pairs * longest < kAppendBefore);
@@ -474,6 +489,11 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
         a.splits = plan.splits;
         a.split_tiles = plan.split_tiles;
         set_positions(a, positions + b0, nb);
+        for (int32_t b = 0; b < nb; ++b) a.order[b] = static_cast<uint8_t>(b);
+        if (nb > 1)
+            std::sort(a.order, a.order + nb, [&](uint8_t x, uint8_t y) {
+                return a.positions[x] != a.positions[y] ? a.positions[x] > a.positions[y] : x < y;
+            });
         const ElementType type = static_cast<ElementType>(dtype);
         SKV_HIP(plan.row_tiles == 0 ? launch_block_prompt(a, nb, type, ctx->stream)
                                     : launch_block_attend(a, nb, plan.row_tiles, type, ctx->stream));

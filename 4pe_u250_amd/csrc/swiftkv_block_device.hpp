@@ -32,6 +32,11 @@ __device__ __forceinline__ int row_token(const BlockAttendArgs& a, int r) {
     return a.group_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_magic));
 }
 
+// Tiles of each split but the last of a sequence that has `splits`: even shares,
+// in whole turns of four waves (so that none is longer than the launch's
+// split_tiles, a multiple of four, and none is empty).
+__device__ __forceinline__ int split_length(int tiles, int splits) { return ((tiles + splits - 1) / splits + 3) & ~3; }
+
 // What one workgroup tells another: write-through stores, loads past the caches.
 __device__ __forceinline__ void publish(float* p, float v) {
     __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -39,6 +44,39 @@ __device__ __forceinline__ void publish(float* p, float v) {
 __device__ __forceinline__ float fetch(const float* p) {
     return __uint_as_float(__hip_atomic_load(const_cast<uint32_t*>(reinterpret_cast<const uint32_t*>(p)),
                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// One output channel d of a row from its splits' (m, l, acc), `step` floats apart,
+// in split order.  Eight splits' loads go out together.
+__device__ __forceinline__ void join_splits(const float* src, int step, int splits, int d, float& m, float& l, float& o) {
+    m = -INFINITY;
+    l = o = 0.0f;
+    for (int j0 = 0; j0 < splits; j0 += 8) {
+        float mj[8], lj[8], oj[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float* at = src + static_cast<int64_t>(min(j0 + j, splits - 1)) * step;
+            mj[j] = fetch(at);
+            lj[j] = fetch(at + 1);
+            oj[j] = fetch(at + 2 + d);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j0 + j >= splits) mj[j] = -INFINITY, lj[j] = oj[j] = 0.0f;
+            top = fmaxf(top, mj[j]);
+        }
+        const float safe = top == -INFINITY ? 0.0f : top, f = fast_exp2(m - safe);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float fj = fast_exp2(mj[j] - safe);
+            l = __builtin_fmaf(lj[j], fj, l);
+            o = __builtin_fmaf(oj[j], fj, o);
+        }
+        m = top;
+    }
 }
 
 // A tile's scales, uniform over the wave.

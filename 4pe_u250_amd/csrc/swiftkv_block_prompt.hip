@@ -69,7 +69,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     const int g = lane >> 4, n16 = lane & 15;
     const int team = wave / kTeamWaves, part = wave % kTeamWaves;
     const int tid = threadIdx.x % kTeamThreads;
-    const int b = blockIdx.y;
+    const int b = a.order[blockIdx.y];
     int id = blockIdx.x;
     const int kh = id % a.view.kv_heads;         // heads fastest: a head's workgroups share an XCD's L2
     id /= a.view.kv_heads;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     const int tiles = (most + kTileTokens - 1) / kTileTokens;
     const int my_splits = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
     if (split >= my_splits) return;
-    const int tile_begin = split * a.split_tiles, tile_end = min(tiles, tile_begin + a.split_tiles);
+    const int per = split_length(tiles, my_splits), tile_begin = split * per, tile_end = min(tiles, tile_begin + per);
 
     const int64_t page = block_page(a.view, a.slot0 + b, a.layer, kh);
     int8_t* const base = a.view.base + page * a.view.page_bytes;
@@ -333,17 +333,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int i = threadIdx.x; i < rows * HD; i += TEAMS * kTeamThreads) {
         const int jr = i / HD, d = i % HD, rr = row_first + jr, ii = row_token(a, rr);
-        float m = -INFINITY, ls = 0.0f, o = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < my_splits; ++j) {
-            const float* src = partial + static_cast<int64_t>(j) * kMergeFloats + jr * (HD + 2);
-            const float mj = fetch(src), lj = fetch(src + 1), oj = fetch(src + 2 + d);
-            const float mn = fmaxf(m, mj), ms = mn == -INFINITY ? 0.0f : mn;
-            const float f = fast_exp2(m - ms), fj = fast_exp2(mj - ms);
-            ls = ls * f + lj * fj;
-            o = o * f + oj * fj;
-            m = mn;
-        }
+        float m, ls, o;
+        join_splits(partial + jr * (HD + 2), kMergeFloats, my_splits, d, m, ls, o);
         static_cast<T*>(a.out)[(static_cast<int64_t>(b) * a.n + ii) * a.out_stride +
                                (kh * a.group + rr - ii * a.group) * HD + d] = static_cast<T>(ls == 0.0f ? 0.0f : o / ls);
     }
