@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 //
 // ONCE (one row chunk, so each page is read once): the codes are read past the
 // caches (nontemporal; 64 sequences of 4096 tokens, 8 key/value heads, 82 us
-// against 100.6), and the call's new rows may be appended here: each workgroup
+// against 100.6 in an earlier form), and the call's new rows may be appended here: each workgroup
 // appends to the blocks of its own range, at most two (n <= 16), writes them to
 // the cache and keeps them in LDS, from where the wave that scans their tile
 // takes them.
@@ -480,25 +480,25 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
     const uint64_t* table = reinterpret_cast<const uint64_t*>(a.view.table + page * a.view.blocks);
     int8_t* const scale_base = base + static_cast<int64_t>(a.view.blocks) * kRecord;
 
+    // A tile's codes, by the two halves of its table entry.
     v4i kb[kTileBlocks][NS], vb[ND];
-    auto load_k = [&](uint32_t low, uint32_t high, int past) {
+    auto load_k = [&](uint32_t low, uint32_t high) {
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
             const int at = static_cast<int>(((j & 2 ? high : low) >> (16 * (j & 1))) & 0xffffu) * kRecord;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
-                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16 + past, at + s * 1024, kPolicy);
+                kb[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, at + s * 1024, kPolicy);
         }
     };
-    auto load_v = [&](uint32_t low, uint32_t high, int past) {
+    auto load_v = [&](uint32_t low, uint32_t high) {
         const uint32_t mine = ((g & 2 ? high : low) >> (16 * (g & 1))) & 0xffffu;
-        const int at = static_cast<int>(mine) * kRecord + kBlockRows * HD + n16 * 16 + past;
+        const int at = static_cast<int>(mine) * kRecord + kBlockRows * HD + n16 * 16;
 #pragma unroll
         for (int i = 0; i < ND; ++i) vb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, i * 256, kPolicy);
     };
 
-    // The first tile's loads go out before any math; a wave without a tile asks
-    // for the split's last again and drops it.
+    // (a wave without a tile, and lanes past its last, ask for the split's last)
     const int last_tile = max(tile_begin, tile_end - 1);
     int tile0 = tile_begin + wave;               // first of the 64 tiles whose heads the wave holds
     TileHeads heads;
@@ -549,11 +549,11 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
     // One tile.  FROM_LDS: it has blocks that this call appends to, which come
     // from LDS over what was loaded; such a tile is its wave's last.  (A second
     // body, not a branch in one: the loop would wait for all loads at its join.)
-    auto scan = [&](auto from_lds, int tile, int at, bool more) {
+    auto scan = [&](auto from_lds, int tile, int at) {
         TileHead head;
         const uint32_t low = heads.low(at), high = heads.high(at);
-        load_k(low, high, 0);
-        load_v(low, high, 0);
+        load_k(low, high);
+        load_v(low, high);
         __builtin_amdgcn_sched_barrier(0);
         heads.scales_of(at, head);
         if constexpr (decltype(from_lds)::value) {
@@ -660,8 +660,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
                 acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 65536.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
             }
         if (LSE) {
-            // The lane n16 == j < 4 has block j's.  After the loads, which would
-            // otherwise wait for these stores.
+            // The lane n16 == j < 4 has block j's.
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const int row = rt * kRowTile + g;
@@ -679,8 +678,8 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         const int end = min(tile_end, tile0 + 64 * kAttendWaves4);
         int tile = tile0, at = 0;
         for (; tile < min(end, plain_end); tile += kAttendWaves4, ++at)
-            scan(std::false_type{}, tile, at, tile + kAttendWaves4 < end);
-        if (ONCE && tile < end) scan(std::true_type{}, tile, at, false);
+            scan(std::false_type{}, tile, at);
+        if (ONCE && tile < end) scan(std::true_type{}, tile, at);
         tile0 += 64 * kAttendWaves4;
         if (tile0 < tile_end) start();
     }

@@ -8,11 +8,13 @@ namespace {
 
 using namespace dev;
 
-// Workgroup (key/value head, 64 rows, split): wave = 16 rows, and one of two
-// halves of the split's tiles (every other one).  Matrix products bound it, so
-// they run on 16-bit floats, which hold a code exactly, and not on the digits of
-// swiftkv_block.hip, which would take four times the rows.  Each half's four
-// waves turn a tile's codes into half floats in LDS, once for their 64 rows
+// Workgroup (key/value head, 64 rows, split): TEAMS teams of four waves take
+// every TEAMS-th tile of the split; a wave has 16 rows.  Matrix products and the
+// work around them bound it, so they run on 16-bit floats, which hold a code
+// exactly, and not on the digits of swiftkv_block.hip, which would take four times
+// the rows (512 tokens onto 4096, 32 heads over 8: 84 us against 161; two teams
+// 101, two row tiles a wave 94, two buffers and two teams 88).  Each team turns a
+// tile's codes into half floats in LDS, once for its 64 rows
 // (0x6400 + byte is 1024 + byte, so a byte permute and a packed subtraction), in
 // the order in which the instruction reads them:
 //

@@ -472,8 +472,12 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  *             (n <= SWIFTKV_BLOCK_WEIGHT_QUERIES).  The first call with weights,
  *             and the first with a larger n, allocates; run it once before a
  *             capture.
- * Scores, softmax sums and outputs are held in FP32; results do not depend on
- * which workgroup ends first. */
+ * Scores, softmax sums and outputs are held in FP32.  With at most 16 rows (n
+ * times the query heads that share a key/value head), or with weights, products
+ * are as exact as FP32's; with more rows queries and softmax weights are 16-bit
+ * floats (each weight good to 2^-12), two of them for FP32 tensors (2^-22).
+ * Results do not depend on which workgroup ends first.  swiftkv_set_split_tokens
+ * applies. */
 #define SWIFTKV_BLOCK_WEIGHT_QUERIES 8
 int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                             const void* v, int64_t v_stride, int32_t dtype, swiftkv_block_cache* cache,

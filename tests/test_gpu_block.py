@@ -196,6 +196,16 @@ def test_prompt_chunks(skv, ctx, t, heads, kv_heads, dim, at, n):
     rig.check_attention(rng, [at], n, spread=20.0)
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_scales(skv, ctx, n):
+    """A negative scale, and one that leaves all weights the same."""
+    rng = np.random.default_rng(16)
+    rig = Rig(skv, ctx, "f32", 1, 4, 2, 64, 256)
+    rig.append(rng, [0], 100)
+    rig.check_attention(rng, [100], n, scale=-0.3)
+    rig.check_attention(rng, [100], n, append=False, scale=1e-30)
+
+
 def test_not_a_number_in_a_chunk(skv, ctx):
     """Within a chunk: a poisoned block reaches the queries that see it and no others."""
     rng = np.random.default_rng(15)
