@@ -12,8 +12,8 @@ using namespace dev;
 // every TEAMS-th tile of the split; a wave has 16 rows.  Matrix products and the
 // work around them bound it, so they run on 16-bit floats, which hold a code
 // exactly, and not on the digits of swiftkv_block.hip, which would take four times
-// the rows (512 tokens onto 4096, 32 heads over 8: 84 us against 161; two teams
-// 101, two row tiles a wave 94, two buffers and two teams 88).  Each team turns a
+// the rows (512 tokens onto 4096, 32 heads over 8, in the first form: 84 us against 161;
+// two teams 101, two row tiles a wave 94, two buffers and two teams 88; now 66).  Each team turns a
 // tile's codes into half floats in LDS, once for its 64 rows
 // (0x6400 + byte is 1024 + byte, so a byte permute and a packed subtraction), in
 // the order in which the instruction reads them:
@@ -24,14 +24,16 @@ using namespace dev;
 //   output  O^T[channel][row] = V^T P^T, with P straight from those registers:
 //           which token stands in which place of the product does not matter as
 //           long as V's layout agrees, so nothing moves between lanes but a row's
-//           maximum.  P = 2^15 p (scale over the largest seen), rounded to a half
+//           maximum.  P = 2^11 p (scale over the largest seen), rounded to a half
 //           float: 2^-12 of each weight, below the output's own rounding in
-//           bfloat16 and at it in float16; FP32 outputs take two, 22 bits.
+//           bfloat16 and at it in float16, or 2^-36 of the row's largest where that
+//           is more; FP32 outputs take two, 22 bits of 2^15 p.
 constexpr int kTeamWaves = 4;                     // 16 rows each
 constexpr int kTeamThreads = kTeamWaves * 64;
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ v2h pack_halves(float a, float b) {
     return v2h{static_cast<_Float16>(a), static_cast<_Float16>(b)};
@@ -47,6 +49,24 @@ __device__ __forceinline__ v2u code_halves(uint32_t w) {
                __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, high) + off)};
 }
 
+// N products with operands from LDS, at(i) after the lane's first, each read
+// kAhead products before it is used.  (Left to itself the compiler saves registers
+// and waits for each read: 74 us against 66 for 512 tokens onto 4096.)
+template <int N, typename At, typename Multiply>
+__device__ __forceinline__ void products(const uint8_t* first, At at, Multiply multiply) {
+    constexpr int kAhead = 4;
+    v8h ring[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ring[i] = *reinterpret_cast<const v8h*>(first + at(i));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(i, ring[i % kAhead]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + kAhead < N) ring[i % kAhead] = *reinterpret_cast<const v8h*>(first + at(i + kAhead));
+    }
+}
+
 __device__ __forceinline__ float across_groups_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
@@ -59,6 +79,10 @@ __device__ __forceinline__ float across_groups_sum(float x) {
 template <typename T, int HD, int TEAMS>
 __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(const BlockAttendArgs a) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;    // half floats of a query value, and of a weight
+    // A row's reference value follows its maximum only when that is more than
+    // 2^kSlack above it, so that most tiles neither exchange maxima nor scale what is there.
+    constexpr int kSlackExp = TERMS == 1 ? 4 : 0, kWeightExp = 15 - kSlackExp;
+    constexpr float kSlack = kSlackExp, kFloatMin = 0x1p-126f;
     constexpr int NS = HD / 32, ND = HD / 16, kRecord = 2 * kBlockRows * HD;
     constexpr int kTileBytes = kTileTokens * HD * 2;         // of K, and of V
     constexpr int NL = kTileBlocks * kRecord / 16 / kTeamThreads;    // a thread's 16-byte pieces of a tile
@@ -105,36 +129,42 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
         Vec8<T> w[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) w[s] = *reinterpret_cast<const Vec8<T>*>(src + 32 * s);
-        float amax = 0.0f;
+        uint32_t amax = 0;                       // of the magnitudes' bits: what is no number is above infinity
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = fabsf(static_cast<float>(w[s].v[j]));
-                amax = fmaxf(amax, x <= kFloatMax ? x : INFINITY);
-            }
-        amax = across_groups_max(amax);
-        const bool poison = amax == INFINITY;
-        const int e = poison ? 0 : max(static_cast<int>(__float_as_uint(amax) >> 23) - 126, -90);   // amax < 2^e
-        qs = poison ? __builtin_nanf("") : ldexpf(a.scale, e - 15);
+            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(static_cast<float>(w[s].v[j])) & 0x7fffffffu);
+        amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16)));
+        amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
+        const bool poison = amax >= 0x7f800000u;
+        const int e = poison ? 0 : max(static_cast<int>(amax >> 23) - 126, -90);     // magnitudes < 2^e
+        qs = poison ? __builtin_nanf("") : ldexpf(fabsf(a.scale), e - 15);
+        const float to_half = (a.scale < 0.0f ? -1.0f : 1.0f) * ldexpf(1.0f, 15 - e);
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = poison ? 0.0f : ldexpf(static_cast<float>(w[s].v[j]), 15 - e);
-                const _Float16 h = static_cast<_Float16>(x);
-                q[0][s][j] = h;
-                if (TERMS == 2) q[TERMS - 1][s][j] = static_cast<_Float16>(x - static_cast<float>(h));
+            for (int j = 0; j < 8; j += 2) {
+                const float x = static_cast<float>(w[s].v[j]) * to_half, y = static_cast<float>(w[s].v[j + 1]) * to_half;
+                const v2h h = pack_halves(x, y);
+                q[0][s][j] = h[0];
+                q[0][s][j + 1] = h[1];
+                if (TERMS == 2) {
+                    const v2h rest = pack_halves(x - static_cast<float>(h[0]), y - static_cast<float>(h[1]));
+                    q[TERMS - 1][s][j] = rest[0];
+                    q[TERMS - 1][s][j + 1] = rest[1];
+                }
             }
     }
 
     uint8_t* const k_lds = lds + team * 2 * kTileBytes;      // [block][32-channel step][lane][16 bytes]
     uint8_t* const v_lds = k_lds + kTileBytes;               // [16 channels][32 tokens][lane][16 bytes]
     TileHeads heads;
+    uint32_t scale_pair[kTileBlocks];            // upper halves (all of a power of two) of a tile's K and V scales
     v4i piece[NL];
-    // Piece i of the thread: unit `unit` of block blk(i).
+    // Piece i of the thread: unit `unit` of block blk(i), so that two pieces are the
+    // same unit of a pair of blocks.
     const int unit = tid % kPieces;
-    auto blk = [&](int i) { return (i * kTeamThreads + part * 64) / kPieces; };
+    auto blk = [&](int i) { return NL == kTileBlocks ? i : part / (kPieces / 64) * NL + i; };
     auto load_tile = [&](int at) {
         const uint32_t low = heads.low(at), high = heads.high(at);
 #pragma unroll
@@ -146,21 +176,26 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     };
     auto store_tile = [&]() {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
+        for (int i = 0; i < NL; i += 2) {
             const int j = blk(i);
-            v2u h[4];
+            v2u h[2][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = code_halves(static_cast<uint32_t>(piece[i][k]));
+            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[o][k] = code_halves(static_cast<uint32_t>(piece[i + o][k]));
             if (unit < HD) {     // K: 16 channels (chunk c) of token t
                 const int c = unit >> 4, t = unit & 15;
-                uint8_t* dst = k_lds + ((j * NS + (c >> 1)) * 64 + (c & 1) * 32 + t) * 16;
-                *reinterpret_cast<v4i*>(dst) = v4i{(int)h[0].x, (int)h[0].y, (int)h[1].x, (int)h[1].y};
-                *reinterpret_cast<v4i*>(dst + 256) = v4i{(int)h[2].x, (int)h[2].y, (int)h[3].x, (int)h[3].y};
-            } else {             // V: 16 tokens of channel d; tokens 4 g' .. go to lane group g'
-                const int d = unit - HD;
-                uint8_t* dst = v_lds + (((d >> 4) * 2 + (j >> 1)) * 64 + (d & 15)) * 16 + (j & 1) * 8;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) *reinterpret_cast<v2u*>(dst + k * 256) = h[k];
+                for (int o = 0; o < 2; ++o) {
+                    v4u* dst = reinterpret_cast<v4u*>(k_lds) + ((j + o) * NS + (c >> 1)) * 64 + (c & 1) * 32 + t;
+                    dst[0] = v4u{h[o][0].x, h[o][0].y, h[o][1].x, h[o][1].y};
+                    dst[16] = v4u{h[o][2].x, h[o][2].y, h[o][3].x, h[o][3].y};
+                }
+            } else {             // V: 16 tokens of channel d of both; tokens 4 g' .. go to lane group g'
+                const int d = unit - HD;
+                v4u* dst = reinterpret_cast<v4u*>(v_lds) + ((d >> 4) * 2 + (j >> 1)) * 64 + (d & 15);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dst[k * 16] = v4u{h[0][k].x, h[0][k].y, h[1][k].x, h[1][k].y};
             }
         }
     };
@@ -168,7 +203,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     v4f acc[ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = -INFINITY, l_run = 0.0f, unit_scale = 0x1p-100f;   // acc counts in unit_scale * 2^-15
+    float m_run = -INFINITY, l_run = 0.0f;
+    int unit_exp = 127 - 100;                    // acc counts in 2^(unit_exp - 127 - kWeightExp)
     bool poison = false;
     const int my_first = tile_begin + team;
     const int turns = (tile_end - tile_begin + TEAMS - 1) / TEAMS;   // every team's
@@ -179,68 +215,98 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             heads.load_entries(table, tile + lane * TEAMS, last_tile);
             heads.load_scales(scale_base);
             load_tile(0);
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j)
+                scale_pair[j] = static_cast<uint32_t>(heads.scale[j]) >> 16 |
+                                (static_cast<uint32_t>(heads.scale[j] >> 32) & 0xffff0000u);
         }
         __syncthreads();                         // everyone is done with the tile before
         store_tile();
         __syncthreads();
-        if (turn + 1 < turns && at != 63) load_tile(at + 1);
-        if (tile >= tile_end || !any_row) continue;
+        if (tile >= tile_end || !any_row) {
+            load_tile((at + 1) & 63);
+            continue;
+        }
         TileHead head;
-        heads.scales_of(at, head);
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j) {
+            const uint32_t both = __builtin_amdgcn_readlane(scale_pair[j], at);
+            head.ks[j] = __uint_as_float(both << 16);
+            head.vs[j] = __uint_as_float(both & 0xffff0000u);
+        }
         const int tok0 = tile * kTileTokens;
         v4f s[kTileBlocks];
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            s[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < kTileBlocks; ++j) s[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        products<NS * kTileBlocks>(
+            k_lds + lane * 16, [](int i) { return (i % kTileBlocks * NS + i / kTileBlocks) * 1024; },
+            [&](int i, v8h kk) {
 #pragma unroll
-            for (int k = 0; k < NS; ++k) {
-                const v8h kk = *reinterpret_cast<const v8h*>(k_lds + ((j * NS + k) * 64 + lane) * 16);
+                for (int t = 0; t < TERMS; ++t)
+                    s[i % kTileBlocks] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[t][i / kTileBlocks], s[i % kTileBlocks], 0, 0, 0);
+            });
+        // The next tile's codes: after the scores, which need the registers, and
+        // without a condition, which would keep the last ones (a tile too many is read).
+        load_tile((at + 1) & 63);
+        // Scores are s * f, f > 0.
+        float f[kTileBlocks];
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[t][k], s[j], 0, 0, 0);
-            }
-        }
-        float top = -INFINITY;
-        const bool masked = __any(tok0 + kTileTokens > limit);
+        for (int j = 0; j < kTileBlocks; ++j) f[j] = qs * head.ks[j];
+        if (__any(tok0 + kTileTokens > limit)) {
+            asm volatile("");                    // a branch, not selects in every tile
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            const float f = qs * head.ks[j];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] *= f;
-            if (masked) {
+            for (int j = 0; j < kTileBlocks; ++j) {
+                // a factor that leaves -inf as it is
+                if (tok0 + kBlockRows * j >= limit || f[j] < kFloatMin) f[j] = kFloatMin;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (tok0 + kBlockRows * j + 4 * g + i >= limit) s[j][i] = -INFINITY;
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
         }
-        top = across_groups_max(top);
-        const float m_new = fmaxf(m_run, top), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kTileBlocks; ++j)
+            top = fmaxf(top, f[j] * fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
         // The largest V scale until now; one that is not a number poisons the rows
-        // that see its block.
-        float v_top = unit_scale;
+        // that see its block.  Scales are powers of two: exponents, in scalar registers.
+        int e_top = unit_exp, ev[kTileBlocks];
+        bool bad = false;
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
-            v_top = fmaxf(v_top, head.vs[j]);
-            if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit) poison = true;
+            ev[j] = static_cast<int>(__float_as_uint(head.vs[j]) >> 23 & 255u);
+            if (ev[j] == 255) {
+                bad = true;
+                ev[j] = 0;
+            }
+            e_top = max(e_top, ev[j]);
         }
-        const float v_inv = pow2_inverse(v_top);
-        const float alpha = fast_exp2(m_run - m_safe);
-        const float shrink = alpha * (unit_scale * v_inv);
-        m_run = m_new;
-        unit_scale = v_top;
-        float sum = 0.0f;
+        if (bad) {
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j)
+                if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit) poison = true;
+        }
+        if (e_top != unit_exp || __any(top > m_run + kSlack)) {
+            top = across_groups_max(top);
+            const float m_new = top > m_run + kSlack ? top : m_run;
+            const float alpha = m_new == -INFINITY ? 0.0f : fast_exp2(m_run - m_new);
+            const float shrink = ldexpf(alpha, unit_exp - e_top);
+            m_run = m_new;
+            unit_exp = e_top;
+            l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= shrink;
+        }
+        const float m_safe = m_run == -INFINITY ? 0.0f : m_run;
         v8h w[TERMS][2];
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
-            const float f = head.vs[j] == head.vs[j] ? head.vs[j] * v_inv * 32768.0f : 0.0f;
+            // weights times 2^up; below 2^-25 they are no half floats, so less does not matter
+            const int up = kWeightExp + max(ev[j] - e_top, -60);
+            const float c = static_cast<float>(up) - m_safe;
             float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = fast_exp2(s[j][i] - m_safe);
-                sum += e;
-                x[i] = e * f;
-            }
+            for (int i = 0; i < 4; ++i) x[i] = fast_exp2(__builtin_fmaf(s[j][i], f[j], c));
+            l_run = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), __uint_as_float(static_cast<uint32_t>(127 - up) << 23), l_run);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const v2h h = pack_halves(x[i], x[i + 1]);
@@ -253,25 +319,19 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
                 }
             }
         }
-        l_run = l_run * alpha + sum;
-        if (__any(shrink != 1.0f)) {
+        products<2 * ND>(
+            v_lds + lane * 16, [](int i) { return (i % ND * 2 + i / ND) * 1024; },
+            [&](int i, v8h vv) {
 #pragma unroll
-            for (int i = 0; i < ND; ++i) acc[i] *= shrink;
-        }
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const v8h vv = *reinterpret_cast<const v8h*>(v_lds + ((i * 2 + k) * 64 + lane) * 16);
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, w[t][k], acc[i], 0, 0, 0);
-            }
+                for (int t = 0; t < TERMS; ++t)
+                    acc[i % ND] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, w[t][i / ND], acc[i % ND], 0, 0, 0);
+            });
     }
 
     // Join the teams in LDS: (m, l, acc) per row of all but the first.
     float l = across_groups_sum(l_run);
     if (poison) l = __builtin_nanf("");
-    const float to_values = unit_scale * (1.0f / 32768.0f);
+    const float to_values = ldexpf(1.0f, unit_exp - 127 - kWeightExp);
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] *= to_values;
     __syncthreads();

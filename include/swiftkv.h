@@ -475,7 +475,9 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  * Scores, softmax sums and outputs are held in FP32.  With at most 16 rows (n
  * times the query heads that share a key/value head), or with weights, products
  * are as exact as FP32's; with more rows queries and softmax weights are 16-bit
- * floats (each weight good to 2^-12), two of them for FP32 tensors (2^-22).
+ * floats (each weight good to 2^-12, or to 2^-36 of the row's largest where that
+ * is more, with weights counted times their block's V scale), two of them for
+ * FP32 tensors (2^-22, 2^-40).
  * Results do not depend on which workgroup ends first.  swiftkv_set_split_tokens
  * applies. */
 #define SWIFTKV_BLOCK_WEIGHT_QUERIES 8
