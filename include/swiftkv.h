@@ -488,7 +488,8 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
 
 /* Drop all but `keep` blocks of each (layer, sequence, key/value head) of layers
  * layer0 .. layer0 + layers - 1 and sequences seq0 .. seq0 + batch - 1 that holds
- * more; positions[b] is the number of cached tokens.  The first `sinks` and the
+ * more; positions[b] is the number of cached tokens (a negative one skips the
+ * sequence: its weights and its part of `kept` stay as they are).  The first `sinks` and the
  * last `recent` blocks stay (recent >= 1: the block that is being filled stays
  * last; sinks + recent <= keep); of the others those of the largest weight, ties
  * to the lower index.  A weight that is negative or NaN counts as 0.  The blocks that stay keep their

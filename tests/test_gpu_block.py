@@ -206,6 +206,34 @@ def test_scales(skv, ctx, n):
     rig.check_attention(rng, [100], n, append=False, scale=1e-30)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("steps", [3, 5])
+def test_rising_scores_in_a_chunk(skv, ctx, t, dim, steps):
+    """Scores that rise 2^steps-fold in 256 tokens, below and above what moves a row's reference value, over V blocks
+    whose scales differ by 2^12."""
+    rng = np.random.default_rng(17)
+    tokens, n, heads, kv_heads = 1160, 40, 4, 2
+    rig = Rig(skv, ctx, t, 1, heads, kv_heads, dim, 1216)
+    along = rng.standard_normal(dim)
+    along /= np.linalg.norm(along)
+    rise = steps * np.log(2.0) / 256 * np.arange(tokens + n)
+    k = rise[None, :, None, None] * along + 0.05 * rng.standard_normal((1, tokens + n, kv_heads, dim))
+    v = rng.standard_normal(k.shape) * np.where(np.arange(tokens + n) // 16 % 3 == 0, 1.0, 2.0 ** -12)[None, :, None, None]
+    q = dim ** 0.5 * along + 0.05 * rng.standard_normal((1, n, heads, dim))
+    (_, k), (_, v), (qr, q) = (R.typed(x, t) for x in (k, v, q))
+    for first, count in ((0, tokens), (tokens, n)):
+        part = slice(first, first + count)
+        dk, dv = (ctx.to_device(R.typed(x[:, part], t)[0]) for x in (k, v))
+        skv.swiftkv_block_append(ctx, dk, dv, rig.cache, 0, [first], n=count, dtype=rig.dt)
+        rig.note([first], k[:, part], v[:, part])
+        ctx.synchronize()
+    dq, dout = ctx.to_device(qr), ctx.alloc(qr.size)
+    skv.swiftkv_block_attention(ctx, dq, None, None, rig.cache, 0, [tokens], dout, n=n, dtype=rig.dt)
+    ctx.synchronize()
+    rig.compare(q, [tokens], n, R.values_of(dout.download(np.uint8, (qr.size,)), t, q.shape), None, None)
+
+
 def test_not_a_number_in_a_chunk(skv, ctx):
     """Within a chunk: a poisoned block reaches the queries that see it and no others."""
     rng = np.random.default_rng(15)
