@@ -264,13 +264,15 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 //           four signed bytes of m as four rows, so a 16-row A holds 4 queries;
 //           B: the K codes as they lie.  The byte sums are exact; one lane has the
 //           four of a (row, token) and joins them into m.k.
-//   output  A: p 2^30 as its four signed bytes, p = 2^(score - the tile's largest), each
-//           times its block's V scale over the tile's largest (a power of two);
+//   output  A: p v as a fraction of 2^30, in four signed bytes, p = 2^(score - the tile's
+//           largest), v its block's V scale, over the power of two above the largest p v
+//           that the row has in the tile (a block's scale alone says nothing: the row may
+//           not see the block, or hardly weigh it);
 //           B: the V codes as they lie, 64 tokens of 16 channels at a time.
 //
 // So a code is never converted, the operator is bound by reading the codes
 // (2 * head_dim + 0.5 bytes a token), and what a product rounds is 2^-30 of a
-// row's largest query value and 2^-31 of a tile's largest weight: less than
+// row's largest query value and 2^-30 of its largest p v in a tile: less than
 // FP32 products would.
 //
 // Wave w takes tiles w, w + 4, ... of the split, each with its own running
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves4 = 4;
 constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
-constexpr float kDigitOne = 1073741824.0f;       // 2^30
+constexpr int kScaleBits = 127 - 100;            // exponent bits of the smallest scale
 
 template <int HD, int RT>
 struct AttendShared {
@@ -589,18 +591,12 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
                 if (tok0 + kBlockRows * j + n16 >= limit[rt]) s[rt][j] = -INFINITY;
             }
 
-        // V scales over the tile's largest; a scale that is not a number poisons
-        // the rows that see its block.
-        float v_top = 0x1p-100f;
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) v_top = fmaxf(v_top, head.vs[j]);
-        const float v_inv = pow2_inverse(v_top);
         v4i pa[RT];
         float alpha[RT], v_mul[RT], block_sum[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float top = -INFINITY;
-            bool poison = false;
+            bool poison = false;                 // by a V scale that is not a number, where the row sees its block
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
                 if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit[rt]) poison = true;
@@ -608,13 +604,19 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             }
             top = row16_max_f(top);
             const float top_safe = top == -INFINITY ? 0.0f : top;    // a row that sees nothing here
-            float sum = 0.0f;
+            float sum = 0.0f, largest = 0.0f;    // of the weights times their V scales
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j) {
                 const float w = fast_exp2(s[rt][j] - top_safe);
                 s[rt][j] = w;
                 sum += w;
-                const uint32_t u = signed_digits(static_cast<int32_t>(__builtin_rintf(w * (head.vs[j] * v_inv) * kDigitOne)));
+                largest = fmaxf(largest, w * head.vs[j]);
+            }
+            // largest < 2^(e - 126)
+            const int e = max(static_cast<int>(__float_as_uint(row16_max_f(largest)) >> 23), kScaleBits);
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) {
+                const uint32_t u = signed_digits(static_cast<int32_t>(__builtin_rintf(ldexpf(s[rt][j] * head.vs[j], 156 - e))));
                 // The four lanes of a quad turn their words (a token's digits) into
                 // digit n16 & 3 of the quad's four tokens.
                 const uint32_t x1 = dpp_u<kDppQuadXor1>(u), x2 = dpp_u<kDppQuadXor2>(u), x3 = dpp_u<kDppQuadXor1>(x2);
@@ -638,7 +640,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             const float beta = fast_exp2(top - m_safe);
             m_run[rt] = m_new;
             l_run[rt] = l_run[rt] * alpha[rt] + sum * beta;
-            v_mul[rt] = poison ? __builtin_nanf("") : beta * v_top * (1.0f / kDigitOne);
+            v_mul[rt] = poison ? __builtin_nanf("") : ldexpf(beta, e - 156);
         }
         // The digits were written by other lanes of this wave, whose LDS accesses
         // stay in order; the fences keep the compiler to it.

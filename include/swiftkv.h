@@ -473,8 +473,10 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  *             and the first with a larger n, allocates; run it once before a
  *             capture.
  * Scores, softmax sums and outputs are held in FP32.  With at most 16 rows (n
- * times the query heads that share a key/value head), or with weights, products
- * are as exact as FP32's; with more rows queries and softmax weights are 16-bit
+ * times the query heads that share a key/value head), or with weights, a query
+ * value is good to 2^-30 of its row's largest, and a softmax weight times its
+ * block's V scale to 2^-30 of the largest such product that the row has among the
+ * 64 tokens around it; with more rows queries and softmax weights are 16-bit
  * floats (each weight good to 2^-12, or to 2^-36 of the row's largest where that
  * is more, with weights counted times their block's V scale), two of them for
  * FP32 tensors (2^-22, 2^-40).
