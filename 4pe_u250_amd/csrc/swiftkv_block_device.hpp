@@ -46,6 +46,12 @@ __device__ __forceinline__ float fetch(const float* p) {
                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
+// l 2^d, d <= 0, also where 2^d leaves FP32's range and the product does not: where the
+// reference value follows weights times V scales, sums of weights may be up to 2^100.
+__device__ __forceinline__ float scaled_sum(float l, float d) {
+    return l * fast_exp2(fmaxf(d, -100.0f)) * fast_exp2(fminf(d + 100.0f, 0.0f));
+}
+
 // One output channel d of a row from its splits' (m, l, acc), `step` floats apart,
 // in split order.  Eight splits' loads go out together.
 __device__ __forceinline__ void join_splits(const float* src, int step, int splits, int d, float& m, float& l, float& o) {
@@ -66,14 +72,13 @@ __device__ __forceinline__ void join_splits(const float* src, int step, int spli
             if (j0 + j >= splits) mj[j] = -INFINITY, lj[j] = oj[j] = 0.0f;
             top = fmaxf(top, mj[j]);
         }
-        const float safe = top == -INFINITY ? 0.0f : top, f = fast_exp2(m - safe);
-        l *= f;
-        o *= f;
+        const float safe = top == -INFINITY ? 0.0f : top;
+        l = scaled_sum(l, m - safe);
+        o *= fast_exp2(m - safe);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float fj = fast_exp2(mj[j] - safe);
-            l = __builtin_fmaf(lj[j], fj, l);
-            o = __builtin_fmaf(oj[j], fj, o);
+            l += scaled_sum(lj[j], mj[j] - safe);
+            o = __builtin_fmaf(oj[j], fast_exp2(mj[j] - safe), o);
         }
         m = top;
     }

@@ -24,10 +24,13 @@ using namespace dev;
 //   output  O^T[channel][row] = V^T P^T, with P straight from those registers:
 //           which token stands in which place of the product does not matter as
 //           long as V's layout agrees, so nothing moves between lanes but a row's
-//           maximum.  P = 2^11 p (scale over the largest seen), rounded to a half
-//           float: 2^-12 of each weight, below the output's own rounding in
-//           bfloat16 and at it in float16, or 2^-36 of the row's largest where that
-//           is more; FP32 outputs take two, 22 bits of 2^15 p.
+//           maximum.  A weight counts times its block's V scale, P = 2^11 p v over a
+//           power of two that follows the largest p v which the row has seen (not the
+//           largest p times the largest v: a block that the row does not see, or hardly
+//           weighs, would take bits from the rest), rounded to a half float: 2^-11 of
+//           each, below the output's own rounding in bfloat16 and at it in float16, or
+//           2^-35 of the row's largest where that is more; FP32 outputs take two, 22 bits
+//           of 2^15 p v, or 2^-39.  The sum of weights is that of P / v, in FP32.
 constexpr int kTeamWaves = 4;                     // 16 rows each
 constexpr int kTeamThreads = kTeamWaves * 64;
 
@@ -79,10 +82,15 @@ __device__ __forceinline__ float across_groups_sum(float x) {
 template <typename T, int HD, int TEAMS>
 __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(const BlockAttendArgs a) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;    // half floats of a query value, and of a weight
-    // A row's reference value follows its maximum only when that is more than
-    // 2^kSlack above it, so that most tiles neither exchange maxima nor scale what is there.
+    // A row's reference value, a whole number, follows the largest score + log2 of the
+    // V scale only when that is more than kSlack above it, so that most tiles neither exchange
+    // maxima nor scale what is there.
     constexpr int kSlackExp = TERMS == 1 ? 4 : 0, kWeightExp = 15 - kSlackExp;
     constexpr float kSlack = kSlackExp, kFloatMin = 0x1p-126f;
+    // Sums of weights count in 2^-kSumExp of them, which keeps them and 1 / v in FP32's range.
+    constexpr int kSumExp = 6, kScaleMin = 127 - 100;    // exponent bits of the smallest scale
+    // Between V scales further apart a weight may vanish beside p v that counts in the sum.
+    constexpr int kWide = 96;
     constexpr int NS = HD / 32, ND = HD / 16, kRecord = 2 * kBlockRows * HD;
     constexpr int kTileBytes = kTileTokens * HD * 2;         // of K, and of V
     constexpr int NL = kTileBlocks * kRecord / 16 / kTeamThreads;    // a thread's 16-byte pieces of a tile
@@ -203,8 +211,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     v4f acc[ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = -INFINITY, l_run = 0.0f;
-    int unit_exp = 127 - 100;                    // acc counts in 2^(unit_exp - 127 - kWeightExp)
+    float m_run = -INFINITY, l_run = 0.0f;       // m_run: kWeightExp above the reference value
+    int scale_low = 255, scale_high = 0;         // exponent bits of the V scales until now
     bool poison = false;
     const int my_first = tile_begin + team;
     const int turns = (tile_end - tile_begin + TEAMS - 1) / TEAMS;   // every team's
@@ -263,50 +271,58 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
                     if (tok0 + kBlockRows * j + 4 * g + i >= limit) s[j][i] = -INFINITY;
             }
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j)
-            top = fmaxf(top, f[j] * fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
-        // The largest V scale until now; one that is not a number poisons the rows
-        // that see its block.  Scales are powers of two: exponents, in scalar registers.
-        int e_top = unit_exp, ev[kTileBlocks];
+        // V scales are powers of two: exponents, in scalar registers.  One that is not a
+        // number poisons the rows that see its block.
+        int ev[kTileBlocks];
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
-            ev[j] = static_cast<int>(__float_as_uint(head.vs[j]) >> 23 & 255u);
+            ev[j] = max(static_cast<int>(__float_as_uint(head.vs[j]) >> 23 & 255u), kScaleMin);
             if (ev[j] == 255) {
                 bad = true;
-                ev[j] = 0;
+                ev[j] = kScaleMin;
             }
-            e_top = max(e_top, ev[j]);
+            scale_low = min(scale_low, ev[j]);
+            scale_high = max(scale_high, ev[j]);
         }
         if (bad) {
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j)
                 if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit) poison = true;
         }
-        if (e_top != unit_exp || __any(top > m_run + kSlack)) {
-            top = across_groups_max(top);
-            const float m_new = top > m_run + kSlack ? top : m_run;
-            const float alpha = m_new == -INFINITY ? 0.0f : fast_exp2(m_run - m_new);
-            const float shrink = ldexpf(alpha, unit_exp - e_top);
-            m_run = m_new;
-            unit_exp = e_top;
-            l_run *= alpha;
+        float top = -INFINITY, vk[kTileBlocks];
 #pragma unroll
-            for (int i = 0; i < ND; ++i) acc[i] *= shrink;
+        for (int j = 0; j < kTileBlocks; ++j) {
+            vk[j] = static_cast<float>(ev[j] - 127 + kWeightExp);
+            top = fmaxf(top, __builtin_fmaf(f[j], fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), vk[j]));
         }
-        const float m_safe = m_run == -INFINITY ? 0.0f : m_run;
+        if (__any(top > m_run + kSlack)) {
+            top = across_groups_max(top);
+            const float m_new = top > m_run + kSlack ? ceilf(top) : m_run;
+            const float alpha = m_new == -INFINITY ? 0.0f : fast_exp2(m_run - m_new);
+            l_run = m_new == -INFINITY ? l_run : scaled_sum(l_run, m_run - m_new);
+            m_run = m_new;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= alpha;
+        }
+        const float base_exp = (m_run == -INFINITY ? 0.0f : m_run) - kWeightExp;
+        const bool wide = scale_high - scale_low > kWide;
+        if (wide) {
+            const float c = (kWeightExp - kSumExp) - base_exp;
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l_run += fast_exp2(__builtin_fmaf(s[j][i], f[j], c));
+        }
         v8h w[TERMS][2];
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
-            // weights times 2^up; below 2^-25 they are no half floats, so less does not matter
-            const int up = kWeightExp + max(ev[j] - e_top, -60);
-            const float c = static_cast<float>(up) - m_safe;
+            const float c = vk[j] - base_exp;
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = fast_exp2(__builtin_fmaf(s[j][i], f[j], c));
-            l_run = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), __uint_as_float(static_cast<uint32_t>(127 - up) << 23), l_run);
+            const float per_scale = wide ? 0.0f : __uint_as_float(static_cast<uint32_t>(254 - kSumExp - ev[j]) << 23);
+            l_run = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), per_scale, l_run);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const v2h h = pack_halves(x[i], x[i + 1]);
@@ -331,9 +347,9 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     // Join the teams in LDS: (m, l, acc) per row of all but the first.
     float l = across_groups_sum(l_run);
     if (poison) l = __builtin_nanf("");
-    const float to_values = ldexpf(1.0f, unit_exp - 127 - kWeightExp);
+    constexpr float kToValues = 1.0f / (1 << kSumExp);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) acc[i] *= to_values;
+    for (int i = 0; i < ND; ++i) acc[i] *= kToValues;
     __syncthreads();
     float* const merge = reinterpret_cast<float*>(lds);
     if (team > 0) {
@@ -359,11 +375,11 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
         const float m_safe = m == -INFINITY ? 0.0f : m;
         const float f1 = fast_exp2(m_run - m_safe);
         float f2[TEAMS - 1];
-        l *= f1;
+        l = scaled_sum(l, m_run - m_safe);
 #pragma unroll
         for (int t = 0; t < TEAMS - 1; ++t) {
             f2[t] = fast_exp2(others[t * kMergeFloats] - m_safe);
-            l += others[t * kMergeFloats + 1] * f2[t];
+            l += scaled_sum(others[t * kMergeFloats + 1], others[t * kMergeFloats] - m_safe);
         }
         float* const dst = partial + static_cast<int64_t>(split) * kMergeFloats + row * (HD + 2);
         if (my_splits > 1 && g == 0) {

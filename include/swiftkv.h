@@ -477,9 +477,9 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  * value is good to 2^-30 of its row's largest, and a softmax weight times its
  * block's V scale to 2^-30 of the largest such product that the row has among the
  * 64 tokens around it; with more rows queries and softmax weights are 16-bit
- * floats (each weight good to 2^-12, or to 2^-36 of the row's largest where that
+ * floats (each weight good to 2^-11, or to 2^-35 of the row's largest where that
  * is more, with weights counted times their block's V scale), two of them for
- * FP32 tensors (2^-22, 2^-40).
+ * FP32 tensors (2^-22, 2^-39).
  * Results do not depend on which workgroup ends first.  swiftkv_set_split_tokens
  * applies. */
 #define SWIFTKV_BLOCK_WEIGHT_QUERIES 8

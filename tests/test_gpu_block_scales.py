@@ -8,8 +8,10 @@ from test_gpu_block import Rig
 
 pytestmark = pytest.mark.gpu
 
-# Query tokens and heads on one key/value head, and weights: 4, 8 and 16 rows in one workgroup, more rows with weights.
-FORMS = [(1, 1, False), (1, 3, True), (1, 5, False), (4, 4, False), (5, 3, True), (8, 5, True)]
+# Query tokens and heads on one key/value head, and weights: every form of the kernels (4, 8 and 16 rows in one
+# workgroup, more rows with weights, more rows without).
+FORMS = [(1, 1, False), (1, 3, True), (1, 5, False), (4, 4, False), (5, 3, True), (8, 5, True), (20, 1, False),
+         (37, 2, False)]
 
 
 def put(rig, at, k, v):
@@ -117,7 +119,8 @@ def test_blocks_dropped_by_eviction(skv, ctx, t, n, heads, weights):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
-@pytest.mark.parametrize("n,heads,weights", [(8, 2, False), (16, 1, False), (8, 6, True)])
+@pytest.mark.parametrize("n,heads,weights", [(8, 2, False), (16, 1, False), (8, 6, True), (60, 1, False), (60, 4, False),
+                                             (200, 1, False)])
 @pytest.mark.parametrize("at", [0, 5, 64])
 def test_later_tokens_of_the_same_call(skv, ctx, t, n, heads, weights, at):
     """V rows 2^40 times those of the block before, two blocks out of three: a query takes nothing from those that come
@@ -172,3 +175,18 @@ def test_weight_and_scale_against_each_other(skv, ctx, t, dim, n, heads, weights
         attend(rig, rng, tokens - n, n, heads, weights, q)
     finally:
         ctx.set_split_tokens(0)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,heads", [(1, 2), (40, 2)])
+def test_small_values_in_channels_of_their_own(skv, ctx, t, n, heads):
+    """Blocks whose scales differ by 2^12 with values in channels of their own, so that the small ones show."""
+    rng = np.random.default_rng(18)
+    rig = rig_of(skv, ctx, t, heads, 64, 640)
+    v = rng.standard_normal((600, 64))
+    large = np.arange(600) // 16 % 3 == 0
+    v[large, 32:] = 0
+    v[~large, :32] = 0
+    v[~large] *= 2.0 ** -12
+    put(rig, 0, rng.standard_normal((600, 64)), v)
+    attend(rig, rng, 600 - n, n, heads, False)
