@@ -295,6 +295,10 @@ constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves4 = 4;
 constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
 constexpr int kScaleBits = 127 - 100;            // exponent bits of the smallest scale
+// A sum of weights times values may leave FP32's range where its quotient does not: waves
+// sum in a unit of their own, not below 2^kUnitMin, and join in 2^kJoinExp, of 2^17 tokens.
+constexpr float kUnitMin = -200.0f;
+constexpr int kJoinExp = 18;
 
 template <int HD, int RT>
 struct AttendShared {
@@ -523,7 +527,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
 
     v4i qa[RT][NS];
     float qs[RT], m_run[RT], l_run[RT];
-    float acc[RT][ND];
+    float acc[RT][ND], unit[RT];                 // acc counts in 2^(m_run + unit)
     int limit[RT];                               // tokens that row (rt, g) sees
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -534,6 +538,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         limit[rt] = row < rows && p >= 0 ? p + row_token(a, row_first + row) + 1 : 0;
         m_run[rt] = -INFINITY;
         l_run[rt] = 0.0f;
+        unit[rt] = kUnitMin;
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[rt][i] = 0.0f;
     }
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             }
 
         v4i pa[RT];
-        float alpha[RT], v_mul[RT], block_sum[RT];
+        float acc_mul[RT], v_mul[RT], block_sum[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float top = -INFINITY;
@@ -636,11 +641,14 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             }
             const float m_new = fmaxf(m_run[rt], top);
             const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
-            alpha[rt] = fast_exp2(m_run[rt] - m_safe);
-            const float beta = fast_exp2(top - m_safe);
+            const float fall = m_run[rt] - m_safe, below = top - m_safe;   // 0 or less
+            l_run[rt] = l_run[rt] * fast_exp2(fall) + sum * fast_exp2(below);
             m_run[rt] = m_new;
-            l_run[rt] = l_run[rt] * alpha[rt] + sum * beta;
-            v_mul[rt] = poison ? __builtin_nanf("") : ldexpf(beta, e - 156);
+            const float tile_unit = static_cast<float>(e - 126);
+            const float to = fmaxf(fmaxf(unit[rt] + ceilf(fall), tile_unit + ceilf(below)), kUnitMin);
+            acc_mul[rt] = fast_exp2(fall + (unit[rt] - to));
+            v_mul[rt] = poison ? __builtin_nanf("") : fast_exp2(below + (tile_unit - 30.0f - to));
+            unit[rt] = to;
         }
         // The digits were written by other lanes of this wave, whose LDS accesses
         // stay in order; the fences keep the compiler to it.
@@ -659,7 +667,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
                 c = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[rt], vb[i], c, 0, 0, 0);
                 const float lower = static_cast<float>(c[0] + c[1] * 256);     // below 2^29
                 const float upper = static_cast<float>(c[2] + c[3] * 256);
-                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 65536.0f, lower), v_mul[rt], acc[rt][i] * alpha[rt]);
+                acc[rt][i] = __builtin_fmaf(__builtin_fmaf(upper, 65536.0f, lower), v_mul[rt], acc[rt][i] * acc_mul[rt]);
             }
         if (LSE) {
             // The lane n16 == j < 4 has block j's.
@@ -713,7 +721,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
             dst[1] = l;
         }
 #pragma unroll
-        for (int i = 0; i < ND; ++i) dst[2 + i * 16 + n16] = acc[rt][i];
+        for (int i = 0; i < ND; ++i) dst[2 + i * 16 + n16] = ldexpf(acc[rt][i], static_cast<int>(unit[rt]) - kJoinExp);
     }
     __syncthreads();
     constexpr int kItems = kRows * HD / kAttendThreads;      // outputs of a thread
@@ -762,7 +770,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
             const int i = threadIdx.x + k * kAttendThreads, row = i / HD, d = i % HD;
-            join_splits(partial + row * (HD + 2), kRows * (HD + 2), my_splits, d, m_all[k], l_all[k], o_all[k]);
+            join_splits<false>(partial + row * (HD + 2), kRows * (HD + 2), my_splits, d, m_all[k], l_all[k], o_all[k]);
         }
     }
     float* const lse = merge;                    // log2 of each row's sum
@@ -774,7 +782,7 @@ __global__ __launch_bounds__(kAttendThreads, RT == 4 ? 1 : RT == 2 ? 2 : 4) void
         const int r = row_first + row, i_q = row_token(a, r);
         const int64_t token = static_cast<int64_t>(b) * a.n + i_q;
         static_cast<T*>(a.out)[token * a.out_stride + (kh * a.group + r - i_q * a.group) * HD + d] =
-            static_cast<T>(l_all[k] == 0.0f ? 0.0f : o_all[k] / l_all[k]);
+            static_cast<T>(l_all[k] == 0.0f ? 0.0f : o_all[k] / l_all[k] * (1 << kJoinExp));
         if (LSE && d == 0) {
             const float v = (m_all[k] == -INFINITY ? 0.0f : m_all[k]) + __log2f(l_all[k]);
             if (ONCE) lse[row] = v;

@@ -46,14 +46,14 @@ __device__ __forceinline__ float fetch(const float* p) {
                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// l 2^d, d <= 0, also where 2^d leaves FP32's range and the product does not: where the
-// reference value follows weights times V scales, sums of weights may be up to 2^100.
-__device__ __forceinline__ float scaled_sum(float l, float d) {
-    return l * fast_exp2(fmaxf(d, -100.0f)) * fast_exp2(fminf(d + 100.0f, 0.0f));
-}
+// x 2^d of a whole d <= 0, also where 2^d leaves FP32's range and the product does not:
+// with a reference value that follows weights times V scales, sums of weights go up to 2^100.
+__device__ __forceinline__ float scaled(float x, float d) { return ldexpf(x, static_cast<int>(fmaxf(d, -400.0f))); }
 
 // One output channel d of a row from its splits' (m, l, acc), `step` floats apart,
-// in split order.  Eight splits' loads go out together.
+// in split order.  Eight splits' loads go out together.  WHOLE: the m are whole
+// numbers and go by weights times V scales.
+template <bool WHOLE>
 __device__ __forceinline__ void join_splits(const float* src, int step, int splits, int d, float& m, float& l, float& o) {
     m = -INFINITY;
     l = o = 0.0f;
@@ -73,13 +73,21 @@ __device__ __forceinline__ void join_splits(const float* src, int step, int spli
             top = fmaxf(top, mj[j]);
         }
         const float safe = top == -INFINITY ? 0.0f : top;
-        l = scaled_sum(l, m - safe);
-        o *= fast_exp2(m - safe);
+        auto add = [&](float mi, float li, float oi) {
+            if (WHOLE) {
+                l += scaled(li, mi - safe);
+                o += scaled(oi, mi - safe);
+            } else {
+                const float f = fast_exp2(mi - safe);
+                l = __builtin_fmaf(li, f, l);
+                o = __builtin_fmaf(oi, f, o);
+            }
+        };
+        const float l0 = l, o0 = o;
+        l = o = 0.0f;
+        add(m, l0, o0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            l += scaled_sum(lj[j], mj[j] - safe);
-            o = __builtin_fmaf(oj[j], fast_exp2(mj[j] - safe), o);
-        }
+        for (int j = 0; j < 8; ++j) add(mj[j], lj[j], oj[j]);
         m = top;
     }
 }

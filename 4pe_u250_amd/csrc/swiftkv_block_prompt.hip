@@ -300,7 +300,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             top = across_groups_max(top);
             const float m_new = top > m_run + kSlack ? ceilf(top) : m_run;
             const float alpha = m_new == -INFINITY ? 0.0f : fast_exp2(m_run - m_new);
-            l_run = m_new == -INFINITY ? l_run : scaled_sum(l_run, m_run - m_new);
+            if (m_new > -INFINITY) l_run = scaled(l_run, m_run - m_new);
             m_run = m_new;
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= alpha;
@@ -375,11 +375,11 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
         const float m_safe = m == -INFINITY ? 0.0f : m;
         const float f1 = fast_exp2(m_run - m_safe);
         float f2[TEAMS - 1];
-        l = scaled_sum(l, m_run - m_safe);
+        l = scaled(l, m_run - m_safe);
 #pragma unroll
         for (int t = 0; t < TEAMS - 1; ++t) {
             f2[t] = fast_exp2(others[t * kMergeFloats] - m_safe);
-            l += scaled_sum(others[t * kMergeFloats + 1], others[t * kMergeFloats] - m_safe);
+            l += scaled(others[t * kMergeFloats + 1], others[t * kMergeFloats] - m_safe);
         }
         float* const dst = partial + static_cast<int64_t>(split) * kMergeFloats + row * (HD + 2);
         if (my_splits > 1 && g == 0) {
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     for (int i = threadIdx.x; i < rows * HD; i += TEAMS * kTeamThreads) {
         const int jr = i / HD, d = i % HD, rr = row_first + jr, ii = row_token(a, rr);
         float m, ls, o;
-        join_splits(partial + jr * (HD + 2), kMergeFloats, my_splits, d, m, ls, o);
+        join_splits<true>(partial + jr * (HD + 2), kMergeFloats, my_splits, d, m, ls, o);
         static_cast<T*>(a.out)[(static_cast<int64_t>(b) * a.n + ii) * a.out_stride +
                                (kh * a.group + rr - ii * a.group) * HD + d] = static_cast<T>(ls == 0.0f ? 0.0f : o / ls);
     }

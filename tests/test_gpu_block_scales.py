@@ -177,6 +177,19 @@ def test_weight_and_scale_against_each_other(skv, ctx, t, dim, n, heads, weights
         ctx.set_split_tokens(0)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n,heads,weights", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** 125, 2.0 ** -88, 0.0])
+def test_largest_and_smallest_values(skv, ctx, t, n, heads, weights, size):
+    """Values whose sum leaves FP32's range though their mean does not, tiny ones, and none."""
+    rng = np.random.default_rng(n)
+    rig = rig_of(skv, ctx, t, heads, 64, 1100)
+    v = size * np.where(rng.random((1050, 64)) < 0.5, 1.0, 0.8)
+    put(rig, 0, rng.standard_normal((1050, 64)), v)
+    for end in (1050, 300):
+        attend(rig, rng, end - n, n, heads, weights)
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,heads", [(1, 2), (40, 2)])
 def test_small_values_in_channels_of_their_own(skv, ctx, t, n, heads):
