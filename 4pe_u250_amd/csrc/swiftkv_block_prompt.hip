@@ -70,6 +70,12 @@ __device__ __forceinline__ void products(const uint8_t* first, At at, Multiply m
     }
 }
 
+// a * b rounded, not part of a fused operation.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 __device__ __forceinline__ float across_groups_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
@@ -91,6 +97,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     constexpr int kSumExp = 6, kScaleMin = 127 - 100;    // exponent bits of the smallest scale
     // Between V scales further apart a weight may vanish beside p v that counts in the sum.
     constexpr int kWide = 96;
+    // Beyond this a score has no room for log2 of a V scale beside it.
+    constexpr float kFar = 0x1p22f;
     constexpr int NS = HD / 32, ND = HD / 16, kRecord = 2 * kBlockRows * HD;
     constexpr int kTileBytes = kTileTokens * HD * 2;         // of K, and of V
     constexpr int NL = kTileBlocks * kRecord / 16 / kTeamThreads;    // a thread's 16-byte pieces of a tile
@@ -212,6 +220,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -INFINITY, l_run = 0.0f;       // m_run: kWeightExp above the reference value
+    float shift = 0.0f;                          // of the row's scores, a whole number; 0 unless one was far
+    bool far = false;                            // some row's was
     int scale_low = 255, scale_high = 0;         // exponent bits of the V scales until now
     bool poison = false;
     const int my_first = tile_begin + team;
@@ -271,6 +281,29 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
                     if (tok0 + kBlockRows * j + 4 * g + i >= limit) s[j][i] = -INFINITY;
             }
         }
+        // Where scores are far, what follows sees them less the row's shift, which is the
+        // largest at the time it was far.
+        auto shift_scores = [&]() {
+            float largest = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[j][i] = rounded_product(s[j][i], f[j]);
+                    largest = fmaxf(largest, s[j][i]);
+                }
+                f[j] = 1.0f;
+            }
+            largest = across_groups_max(largest);
+            if (fabsf(largest) < INFINITY && (m_run == -INFINITY ? fabsf(largest) > kFar : largest - shift > kFar)) {
+                const float next = rintf(largest);
+                m_run -= next - shift;
+                shift = next;
+            }
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j) s[j] -= shift;
+        };
+        if (far) shift_scores();
         // V scales are powers of two: exponents, in scalar registers.  One that is not a
         // number poisons the rows that see its block.
         int ev[kTileBlocks];
@@ -290,14 +323,24 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             for (int j = 0; j < kTileBlocks; ++j)
                 if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit) poison = true;
         }
-        float top = -INFINITY, vk[kTileBlocks];
+        float vk[kTileBlocks];
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            vk[j] = static_cast<float>(ev[j] - 127 + kWeightExp);
-            top = fmaxf(top, __builtin_fmaf(f[j], fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), vk[j]));
-        }
+        for (int j = 0; j < kTileBlocks; ++j) vk[j] = static_cast<float>(ev[j] - 127 + kWeightExp);
+        auto largest_weight = [&]() {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < kTileBlocks; ++j)
+                top = fmaxf(top, __builtin_fmaf(f[j], fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), vk[j]));
+            return top;
+        };
+        float top = largest_weight();
         if (__any(top > m_run + kSlack)) {
             top = across_groups_max(top);
+            if (!far && __any(fabsf(top) > kFar && fabsf(top) < INFINITY)) {
+                far = true;
+                shift_scores();
+                top = across_groups_max(largest_weight());
+            }
             const float m_new = top > m_run + kSlack ? ceilf(top) : m_run;
             const float alpha = m_new == -INFINITY ? 0.0f : fast_exp2(m_run - m_new);
             if (m_new > -INFINITY) l_run = scaled(l_run, m_run - m_new);
@@ -347,6 +390,17 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     // Join the teams in LDS: (m, l, acc) per row of all but the first.
     float l = across_groups_sum(l_run);
     if (poison) l = __builtin_nanf("");
+    if (far) {
+        // The reference value of the scores themselves, as near as FP32 has it.
+        const float all = m_run + shift;
+        const int rest = static_cast<int>(fminf(fmaxf(m_run - (all - shift), -60.0f), 60.0f));
+        m_run = all;
+        l = ldexpf(l, rest);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][k] = ldexpf(acc[i][k], rest);
+    }
     constexpr float kToValues = 1.0f / (1 << kSumExp);
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] *= kToValues;

@@ -190,6 +190,37 @@ def test_largest_and_smallest_values(skv, ctx, t, n, heads, weights, size):
         attend(rig, rng, end - n, n, heads, weights)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n,heads,weights", FORMS)
+@pytest.mark.parametrize("height", [2.0 ** 18, -2.0 ** 18, 2.0 ** 24, 2.0 ** 29, -2.0 ** 29, 2.0 ** 60])
+def test_scores_far_from_zero(skv, ctx, t, n, heads, weights, height):
+    """Scores so large that FP32 has no fraction of them: the two tokens of the largest, the same in all their bits, share
+    the weight, though their blocks' V scales differ.  Before them others hold it for a while."""
+    rng = np.random.default_rng(n)
+    dim, tokens = 64, 700
+    part = 0.9 * rng.random(tokens) if height > 0 else 1.3 + rng.random(tokens)
+    part[[100, 101, 390]] = 0.95 if height > 0 else 1.2
+    for token in (420, 600):                    # in blocks of the same K scale, so of the same code
+        part[token // 16 * 16:token // 16 * 16 + 16] = 0.5 if height > 0 else 2.0
+        part[token] = 1.0
+    q = np.tile(dim ** 0.25 * rng.standard_normal(dim), (n, heads, 1))
+    _, q = R.typed(q, t)
+    k = np.outer(part * height, q[0, 0] / (q[0, 0] @ q[0, 0] * dim ** -0.5))
+    rig = rig_of(skv, ctx, t, heads, dim, 704)
+    put(rig, 0, k, rng.standard_normal((tokens, dim)) * 2.0 ** (np.arange(tokens) // 16 * 7 % 13)[:, None])
+    q, out, _ = run(rig, q, tokens - n, weights)
+    page = rig.pages[0, 0, 0]
+    keys, v = page.values(tokens)
+    s = keys @ q[0, 0] * dim ** -0.5
+    # the definition's own two, so far above the rest that no rounding of a score (2^-24 of it a few times) matters
+    first, rest = np.flatnonzero(s == s.max()), np.sort(s)[:-2]
+    assert first.tolist() == [420, 600] and rest.max() < s.max() - 0.01 * abs(height)
+    want, size = v[first].mean(0), np.abs(v[first]).mean(0)
+    step = 2.0 ** -20 + (0 if heads * n <= 16 or weights else 2.0 ** -22 if t == "f32" else 2.0 ** -11)
+    bound = step * size + R.HALF_STEP[t] * np.abs(want) * (1 + step) + 256 * 2.0 ** -29 * page.scales[1].max()
+    assert (np.abs(out - want) <= bound).all()
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,heads", [(1, 2), (40, 2)])
 def test_small_values_in_channels_of_their_own(skv, ctx, t, n, heads):
