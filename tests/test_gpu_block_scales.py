@@ -1,5 +1,6 @@
 """The block cache's attention where blocks have V scales far apart: what a row does not see, or hardly weighs, takes
-nothing from the rest.  Bounds here go by each row's own visible tokens."""
+nothing from the rest.  Bounds here go by each row's own visible tokens.  Long splits, whose tiles are more than one
+window of the table."""
 import numpy as np
 import pytest
 
@@ -234,3 +235,19 @@ def test_small_values_in_channels_of_their_own(skv, ctx, t, n, heads):
     v[~large] *= 2.0 ** -12
     put(rig, 0, rng.standard_normal((600, 64)), v)
     attend(rig, rng, 600 - n, n, heads, False)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 4, 70])
+def test_second_window_of_the_table(skv, ctx, t, n):
+    """One split of 20011 tokens and those that the call appends: a wave or team takes more tiles than the 64 whose table
+    entries it reads at a time, and the appended ones lie in its second window."""
+    rng = np.random.default_rng(n)
+    rig = Rig(skv, ctx, t, 1, 4, 1, 64, 20100)
+    rig.append(rng, [0], 20011)
+    ctx.set_split_tokens(32768)
+    try:
+        rig.check_attention(rng, [20011], n, weights=n == 4)
+        rig.check_attention(rng, [20010 + n], 1, append=False)
+    finally:
+        ctx.set_split_tokens(0)
