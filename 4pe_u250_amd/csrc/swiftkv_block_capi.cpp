@@ -26,11 +26,10 @@ struct swiftkv_block_cache {
     int32_t capacity = 0;      // tokens
     BlockView view{};
     size_t bytes = 0;
-    // Log-sums of the blocks and rows of one launch with weights.  A buffer
-    // that a larger n outgrows is kept: a graph may have recorded it.
+    // Log-sums of the rows and blocks of one launch with weights, for the most
+    // queries that such a call takes (a graph may record it at any time):
+    // allocated with the first of them.
     float* log_sums = nullptr;
-    size_t log_sum_floats = 0;
-    float* outgrown[kBlockWeightQueries] = {};
 };
 
 namespace {
@@ -358,8 +357,6 @@ int swiftkv_block_cache_destroy(swiftkv_block_cache* cache) {
     (void)hipStreamSynchronize(ctx->stream);
     (void)hipFree(cache->view.base);
     if (cache->log_sums) (void)hipFree(cache->log_sums);
-    for (float* p : cache->outgrown)
-        if (p) (void)hipFree(p);
     delete cache;
     release_child(ctx);
     return ok();
@@ -444,20 +441,15 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.counters = ctx->block_workspace;
     a.partials = reinterpret_cast<float*>(ctx->block_workspace + kMaxSplitGroups * kCounterStride);
     if (weights) {
-        const size_t rows = static_cast<size_t>(std::min(cache->max_batch, kBlockBatch)) * cache->heads * n;
-        const size_t need = rows * (static_cast<size_t>(view.blocks) + 1);
-        if (need > cache->log_sum_floats) {
-            if ((rc = not_capturing(ctx, "the first attention with weights (or with more queries)"))) return rc;
+        const size_t rows =
+            static_cast<size_t>(std::min(cache->max_batch, kBlockBatch)) * cache->heads * kBlockWeightQueries;
+        if (!cache->log_sums) {
+            if ((rc = not_capturing(ctx, "the first attention with weights"))) return rc;
+            const size_t bytes = rows * (static_cast<size_t>(view.blocks) + 1) * sizeof(float);
             void* p = nullptr;
-            if (hipMalloc(&p, need * sizeof(float)) != hipSuccess)
-                return fail(SWIFTKV_ENOMEM, "hipMalloc of %zu bytes failed", need * sizeof(float));
-            for (float*& old : cache->outgrown)      // n grows at most kBlockWeightQueries - 1 times
-                if (!old) {
-                    old = cache->log_sums;
-                    break;
-                }
+            if (hipMalloc(&p, bytes) != hipSuccess) return fail(SWIFTKV_ENOMEM, "hipMalloc of %zu bytes failed", bytes);
             cache->log_sums = static_cast<float*>(p);
-            cache->log_sum_floats = need;
+            cache->bytes += bytes;
         }
         a.row_lse = cache->log_sums;
         a.block_lse = cache->log_sums + rows;

@@ -439,6 +439,7 @@ int swiftkv_block_cache_create(swiftkv_context* ctx, int32_t layers, int32_t max
                                int32_t kv_heads, int32_t head_dim, int32_t max_seq_len,
                                swiftkv_block_cache** out);
 int swiftkv_block_cache_destroy(swiftkv_block_cache* cache);
+/* Device memory of the cache, with what its first attention with weights added. */
 size_t swiftkv_block_cache_bytes(const swiftkv_block_cache* cache);
 /* Blocks of one (sequence, layer, key/value head): capacity / 16. */
 int32_t swiftkv_block_cache_blocks(const swiftkv_block_cache* cache);
@@ -469,9 +470,9 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  *   weights   NULL, or device FP32 [batch][kv_heads][blocks of the cache], in the
  *             blocks' present order: the softmax weight that the n queries of the
  *             key/value head's query heads give the tokens of each block is added
- *             (n <= SWIFTKV_BLOCK_WEIGHT_QUERIES).  The first call with weights,
- *             and the first with a larger n, allocates; run it once before a
- *             capture.
+ *             (n <= SWIFTKV_BLOCK_WEIGHT_QUERIES).  The first call with weights
+ *             allocates: FP32 [min(max_batch, 64) sequences][heads][8 queries]
+ *             [blocks + 1]; run it once before a capture.
  * Scores, softmax sums and outputs are held in FP32.  With at most 16 rows (n
  * times the query heads that share a key/value head), or with weights, a query
  * value is good to 2^-30 of its row's largest, and a softmax weight times its
