@@ -39,6 +39,8 @@ static_assert(SWIFTKV_BLOCK_WEIGHT_QUERIES == kBlockWeightQueries, "queries with
 static_assert(SWIFTKV_F32 == kF32 && SWIFTKV_BF16 == kBF16 && SWIFTKV_F16 == kF16, "element types");
 
 constexpr float kLog2E = 1.4426950408889634f;
+// Workgroups of up to 1024 threads that a launch's x extent holds.
+constexpr int64_t kMaxPromptGroups = int64_t(1) << 22;
 // Workgroups of an attention launch that splits its sequences, at most, and
 // what their partials take (17 MB).
 constexpr int64_t kMaxSplitGroups = 2048;
@@ -426,6 +428,10 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     if (weights && n > kBlockWeightQueries)
         return fail(SWIFTKV_ERANGE, "weights are gathered from at most %d queries a call, not %d", kBlockWeightQueries, n);
     if (reinterpret_cast<uintptr_t>(weights) & 3u) return fail(SWIFTKV_EINVAL, "weights must be aligned to 4 bytes");
+    const int32_t group = cache->heads / view.kv_heads;
+    if (!weights && (static_cast<int64_t>(group) * n + kPromptRows - 1) / kPromptRows * view.kv_heads >= kMaxPromptGroups)
+        return fail(SWIFTKV_ERANGE, "n = %d: %d heads take %lld workgroups and more", n, cache->heads,
+                    static_cast<long long>(kMaxPromptGroups));
     if (n == 0) return ok();
     if ((rc = set_device(ctx))) return rc;
 
@@ -434,7 +440,7 @@ int swiftkv_block_attention(swiftkv_context* ctx, const void* q, int64_t q_strid
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.scale = (scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(view.head_dim)) : scale) * kLog2E;
-    a.group = cache->heads / view.kv_heads;
+    a.group = group;
     a.group_magic = a.group == 1 ? 0u : static_cast<uint32_t>(((uint64_t(1) << 32) + a.group - 1) / a.group);
     a.n = n;
     a.layer = layer_index;

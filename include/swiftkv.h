@@ -466,6 +466,7 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  * no part, and its output rows are zero.
  *   q, out    [batch * n][heads * head_dim], q_stride and out_stride apart; out
  *             has q's type and must not overlap the inputs
+ *   n         0 to the capacity; n * heads < 2^28 - 64 * kv_heads without weights
  *   scale     multiplies q.k; 0 stands for 1 / sqrt(head_dim)
  *   weights   NULL, or device FP32 [batch][kv_heads][blocks of the cache], in the
  *             blocks' present order: the softmax weight that the n queries of the

@@ -1,4 +1,4 @@
-"""What the block cache's attention allocates, and when."""
+"""What the block cache's attention allocates and when, and what is too large for a launch."""
 import numpy as np
 import pytest
 
@@ -32,3 +32,22 @@ def test_weights_allocate_once(skv, ctx):
     out, after = dout.download(np.float32, q.shape).astype(np.float64), dw.download(np.float32, before.shape)
     rig.compare(q, [13, 13, 13], 8, out, before, after / 2)
     graph.close()
+
+
+def test_more_workgroups_than_a_launch_takes(skv, ctx):
+    """Refused before the rows are appended or a tensor is read."""
+    cache = skv.BlockCache(ctx, 1, 1, 256 * 64, 256, 64, 16384)
+    k = np.random.default_rng(20).standard_normal((1, 256 * 64)).astype(np.float32)
+    buf = ctx.to_device(k)
+    skv.swiftkv_block_append(ctx, buf, buf, cache, 0, 0, dtype=skv.F32)
+    got = ctx.alloc(4 * 256 * 64), ctx.alloc(4 * 256 * 64)
+    values = []
+    for _ in range(2):
+        skv.swiftkv_block_values(ctx, cache, 0, 0, *got, dtype=skv.F32)
+        ctx.synchronize()
+        values.append(got[0].download(np.float32, k.shape))
+        with pytest.raises(skv.SwiftKVError) as e:
+            skv.swiftkv_block_attention(ctx, buf, buf, buf, cache, 0, 0, buf, n=16384, dtype=skv.F32)
+        assert e.value.code == skv.ERANGE
+    np.testing.assert_array_equal(*values)
+    assert np.abs(values[0] - k).max() <= np.abs(k).max() / 64
