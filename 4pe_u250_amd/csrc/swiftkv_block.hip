@@ -1004,15 +1004,13 @@ void attend(const BlockAttendArgs& a, int batch, hipStream_t s) {
         block_attend_kernel<T, HD, RT, LSE, true><<<grid, kAttendThreads, 0, s>>>(a);
         return;
     }
-    if constexpr (RT == kMaxRowTiles) {
-        block_attend_kernel<T, HD, RT, LSE, false><<<grid, kAttendThreads, 0, s>>>(a);
-        if (LSE) {
-            int most = 0;
-            for (int b = 0; b < batch; ++b) most = a.positions[b] + a.n > most ? a.positions[b] + a.n : most;
-            const int blocks = (most + kBlockRows - 1) / kBlockRows;
-            if (blocks > 0)
-                block_weights_kernel<<<dim3((blocks + 255) / 256, a.view.kv_heads, batch), 256, 0, s>>>(a);
-        }
+    if constexpr (RT == kMaxRowTiles && LSE) {   // more rows without weights: the prompt kernel
+        block_attend_kernel<T, HD, RT, true, false><<<grid, kAttendThreads, 0, s>>>(a);
+        int most = 0;
+        for (int b = 0; b < batch; ++b) most = a.positions[b] + a.n > most ? a.positions[b] + a.n : most;
+        const int blocks = (most + kBlockRows - 1) / kBlockRows;
+        if (blocks > 0)
+            block_weights_kernel<<<dim3((blocks + 255) / 256, a.view.kv_heads, batch), 256, 0, s>>>(a);
     }
 }
 }  // namespace
