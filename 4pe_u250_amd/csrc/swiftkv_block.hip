@@ -276,10 +276,13 @@ __global__ __launch_bounds__(256) void block_table_kernel(uint16_t* table, int64
 // FP32 products would.
 //
 // Wave w takes tiles w, w + 4, ... of the split, each with its own running
-// (max, sum, output); the waves meet in LDS.  A tile's loads all go out together
-// and four workgroups fill a CU (128 registers), so that others' loads fly while
-// one computes: 64 sequences x 32 heads of 4096 tokens 308 us, 7.0 TB/s.  Asking
-// for the next tile's codes ahead took 154 registers and 328 us.
+// (max, sum, output); the waves meet in LDS.  A tile's loads all go out together;
+// with up to 4 rows four workgroups fill a CU (128 registers), so that others' loads
+// fly while one computes: 64 sequences x 32 heads of 4096 tokens 308 us, 7.0 TB/s.
+// Asking for the next tile's codes ahead took 154 registers and 328 us.  Heads of 128
+// with 8 rows take 161 to 178 registers (two or three workgroups a CU), with 16 rows 202
+// to 256 (one), where little hides a tile's loads: 64 sequences of 4096 tokens, 8
+// key/value heads, 86.5, 94 and 138 us for 4, 8 and 16 rows.
 //
 // ONCE (one row chunk, so each page is read once): the codes are read past the
 // caches (nontemporal; 64 sequences of 4096 tokens, 8 key/value heads, 82 us
@@ -836,7 +839,9 @@ __global__ __launch_bounds__(256) void block_weights_kernel(const BlockAttendArg
 // into few bins, whose atomics wait for each other: 32 layers x 8 sequences x 8
 // heads of 2032 blocks took 32.8 us.)  Ballots and one prefix over (turn, wave)
 // give each block its place.  A few KiB are read and written a workgroup: latency
-// bounds it.
+// bounds it, twice where PER is 8, whose 88 registers leave 1280 of those 2048
+// workgroups resident.  That launch takes 21.6 us on weights as they gather, and 20.5 on
+// what an eviction left, mostly zeros.
 constexpr int kEvictThreads = 256;
 constexpr int kEvictBins = 2048;
 

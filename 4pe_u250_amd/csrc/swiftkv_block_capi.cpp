@@ -128,6 +128,17 @@ int append_rows(const swiftkv_context* ctx, const void* k, int64_t k_stride, con
 // Sequences of different lengths take a quarter more workgroups: 16 of 2000 to
 // 32511 tokens 105.8 with 8192 tokens, 116.9 with the 9700 of one for each CU.
 //
+// Rows (query tokens times grouped heads) choose the kernel: the digits' row tiles
+// of 4, 8 or 16, the fewest that hold the rows, and half floats, 64 rows a
+// workgroup, for more than 16 without weights.  us of a step onto 4095 tokens, 64 / 8 /
+// 1 sequences, 8 key/value heads (4 where groups are 5), the kernel taken against the
+// next: 4 rows 86.5 / 17.7 / 10.8 against 88.7 / 19.9 / 13.2; 5 rows 47.6 / 14.5 / 12.9
+// against 67.0 / 20.8 / 19.3; 8 rows 93.7 / 20.4 / 15.7 against 137 / 31.2 / 23.9; 16 rows
+// 140 / 31.9 / 23.5 against 129 / 37.5 / 25.8 (FP32 139 / 31.8 / 23.4 against 163 / 43.4 /
+// 28.5); more rows, half floats against 16 at a time: 20 rows 72.9 / 31.3 / 26.9 against
+// 99.3 / 34.7 / 26.9, 32 rows 128 / 40.5 / 30.9 against 181 / 48.1 / 27.3 (FP32 168 / 47.1 /
+// 34.4 against 184 / 46.2 / 26.2).
+//
 // One row chunk may append the call's rows in the attention's own launch, which
 // costs each sequence's last workgroup five trips to memory, or leave them to a
 // launch before it.  us of a step, own launch against one before: batch 1 / 8 /

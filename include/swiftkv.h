@@ -470,13 +470,14 @@ int swiftkv_block_values(swiftkv_context* ctx, const swiftkv_block_cache* cache,
  *   scale     multiplies q.k; 0 stands for 1 / sqrt(head_dim)
  *   weights   NULL, or device FP32 [batch][kv_heads][blocks of the cache], in the
  *             blocks' present order: the softmax weight that the n queries of the
- *             key/value head's query heads give the tokens of each block is added
+ *             key/value head's query heads give the tokens of each block is added,
+ *             good to 2^-20 (S + 20) of it where the sums of scale |q k| are up to S in log2
  *             (n <= SWIFTKV_BLOCK_WEIGHT_QUERIES).  The first call with weights
  *             allocates: FP32 [min(max_batch, 64) sequences][heads][8 queries]
  *             [blocks + 1]; run it once before a capture.
  * Scores, softmax sums and outputs are held in FP32.  With at most 16 rows (n
  * times the query heads that share a key/value head), or with weights, a query
- * value is good to 2^-30 of its row's largest, and a softmax weight times its
+ * value is good to 2^-30 of its row's largest (or 2^-120), and a softmax weight times its
  * block's V scale to 2^-30 of the largest such product that the row has among the
  * 64 tokens around it; with more rows queries and softmax weights are 16-bit
  * floats (each weight good to 2^-11, or to 2^-35 of the row's largest where that
