@@ -137,6 +137,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     const int r = row_first + min(row, rows - 1), i_q = row_token(a, r);
     const int limit = row < rows && p >= 0 ? p + i_q + 1 : 0;
     const bool any_row = part * 16 < rows;
+    const int wave_limit = p + row_token(a, row_first + min(part * 16 + 15, rows - 1)) + 1;      // of its last row
     v8h q[TERMS][NS];
     float qs;
     {
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     float m_run = -INFINITY, l_run = 0.0f;       // m_run: kWeightExp above the reference value
     float shift = 0.0f;                          // of the row's scores, a whole number; 0 unless one was far
     bool far = false;                            // some row's was
-    int scale_low = 255, scale_high = 0;         // exponent bits of the V scales until now
+    int scale_low = 255, scale_high = 0;         // exponent bits of the V scales that the wave's rows have seen
     bool poison = false;
     const int my_first = tile_begin + team;
     const int turns = (tile_end - tile_begin + TEAMS - 1) / TEAMS;   // every team's
@@ -315,8 +316,10 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
                 bad = true;
                 ev[j] = kScaleMin;
             }
-            scale_low = min(scale_low, ev[j]);
-            scale_high = max(scale_high, ev[j]);
+            if (tok0 + kBlockRows * j < wave_limit) {
+                scale_low = min(scale_low, ev[j]);
+                scale_high = max(scale_high, ev[j]);
+            }
         }
         if (bad) {
 #pragma unroll

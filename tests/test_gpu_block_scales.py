@@ -100,6 +100,25 @@ def test_rows_left_behind_a_restarted_sequence(skv, ctx, t, n, heads, weights, u
             attend(rig, rng, end - n, n, heads, weights)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,heads,weights", FORMS)
+def test_what_is_left_behind_changes_no_bit(skv, ctx, t, n, heads, weights):
+    """The same tokens in an empty slot and in slots that held large, small and no numbers."""
+    seen = []
+    for size in (None, 2.0 ** 110, 2.0 ** -99, np.nan):
+        rng = np.random.default_rng(n)
+        rig = rig_of(skv, ctx, t, heads, 64, 256)
+        k, v, q = rng.standard_normal((90, 64)), rng.standard_normal((90, 64)), rng.standard_normal((n, heads, 64))
+        if size is not None:
+            put(rig, 0, *(rng.standard_normal((2, 250, 64)) * size))
+        put(rig, 0, k, v)
+        seen.append([])
+        for end in (40, 65, 90):
+            _, out, w = run(rig, q, end - n, weights)
+            seen[-1].append(out.tobytes() + (w[:6].tobytes() if weights else b""))
+    assert all(x == seen[0] for x in seen[1:])
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 @pytest.mark.parametrize("n,heads,weights", FORMS)
 def test_blocks_dropped_by_eviction(skv, ctx, t, n, heads, weights):
