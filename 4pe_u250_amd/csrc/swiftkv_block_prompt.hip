@@ -76,6 +76,16 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
     return a * b;
 }
 
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = max(x, dpp_u<kDppQuadXor1>(x));
+    x = max(x, dpp_u<kDppQuadXor2>(x));
+    x = max(x, dpp_u<kDppHalfMirror>(x));
+    x = max(x, dpp_u<kDppRowRor8>(x));
+    const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16),
+                   c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    return max(max(a, b), max(c, d));
+}
+
 __device__ __forceinline__ float across_groups_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
@@ -94,9 +104,10 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     constexpr int kSlackExp = TERMS == 1 ? 4 : 0, kWeightExp = 15 - kSlackExp;
     constexpr float kSlack = kSlackExp, kFloatMin = 0x1p-126f;
     // Sums of weights count in 2^-kSumExp of them, which keeps them and 1 / v in FP32's range.
-    constexpr int kSumExp = 6, kScaleMin = 127 - 100;    // exponent bits of the smallest scale
+    constexpr int kSumExp = 6;
+    constexpr uint32_t kScaleMin = 127 - 100;    // exponent bits of the smallest scale
     // Between V scales further apart a weight may vanish beside p v that counts in the sum.
-    constexpr int kWide = 96;
+    constexpr uint32_t kWide = 96;
     // Beyond this a score has no room for log2 of a V scale beside it.
     constexpr float kFar = 0x1p22f;
     constexpr int NS = HD / 32, ND = HD / 16, kRecord = 2 * kBlockRows * HD;
@@ -223,7 +234,8 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
     float m_run = -INFINITY, l_run = 0.0f;       // m_run: kWeightExp above the reference value
     float shift = 0.0f;                          // of the row's scores, a whole number; 0 unless one was far
     bool far = false;                            // some row's was
-    int scale_low = 255, scale_high = 0;         // exponent bits of the V scales that the wave's rows have seen
+    uint32_t scale_low = 255, scale_high = 0;    // exponent bits of the V scales that the wave's rows see until the window's end
+    bool wide = false, bad = false;
     bool poison = false;
     const int my_first = tile_begin + team;
     const int turns = (tile_end - tile_begin + TEAMS - 1) / TEAMS;   // every team's
@@ -234,10 +246,24 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             heads.load_entries(table, tile + lane * TEAMS, last_tile);
             heads.load_scales(scale_base);
             load_tile(0);
+            // V scales are powers of two: exponents will do, 255 for one that is not a number.
+            const int first = min(tile + lane * TEAMS, last_tile) * kTileTokens;
+            uint32_t low = 255, high = 0;
+            bool nan = false;
 #pragma unroll
-            for (int j = 0; j < kTileBlocks; ++j)
-                scale_pair[j] = static_cast<uint32_t>(heads.scale[j]) >> 16 |
-                                (static_cast<uint32_t>(heads.scale[j] >> 32) & 0xffff0000u);
+            for (int j = 0; j < kTileBlocks; ++j) {
+                const uint32_t e = max(static_cast<uint32_t>(heads.scale[j] >> 55) & 255u, kScaleMin);
+                scale_pair[j] = static_cast<uint32_t>(heads.scale[j]) >> 16 | e << 23;
+                nan |= e == 255;
+                if (e < 255 && first + kBlockRows * j < wave_limit) {
+                    low = min(low, e);
+                    high = max(high, e);
+                }
+            }
+            bad = __any(nan);
+            scale_low = min(scale_low, ~wave_max(~low));
+            scale_high = max(scale_high, wave_max(high));
+            wide = scale_high > scale_low + kWide;
         }
         __syncthreads();                         // everyone is done with the tile before
         store_tile();
@@ -246,12 +272,13 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             load_tile((at + 1) & 63);
             continue;
         }
-        TileHead head;
+        float ks[kTileBlocks];
+        uint32_t ev[kTileBlocks];                // exponent bits of the V scales
 #pragma unroll
         for (int j = 0; j < kTileBlocks; ++j) {
             const uint32_t both = __builtin_amdgcn_readlane(scale_pair[j], at);
-            head.ks[j] = __uint_as_float(both << 16);
-            head.vs[j] = __uint_as_float(both & 0xffff0000u);
+            ks[j] = __uint_as_float(both << 16);
+            ev[j] = both >> 23;
         }
         const int tok0 = tile * kTileTokens;
         v4f s[kTileBlocks];
@@ -270,7 +297,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
         // Scores are s * f, f > 0.
         float f[kTileBlocks];
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) f[j] = qs * head.ks[j];
+        for (int j = 0; j < kTileBlocks; ++j) f[j] = qs * ks[j];
         if (__any(tok0 + kTileTokens > limit)) {
             asm volatile("");                    // a branch, not selects in every tile
 #pragma unroll
@@ -305,30 +332,18 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             for (int j = 0; j < kTileBlocks; ++j) s[j] -= shift;
         };
         if (far) shift_scores();
-        // V scales are powers of two: exponents, in scalar registers.  One that is not a
-        // number poisons the rows that see its block.
-        int ev[kTileBlocks];
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) {
-            ev[j] = max(static_cast<int>(__float_as_uint(head.vs[j]) >> 23 & 255u), kScaleMin);
-            if (ev[j] == 255) {
-                bad = true;
-                ev[j] = kScaleMin;
-            }
-            if (tok0 + kBlockRows * j < wave_limit) {
-                scale_low = min(scale_low, ev[j]);
-                scale_high = max(scale_high, ev[j]);
-            }
-        }
         if (bad) {
+            // A V scale that is not a number poisons the rows that see its block.
 #pragma unroll
             for (int j = 0; j < kTileBlocks; ++j)
-                if (head.vs[j] != head.vs[j] && tok0 + kBlockRows * j < limit) poison = true;
+                if (ev[j] == 255) {
+                    ev[j] = kScaleMin;
+                    if (tok0 + kBlockRows * j < limit) poison = true;
+                }
         }
         float vk[kTileBlocks];
 #pragma unroll
-        for (int j = 0; j < kTileBlocks; ++j) vk[j] = static_cast<float>(ev[j] - 127 + kWeightExp);
+        for (int j = 0; j < kTileBlocks; ++j) vk[j] = static_cast<float>(static_cast<int>(ev[j]) - 127 + kWeightExp);
         auto largest_weight = [&]() {
             float top = -INFINITY;
 #pragma unroll
@@ -352,7 +367,6 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             for (int i = 0; i < ND; ++i) acc[i] *= alpha;
         }
         const float base_exp = (m_run == -INFINITY ? 0.0f : m_run) - kWeightExp;
-        const bool wide = scale_high - scale_low > kWide;
         if (wide) {
             const float c = (kWeightExp - kSumExp) - base_exp;
 #pragma unroll
@@ -367,7 +381,7 @@ __global__ __launch_bounds__(TEAMS * kTeamThreads) void block_prompt_kernel(cons
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = fast_exp2(__builtin_fmaf(s[j][i], f[j], c));
-            const float per_scale = wide ? 0.0f : __uint_as_float(static_cast<uint32_t>(254 - kSumExp - ev[j]) << 23);
+            const float per_scale = wide ? 0.0f : __uint_as_float((254u - kSumExp - ev[j]) << 23);
             l_run = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), per_scale, l_run);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
