@@ -13,7 +13,7 @@ using namespace dev;
 // work around them bound it, so they run on 16-bit floats, which hold a code
 // exactly, and not on the digits of swiftkv_block.hip, which would take four times
 // the rows (512 tokens onto 4096, 32 heads over 8, in the first form: 84 us against 161;
-// two teams 101, two row tiles a wave 94, two buffers and two teams 88; now 68).  Each team turns a
+// two teams 101, two row tiles a wave 94, two buffers and two teams 88; now 66).  Each team turns a
 // tile's codes into half floats in LDS, once for its 64 rows
 // (0x6400 + byte is 1024 + byte, so a byte permute and a packed subtraction), in
 // the order in which the instruction reads them:
