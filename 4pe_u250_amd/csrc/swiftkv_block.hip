@@ -298,8 +298,9 @@ constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves4 = 4;
 constexpr int kDigitStride = kTileTokens + 16;   // bytes between rows of digits: rows of a 4-row step apart in banks
 constexpr int kScaleBits = 127 - 100;            // exponent bits of the smallest scale
-// A sum of weights times values may leave FP32's range where its quotient does not: waves
-// sum in a unit of their own, not below 2^kUnitMin, and join in 2^kJoinExp, of 2^17 tokens.
+// A sum of weights times values may leave FP32's range where its quotient does not (2^17
+// tokens, values below 2^127): a wave sums in a power of two of its own, 2^kUnitMin at
+// least, and waves and splits join what they have over 2^kJoinExp.
 constexpr float kUnitMin = -200.0f;
 constexpr int kJoinExp = 18;
 

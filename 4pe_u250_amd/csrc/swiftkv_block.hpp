@@ -76,7 +76,7 @@ struct BlockAttendArgs {
     int32_t chunks;       // row chunks per (sequence, key/value head)
     int32_t splits;       // of the longest sequence
     int32_t split_tiles;  // tiles per split at most, a multiple of 4
-    float* partials;      // [pair][split][rows of a chunk][2 + head_dim]: m, l, acc
+    float* partials;      // [pair][split][rows of a chunk][2 + head_dim]: m, l, acc, each kernel's own units
     uint32_t* counters;   // [pair] arrived splits, kCounterStride apart, zero between launches
     float* block_lse;     // null, or [sequence][kv head][row][blocks]: log2 of each block's sum of 2^score
     float* row_lse;       // [sequence][kv head][row]: the same of the whole row
