@@ -50,6 +50,10 @@ BLOCK_TOKENS = 16
 BLOCK_MAX_SEQ = 131072
 BLOCK_WEIGHT_QUERIES = 8
 ROTARY_MAX_POSITIONS = 1048576
+PAGE_TOKENS = 64
+TREE_TOKENS = 64
+PAGED_MAX_SEQ = 131072
+TREE_ROOT, TREE_NONE = -1, -2                           # parents of a tree's first tokens; rows without one
 KERNEL_APPEND, KERNEL_STEP, KERNEL_EXACT = 0, 1, 2
 KERNEL_KINDS = 3
 _STATUS_NAMES = {EINVAL: "EINVAL", ERANGE: "ERANGE", EHIP: "EHIP", ENOMEM: "ENOMEM", ESTATE: "ESTATE"}
@@ -116,6 +120,17 @@ _SIGNATURES = {
     "swiftkv_block_attention": (C.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _vp, _i32, _i32,
                                           C.c_float, _vp, _vp, _i64]),
     "swiftkv_block_evict": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "swiftkv_paged_cache_create": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_vp)]),
+    "swiftkv_paged_cache_destroy": (C.c_int, [_vp]),
+    "swiftkv_paged_cache_bytes": (_sz, [_vp]),
+    "swiftkv_paged_map": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32]),
+    "swiftkv_paged_copy": (C.c_int, [_vp, _vp, _i32, _i32]),
+    "swiftkv_paged_append": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _i32]),
+    "swiftkv_paged_values": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp]),
+    "swiftkv_paged_attention": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp,
+                                          _i32, _i32, C.c_float, _vp, _i64]),
+    "swiftkv_paged_keep": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp]),
+    "swiftkv_debug_paged_plan": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "swiftkv_device_alloc": (C.c_int, [_vp, _sz, C.POINTER(_vp)]),
     "swiftkv_device_free": (C.c_int, [_vp, _vp]),
     "swiftkv_memcpy_h2d": (C.c_int, [_vp, _vp, _vp, _sz]),
@@ -551,6 +566,71 @@ class BlockCache:
             pass
 
 
+class PagedCache:
+    """GPU-resident cache of 16-bit rows in pages of 64 tokens that a table shares out among sequences."""
+
+    def __init__(self, ctx: Context, layers: int, pages: int, max_batch: int, heads: int, kv_heads: int, head_dim: int,
+                 max_seq_len: int, dtype: int = BF16):
+        h = C.c_void_p()
+        _check(lib().swiftkv_paged_cache_create(ctx.handle, layers, pages, max_batch, heads, kv_heads, head_dim,
+                                                max_seq_len, dtype, C.byref(h)))
+        self.ctx, self.handle = ctx, h.value
+        self.layers, self.pages, self.max_batch, self.max_seq_len = layers, pages, max_batch, max_seq_len
+        self.heads, self.kv_heads, self.head_dim, self.dtype = heads, kv_heads, head_dim, dtype
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().swiftkv_paged_cache_bytes(self.handle))
+
+    def map(self, seq: int, pages, first: int = 0) -> None:
+        """Entries first, first + 1, ... of the sequence, 64 tokens each, name `pages` (-1: none)."""
+        at, n, _keep = _int32s(pages)
+        _check(lib().swiftkv_paged_map(self.ctx.handle, self.handle, seq, first, at, n))
+
+    def copy(self, source: int, target: int) -> None:
+        """Page `target` gets what page `source` holds, in every layer."""
+        _check(lib().swiftkv_paged_copy(self.ctx.handle, self.handle, source, target))
+
+    def close(self) -> None:
+        if self.handle:
+            h, self.handle = self.handle, None
+            _check(lib().swiftkv_paged_cache_destroy(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _int32s(x):
+    """(address, count, owner) of host numbers as int32; a list goes through an array of C ints, which refuses what
+    does not fit one (and takes a tenth of numpy's time for a tree's)."""
+    if type(x) is list:
+        try:
+            a = array.array("i", x)
+            return (*a.buffer_info(), a)
+        except TypeError:
+            pass
+    a = np.asarray(x)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or int(a.min()) < _INT32_MIN or int(a.max()) > _INT32_MAX):
+            raise ValueError("expected whole numbers of 32 bits")
+        a = a.astype(np.int32)
+    a = np.ascontiguousarray(a)
+    return a.ctypes.data, int(a.size), a
+
+
+def _tree(parents, batch: int, n: int):
+    """(address or None, owner) of a call's trees."""
+    if parents is None:
+        return None, None
+    at, count, owner = _int32s(parents)
+    if count != batch * n:
+        raise ValueError(f"{count} parents for {batch} sequences of {n} tokens")
+    return at, owner
+
+
 def _ptr(x) -> Optional[int]:
     if x is None or type(x) is int:
         return x
@@ -783,6 +863,73 @@ def swiftkv_block_evict(ctx: Context, cache: BlockCache, layer0: int, layers: in
     _check(lib().swiftkv_block_evict(ctx.handle, cache.handle, layer0, layers, seq0, pos, batch, keep, sinks, recent,
                                      _ptr(weights), _ptr(kept), left))
     return list(left)
+
+
+def swiftkv_paged_append(ctx: Context, k, v, cache: PagedCache, layer_index: int, position, n: int = 1,
+                         table: Optional[RotaryTable] = None, halves: bool = True, parents=None, seq0: int = 0,
+                         k_stride: Optional[int] = None, v_stride: Optional[int] = None) -> None:
+    """Append n tokens to each of sequences seq0, seq0 + 1, ... at cached tokens
+    position[b] ..; a negative position skips its sequence.  k, v: device
+    [batch * n][kv_heads * head_dim], rows k_stride and v_stride elements apart
+    (default dense); keys are turned by `table`, if one is given.
+    parents: [batch * n], the token of the call that each token continues, TREE_ROOT
+    for the last cached one, TREE_NONE for rows without a token; None: chains."""
+    pos, batch, _keep = _positions(ctx, position)
+    tree, _owner = _tree(parents, batch, n)
+    row = cache.kv_heads * cache.head_dim
+    _check(lib().swiftkv_paged_append(ctx.handle, None if table is None else table.handle, 1 if halves else 0, _ptr(k),
+                                      row if k_stride is None else k_stride, _ptr(v),
+                                      row if v_stride is None else v_stride, cache.handle, layer_index, seq0, pos,
+                                      tree, batch, n))
+
+
+def swiftkv_paged_values(ctx: Context, cache: PagedCache, layer0: int, position, k, v, n: int = 1, layers: int = 1,
+                         seq0: int = 0) -> None:
+    """Cached tokens [position[b], position[b] + n) of `layers` layers to device k and
+    v, [layers][batch * n][kv_heads * head_dim] each."""
+    pos, batch, _keep = _positions(ctx, position)
+    _check(lib().swiftkv_paged_values(ctx.handle, cache.handle, layer0, layers, seq0, pos, batch, n, _ptr(k), _ptr(v)))
+
+
+def swiftkv_paged_attention(ctx: Context, q, k, v, cache: PagedCache, layer_index: int, position, out, n: int = 1,
+                            table: Optional[RotaryTable] = None, halves: bool = True, parents=None, scale: float = 0.0,
+                            seq0: int = 0, q_stride: Optional[int] = None, k_stride: Optional[int] = None,
+                            v_stride: Optional[int] = None, out_stride: Optional[int] = None) -> None:
+    """Append n tokens to each sequence (unless k and v are None; queries and keys
+    turned by `table`) and attend: a token sees the cached tokens before
+    position[b], its ancestors (parents as for swiftkv_paged_append) and itself.
+    q, out: device [batch * n][heads * head_dim]; rows without a token are zero."""
+    pos, batch, _keep = _positions(ctx, position)
+    tree, _owner = _tree(parents, batch, n)
+    row, kv_row = cache.heads * cache.head_dim, cache.kv_heads * cache.head_dim
+    _check(lib().swiftkv_paged_attention(ctx.handle, None if table is None else table.handle, 1 if halves else 0, _ptr(q),
+                                         row if q_stride is None else q_stride, _ptr(k),
+                                         kv_row if k_stride is None else k_stride, _ptr(v),
+                                         kv_row if v_stride is None else v_stride, cache.handle, layer_index, seq0, pos,
+                                         tree, batch, n, scale, _ptr(out), row if out_stride is None else out_stride))
+
+
+def swiftkv_paged_keep(ctx: Context, cache: PagedCache, layer0: int, layers: int, position, accepted, m: int,
+                       seq0: int = 0) -> list:
+    """Move the rows of each sequence's accepted drafted tokens (accepted [batch * m],
+    rising, then -1) to cached tokens position[b], position[b] + 1, ... of `layers`
+    layers.  Returns the numbers of tokens then cached."""
+    pos, batch, _keep = _positions(ctx, position)
+    at, count, _owner = _int32s(accepted)
+    if count != batch * m:
+        raise ValueError(f"{count} accepted tokens for {batch} sequences of {m}")
+    left = (C.c_int32 * batch)()
+    _check(lib().swiftkv_paged_keep(ctx.handle, cache.handle, layer0, layers, seq0, pos, at, batch, m, left))
+    return list(left)
+
+
+def paged_plan(heads: int, kv_heads: int, n: int, positions, cus: int = 256, split_tokens: int = 0):
+    """The plan of one launch of swiftkv_paged_attention (host-only, no device
+    needed): (rows of a workgroup, row chunks, splits, tokens of a split)."""
+    at, batch, _owner = _int32s(positions)
+    r = [C.c_int32() for _ in range(4)]
+    _check(lib().swiftkv_debug_paged_plan(cus, split_tokens, heads, kv_heads, n, at, batch, *(C.addressof(x) for x in r)))
+    return tuple(x.value for x in r)
 
 
 def a14_unpack(words: np.ndarray) -> np.ndarray:

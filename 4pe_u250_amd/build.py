@@ -9,10 +9,12 @@ built with packed-FP32 instruction selection disabled.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
@@ -27,7 +29,6 @@ HIP_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # Atomics with a returned value stay single-lane operations whose result
@@ -43,7 +44,8 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=8",
 ]
 SOURCES = ["swiftkv_kernels.hip", "swiftkv_synth.hip", "swiftkv_exact.hip", "swiftkv_exact_short.hip",
-           "swiftkv_block.hip", "swiftkv_block_prompt.hip", "swiftkv_rotary.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp"]
+           "swiftkv_block.hip", "swiftkv_block_prompt.hip", "swiftkv_rotary.hip", "swiftkv_paged.hip",
+           "swiftkv_paged_attend.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp", "swiftkv_paged_capi.cpp"]
 HOST_SRC = os.path.join(PKG_DIR, "host", "swiftkv_host.cpp")
 HOST_BIN = os.path.join(PKG_DIR, "swiftkv_host")
 
@@ -58,31 +60,47 @@ def _run(cmd, cwd=None):
     return "\n".join(lines)
 
 
-def build_library(verbose: bool = False) -> str:
-    srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    tmp = LIB + ".tmp"
-    cmd = [HIPCC, *HIP_FLAGS, "-I", os.path.join(REPO, "include"), *srcs, "-o", tmp]
-    out = _run(cmd)
-    if verbose and out.strip():
-        print(out)
-    os.replace(tmp, LIB)
-    return LIB
+def _compile(sources, extra, folder):
+    """Objects of the sources, compiled side by side."""
+    def one(name):
+        obj = os.path.join(folder, name + ".o")
+        out = _run([HIPCC, *HIP_FLAGS, *extra, "-I", os.path.join(REPO, "include"), "-c", os.path.join(CSRC, name), "-o", obj])
+        return obj, out
+    jobs = min(8, int(os.environ.get("MAX_JOBS") or 8))
+    with concurrent.futures.ThreadPoolExecutor(jobs) as pool:
+        done = list(pool.map(one, sources))
+    return [obj for obj, _ in done], "\n".join(out for _, out in done if out.strip())
+
+
+def _link(objects, lib):
+    tmp = lib + ".tmp"
+    out = _run([HIPCC, f"--offload-arch={ARCH}", "-shared", *objects, "-o", tmp])
+    os.replace(tmp, lib)
+    return out
 
 
 STAMPS_LIB = os.path.join(PKG_DIR, "libswiftkv_stamps.so")
+STAMPED = ["swiftkv_kernels.hip"]
 
 
-def build_stamps(verbose: bool = False) -> str:
-    """The instrumented library for phase_stamps.py: the same sources with the
-    step kernel's s_memrealtime phase stamps compiled in (SWIFTKV_PHASE_STAMPS).
-    Diagnostics only; the product is libswiftkv.so."""
-    srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    tmp = STAMPS_LIB + ".tmp"
-    out = _run([HIPCC, *HIP_FLAGS, "-DSWIFTKV_PHASE_STAMPS", "-I", os.path.join(REPO, "include"), *srcs, "-o", tmp])
+def build_libraries(verbose: bool = False) -> str:
+    """libswiftkv.so, and the instrumented library for phase_stamps.py: the same
+    objects but for the step kernel's, which has its s_memrealtime phase stamps
+    compiled in (SWIFTKV_PHASE_STAMPS).  Diagnostics only; the product is
+    libswiftkv.so."""
+    with tempfile.TemporaryDirectory() as folder:
+        stamped = os.path.join(folder, "stamped")
+        os.mkdir(stamped)
+        with concurrent.futures.ThreadPoolExecutor(1) as pool:
+            job = pool.submit(_compile, STAMPED, ["-DSWIFTKV_PHASE_STAMPS"], stamped)
+            objects, out = _compile(SOURCES, [], folder)
+            extra, _ = job.result()
+        out += _link(objects, LIB)
+        names = {os.path.basename(o): o for o in extra}
+        _link([names.get(os.path.basename(o), o) for o in objects], STAMPS_LIB)
     if verbose and out.strip():
         print(out)
-    os.replace(tmp, STAMPS_LIB)
-    return STAMPS_LIB
+    return LIB
 
 
 def build_host(verbose: bool = False) -> str:
@@ -111,9 +129,8 @@ def build_oracle(verbose: bool = False) -> None:
 
 def main() -> int:
     build_oracle(verbose=True)
-    print(build_library(verbose=True))
+    print(build_libraries(verbose=True))
     print(build_host(verbose=True))
-    print(build_stamps(verbose=True))
     return 0
 
 

@@ -2,22 +2,13 @@
 // cache (include/swiftkv.h): objects, argument checks, launch plans.  Kernels:
 // swiftkv_block.hip, swiftkv_rotary.hip.  As in swiftkv_capi.cpp no exception
 // crosses the C boundary, and a refused call enqueues nothing.
-#include "swiftkv_internal.hpp"
+#include "swiftkv_block_host.hpp"
 
 #include <algorithm>
 #include <cstring>
 #include <new>
 
-#include "swiftkv_block.hpp"
-
 using namespace swiftkv;
-
-struct swiftkv_rotary_table {
-    swiftkv_context* ctx = nullptr;
-    int32_t rotary_dim = 0;
-    int32_t positions = 0;
-    float2* table = nullptr;   // device [positions][rotary_dim / 2] (cos, sin)
-};
 
 struct swiftkv_block_cache {
     swiftkv_context* ctx = nullptr;
@@ -46,27 +37,8 @@ constexpr int64_t kMaxPromptGroups = int64_t(1) << 22;
 constexpr int64_t kMaxSplitGroups = 2048;
 constexpr size_t kPartialFloats = static_cast<size_t>(kMaxSplitGroups) * kMaxRowTiles * kRowTile * (2 + 128);
 
-int check_tensor(const char* name, const void* p, int64_t stride, int64_t row, int32_t dtype) {
-    if (!p) return fail(SWIFTKV_EINVAL, "null %s", name);
-    if (reinterpret_cast<uintptr_t>(p) & 15u) return fail(SWIFTKV_EINVAL, "%s must be 16-byte aligned", name);
-    if (stride < row || stride > (int64_t(1) << 40))
-        return fail(SWIFTKV_EINVAL, "%s stride %lld outside [%lld, 2^40]", name, static_cast<long long>(stride),
-                    static_cast<long long>(row));
-    if (stride * static_cast<int64_t>(element_bytes(dtype)) % 16 != 0)
-        return fail(SWIFTKV_EINVAL, "%s stride %lld is not a multiple of 16 bytes", name,
-                    static_cast<long long>(stride));
-    return SWIFTKV_OK;
-}
-
 int check_type(int32_t dtype) {
     return dtype < kF32 || dtype > kF16 ? fail(SWIFTKV_EINVAL, "unknown element type %d", dtype) : SWIFTKV_OK;
-}
-
-int check_idle_io(const swiftkv_context* ctx) {
-    if (!ctx) return fail(SWIFTKV_EINVAL, "null context");
-    if (ctx->released) return fail(SWIFTKV_ESTATE, "the context has been destroyed");
-    if (ctx->host_io) return fail(SWIFTKV_ESTATE, "this entry takes device pointers: switch host-memory I/O mode off");
-    return SWIFTKV_OK;
 }
 
 // What every call on a range of sequences of a block cache checks; n tokens at

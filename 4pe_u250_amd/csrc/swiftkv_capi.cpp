@@ -659,6 +659,7 @@ void swiftkv::free_context(swiftkv_context* ctx) {
     if (ctx->arrivals) (void)hipFree(ctx->arrivals);
     if (ctx->exact_workspace) (void)hipFree(ctx->exact_workspace);
     if (ctx->block_workspace) (void)hipFree(ctx->block_workspace);
+    if (ctx->paged_workspace) (void)hipFree(ctx->paged_workspace);
     if (ctx->io_stage) (void)hipFree(ctx->io_stage);
     if (ctx->fault_host) (void)hipHostFree(ctx->fault_host);
     for (auto& t : ctx->timers)

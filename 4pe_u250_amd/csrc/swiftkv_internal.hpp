@@ -44,6 +44,14 @@ inline int ok() {
                         __LINE__);                                                             \
     } while (0)
 
+// Device memory; where there is none, no error stays behind for the next launch's
+// check to report.
+inline bool device_malloc(void** p, size_t bytes) {
+    if (hipMalloc(p, bytes) == hipSuccess) return true;
+    (void)hipGetLastError();
+    return false;
+}
+
 struct ProfilePair {
     hipEvent_t begin;
     hipEvent_t end;
@@ -109,6 +117,8 @@ struct swiftkv_context {
     // fixed size (a graph may record them at any time): allocated with the first
     // block cache.
     uint32_t* block_workspace = nullptr;
+    // The same of the paged cache's attention, allocated with the first paged cache.
+    uint32_t* paged_workspace = nullptr;
 };
 
 struct swiftkv_graph {

@@ -510,6 +510,114 @@ int swiftkv_block_evict(swiftkv_context* ctx, swiftkv_block_cache* cache, int32_
                         int32_t recent, float* weights, int32_t* kept, int32_t* out_positions);
 
 /* --------------------------------------------------------------------------
+ * The paged cache: 16-bit rows in pages of SWIFTKV_PAGE_TOKENS tokens that a table
+ * shares out, and decoding with drafted tokens over it.  It has no counterpart in
+ * the reference.  A program maps pages to a sequence before it needs them, calls
+ * swiftkv_paged_attention for each layer (which turns the queries and keys,
+ * appends the new rows and attends) with one token, a prompt's chunk or a tree of
+ * drafted tokens of each sequence, and swiftkv_paged_keep once the accepted path
+ * is known.
+ *
+ * Tensors, strides, positions and host-memory I/O are as for the block cache; the
+ * element type is the cache's.
+ *
+ * Trees.  `parents`, host [batch * n] (n <= SWIFTKV_TREE_TOKENS): token i of
+ * sequence b continues token parents[b * n + i] < i of the same call, or with -1 the
+ * last cached one; -2, from some i on, marks rows without a token, so sequences may
+ * bring different numbers.  parents NULL: chains, token i continues token i - 1 (any
+ * n).  A token's row is cached token positions[b] + i, whatever its parent; its
+ * position in the text, by which its query and key are turned, is positions[b] plus
+ * its depth (0 where it continues the cached tokens).  It attends to cached tokens
+ * [0, positions[b]), its ancestors and itself.
+ * ------------------------------------------------------------------------ */
+#define SWIFTKV_PAGE_TOKENS 64
+#define SWIFTKV_TREE_TOKENS 64
+#define SWIFTKV_PAGED_MAX_SEQ 131072
+typedef struct swiftkv_paged_cache swiftkv_paged_cache;
+/*   pages        of each layer, shared by all sequences: 4 * 64 * kv_heads * head_dim
+ *                bytes a layer
+ *   max_batch    sequences
+ *   heads, kv_heads, head_dim   as for the block cache
+ *   max_seq_len  <= SWIFTKV_PAGED_MAX_SEQ; the capacity is the next multiple of 64
+ *   dtype        SWIFTKV_BF16 or SWIFTKV_F16
+ * Zero-filled; no sequence has a page. */
+int swiftkv_paged_cache_create(swiftkv_context* ctx, int32_t layers, int32_t pages, int32_t max_batch, int32_t heads,
+                               int32_t kv_heads, int32_t head_dim, int32_t max_seq_len, int32_t dtype,
+                               swiftkv_paged_cache** out);
+int swiftkv_paged_cache_destroy(swiftkv_paged_cache* cache);
+/* Device memory of the cache. */
+size_t swiftkv_paged_cache_bytes(const swiftkv_paged_cache* cache);
+
+/* Entries [first, first + n) of the sequence's table, 64 tokens each, name `pages`
+ * (host) in every layer; -1: none.  Several entries may name one page (a prefix that
+ * sequences share); calls that would write a token of such a page are refused
+ * (SWIFTKV_ESTATE), and so are calls whose tokens have no page.  In the order of
+ * the context's stream; not during a capture.  A captured call uses the table as it
+ * is at each replay, without these checks: the table must still give its tokens
+ * pages, and those that it writes to it alone (a row without a page is not written; one
+ * that is read holds some page's values). */
+int swiftkv_paged_map(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t seq, int32_t first, const int32_t* pages,
+                      int32_t n);
+/* Copy page `from` to page `to` in every layer (`to` named by one entry at most): what a
+ * sequence does before it writes to a page that it shares. */
+int swiftkv_paged_copy(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t from, int32_t to);
+
+/* Append n tokens, or trees, to each of the sequences seq0 .. seq0 + batch - 1 of one
+ * layer.  k, v: [batch * n][kv_heads * head_dim]; a negative position skips its
+ * sequence.  Keys are turned by `table` (NULL: not), with the pairs that `halves`
+ * chooses as for swiftkv_rotary: in FP32, rounded once.
+ *   table   rotary_dim <= head_dim; every token's position within it */
+int swiftkv_paged_append(swiftkv_context* ctx, const swiftkv_rotary_table* table, int32_t halves, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, swiftkv_paged_cache* cache,
+                         int32_t layer_index, int32_t seq0, const int32_t* positions, const int32_t* parents,
+                         int32_t batch, int32_t n);
+
+/* Cached tokens [positions[b], positions[b] + n) of layers layer0 .. layer0 + layers - 1
+ * to k and v: device [layers][batch * n][kv_heads * head_dim], dense.  A negative
+ * position leaves its sequence's rows as they are. */
+int swiftkv_paged_values(swiftkv_context* ctx, const swiftkv_paged_cache* cache, int32_t layer0, int32_t layers,
+                         int32_t seq0, const int32_t* positions, int32_t batch, int32_t n, void* k, void* v);
+
+/* Attention of n query tokens, or a tree's, of each sequence.  With k and v (both, or
+ * neither) it first appends their rows as swiftkv_paged_append does; without, the rows
+ * have to be there.  The queries are turned as the keys are and rounded to their type.
+ *   q, out    [batch * n][heads * head_dim], q_stride and out_stride apart; out must not
+ *             overlap the inputs; rows without a token, and of sequences with a negative
+ *             position, are zero
+ *   scale     multiplies q.k; 0 stands for 1 / sqrt(head_dim); its magnitude within
+ *             [2^-100, 2^100]
+ * What a row does not see does not reach it, infinities and NaN included.  Scores,
+ * softmax sums and outputs are held in FP32; a softmax weight is rounded to the element
+ * type (bfloat16: 2^-8 of it, or 2^-16 with at most 16 rows, n times the query heads that
+ * share a key/value head; float16: 2^-11, or 2^-36 of the row's largest where that is
+ * more).  Results do not depend on which workgroup ends first.
+ * swiftkv_set_split_tokens applies. */
+int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* table, int32_t halves, const void* q,
+                            int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            swiftkv_paged_cache* cache, int32_t layer_index, int32_t seq0, const int32_t* positions,
+                            const int32_t* parents, int32_t batch, int32_t n, float scale, void* out,
+                            int64_t out_stride);
+
+/* Keep the accepted path of each sequence's tree: the row of drafted token accepted[b * m +
+ * j] (cached token positions[b] + accepted) moves to cached token positions[b] + j, in
+ * layers layer0 .. layer0 + layers - 1.  accepted: host [batch * m], rising within
+ * [0, SWIFTKV_TREE_TOKENS), each a descendant of the one before (so that its key has been
+ * turned by the position that it gets), then -1; m <= SWIFTKV_TREE_TOKENS.  A negative
+ * position skips its sequence.
+ *   out_positions   NULL, or host [batch]: the number of tokens then cached */
+int swiftkv_paged_keep(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t layer0, int32_t layers, int32_t seq0,
+                       const int32_t* positions, const int32_t* accepted, int32_t batch, int32_t m,
+                       int32_t* out_positions);
+
+/* Testing aid with no counterpart in the reference, host-only: the plan of one attention
+ * launch of batch <= 64 sequences on a device of `cus` compute units: rows of a
+ * workgroup's chunk, chunks of a (sequence, key/value head), splits of the longest
+ * sequence, tokens of a split. */
+int swiftkv_debug_paged_plan(int32_t cus, int32_t split_tokens, int32_t heads, int32_t kv_heads, int32_t n,
+                             const int32_t* positions, int32_t batch, int32_t* out_rows, int32_t* out_chunks,
+                             int32_t* out_splits, int32_t* out_split_tokens);
+
+/* --------------------------------------------------------------------------
  * Device-memory helpers for FFI callers without a GPU framework (ctypes).
  * swiftkv_device_free takes only pointers from swiftkv_device_alloc on the
  * same context (anything else, or a second free: SWIFTKV_EINVAL); it waits
