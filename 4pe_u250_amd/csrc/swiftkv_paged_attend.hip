@@ -99,7 +99,7 @@ __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask
 // themselves; the last to arrive joins all in split order, so the result does not
 // depend on who that is.
 template <typename T, int HD, int R, int RT, typename Tree>
-__global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void paged_attend_kernel(const PagedAttendArgs a,
+__global__ __launch_bounds__(kAttendThreads, R == 16 ? 3 : RT == 1 ? 2 : 1) void paged_attend_kernel(const PagedAttendArgs a,
                                                                                                  const Tree tree) {
     using P = Product<T, R>;
     using Sum = typename P::Sum;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
     constexpr int kPolicy = ROWS < 64 ? 2 : 0;   // nontemporal where a page is read once
     constexpr int kStepBytes = 2 * kStepTokens * HD * 2, kChunks = HD / 8;
     constexpr int CG = HD / 4;                   // quads of output channels
-    __shared__ __align__(16) v4f merge[kWaves * CG * (ROWS + 1)];
+    __shared__ __align__(16) v4f lds[kWaves * CG * (ROWS + 1)];  // queries, then the waves' sums
     __shared__ float stats[kWaves][ROWS][2];
     __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -190,31 +190,36 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
         if (wrote) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the scan's loads find them
     }
 
-    // The rows of this lane: queries as B operands, what they see past all_see.
-    Half8<T> q[RT][NS];
+    // The chunk's queries, turned once for the workgroup and read as B operands.
+    constexpr int kPitch = HD + 8;
+    T* const staged = reinterpret_cast<T*>(lds);
+#pragma unroll
+    for (int it = 0; it < (ROWS * kChunks + kAttendThreads - 1) / kAttendThreads; ++it) {
+        const int item = min(it * kAttendThreads + static_cast<int>(threadIdx.x), ROWS * kChunks - 1), row = item / kChunks, c = item % kChunks;
+        const int r = row_first + min(row, rows - 1), i = row_token(a.group_magic, r);
+        int position = p + i;
+        if constexpr (kTree) position = p + __popcll(from_lane(at_place.mask, i)) - 1;
+        Half8<T> x = turned(static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride + (kh * a.group + r - i * a.group) * HD,
+                            c, a.rotation, angles(a.rotation, max(position, 0)));
+        if (a.negative) x = -x;
+        *reinterpret_cast<Half8<T>*>(staged + row * kPitch + 8 * c) = x;
+    }
+    // What the lane's rows see past all_see.
     uint64_t mask[RT];
     int first[RT];                               // seen_bits' argument
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int row = rt * R + place;
-        const int r = row_first + min(row, rows - 1), i = row_token(a.group_magic, r);
-        int position = p + i;
-        if constexpr (kTree) {
-            mask[rt] = from_lane(at_place.mask, i);
-            first[rt] = p;
-            position = p + __popcll(mask[rt]) - 1;
-        } else {
-            mask[rt] = 0;
-            first[rt] = p + i + 1;
-        }
-        const T* src = static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride + (kh * a.group + r - i * a.group) * HD;
-        const float2* cs = angles(a.rotation, max(position, 0));
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            q[rt][s] = turned(src, s * G + g, a.rotation, cs);
-            if (a.negative) q[rt][s] = -q[rt][s];
-        }
+        const int i = row_token(a.group_magic, row_first + min(rt * R + place, rows - 1));
+        mask[rt] = kTree ? from_lane(at_place.mask, i) : 0;
+        first[rt] = kTree ? p : p + i + 1;
     }
+    __syncthreads();
+    Half8<T> q[RT][NS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+            q[rt][s] = *reinterpret_cast<const Half8<T>*>(staged + (rt * R + place) * kPitch + (s * G + g) * 8);
 
     const int k_lane = R == 16 ? lane * 16 : (((place >> 3) & 1) * 64 + g * 16 + (place >> 4) * 8 + ((place >> 2) & 1) * 4 + (place & 3)) * 16;
     const int v_lane = R == 16 ? lane * 16 : ((place >> 4) * 64 + g * 16 + (place & 15)) * 16;
@@ -230,53 +235,66 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
         for (int i = 0; i < ND; ++i) acc[rt][i] = Sum{};
     }
 
-    // One step; MASKED: rows see different tokens of it.
-    auto scan = [&](auto masked, int step, int page) {
+    // A step's K and V are asked for as soon as the registers of the one before are
+    // free, K during its softmax and V after its products; past the wave's last step
+    // the resource is empty, and nothing is fetched.
+    Half8<T> kb[NL], vb[NL];
+    auto cells_of = [&](int step, int at) {
+        const int page = __builtin_amdgcn_readlane(pages, at);
+        return __builtin_amdgcn_make_buffer_rsrc(step_cells(max(page, 0), step), static_cast<short>(0),
+                                                 step < step_end ? kStepBytes : 0, kBufferWord3);
+    };
+    // (offsets up to 4095 travel in the instruction)
+    auto load = [&](__amdgpu_buffer_rsrc_t cells, int lane_at, int at) {
+        return __builtin_bit_cast(Half8<T>, __builtin_amdgcn_raw_buffer_load_b128(cells, lane_at + (at & 4095), at & ~4095, kPolicy));
+    };
+    auto load_k = [&](__amdgpu_buffer_rsrc_t cells) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) kb[i] = load(cells, k_lane, cell_at(i));
+    };
+    auto load_v = [&](__amdgpu_buffer_rsrc_t cells) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vb[i] = load(cells, v_lane, kStepBytes / 2 + cell_at(i));
+    };
+
+    // One step, and the loads of the next; MASKED: rows see different tokens of it.
+    auto scan = [&](auto masked, int step, __amdgpu_buffer_rsrc_t next) {
         constexpr bool kMasked = decltype(masked)::value;
-        const __amdgpu_buffer_rsrc_t cells = __builtin_amdgcn_make_buffer_rsrc(
-            step_cells(max(page, 0), step), static_cast<short>(0), kStepBytes, kBufferWord3);
-        Half8<T> kb[NL], vb[NL];
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            kb[i] = __builtin_bit_cast(Half8<T>, __builtin_amdgcn_raw_buffer_load_b128(cells, k_lane, cell_at(i), kPolicy));
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            vb[i] = __builtin_bit_cast(Half8<T>, __builtin_amdgcn_raw_buffer_load_b128(cells, v_lane, kStepBytes / 2 + cell_at(i), kPolicy));
-        __builtin_amdgcn_sched_barrier(0);
+        uint32_t bits[RT];
         Half8<T> w[RT][TERMS][NP];
-        Half8<T> sees[RT][NP];                   // 1 where the row sees the token
+        float s[RT][NV];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float s[NV];
             if constexpr (R == 16) {
                 Sum c[2] = {Sum{}, Sum{}};
 #pragma unroll
                 for (int i = 0; i < NL; ++i) c[i & 1] = P::add(kb[i], q[rt][i >> 1], c[i & 1]);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) s[i] = c[i >> 2][i & 3];
+                for (int i = 0; i < NV; ++i) s[rt][i] = c[i >> 2][i & 3];
             } else {
                 Sum c = Sum{};
 #pragma unroll
                 for (int i = 0; i < NL; ++i) c = P::add(kb[i], q[rt][i], c);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) s[i] = c[i];
+                for (int i = 0; i < NV; ++i) s[rt][i] = c[i];
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
             if constexpr (kMasked) {
-                const uint32_t bits = seen_bits(step * kStepTokens, first[rt], mask[rt]);
+                bits[rt] = seen_bits(step * kStepTokens, first[rt], mask[rt]) >> (8 * g);
 #pragma unroll
-                for (int o = 0; o < NP; ++o) {
-                    const uint32_t octet = bits >> (8 * (o * G + g));
+                for (int o = 0; o < NP; ++o)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool sees_it = (octet >> j) & 1u;
-                        if (!sees_it) s[8 * o + j] = -INFINITY;
-                        sees[rt][o][j] = static_cast<T>(sees_it ? 1.0f : 0.0f);
-                    }
-                }
+                    for (int j = 0; j < 8; ++j)
+                        if (!(bits[rt] >> (8 * o * G + j) & 1u)) s[rt][8 * o + j] = -INFINITY;
             }
-            float top = s[0];
+            float top = s[rt][0];
 #pragma unroll
-            for (int i = 1; i < NV; ++i) top = fmaxf(top, s[i]);
+            for (int i = 1; i < NV; ++i) top = fmaxf(top, s[rt][i]);
             top *= a.scale;
             if (__any(top > m[rt] + kSlack)) {
                 top = groups_max<R>(top);
@@ -292,7 +310,7 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
             for (int o = 0; o < NP; ++o)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = fast_exp2(__builtin_fmaf(s[8 * o + j], a.scale, c));
+                    const float x = fast_exp2(__builtin_fmaf(s[rt][8 * o + j], a.scale, c));
                     l[rt] += x;
                     w[rt][0][o][j] = static_cast<T>(x);
                     if constexpr (TERMS == 2) w[rt][TERMS - 1][o][j] = static_cast<T>(x - static_cast<float>(w[rt][0][o][j]));
@@ -301,34 +319,46 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
         if constexpr (kMasked) {
             // 0 times an infinity or a NaN is a NaN, so what is no number leaves V here and
             // reaches the rows that see it by itself: products of ones count such values.
-            typedef uint16_t Bits __attribute__((ext_vector_type(8)));
-            constexpr uint16_t kInf = kHalf ? 0x7c00 : 0x7f80;
-            bool bad = false;
+            typedef uint32_t Pairs __attribute__((ext_vector_type(4)));
+            constexpr uint32_t kInf = kHalf ? 0x7c00 : 0x7f80, kInfs = kInf << 16 | kInf, kOne = kHalf ? 0x3c00 : 0x3f80;
+            uint32_t bad = 0;                    // a half of `rest` is 0 where its exponent is all ones
 #pragma unroll
             for (int i = 0; i < NL; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) bad |= (__builtin_bit_cast(Bits, vb[i])[j] & kInf) == kInf;
-            if (__any(bad)) {
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t rest = ~__builtin_bit_cast(Pairs, vb[i])[j] & kInfs;
+                    bad |= (rest - 0x00010001u) & ~rest & 0x80008000u;
+                }
+            if (__any(bad != 0)) {
 #pragma unroll 1
-                for (int kind = 0; kind < 3; ++kind) {
+                for (int kind = 0; kind < 3; ++kind) {       // NaN, inf, -inf: from `low` on, `span` patterns
                     const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+                    const uint32_t sign = kind == 0 ? 0x7fffu : 0xffffu, low = kind == 0 ? kInf + 1 : kind == 1 ? kInf : kInf | 0x8000u;
+                    const uint32_t span = kind == 0 ? 0x8000u - low : 1u;
+                    auto count_of = [&](uint32_t u) { return ((u & sign) - low) < span ? kOne : 0u; };
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
                         Half8<T> is[NP];
 #pragma unroll
                         for (int o = 0; o < NP; ++o) {
-                            const Bits u = __builtin_bit_cast(Bits, vb[d * NP + o]);
+                            Pairs u = __builtin_bit_cast(Pairs, vb[d * NP + o]);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const bool yes = kind == 0 ? (u[j] & 0x7fff) > kInf : u[j] == (kind == 1 ? kInf : (kInf | 0x8000));
-                                is[o][j] = static_cast<T>(yes ? 1.0f : 0.0f);
-                            }
+                            for (int j = 0; j < 4; ++j) u[j] = count_of(u[j] >> 16) << 16 | count_of(u[j] & 0xffffu);
+                            is[o] = __builtin_bit_cast(Half8<T>, u);
                         }
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) {
                             Sum n = Sum{};
 #pragma unroll
-                            for (int o = 0; o < NP; ++o) n = P::add(is[o], sees[rt][o], n);
+                            for (int o = 0; o < NP; ++o) {
+                                Pairs sees;
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint32_t two = bits[rt] >> (8 * o * G + 2 * j);
+                                    sees[j] = (two & 1u) * kOne | (two & 2u) * (kOne << 15);
+                                }
+                                n = P::add(is[o], __builtin_bit_cast(Half8<T>, sees), n);
+                            }
 #pragma unroll
                             for (int e = 0; e < R * R / 64; ++e) acc[rt][d][e] += n[e] > 0.0f ? value : 0.0f;
                         }
@@ -336,9 +366,12 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
                 }
 #pragma unroll
                 for (int i = 0; i < NL; ++i) {
-                    Bits u = __builtin_bit_cast(Bits, vb[i]);
+                    Pairs u = __builtin_bit_cast(Pairs, vb[i]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = (u[j] & kInf) == kInf ? 0 : u[j];
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t high = u[j] >> 16, lower = u[j] & 0xffffu;
+                        u[j] = ((high & kInf) == kInf ? 0u : high << 16) | ((lower & kInf) == kInf ? 0u : lower);
+                    }
                     vb[i] = __builtin_bit_cast(Half8<T>, u);
                 }
             }
@@ -353,17 +386,28 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
                     for (int t = 0; t < TERMS; ++t) acc[rt][d] = P::add(vb[d * NP + o], w[rt][t][o], acc[rt][d]);
     };
     const int plain_end = min(step_end, all_see / kStepTokens);
-    int step = step_begin + wave;
-    for (int at = 0; step < step_end; step += kWaves, ++at) {
-        if (at == 64) {
-            load_pages(step);
-            at = 0;
-        }
-        const int page = __builtin_amdgcn_readlane(pages, at);
-        if (step < plain_end) scan(std::false_type{}, step, page);
-        else scan(std::true_type{}, step, page);
+    int step = step_begin + wave, at = 0;
+    if (step < step_end) {
+        const __amdgpu_buffer_rsrc_t cells = cells_of(step, 0);
+        load_k(cells);
+        load_v(cells);
     }
+    auto run = [&](auto masked, int end) {
+        for (; step < end; step += kWaves) {
+            if (++at == 64) {
+                load_pages(step + kWaves);
+                at = 0;
+            }
+            const __amdgpu_buffer_rsrc_t next = cells_of(step + kWaves, at);
+            scan(masked, step, next);
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(next);
+        }
+    };
+    run(std::false_type{}, plain_end);
+    run(std::true_type{}, step_end);
 
+    __syncthreads();                             // everyone has its queries
     // The waves' sums meet in LDS, quads of channels of a row together.
     const int row_of = place;
 #pragma unroll
@@ -378,7 +422,7 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
 #pragma unroll
             for (int e = 0; e < R * R / 256; ++e) {
                 const int quad = d * (R / 4) + e * G + g;
-                merge[(wave * CG + quad) * (ROWS + 1) + rt * R + row_of] =
+                lds[(wave * CG + quad) * (ROWS + 1) + rt * R + row_of] =
                     v4f{acc[rt][d][4 * e], acc[rt][d][4 * e + 1], acc[rt][d][4 * e + 2], acc[rt][d][4 * e + 3]};
             }
     }
@@ -413,7 +457,7 @@ __global__ __launch_bounds__(kAttendThreads, R == 16 ? 4 : RT == 1 ? 2 : 1) void
         for (int w = 0; w < kWaves; ++w) {
             const float f = fast_exp2(stats[w][row][0] - safe);
             l_all += stats[w][row][1] * f;
-            o += merge[(w * CG + quad) * (ROWS + 1) + row] * f;
+            o += lds[(w * CG + quad) * (ROWS + 1) + row] * f;
         }
         if (my_splits == 1) {
             finish(row, quad, l_all, o);
