@@ -120,7 +120,7 @@ struct PagedMapArgs {
 };
 
 // Rows of an attention workgroup's chunk.
-constexpr int kSplitQuantumSteps = 8;
+constexpr int kSplitQuantumSteps = 4;
 
 hipError_t launch_paged_map(const PagedMapArgs& a, hipStream_t s);
 // tree null: chains
@@ -128,7 +128,11 @@ hipError_t launch_paged_append(const PagedRowsArgs& a, const PagedTree* tree, in
 hipError_t launch_paged_values(const PagedRowsArgs& a, int layers, int batch, hipStream_t s);
 hipError_t launch_paged_keep(const PagedKeepArgs& a, int layers, int batch, hipStream_t s);
 hipError_t launch_paged_copy(const PagedView& v, int64_t from, int64_t to, hipStream_t s);
-// rows: of a chunk, 16, 32 or 64
+// rows: of a chunk, 16 or 32 (a.chunks == 1)
 hipError_t launch_paged_attend(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);
+// rows: 64, 128 or 256; a.k null
+hipError_t launch_paged_many(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);
+// The splits of such calls, of more than 16 rows
+hipError_t launch_paged_join(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);
 
 }  // namespace swiftkv

@@ -1,0 +1,399 @@
+// swiftkv_paged_attend_device.hpp -- what the paged attention's kernels share: the
+// products on 16-bit matrix instructions, the softmax of one step of 32 cached
+// tokens, a workgroup's share of a call, and how partial results are joined.
+#pragma once
+
+#include "swiftkv_paged_device.hpp"
+
+namespace swiftkv {
+namespace dev {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// D[R][R] += A B.  Lane = (group g, place m): A has row m and contraction places
+// 8 g .., B column m and the same places; D column m, rows 4 g .. of every
+// 4 * 64 / R.
+template <typename T, int R>
+struct Product;
+template <>
+struct Product<__bf16, 16> {
+    using Sum = v4f;
+    static __device__ __forceinline__ Sum add(Half8<__bf16> a, Half8<__bf16> b, Sum c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Product<_Float16, 16> {
+    using Sum = v4f;
+    static __device__ __forceinline__ Sum add(Half8<_Float16> a, Half8<_Float16> b, Sum c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Product<__bf16, 32> {
+    using Sum = v16f;
+    static __device__ __forceinline__ Sum add(Half8<__bf16> a, Half8<__bf16> b, Sum c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Product<_Float16, 32> {
+    using Sum = v16f;
+    static __device__ __forceinline__ Sum add(Half8<_Float16> a, Half8<_Float16> b, Sum c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ int row_token(uint32_t group_magic, int r) {
+    return group_magic == 0 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), group_magic));
+}
+
+// The bits of tokens tok0 .. tok0 + 31 that a row sees: all before `first`, and
+// those of `mask` from there on.
+__device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask) {
+    const int d = tok0 - first;
+    if (d >= 0) return d < 64 ? static_cast<uint32_t>(mask >> d) : 0u;
+    if (d <= -kStepTokens) return ~0u;
+    return ((1u << -d) - 1u) | static_cast<uint32_t>(mask << -d);
+}
+
+// R rows of a wave: their queries as B operands, and softmax(scale q k^T) v over the
+// steps that the wave takes, 32 cached tokens each:
+//
+//   scores  S^T[token][row] = K Q^T: a lane ends with one row and, of the step's
+//           four octets of tokens, whole ones;
+//   output  O^T[channel][row] = V^T P^T, with P straight from those registers,
+//           rounded to the cache's type.
+//
+// Both A operands are the cache's cells as they lie (swiftkv_paged.hpp).  Nothing
+// moves between lanes but, now and then, a row's maximum: the reference value that
+// weights are taken over follows it only when a score is more than 2^kSlack above,
+// with p <= 2^kSlack until then.  (That branch is marked unlikely, which also keeps
+// the sums' registers where the products want them.)
+//
+// 16 rows leave the matrix instructions idle, so a bfloat16 weight is two terms there
+// (2^-16 of it); with more rows it is one, 2^-8.  A float16 weight is 2^(kShift +
+// kSlack) at most and is good to 2^-11, or to 2^-36 of the row's largest.
+template <typename T, int HD, int R>
+struct RowTile {
+    using P = Product<T, R>;
+    using Sum = typename P::Sum;
+    static constexpr bool kHalf = std::is_same<T, _Float16>::value;
+    static constexpr int G = 64 / R;             // lane groups
+    static constexpr int NV = kStepTokens / G;   // scores of a lane
+    static constexpr int NP = NV / 8;            // octets of a lane
+    static constexpr int NL = HD / 16;           // operands of K, and of V, a step
+    static constexpr int NS = HD / (8 * G);      // products of a score
+    static constexpr int ND = HD / R;            // output tiles
+    static constexpr int NE = R * R / 64;        // sums of a lane in one
+    static constexpr int TERMS = R == 16 && !kHalf ? 2 : 1;
+    static constexpr float kSlack = 4.0f, kShift = kHalf ? 11.0f : 0.0f;
+    typedef uint32_t Pairs __attribute__((ext_vector_type(4)));
+
+    Half8<T> q[NS];
+    Sum acc[ND];
+    float m, l;
+    uint64_t mask;
+    int first;                                   // what the row sees: seen_bits' arguments
+
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[i] = Sum{};
+    }
+
+    __device__ __forceinline__ void scores(const Half8<T> (&kb)[NL], float (&s)[NV]) const {
+        if constexpr (R == 16) {
+            Sum c[2] = {Sum{}, Sum{}};
+#pragma unroll
+            for (int i = 0; i < NL; ++i) c[i & 1] = P::add(kb[i], q[i >> 1], c[i & 1]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) s[i] = c[i >> 2][i & 3];
+        } else {
+            Sum c = Sum{};
+#pragma unroll
+            for (int i = 0; i < NL; ++i) c = P::add(kb[i], q[i], c);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) s[i] = c[i];
+        }
+    }
+
+    // The lane's part of what the row sees of the step: its octet o at bit 8 o G.
+    __device__ __forceinline__ uint32_t seen(int step, int g) const { return seen_bits(step * kStepTokens, first, mask) >> (8 * g); }
+    static __device__ __forceinline__ void hide(uint32_t bits, float (&s)[NV]) {
+#pragma unroll
+        for (int o = 0; o < NP; ++o)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(bits >> (8 * o * G + j) & 1u)) s[8 * o + j] = -INFINITY;
+    }
+
+    static __device__ __forceinline__ float groups_max(float x) {
+        if (R == 16) x = fmaxf(x, __shfl_xor(x, 16));
+        return fmaxf(x, __shfl_xor(x, 32));
+    }
+    static __device__ __forceinline__ float groups_sum(float x) {
+        if (R == 16) x += __shfl_xor(x, 16);
+        return x + __shfl_xor(x, 32);
+    }
+
+    // The reference value follows scores that are far above it.
+    __device__ __forceinline__ void rise(const float (&s)[NV], float scale) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) top = fmaxf(top, s[i]);
+        top *= scale;
+        if (__builtin_expect(__any(top > m + kSlack), 0)) {
+            top = groups_max(top);
+            const float next = top > m + kSlack ? top : m;
+            const float fall = next == -INFINITY ? 1.0f : fast_exp2(m - next);
+            m = next;
+            l *= fall;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= fall;
+        }
+    }
+    // Scores to weights, as B operands.
+    __device__ __forceinline__ void weights(const float (&s)[NV], float scale, Half8<T> (&w)[TERMS][NP]) {
+        const float c = kShift - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int o = 0; o < NP; ++o) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = fast_exp2(__builtin_fmaf(s[8 * o + j], scale, c));
+                w[0][o][j] = static_cast<T>(x[j]);
+                if constexpr (TERMS == 2) w[TERMS - 1][o][j] = static_cast<T>(x[j] - static_cast<float>(w[0][o][j]));
+            }
+            l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        }
+    }
+
+    static constexpr uint32_t kInf = kHalf ? 0x7c00 : 0x7f80, kOne = kHalf ? 0x3c00 : 0x3f80;
+    // Not zero where one of a cell's values is no number: a half of `rest` is 0 where its
+    // exponent is all ones.
+    static __device__ __forceinline__ uint32_t no_numbers(Pairs cell) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t rest = ~cell[j] & (kInf << 16 | kInf);
+            bad |= (rest - 0x00010001u) & ~rest & 0x80008000u;
+        }
+        return bad;
+    }
+    static __device__ __forceinline__ bool no_numbers(const Half8<T> (&vb)[NL]) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) bad |= no_numbers(__builtin_bit_cast(Pairs, vb[i]));
+        return __any(bad != 0);
+    }
+
+    // 0 times an infinity or a NaN is a NaN, so where rows see different tokens, what is
+    // no number leaves V and reaches the rows that see it by itself: products of ones
+    // count such values.
+    __device__ __forceinline__ void part_with_no_numbers(Half8<T> (&vb)[NL], uint32_t bits) {
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {   // NaN, inf, -inf: from `low` on, `span` patterns
+            const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+            const uint32_t sign = kind == 0 ? 0x7fffu : 0xffffu, low = kind == 0 ? kInf + 1 : kind == 1 ? kInf : kInf | 0x8000u;
+            const uint32_t span = kind == 0 ? 0x8000u - low : 1u;
+            auto count_of = [&](uint32_t u) { return ((u & sign) - low) < span ? kOne : 0u; };
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                Sum n = Sum{};
+#pragma unroll
+                for (int o = 0; o < NP; ++o) {
+                    Pairs u = __builtin_bit_cast(Pairs, vb[d * NP + o]), sees;
+                    asm volatile("" : "+v"(u), "+v"(bits));      // nothing of this is worth a register outside the loop
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u[j] = count_of(u[j] >> 16) << 16 | count_of(u[j] & 0xffffu);
+                        const uint32_t two = bits >> (8 * o * G + 2 * j);
+                        sees[j] = (two & 1u) * kOne | (two & 2u) * (kOne << 15);
+                    }
+                    n = P::add(__builtin_bit_cast(Half8<T>, u), __builtin_bit_cast(Half8<T>, sees), n);
+                }
+#pragma unroll
+                for (int e = 0; e < NE; ++e) acc[d][e] += n[e] > 0.0f ? value : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            Pairs u = __builtin_bit_cast(Pairs, vb[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t high = u[j] >> 16, lower = u[j] & 0xffffu;
+                u[j] = ((high & kInf) == kInf ? 0u : high << 16) | ((lower & kInf) == kInf ? 0u : lower);
+            }
+            vb[i] = __builtin_bit_cast(Half8<T>, u);
+        }
+    }
+
+    __device__ __forceinline__ void add(const Half8<T> (&vb)[NL], const Half8<T> (&w)[TERMS][NP]) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int o = 0; o < NP; ++o)
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) acc[d] = P::add(vb[d * NP + o], w[t][o], acc[d]);
+    }
+
+    // The sums as quads of channels: quads[quad * pitch + row].
+    __device__ __forceinline__ void leave(v4f* quads, int pitch, int row, int g) const {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < NE / 4; ++e)
+                quads[(d * (R / 4) + e * G + g) * pitch + row] = v4f{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+    }
+};
+
+// A workgroup's share of a call: ROWS rows of a chunk, the steps of a split.
+template <int ROWS, typename Tree>
+struct Share {
+    static constexpr bool kTree = std::is_same<Tree, PagedTree>::value;
+    int b, kh, split, chunk;
+    int row_first, rows;
+    int p, count;                                // cached tokens before the call (negative: none), tokens of the call
+    int my_splits, step_begin, step_end;
+    int plain_end;                               // up to here every row sees whole steps
+    TreePlace place;
+    uint64_t live;                               // tokens of the tree
+
+    // `id`: the workgroup's (split, chunk, head), heads fastest, so that a head's workgroups
+    // share an XCD's L2.
+    __device__ __forceinline__ void start(const PagedAttendArgs& a, const Tree& tree, int id, int lane) {
+        b = a.order[blockIdx.y];
+        kh = id % a.view.kv_heads;
+        id /= a.view.kv_heads;
+        split = id % a.splits;
+        chunk = a.chunks - 1 - id / a.splits;    // the longest first
+        row_first = chunk * ROWS;
+        rows = min(ROWS, a.group * a.n - row_first);
+        p = a.positions[b];
+        count = a.n;
+        live = 0;
+        if constexpr (kTree) {
+            place = tree_place(tree.parents + b * a.n, a.n, lane);
+            live = __ballot(place.live);
+            count = __popcll(live);
+        }
+        // Tokens that some row sees, and those that all do.
+        int most = 0, all_see = 0;
+        if (p >= 0) {
+            most = kTree ? p + count : p + row_token(a.group_magic, row_first + rows - 1) + 1;
+            all_see = kTree ? p : p + row_token(a.group_magic, row_first) + 1;
+        }
+        const int steps = (most + kStepTokens - 1) / kStepTokens;
+        my_splits = max(1, (steps + a.split_steps - 1) / a.split_steps);
+        const int per = split_length(steps, my_splits);
+        step_begin = split * per;
+        step_end = min(steps, step_begin + per);
+        plain_end = min(step_end, all_see / kStepTokens);
+    }
+    // The query token of a row, clamped to the chunk's.
+    __device__ __forceinline__ int token(const PagedAttendArgs& a, int row) const {
+        return row_token(a.group_magic, row_first + min(row, rows - 1));
+    }
+    __device__ __forceinline__ int position(int i) const {
+        if constexpr (kTree) return p + __popcll(from_lane(place.mask, i)) - 1;
+        else return p + i;
+    }
+    template <typename Tile>
+    __device__ __forceinline__ void sees(const PagedAttendArgs& a, Tile& tile, int row) const {
+        const int i = token(a, row);
+        tile.mask = kTree ? from_lane(place.mask, i) : 0;
+        tile.first = kTree ? p : p + i + 1;
+    }
+    // All rows' queries, turned, to LDS with a pitch of HD + 8.
+    template <typename T, int HD, int THREADS>
+    __device__ __forceinline__ void stage_queries(const PagedAttendArgs& a, T* staged) const {
+        constexpr int kChunks = HD / 8;
+#pragma unroll
+        for (int it = 0; it < (ROWS * kChunks + THREADS - 1) / THREADS; ++it) {
+            const int item = min(it * THREADS + static_cast<int>(threadIdx.x), ROWS * kChunks - 1), row = item / kChunks, c = item % kChunks;
+            const int r = row_first + min(row, rows - 1), i = row_token(a.group_magic, r);
+            Half8<T> x = turned(static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride + (kh * a.group + r - i * a.group) * HD,
+                                c, a.rotation, angles(a.rotation, max(position(i), 0)));
+            if (a.negative) x = -x;
+            *reinterpret_cast<Half8<T>*>(staged + row * (HD + 8) + 8 * c) = x;
+        }
+    }
+    // The call's rows that fall into steps of the split -- of every WAVES-th step, the
+    // wave-th -- to the cache, by THREADS threads; whether there were any.
+    template <typename T, int HD, int THREADS>
+    __device__ __forceinline__ bool append(const PagedAttendArgs& a, const int32_t* table, uint8_t* layer_head, int64_t page_bytes, int thread,
+                                           int waves, int wave) const {
+        constexpr int kChunks = HD / 8;
+        if (p < 0) return false;
+        const int last = min(step_end, (p + count - 1) / kStepTokens + 1);
+        int step = max(step_begin, p / kStepTokens);
+        step += (wave - (step - step_begin)) & (waves - 1);
+        bool wrote = false;
+        for (; step < last; step += waves) {
+            const int page = table[step / kPageSteps];
+            const int t0 = max(p, step * kStepTokens), t1 = min(p + count, (step + 1) * kStepTokens);
+            if (page < 0) continue;
+            uint8_t* const cells = layer_head + page * page_bytes + (step % kPageSteps) * paged_step_bytes(HD);
+            const int items = (t1 - t0) * kChunks;
+            for (int base = 0; base < items; base += THREADS) {
+                const int item = min(base + thread, items - 1), tok = t0 + item / kChunks, c = item % kChunks, i = tok - p;
+                const int64_t at = static_cast<int64_t>(b) * a.n + i;
+                const Half8<T> kk = turned(static_cast<const T*>(a.k) + at * a.k_stride + kh * HD, c, a.rotation, angles(a.rotation, position(i)));
+                const Half8<T> vv = *reinterpret_cast<const Half8<T>*>(static_cast<const T*>(a.v) + at * a.v_stride + kh * HD + 8 * c);
+                const int t = tok % kStepTokens;
+                *reinterpret_cast<Half8<T>*>(cells + k_cell(t, c)) = kk;
+                T* const dst = reinterpret_cast<T*>(cells + v_cell(t / 8, 8 * c, HD)) + t % 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dst[8 * j] = vv[j];
+            }
+            wrote = true;
+        }
+        return wrote;
+    }
+    // A row's values, sums over the sum of weights: zero for rows without a token.
+    template <typename T, int HD>
+    __device__ __forceinline__ void finish(const PagedAttendArgs& a, int row, int quad, float l, v4f o) const {
+        if (row >= rows) return;
+        const int r = row_first + row, i = row_token(a.group_magic, r);
+        bool is_live = p >= 0;
+        if constexpr (kTree) is_live &= (live >> i & 1) != 0;
+        struct alignas(sizeof(T) * 4) Four { T v[4]; } t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t.v[e] = static_cast<T>(is_live ? o[e] / l : 0.0f);
+        *reinterpret_cast<Four*>(static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.n + i) * a.out_stride +
+                                 (kh * a.group + r - i * a.group) * HD + 4 * quad) = t;
+    }
+    // Where split j leaves (m, l) of a row, and a row's quads behind them.
+    template <int HD>
+    __device__ __forceinline__ float* partial(const PagedAttendArgs& a, int j) const {
+        return a.partials + (((static_cast<int64_t>(b) * a.view.kv_heads + kh) * a.chunks + chunk) * a.splits + j) * (ROWS * (HD + 2));
+    }
+};
+
+// Partial results (m, l, sums) joined one after another.
+struct Joined {
+    float m = -INFINITY, l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    // N of them at once.
+    template <int N>
+    __device__ __forceinline__ void add(const v2f (&ml)[N], const v4f (&sums)[N]) {
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = fmaxf(top, ml[j][0]);
+        const float safe = top == -INFINITY ? 0.0f : top, f0 = fast_exp2(m - safe);
+        l *= f0;
+        o *= f0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float f = fast_exp2(ml[j][0] - safe);
+            l += ml[j][1] * f;
+            o += sums[j] * f;
+        }
+        m = top;
+    }
+};
+
+// The page of `step` and on it its cells as a resource; past `end` an empty one, from
+// which nothing is fetched.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_resource(uint8_t* layer_head, int64_t page_bytes, int page, int step, int end,
+                                                                int step_bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(layer_head + max(page, 0) * page_bytes + (step % kPageSteps) * step_bytes,
+                                             static_cast<short>(0), step < end ? step_bytes : 0, kBufferWord3);
+}
+
+}  // namespace dev
+}  // namespace swiftkv

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <cstdlib>
 #include <new>
 
 #include "swiftkv_paged.hpp"
@@ -140,7 +141,8 @@ PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t group, int32
                          const int32_t* positions, int32_t batch) {
     PagedPlan p{};
     const int64_t rows = static_cast<int64_t>(group) * n;
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    if (getenv("PROWS") && p.rows > 32) p.rows = atoi(getenv("PROWS"));
     p.chunks = static_cast<int32_t>((rows + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.chunks;
     int64_t longest = 0, total = 0;
@@ -161,7 +163,7 @@ PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t group, int32
     per = (per + kSplitQuantumSteps - 1) / kSplitQuantumSteps * kSplitQuantumSteps;
     p.split_steps = static_cast<int32_t>(per);
     p.splits = static_cast<int32_t>((longest + per - 1) / per);
-    p.appends = p.chunks == 1;
+    p.appends = n <= kTreeTokens;
     return p;
 }
 
@@ -413,7 +415,11 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
                 return a.positions[x] != a.positions[y] ? a.positions[x] > a.positions[y] : x < y;
             });
         PagedTree tree;
-        SKV_HIP(launch_paged_attend(a, tree_of(tree, parents, b0, nb, n), nb, plan.rows, cache->type, ctx->stream));
+        const PagedTree* const trees = tree_of(tree, parents, b0, nb, n);
+        SKV_HIP(plan.rows <= (getenv("PD64") ? 64 : 32) ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)
+                                : launch_paged_many(a, trees, nb, plan.rows, cache->type, ctx->stream));
+        if (plan.splits > 1 && plan.rows > 16)
+            SKV_HIP(launch_paged_join(a, trees, nb, plan.rows, cache->type, ctx->stream));
     }
     return ok();
 }

@@ -42,57 +42,51 @@ __device__ __forceinline__ TreePlace tree_place(const uint8_t* parents, int n, i
     return t;
 }
 
-// A pair (a, b) turned by (cos, sin), in FP32 and one order of operations in every
-// kernel, so that a key's row does not depend on which of them appends it.  (The
-// empty asm keeps the compiler from one instruction that multiplies, adds and rounds
-// to float16 at once, which it took in some places.)
-__device__ __forceinline__ float in_fp32(float x) {
-    asm("" : "+v"(x));
-    return x;
+// x cos -+ y sin, in FP32 and one order of operations in every kernel, so that a
+// key's row does not depend on which of them appends it.  (The empty asm keeps the
+// compiler from one instruction that multiplies, adds and rounds to float16 at once,
+// which it took in some places.)
+__device__ __forceinline__ float turn(float x, float y, float c, float s, bool second) {
+    float z = __builtin_fmaf(x, c, second ? y * s : -(y * s));
+    asm("" : "+v"(z));
+    return z;
 }
-__device__ __forceinline__ float turn_first(float a, float b, float2 f) { return in_fp32(__builtin_fmaf(a, f.x, -(b * f.y))); }
-__device__ __forceinline__ float turn_second(float a, float b, float2 f) { return in_fp32(__builtin_fmaf(a, f.y, b * f.x)); }
 
-// 8 channels, 8 * chunk .., of a head's row turned by the angles of `cs`, rounded
-// once.  Both pairings; a pair's other half is read from the row again.
+// 8 channels, 8 * chunk .., of a head's row turned by the angles `cs` (of its
+// position), rounded once.  A channel's partner is its neighbour, or `halves` a channel
+// half the rotary channels away, which is read from the row again.  Small code: a
+// workgroup runs it once, and fetches it for that.
 template <typename T>
 __device__ __forceinline__ Half8<T> turned(const T* row, int chunk, const PagedRotation& r, const float2* cs) {
-    const Half8<T> own = *reinterpret_cast<const Half8<T>*>(row + 8 * chunk);
-    if (r.table == nullptr) return own;
     const int half = r.rotary_dim / 2, c0 = 8 * chunk;
-    Half8<T> out = own;
-    if (!r.halves) {
+    const Half8<T> own = *reinterpret_cast<const Half8<T>*>(row + c0);
+    if (c0 >= r.rotary_dim) return own;
+    if (r.halves ? (half & 7) != 0 : (r.rotary_dim & 7) != 0) {
+        Half8<T> out = own;
+#pragma unroll 1
+        for (int c = c0; c < min(c0 + 8, r.rotary_dim); ++c) {
+            const bool second = r.halves ? c >= half : c & 1;
+            const int other = r.halves ? (second ? c - half : c + half) : c ^ 1, j = r.halves ? (second ? c - half : c) : c >> 1;
+            const T z = static_cast<T>(turn(static_cast<float>(row[c]), static_cast<float>(row[other]), cs[j].x, cs[j].y, second));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool turns = c0 + 2 * i < r.rotary_dim;
-            const float2 f = cs[turns ? 4 * chunk + i : 0];
-            const float a = static_cast<float>(own[2 * i]), b = static_cast<float>(own[2 * i + 1]);
-            if (turns) {
-                out[2 * i] = static_cast<T>(turn_first(a, b, f));
-                out[2 * i + 1] = static_cast<T>(turn_second(a, b, f));
-            }
+            for (int k = 0; k < 8; ++k)
+                if (c - c0 == k) out[k] = z;
         }
-    } else if ((half & 7) == 0) {
-        const bool turns = c0 < r.rotary_dim, second = c0 >= half;
-        const int other = !turns ? c0 : second ? c0 - half : c0 + half, j = !turns ? 0 : second ? c0 - half : c0;
-        const Half8<T> pair = *reinterpret_cast<const Half8<T>*>(row + other);
+        return out;
+    }
+    const bool upper = r.halves && c0 >= half;
+    const Half8<T> other = *reinterpret_cast<const Half8<T>*>(row + (r.halves ? (upper ? c0 - half : c0 + half) : c0));
+    const v4f* const angle = reinterpret_cast<const v4f*>(cs + (r.halves ? (upper ? c0 - half : c0) : c0 / 2));
+    v4f f[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 f = cs[j + i];
-            const float x = static_cast<float>(own[i]), y = static_cast<float>(pair[i]);
-            const float z = second ? turn_second(y, x, f) : turn_first(x, y, f);
-            if (turns) out[i] = static_cast<T>(z);
-        }
-    } else {
+    for (int i = 0; i < 4; ++i) f[i] = angle[r.halves ? i : i & 1];
+    Half8<T> out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = c0 + i;
-            if (c >= r.rotary_dim) continue;
-            const bool second = c >= half;
-            const float2 f = cs[second ? c - half : c];
-            const float x = static_cast<float>(own[i]), y = static_cast<float>(row[second ? c - half : c + half]);
-            out[i] = static_cast<T>(second ? turn_second(y, x, f) : turn_first(x, y, f));
-        }
+    for (int j = 0; j < 8; ++j) {
+        const float c = r.halves ? f[j >> 1][2 * (j & 1)] : f[j >> 2][2 * (j >> 1 & 1)];
+        const float s = r.halves ? f[j >> 1][2 * (j & 1) + 1] : f[j >> 2][2 * (j >> 1 & 1) + 1];
+        const float y = static_cast<float>(r.halves ? other[j] : own[j ^ 1]);
+        out[j] = static_cast<T>(turn(static_cast<float>(own[j]), y, c, s, r.halves ? upper : j & 1));
     }
     return out;
 }

@@ -33,8 +33,8 @@ def places(parents):
 
 
 class Rotation:
-    """The device's rotation: cos and sin computed in 64 bits and kept as FP32; a c - b s and a s + b c as one product
-    rounded to FP32 and a fused multiply-add, then one rounding to the type."""
+    """The device's rotation: cos and sin computed in 64 bits and kept as FP32; a c - b s and b c + a s, the sine's product
+    rounded to FP32 and then a fused multiply-add, then one rounding to the type."""
 
     def __init__(self, rotary_dim, positions=4096, theta=10000.0, halves=True):
         self.dim, self.positions, self.theta, self.halves = rotary_dim, positions, theta, halves
@@ -55,7 +55,7 @@ class Rotation:
         single = lambda v: v.astype(np.float32).astype(np.float64)
         with np.errstate(all="ignore"):
             y[..., i] = R.typed(single(a * c - single(b * s)), t)[1]
-            y[..., j] = R.typed(single(a * s + single(b * c)), t)[1]
+            y[..., j] = R.typed(single(b * c + single(a * s)), t)[1]
         return y
 
 

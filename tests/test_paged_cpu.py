@@ -82,7 +82,7 @@ def test_plan_stays_within_the_workspace(skv, heads, kv, n, batch, split):
         at = [longest] + [int(x) for x in rng.integers(-1, longest + 1, batch - 1)]
         rows, chunks, splits, tokens = skv.paged_plan(heads, kv, n, at, split_tokens=split)
         assert rows * chunks >= n * (heads // kv) > rows * (chunks - 1)
-        assert tokens % 256 == 0 and splits * tokens >= longest + n > (splits - 1) * tokens
+        assert tokens % 128 == 0 and splits * tokens >= longest + n > (splits - 1) * tokens
         if splits > 1:
             assert batch * kv * chunks * splits <= 2048
             assert batch * kv * chunks * splits * rows <= 65536
