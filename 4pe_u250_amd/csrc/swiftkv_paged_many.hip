@@ -14,19 +14,21 @@ constexpr int kManyWaves = 8;
 // TEAMS = 8 / RW such teams take steps of the split in turn.  Vector instructions and
 // matrix products bound it, so a step's cells come from memory once for all rows of a
 // team (as operands straight from memory they are bound by what a CU's loads deliver,
-// 64 bytes a clock), through registers into LDS, in the order in which the lanes of the
+// 64 bytes a clock), straight into LDS, in the order in which the lanes of the
 // 32x32x16 form read them.  A turn, one step of each team, forms the scores of the next
-// step while it forms the weights of this one, so K lies one turn ahead of V, each in
-// two slots: what a turn reads nobody writes in it, and one barrier ends it.
+// step while it forms the weights of this one, so K lies one turn ahead of V.  Each has
+// SLOTS slots: a turn asks for cells SLOTS - 1 turns ahead, into the slots that nobody
+// reads in it, waits for those that it asked for SLOTS - 2 turns before, and ends with a
+// barrier.
 template <int HD, int RW>
 struct ManyShape {
     static constexpr int TEAMS = kManyWaves / RW, ROWS = 32 * RW;
     static constexpr int kHalfBytes = kStepTokens * HD * 2;  // K or V of a step
-    static constexpr int kRing = 4 * TEAMS * kHalfBytes;
+    static constexpr int SLOTS = TEAMS < 4 || HD == 64 ? 3 : 2;
+    static constexpr int kRing = 2 * SLOTS * TEAMS * kHalfBytes;
     static constexpr int kMerge = TEAMS * (HD / 4) * (ROWS + 1) * 16;
     static constexpr int kQueries = ROWS * (HD + 8) * 2;
-    static constexpr int kMost = kRing > kMerge ? kRing : kMerge;
-    static constexpr int kBytes = kMost > kQueries ? kMost : kQueries;
+    static constexpr int kBytes = kRing + kQueries > kMerge ? kRing + kQueries : kMerge;
 };
 
 template <typename T, int HD, int RW, typename Tree>
@@ -35,12 +37,10 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     using Tile = RowTile<T, HD, 32>;
     constexpr int TEAMS = M::TEAMS, ROWS = M::ROWS, kHalfBytes = M::kHalfBytes, kStepBytes = 2 * kHalfBytes;
     constexpr int NL = Tile::NL, CG = HD / 4, kPitch = HD + 8;
-    constexpr int kCells = HD * 4;               // of K, and of V, in a step
-    constexpr int NH = TEAMS * 2 * kCells / kManyThreads;    // a thread's cells of a turn
-    static_assert(NH >= 1 && kCells % 64 == 0, "a wave's cells are of one step");
+    constexpr int SLOTS = M::SLOTS, NH = TEAMS * 2 * NL / kManyWaves;    // a wave's loads of a turn
+    static_assert(NH >= 1 && TEAMS * 2 * NL % kManyWaves == 0, "a turn's loads are shared evenly");
     __shared__ __align__(16) uint8_t lds[M::kBytes];
     __shared__ float stats[TEAMS][ROWS][2];
-    __shared__ int no_numbers[2][TEAMS];         // of a V slot: 1 + the step whose values are not all numbers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane / 32, place = lane % 32, row = wave % RW * 32 + place, team = wave / RW;
     Share<ROWS, Tree> share;
@@ -62,48 +62,32 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
         __syncthreads();
     }
 
-    // Cell i * kManyThreads + thread of a turn: first the teams' K cells, then their V
-    // cells.  A K cell [c][h][g'][m] is read by product 2 c + (g' >> 1)'s lane (g' & 1, 16 (m >> 3) +
-    // 8 h + (m & 7)), a V cell [c][g'][m] by product (c >> 1, g' >> 1)'s lane (g' & 1, 16 (c & 1) + m).
-    const int first_cell = wave * 64;            // of the wave, in a turn's first kManyThreads
-    auto cell_of = [&](int i) { return i * kManyThreads + first_cell; };
-    auto reader = [&](int cell, bool is_v) {
-        const int m = cell & 15, gg = (cell >> 4) & 3, c = is_v ? cell >> 6 : cell >> 7, h = (cell >> 6) & 1;
-        const int product = (is_v ? c >> 1 : c) * 2 + (gg >> 1);
-        return product * 1024 + ((gg & 1) * 32 + (is_v ? (c & 1) * 16 + m : (m >> 3) * 16 + h * 8 + (m & 7))) * 16;
-    };
-    // K of turn `k_step`, V of turn `v_step` (first steps of their turns).
-    auto load_turn = [&](v4i (&held)[NH], int k_step, int v_step) {
+    // A wave's loads of a turn: NH of its 1 KiB blocks, first the teams' K, then their V.
+    // Product x of K reads, with lane (g', 16 m' + 8 h + m''), cell [x / 2][h][2 (x & 1) + g'][8 m' + m''];
+    // product (c / 2, x & 1) of V, with lane (g', 16 (c & 1) + m), cell [c][2 (x & 1) + g'][m].
+    const int k_lane = (((place >> 3) & 1) * 64 + g * 16 + (place >> 4) * 8 + (place & 7)) * 16;
+    const int v_lane = ((place >> 4) * 64 + g * 16 + (place & 15)) * 16;
+    auto load_turn = [&](int k_step, int v_step, int k_slot, int v_slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NH; ++i) {
-            const bool is_v = cell_of(i) >= TEAMS * kCells;
-            const int in_kind = cell_of(i) - (is_v ? TEAMS * kCells : 0), step = (is_v ? v_step : k_step) + in_kind / kCells;
-            const int at = step - window;        // below 128: the window follows K
+            const int block = i * kManyWaves + wave, of_kind = block % (TEAMS * NL), of_step = of_kind % NL;
+            const bool is_v = block >= TEAMS * NL;
+            const int step = (is_v ? v_step : k_step) + of_kind / NL, at = step - window;    // below 128: the window follows K
             const int page = at < 64 ? __builtin_amdgcn_readlane(pages, max(at, 0)) : __builtin_amdgcn_readlane(pages_next, min(at - 64, 63));
-            held[i] = __builtin_amdgcn_raw_buffer_load_b128(step_resource(layer_head, page_bytes, page, step, step_end, kStepBytes), lane * 16,
-                                                            (is_v ? kHalfBytes : 0) + in_kind % kCells * 16, 0);
-        }
-    };
-    // CHECK: of V cells (turn v_step) that a turn of the tail reads.
-    auto store_turn = [&](auto check, const v4i (&held)[NH], int k_slot, int v_slot, int v_step) {
-#pragma unroll
-        for (int i = 0; i < NH; ++i) {
-            const bool is_v = cell_of(i) >= TEAMS * kCells;
-            const int in_kind = cell_of(i) - (is_v ? TEAMS * kCells : 0);
-            uint8_t* const slot = lds + (((is_v ? 2 + v_slot : k_slot) * TEAMS) + in_kind / kCells) * kHalfBytes;
-            *reinterpret_cast<v4i*>(slot + reader(in_kind % kCells + lane, is_v)) = held[i];
-            if (decltype(check)::value && is_v && Tile::no_numbers(__builtin_bit_cast(typename Tile::Pairs, held[i])) != 0)
-                no_numbers[v_slot][in_kind / kCells] = v_step + in_kind / kCells + 1;
+            uint8_t* const to = lds + ((is_v ? SLOTS + v_slot : k_slot) * TEAMS * NL + of_kind) * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(step_resource(layer_head, page_bytes, page, step, step_end, kStepBytes),
+                                                     reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(to)), 16,
+                                                     is_v ? v_lane : k_lane, (is_v ? kHalfBytes : 0) + (of_step >> 1) * 2048 + (of_step & 1) * 512, 0, 0);
         }
     };
     auto k_cells = [&](int slot) { return lds + (slot * TEAMS + team) * kHalfBytes + lane * 16; };
-    auto v_cells = [&](int slot) { return lds + ((2 + slot) * TEAMS + team) * kHalfBytes + lane * 16; };
-    if (threadIdx.x < 2 * TEAMS) no_numbers[threadIdx.x / TEAMS][threadIdx.x % TEAMS] = 0;
-    v4i held[NH], held_first[NH];
-    load_turn(held_first, step_begin, step_begin);
-    load_turn(held, step_begin + TEAMS, step_end);
+    auto v_cells = [&](int slot) { return lds + ((SLOTS + slot) * TEAMS + team) * kHalfBytes + lane * 16; };
 
-    T* const staged = reinterpret_cast<T*>(lds);
+    // K lies one turn ahead of V.
+    load_turn(step_begin, step_end, 0, SLOTS - 1);
+#pragma unroll
+    for (int t = 1; t < SLOTS; ++t) load_turn(step_begin + t * TEAMS, step_begin + (t - 1) * TEAMS, t, t - 1);
+    T* const staged = reinterpret_cast<T*>(lds + M::kRing);
     share.template stage_queries<T, HD, kManyThreads>(a, staged);
     __syncthreads();
     Tile tile;
@@ -111,15 +95,21 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     share.sees(a, tile, row);
 #pragma unroll
     for (int s = 0; s < Tile::NS; ++s) tile.q[s] = *reinterpret_cast<const Half8<T>*>(staged + row * kPitch + (s * 2 + g) * 8);
-    __syncthreads();
-    store_turn(std::true_type{}, held_first, 0, 0, step_begin);
-    __syncthreads();
-    float s[Tile::NV];
-    auto seen = [&](int st) { return st < step_end ? tile.seen(st, g) : 0u; };
-    auto operands = [&](Half8<T> (&x)[NL], const uint8_t* cells) {
+    // All but the last `left` turns' loads are there, for everyone.
+    auto arrive = [&](auto left) __attribute__((always_inline)) {
+        constexpr int N = decltype(left)::value * NH;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    using std::integral_constant;
+    auto operands = [&](Half8<T> (&x)[NL], const uint8_t* cells) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) x[i] = *reinterpret_cast<const Half8<T>*>(cells + i * 1024);
     };
+    auto seen = [&](int st) { return st < step_end ? tile.seen(st, g) : 0u; };
+    float s[Tile::NV], s1[Tile::NV];
+    arrive(integral_constant<int, SLOTS - 1>{});
     {
         Half8<T> kb[NL];
         operands(kb, k_cells(0));
@@ -127,48 +117,48 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
         tile.hide(seen(step_begin + team), s);
         tile.rise(s, a.scale);
     }
-    store_turn(std::false_type{}, held, 1, 1, 0);
-    load_turn(held, step_begin + 2 * TEAMS, step_begin + TEAMS);
-    __syncthreads();
+    arrive(integral_constant<int, SLOTS - 2>{});
 
-    int step0 = step_begin, odd = 0;
+    // Slots of this turn's V and the next turn's K, and of what this turn asks for.
+    int step0 = step_begin, v_slot = 0, k_slot = 1;
     // One turn: weights and sums of the scores `now`, scores `then` of the next.
     auto turn = [&](auto masked, const float (&now)[Tile::NV], float (&then)[Tile::NV]) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         const int step = step0 + team;
+        const int k_free = k_slot == 0 ? SLOTS - 1 : k_slot - 1, v_free = v_slot == 0 ? SLOTS - 1 : v_slot - 1;
+        load_turn(step0 + SLOTS * TEAMS, step0 + (SLOTS - 1) * TEAMS, k_free, v_free);
         if (!kMasked || step < step_end) {
             Half8<T> kb[NL], vb[NL], w[Tile::TERMS][Tile::NP];
-            operands(kb, k_cells(odd ^ 1));
-            operands(vb, v_cells(odd));
-            __builtin_amdgcn_sched_barrier(0);   // all asked for before the first is waited for
+            operands(kb, k_cells(k_slot));
+            operands(vb, v_cells(v_slot));
             tile.scores(kb, then);
             tile.weights(now, a.scale, w);
             if constexpr (kMasked)
-                if (__builtin_expect(no_numbers[odd][team] == step + 1, 0)) tile.part_with_no_numbers(vb, seen(step));
+                if (step >= share.plain_end && __builtin_expect(tile.no_numbers(vb), 0)) tile.part_with_no_numbers(vb, seen(step));
             tile.add(vb, w);
             if constexpr (kMasked) tile.hide(seen(step + TEAMS), then);
             tile.rise(then, a.scale);
         }
-        store_turn(masked, held, odd, odd ^ 1, step0 + TEAMS);
-        if (__builtin_expect(step0 + 3 * TEAMS + TEAMS > window + 128, 0)) {
+        if (__builtin_expect(step0 + (SLOTS + 2) * TEAMS > window + 128, 0)) {
             window += 64;
             pages = pages_next;
             pages_next = pages_from(window + 64);
         }
-        load_turn(held, step0 + 3 * TEAMS, step0 + 2 * TEAMS);
-        odd ^= 1;
         step0 += TEAMS;
-        __syncthreads();
+        k_slot = k_slot == SLOTS - 1 ? 0 : k_slot + 1;
+        v_slot = v_slot == SLOTS - 1 ? 0 : v_slot + 1;
+        arrive(integral_constant<int, SLOTS - 2>{});
     };
-    float s1[Tile::NV];
     auto run = [&](auto masked, int end) __attribute__((always_inline)) {
         while (step0 < end) {                    // an even number of turns: a turn past the last does nothing
             turn(masked, s, s1);
             turn(masked, s1, s);
         }
     };
-    run(std::false_type{}, share.plain_end - 4 * TEAMS + 1);   // (the tail's V cells are checked a turn ahead)
+    run(std::false_type{}, share.plain_end - 3 * TEAMS + 1);
     run(std::true_type{}, step_end);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // nothing is on its way to LDS any more
+    __syncthreads();
 
     // The teams' sums meet in LDS, quads of channels of a row together.
     v4f* const quads = reinterpret_cast<v4f*>(lds);
