@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
 
     // A wave appends the call's rows to the steps that it will scan.  (Another wave or
     // workgroup that reads them for other rows writes the same bytes.)
-    if (a.k != nullptr && share.template append<T, HD, 64>(a, table, layer_head, page_bytes, lane, kWaves, wave))
+    if (a.k != nullptr && share.template append<T, HD, 64, kWaves>(a, table, layer_head, page_bytes, lane, wave))
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the scan's loads find them
 
     T* const staged = reinterpret_cast<T*>(lds);
@@ -219,8 +219,9 @@ template <typename T, int HD, int ROWS, typename Tree>
 __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(const PagedAttendArgs a, const Tree tree) {
     constexpr int CG = HD / 4, kRows = kAttendThreads / CG, kAtOnce = 8;
     Share<ROWS, Tree> share;
-    const int part = blockIdx.x % (ROWS / kRows), id = blockIdx.x / (ROWS / kRows);
-    share.start(a, tree, id % a.view.kv_heads + id / a.view.kv_heads * a.view.kv_heads * a.splits, threadIdx.x & 63);
+    // (heads fastest, as the workgroups that left the partial results)
+    const int kh = blockIdx.x % a.view.kv_heads, id = blockIdx.x / a.view.kv_heads, part = id % (ROWS / kRows);
+    share.start(a, tree, kh + id / (ROWS / kRows) * a.view.kv_heads * a.splits, threadIdx.x & 63);
     const int row = part * kRows + threadIdx.x / CG, quad = threadIdx.x % CG;
     if (share.my_splits == 1 || row >= share.rows) return;
     Joined all;

@@ -301,48 +301,88 @@ struct Share {
     // All rows' queries, turned, to LDS with a pitch of HD + 8.
     template <typename T, int HD, int THREADS>
     __device__ __forceinline__ void stage_queries(const PagedAttendArgs& a, T* staged) const {
-        constexpr int kChunks = HD / 8;
-#pragma unroll
-        for (int it = 0; it < (ROWS * kChunks + THREADS - 1) / THREADS; ++it) {
-            const int item = min(it * THREADS + static_cast<int>(threadIdx.x), ROWS * kChunks - 1), row = item / kChunks, c = item % kChunks;
-            const int r = row_first + min(row, rows - 1), i = row_token(a.group_magic, r);
-            Half8<T> x = turned(static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride + (kh * a.group + r - i * a.group) * HD,
-                                c, a.rotation, angles(a.rotation, max(position(i), 0)));
+        constexpr int kChunks = HD / 8, kItems = (ROWS * kChunks + THREADS - 1) / THREADS, kAtOnce = kItems < 8 ? kItems : 8;
+        static_assert(kItems % kAtOnce == 0 && THREADS % kChunks == 0, "whole batches");
+        const int c = threadIdx.x % kChunks;
+        // (threads past the last row take that one again)
+        auto row_of = [&](int it) { return min(it * (THREADS / kChunks) + static_cast<int>(threadIdx.x) / kChunks, ROWS - 1); };
+        auto source = [&](int i, int row) {
+            const int r = row_first + min(row, rows - 1);
+            return static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.n + i) * a.q_stride + (kh * a.group + r - i * a.group) * HD;
+        };
+        auto leave = [&](int row, Half8<T> x) {
             if (a.negative) x = -x;
             *reinterpret_cast<Half8<T>*>(staged + row * (HD + 8) + 8 * c) = x;
+        };
+        if (aligned_rotation(a.rotation)) {
+#pragma unroll 1
+            for (int it0 = 0; it0 < kItems; it0 += kAtOnce) {
+                Chunk<T> x[kAtOnce];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int row = row_of(it0 + k), i = token(a, row);
+                    x[k].load(source(i, row), c, a.rotation, angles(a.rotation, max(position(i), 0)));
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) leave(row_of(it0 + k), x[k].turned(c, a.rotation));
+            }
+        } else {
+#pragma unroll 1
+            for (int it = 0; it < kItems; ++it) {
+                const int row = row_of(it), i = token(a, row);
+                leave(row, turned(source(i, row), c, a.rotation, angles(a.rotation, max(position(i), 0))));
+            }
         }
     }
-    // The call's rows that fall into steps of the split -- of every WAVES-th step, the
-    // wave-th -- to the cache, by THREADS threads; whether there were any.
-    template <typename T, int HD, int THREADS>
+    // The call's rows that fall into steps [begin, end) of the split -- with WAVES, a step of
+    // each WAVES-th from the wave-th -- to the cache, by THREADS threads, two chunks' loads of
+    // each at a time; whether there were any.
+    template <typename T, int HD, int THREADS, int WAVES>
     __device__ __forceinline__ bool append(const PagedAttendArgs& a, const int32_t* table, uint8_t* layer_head, int64_t page_bytes, int thread,
-                                           int waves, int wave) const {
+                                           int wave) const {
         constexpr int kChunks = HD / 8;
+        const bool fast = aligned_rotation(a.rotation);
+        bool any = false;
         if (p < 0) return false;
-        const int last = min(step_end, (p + count - 1) / kStepTokens + 1);
-        int step = max(step_begin, p / kStepTokens);
-        step += (wave - (step - step_begin)) & (waves - 1);
-        bool wrote = false;
-        for (; step < last; step += waves) {
-            const int page = table[step / kPageSteps];
-            const int t0 = max(p, step * kStepTokens), t1 = min(p + count, (step + 1) * kStepTokens);
-            if (page < 0) continue;
-            uint8_t* const cells = layer_head + page * page_bytes + (step % kPageSteps) * paged_step_bytes(HD);
-            const int items = (t1 - t0) * kChunks;
-            for (int base = 0; base < items; base += THREADS) {
-                const int item = min(base + thread, items - 1), tok = t0 + item / kChunks, c = item % kChunks, i = tok - p;
+        const int first_step = max(p / kStepTokens, step_begin), my_step = first_step + ((wave - (first_step - step_begin)) & (WAVES - 1));
+#pragma unroll 1
+        for (int s = my_step; WAVES == 1 ? !any : s < step_end; s += WAVES) {
+        const int t0 = max(p, (WAVES == 1 ? step_begin : s) * kStepTokens), t1 = min(p + count, (WAVES == 1 ? step_end : s + 1) * kStepTokens);
+        if (t0 >= t1) break;
+        const int items = (t1 - t0) * kChunks;
+        any = true;
+#pragma unroll 1
+        for (int base = 0; base < items; base += 2 * THREADS) {
+            Chunk<T> k[2];
+            Half8<T> v[2];
+            int page[2];
+            auto token_of = [&](int x) { return t0 + min(base + x * THREADS + thread, items - 1) / kChunks; };
+            const int c = thread % kChunks;
+            static_assert(THREADS % kChunks == 0, "a thread's chunk stays");
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int tok = token_of(x), i = tok - p;
                 const int64_t at = static_cast<int64_t>(b) * a.n + i;
-                const Half8<T> kk = turned(static_cast<const T*>(a.k) + at * a.k_stride + kh * HD, c, a.rotation, angles(a.rotation, position(i)));
-                const Half8<T> vv = *reinterpret_cast<const Half8<T>*>(static_cast<const T*>(a.v) + at * a.v_stride + kh * HD + 8 * c);
-                const int t = tok % kStepTokens;
-                *reinterpret_cast<Half8<T>*>(cells + k_cell(t, c)) = kk;
+                const T* const row = static_cast<const T*>(a.k) + at * a.k_stride + kh * HD;
+                const float2* const cs = angles(a.rotation, position(i));
+                page[x] = table[tok / kPageTokens];
+                v[x] = *reinterpret_cast<const Half8<T>*>(static_cast<const T*>(a.v) + at * a.v_stride + kh * HD + 8 * c);
+                if (fast) k[x].load(row, c, a.rotation, cs);
+                else k[x].own = turned(row, c, a.rotation, cs);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int tok = token_of(x), step = tok / kStepTokens, t = tok % kStepTokens;
+                if (base + x * THREADS + thread >= items || page[x] < 0) continue;
+                uint8_t* const cells = layer_head + page[x] * page_bytes + (step % kPageSteps) * paged_step_bytes(HD);
+                *reinterpret_cast<Half8<T>*>(cells + k_cell(t, c)) = fast ? k[x].turned(c, a.rotation) : k[x].own;
                 T* const dst = reinterpret_cast<T*>(cells + v_cell(t / 8, 8 * c, HD)) + t % 8;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) dst[8 * j] = vv[j];
+                for (int j = 0; j < 8; ++j) dst[8 * j] = v[x][j];
             }
-            wrote = true;
         }
-        return wrote;
+        }
+        return any;
     }
     // A row's values, sums over the sum of weights: zero for rows without a token.
     template <typename T, int HD>

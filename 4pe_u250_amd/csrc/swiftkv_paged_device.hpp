@@ -52,41 +52,63 @@ __device__ __forceinline__ float turn(float x, float y, float c, float s, bool s
     return z;
 }
 
-// 8 channels, 8 * chunk .., of a head's row turned by the angles `cs` (of its
-// position), rounded once.  A channel's partner is its neighbour, or `halves` a channel
-// half the rotary channels away, which is read from the row again.  Small code: a
-// workgroup runs it once, and fetches it for that.
+// 8 channels, 8 * chunk .., of a head's row, and what turns them: a channel's partner is
+// its neighbour, or with `halves` a channel half the rotary channels away, which is read
+// from the row again.  Loads and arithmetic apart, so that several chunks' loads can be on
+// their way; small code, since a workgroup runs it once, and fetches it for that.
 template <typename T>
-__device__ __forceinline__ Half8<T> turned(const T* row, int chunk, const PagedRotation& r, const float2* cs) {
-    const int half = r.rotary_dim / 2, c0 = 8 * chunk;
-    const Half8<T> own = *reinterpret_cast<const Half8<T>*>(row + c0);
-    if (c0 >= r.rotary_dim) return own;
-    if (r.halves ? (half & 7) != 0 : (r.rotary_dim & 7) != 0) {
-        Half8<T> out = own;
-#pragma unroll 1
-        for (int c = c0; c < min(c0 + 8, r.rotary_dim); ++c) {
-            const bool second = r.halves ? c >= half : c & 1;
-            const int other = r.halves ? (second ? c - half : c + half) : c ^ 1, j = r.halves ? (second ? c - half : c) : c >> 1;
-            const T z = static_cast<T>(turn(static_cast<float>(row[c]), static_cast<float>(row[other]), cs[j].x, cs[j].y, second));
+struct Chunk {
+    Half8<T> own, other;
+    v4f angle[4];
+
+    // ok: aligned_rotation(r)
+    __device__ __forceinline__ void load(const T* row, int chunk, const PagedRotation& r, const float2* cs) {
+        const int half = r.rotary_dim / 2, c0 = 8 * chunk;
+        const bool turns = c0 < r.rotary_dim, upper = c0 >= half;
+        own = *reinterpret_cast<const Half8<T>*>(row + c0);
+        const int partner = upper ? c0 - half : c0 + half, at = r.halves ? (upper ? c0 - half : c0) : c0 / 2;
+        other = *reinterpret_cast<const Half8<T>*>(row + (turns && r.halves ? partner : c0));
+        const v4f* const angles = reinterpret_cast<const v4f*>(cs + (turns ? at : 0));
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c - c0 == k) out[k] = z;
+        for (int i = 0; i < 4; ++i) angle[i] = angles[r.halves ? i : i & 1];
+    }
+    __device__ __forceinline__ Half8<T> turned(int chunk, const PagedRotation& r) const {
+        const int half = r.rotary_dim / 2, c0 = 8 * chunk;
+        const bool turns = c0 < r.rotary_dim, upper = c0 >= half;
+        Half8<T> out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float c = r.halves ? angle[j >> 1][2 * (j & 1)] : angle[j >> 2][2 * (j >> 1 & 1)];
+            const float s = r.halves ? angle[j >> 1][2 * (j & 1) + 1] : angle[j >> 2][2 * (j >> 1 & 1) + 1];
+            const float y = static_cast<float>(r.halves ? other[j] : own[j ^ 1]);
+            const T z = static_cast<T>(turn(static_cast<float>(own[j]), y, c, s, r.halves ? upper : j & 1));
+            out[j] = turns ? z : own[j];
         }
         return out;
     }
-    const bool upper = r.halves && c0 >= half;
-    const Half8<T> other = *reinterpret_cast<const Half8<T>*>(row + (r.halves ? (upper ? c0 - half : c0 + half) : c0));
-    const v4f* const angle = reinterpret_cast<const v4f*>(cs + (r.halves ? (upper ? c0 - half : c0) : c0 / 2));
-    v4f f[4];
+};
+// Whether whole chunks turn and their partners and angles are whole 16-byte pieces.
+__device__ __forceinline__ bool aligned_rotation(const PagedRotation& r) {
+    return r.table != nullptr && (r.halves ? (r.rotary_dim & 15) == 0 : (r.rotary_dim & 7) == 0);
+}
+// One chunk, by any rotation or none.
+template <typename T>
+__device__ __forceinline__ Half8<T> turned(const T* row, int chunk, const PagedRotation& r, const float2* cs) {
+    if (aligned_rotation(r)) {
+        Chunk<T> x;
+        x.load(row, chunk, r, cs);
+        return x.turned(chunk, r);
+    }
+    const int half = r.rotary_dim / 2, c0 = 8 * chunk;
+    Half8<T> out = *reinterpret_cast<const Half8<T>*>(row + c0);
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + 8, r.rotary_dim); ++c) {
+        const bool second = r.halves ? c >= half : c & 1;
+        const int other = r.halves ? (second ? c - half : c + half) : c ^ 1, j = r.halves ? (second ? c - half : c) : c >> 1;
+        const T z = static_cast<T>(turn(static_cast<float>(row[c]), static_cast<float>(row[other]), cs[j].x, cs[j].y, second));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = angle[r.halves ? i : i & 1];
-    Half8<T> out;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float c = r.halves ? f[j >> 1][2 * (j & 1)] : f[j >> 2][2 * (j >> 1 & 1)];
-        const float s = r.halves ? f[j >> 1][2 * (j & 1) + 1] : f[j >> 2][2 * (j >> 1 & 1) + 1];
-        const float y = static_cast<float>(r.halves ? other[j] : own[j ^ 1]);
-        out[j] = static_cast<T>(turn(static_cast<float>(own[j]), y, c, s, r.halves ? upper : j & 1));
+        for (int k = 0; k < 8; ++k)
+            if (c - c0 == k) out[k] = z;
     }
     return out;
 }

@@ -55,13 +55,6 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     uint8_t* const layer_head = a.view.base + paged_record(a.view, a.layer, 0, share.kh);
     const int64_t page_bytes = a.view.kv_heads * paged_record_bytes(HD);
 
-    // A tree's rows (a few steps) are appended by every workgroup that reads them, with the
-    // same bytes: its own writes are what it finds then.
-    if (a.k != nullptr && share.template append<T, HD, kManyThreads>(a, table, layer_head, page_bytes, threadIdx.x, 1, 0)) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-    }
-
     // A wave's loads of a turn: NH of its 1 KiB blocks, first the teams' K, then their V.
     // Product x of K reads, with lane (g', 16 m' + 8 h + m''), cell [x / 2][h][2 (x & 1) + g'][8 m' + m''];
     // product (c / 2, x & 1) of V, with lane (g', 16 (c & 1) + m), cell [c][2 (x & 1) + g'][m].
@@ -84,9 +77,17 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     auto v_cells = [&](int slot) { return lds + ((SLOTS + slot) * TEAMS + team) * kHalfBytes + lane * 16; };
 
     // K lies one turn ahead of V.
-    load_turn(step_begin, step_end, 0, SLOTS - 1);
+    auto load_first = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 1; t < SLOTS; ++t) load_turn(step_begin + t * TEAMS, step_begin + (t - 1) * TEAMS, t, t - 1);
+        for (int t = 0; t < SLOTS; ++t)
+            load_turn(step_begin + t * TEAMS, t == 0 ? step_end : step_begin + (t - 1) * TEAMS, t, t == 0 ? SLOTS - 1 : t - 1);
+    };
+    // A tree's rows (a few steps) are appended by every workgroup that reads them, with the
+    // same bytes: its own writes are what it finds then.
+    const bool late = a.k != nullptr && share.p >= 0 && (step_begin + SLOTS * TEAMS) * kStepTokens > share.p;
+    if (!late) load_first();
+    if (a.k != nullptr && share.template append<T, HD, kManyThreads, 1>(a, table, layer_head, page_bytes, threadIdx.x, 0))
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     T* const staged = reinterpret_cast<T*>(lds + M::kRing);
     share.template stage_queries<T, HD, kManyThreads>(a, staged);
     __syncthreads();
@@ -95,6 +96,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     share.sees(a, tile, row);
 #pragma unroll
     for (int s = 0; s < Tile::NS; ++s) tile.q[s] = *reinterpret_cast<const Half8<T>*>(staged + row * kPitch + (s * 2 + g) * 8);
+    if (late) load_first();
     // All but the last `left` turns' loads are there, for everyone.
     auto arrive = [&](auto left) __attribute__((always_inline)) {
         constexpr int N = decltype(left)::value * NH;
