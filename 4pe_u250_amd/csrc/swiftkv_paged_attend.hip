@@ -214,10 +214,10 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
 }
 
 // Splits of chunks of ROWS rows joined in split order: workgroup (a few rows, chunk and
-// key/value head; sequence), a quad of channels a thread, eight splits' loads at a time.
+// key/value head; sequence), a quad of channels a thread, four or eight splits' loads at a time.
 template <typename T, int HD, int ROWS, typename Tree>
 __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(const PagedAttendArgs a, const Tree tree) {
-    constexpr int CG = HD / 4, kRows = kAttendThreads / CG, kAtOnce = 8;
+    constexpr int CG = HD / 4, kRows = kAttendThreads / CG, kAtOnce = ROWS < 64 ? 8 : 4;
     Share<ROWS, Tree> share;
     // (heads fastest, as the workgroups that left the partial results)
     const int kh = blockIdx.x % a.view.kv_heads, id = blockIdx.x / a.view.kv_heads, part = id % (ROWS / kRows);

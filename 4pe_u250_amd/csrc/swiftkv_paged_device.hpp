@@ -42,12 +42,12 @@ __device__ __forceinline__ TreePlace tree_place(const uint8_t* parents, int n, i
     return t;
 }
 
-// x cos -+ y sin, in FP32 and one order of operations in every kernel, so that a
-// key's row does not depend on which of them appends it.  (The empty asm keeps the
-// compiler from one instruction that multiplies, adds and rounds to float16 at once,
-// which it took in some places.)
-__device__ __forceinline__ float turn(float x, float y, float c, float s, bool second) {
-    float z = __builtin_fmaf(x, c, second ? y * s : -(y * s));
+// x cos + y sin (the sine's sign is the caller's), in FP32 and one order of operations
+// in every kernel, so that a key's row does not depend on which of them appends it.  (The
+// empty asm keeps the compiler from one instruction that multiplies, adds and rounds to
+// float16 at once, which it took in some places.)
+__device__ __forceinline__ float turn(float x, float y, float c, float s) {
+    float z = __builtin_fmaf(x, c, y * s);
     asm("" : "+v"(z));
     return z;
 }
@@ -73,18 +73,22 @@ struct Chunk {
         for (int i = 0; i < 4; ++i) angle[i] = angles[r.halves ? i : i & 1];
     }
     __device__ __forceinline__ Half8<T> turned(int chunk, const PagedRotation& r) const {
-        const int half = r.rotary_dim / 2, c0 = 8 * chunk;
-        const bool turns = c0 < r.rotary_dim, upper = c0 >= half;
+        const int c0 = 8 * chunk;
         Half8<T> out;
+        if (r.halves) {
+            const uint32_t sign = c0 >= r.rotary_dim / 2 ? 0u : 0x80000000u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float c = r.halves ? angle[j >> 1][2 * (j & 1)] : angle[j >> 2][2 * (j >> 1 & 1)];
-            const float s = r.halves ? angle[j >> 1][2 * (j & 1) + 1] : angle[j >> 2][2 * (j >> 1 & 1) + 1];
-            const float y = static_cast<float>(r.halves ? other[j] : own[j ^ 1]);
-            const T z = static_cast<T>(turn(static_cast<float>(own[j]), y, c, s, r.halves ? upper : j & 1));
-            out[j] = turns ? z : own[j];
+            for (int j = 0; j < 8; ++j)
+                out[j] = static_cast<T>(turn(static_cast<float>(own[j]), static_cast<float>(other[j]), angle[j >> 1][2 * (j & 1)],
+                                             __uint_as_float(__float_as_uint(angle[j >> 1][2 * (j & 1) + 1]) ^ sign)));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float s = angle[j >> 2][2 * (j >> 1 & 1) + 1];
+                out[j] = static_cast<T>(turn(static_cast<float>(own[j]), static_cast<float>(own[j ^ 1]), angle[j >> 2][2 * (j >> 1 & 1)], j & 1 ? s : -s));
+            }
         }
-        return out;
+        return c0 < r.rotary_dim ? out : own;
     }
 };
 // Whether whole chunks turn and their partners and angles are whole 16-byte pieces.
@@ -105,7 +109,7 @@ __device__ __forceinline__ Half8<T> turned(const T* row, int chunk, const PagedR
     for (int c = c0; c < min(c0 + 8, r.rotary_dim); ++c) {
         const bool second = r.halves ? c >= half : c & 1;
         const int other = r.halves ? (second ? c - half : c + half) : c ^ 1, j = r.halves ? (second ? c - half : c) : c >> 1;
-        const T z = static_cast<T>(turn(static_cast<float>(row[c]), static_cast<float>(row[other]), cs[j].x, cs[j].y, second));
+        const T z = static_cast<T>(turn(static_cast<float>(row[c]), static_cast<float>(row[other]), cs[j].x, second ? cs[j].y : -cs[j].y));
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (c - c0 == k) out[k] = z;
