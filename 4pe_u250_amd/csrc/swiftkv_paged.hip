@@ -38,7 +38,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append_kernel(const PagedRo
     TreePlace place{};
     int end = p + a.n;
     if constexpr (kTree) {
-        place = tree_place(tree.parents + b * a.n, a.n, lane);
+        place = tree_place(tree.parents, b, a.n, lane);
         end = p + __popcll(__ballot(place.live));
     }
     if (tok0 >= end) return;
@@ -97,6 +97,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_values_kernel(const PagedRo
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
         const int item = it * kRowThreads + threadIdx.x, octet = item / HD, channel = item % HD;
+        if (tok0 + octet * 8 >= end || tok0 + octet * 8 + 8 <= p) continue;
         const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(cells + v_cell(octet, channel, HD));
 #pragma unroll
         for (int j = 0; j < 8; ++j) rows[(octet * 8 + j) * kPitch + channel] = w.v[j];
@@ -115,61 +116,74 @@ __global__ __launch_bounds__(kRowThreads) void paged_values_kernel(const PagedRo
     }
 }
 
-// Workgroup (layer and key/value head, sequence): row accepted[j] goes to row j.  A
-// row may be a source and a target, so all are read before any is written.
+// Workgroup (layer and `heads` key/value heads, sequence): row accepted[j] goes to row j.
+// A row may be a source and a target, so all are read, into LDS, before any is written.  K
+// moves by its cells, V by whole target cells, each of whose 8 tokens comes from its source
+// or from where it is.  Few instructions count here more than few loads: a workgroup runs
+// each once, and unrolled forms of this spent 13 us a launch on fetching them.
 template <int HD, int ROWS>
-__global__ __launch_bounds__(kRowThreads) void paged_keep_kernel(const PagedKeepArgs a) {
-    constexpr int kChunks = HD / 8;
-    constexpr int kCells = (ROWS * kChunks + kRowThreads - 1) / kRowThreads, kValues = ROWS * HD / kRowThreads;
-    const int layer = a.layer0 + static_cast<int>(blockIdx.x) / a.view.kv_heads, kh = blockIdx.x % a.view.kv_heads;
-    const int b = blockIdx.y, p = a.positions[b];
+__global__ __launch_bounds__(kRowThreads) void paged_keep_kernel(const PagedKeepArgs a, int heads) {
+    constexpr int kChunks = HD / 8, kOctets = (ROWS + 14) / 8, kHeads = ROWS <= 8 ? 4 : 1;
+    constexpr int64_t kRecord = 2 * kStepTokens * 2 * 2 * HD;        // between two heads
+    __shared__ __align__(16) Vec8<uint16_t> held[kHeads * (ROWS * kChunks + kOctets * HD)];
+    // Of token 8 (p / 8) + s: the K cells and V values that go there, from the layer's first
+    // head on, and its own; whether a row comes to its octet.
+    __shared__ int64_t k_from[kOctets * 8], k_to[kOctets * 8], v_from[kOctets * 8], v_to[kOctets * 8];
+    __shared__ int comes[kOctets];
+    const int parts = a.view.kv_heads / heads, layer = a.layer0 + static_cast<int>(blockIdx.x) / parts;
+    const int kh0 = static_cast<int>(blockIdx.x) % parts * heads, b = blockIdx.y, p = a.positions[b], tid = threadIdx.x;
     if (p < 0) return;
-    const uint8_t* const accepted = a.accepted + b * a.m;
-    const int32_t* const table = a.view.table + static_cast<int64_t>(a.slot0 + b) * a.view.entries;
-    // Cells of a token's step; its place in the step.
-    auto cells_of = [&](int tok) -> uint8_t* {
-        const int page = table[tok / kPageTokens];
-        if (page < 0) return nullptr;
-        return a.view.base + paged_record(a.view, layer, page, kh) + (tok / kStepTokens % kPageSteps) * paged_step_bytes(HD);
-    };
-    Vec8<uint16_t> k[kCells];
-    uint16_t v[kValues];
-    auto source = [&](int j) {       // of row j, or -1 where it stays
-        const int from = j < a.m ? accepted[j] : 255;
-        return from < kTreeTokens && from != j ? from : -1;
-    };
-    auto k_at = [&](uint8_t* cells, int tok, int chunk) {
-        return reinterpret_cast<Vec8<uint16_t>*>(cells + k_cell(tok % kStepTokens, chunk));
-    };
-    auto v_at = [&](uint8_t* cells, int tok, int channel) {
-        const int t = tok % kStepTokens;
-        return reinterpret_cast<uint16_t*>(cells + v_cell(t / 8, channel, HD)) + t % 8;
-    };
-#pragma unroll
-    for (int it = 0; it < kCells; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, j = item / kChunks, from = j < ROWS ? source(j) : -1;
-        uint8_t* const cells = from < 0 ? nullptr : cells_of(p + from);
-        if (cells != nullptr) k[it] = *k_at(cells, p + from, item % kChunks);
+    const int tok0 = p & ~7, octets = (p - tok0 + a.m + 7) / 8;
+    if (tid < kOctets) comes[tid] = 0;
+    const uint32_t accepted = tree_byte(a.accepted, b, a.m, (tok0 + tid - p) & (kTreeTokens - 1));
+    __syncthreads();
+    if (tid < octets * 8) {
+        const int32_t* const table = a.view.table + static_cast<int64_t>(a.slot0 + b) * a.view.entries;
+        const int64_t page_bytes = a.view.kv_heads * paged_record_bytes(HD);
+        const int to = tok0 + tid, j = to - p, from = j >= 0 && j < a.m && accepted < kTreeTokens ? p + static_cast<int>(accepted) : to;
+        const int page = table[min(from / kPageTokens, a.view.entries - 1)], to_page = table[min(to / kPageTokens, a.view.entries - 1)];
+        const bool moves = from != to && page >= 0 && to_page >= 0;
+        auto step_of = [&](int64_t on, int tok) { return on * page_bytes + tok / kStepTokens % kPageSteps * paged_step_bytes(HD); };
+        auto key = [&](int tok) { return k_cell(tok % kStepTokens, 0); };
+        auto value = [&](int tok) { return v_cell(tok % kStepTokens / 8, 0, HD); };
+        k_from[tid] = moves ? step_of(page, from) + key(from) : -1;
+        k_to[tid] = step_of(max(to_page, 0), to) + key(to);
+        v_from[tid] = moves ? step_of(page, from) + value(from) + 2 * (from % 8) : step_of(max(to_page, 0), to) + value(to) + 2 * (to % 8);
+        v_to[tid] = step_of(max(to_page, 0), to) + value(to);
+        if (moves) comes[tid / 8] = 1;
     }
+    __syncthreads();
+    uint8_t* const base = a.view.base + paged_record(a.view, layer, 0, kh0);
+    const int keys = a.m * kChunks, cells = octets * HD;
+    Vec8<uint16_t>* const held_v = held + kHeads * ROWS * kChunks;
+    auto key_at = [&](int item) { return item / keys * kRecord + k_cell(0, item % kChunks); };
+    auto value_at = [&](int item) { return item / cells * kRecord + (item % HD >> 4) * 1024 + (item % HD & 15) * 16; };
+    const int skip = p - tok0;
+#pragma unroll 1
+    for (int item = tid; item < heads * keys; item += kRowThreads) {
+        const int64_t from = k_from[skip + item % keys / kChunks];
+        if (from >= 0) held[item] = *reinterpret_cast<const Vec8<uint16_t>*>(base + from + key_at(item));
+    }
+#pragma unroll 1
+    for (int item = tid; item < heads * cells; item += kRowThreads) {
+        const int octet = item % cells / HD;
+        if (!comes[octet]) continue;
+        Vec8<uint16_t> w;
 #pragma unroll
-    for (int it = 0; it < kValues; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, from = source(item / HD);
-        uint8_t* const cells = from < 0 ? nullptr : cells_of(p + from);
-        if (cells != nullptr) v[it] = *v_at(cells, p + from, item % HD);
+        for (int e = 0; e < 8; ++e) w.v[e] = *reinterpret_cast<const uint16_t*>(base + v_from[octet * 8 + e] + value_at(item));
+        held_v[item] = w;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // read, and not only asked for
     __syncthreads();
-#pragma unroll
-    for (int it = 0; it < kCells; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, j = item / kChunks;
-        uint8_t* const cells = j < ROWS && source(j) >= 0 && cells_of(p + source(j)) != nullptr ? cells_of(p + j) : nullptr;
-        if (cells != nullptr) *k_at(cells, p + j, item % kChunks) = k[it];
+#pragma unroll 1
+    for (int item = tid; item < heads * keys; item += kRowThreads) {
+        const int s = skip + item % keys / kChunks;
+        if (k_from[s] >= 0) *reinterpret_cast<Vec8<uint16_t>*>(base + k_to[s] + key_at(item)) = held[item];
     }
-#pragma unroll
-    for (int it = 0; it < kValues; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, j = item / HD;
-        uint8_t* const cells = source(j) >= 0 && cells_of(p + source(j)) != nullptr ? cells_of(p + j) : nullptr;
-        if (cells != nullptr) *v_at(cells, p + j, item % HD) = v[it];
+#pragma unroll 1
+    for (int item = tid; item < heads * cells; item += kRowThreads) {
+        const int octet = item % cells / HD;
+        if (comes[octet]) *reinterpret_cast<Vec8<uint16_t>*>(base + v_to[octet * 8] + value_at(item)) = held_v[item];
     }
 }
 
@@ -187,6 +201,9 @@ void with_half(ElementType t, F&& f) {
     if (t == kBF16) f(__bf16{});
     else f(_Float16{});
 }
+
+// (layer, key/value head, sequence) triples from which a workgroup keeps four heads' rows.
+constexpr int kManyKeeps = 4096;
 
 int touched_steps(int n) { return (n + 2 * kStepTokens - 2) / kStepTokens; }
 
@@ -217,11 +234,12 @@ hipError_t launch_paged_values(const PagedRowsArgs& a, int layers, int batch, hi
 }
 
 hipError_t launch_paged_keep(const PagedKeepArgs& a, int layers, int batch, hipStream_t s) {
-    const dim3 grid(layers * a.view.kv_heads, batch);
+    const int heads = a.m <= 8 && a.view.kv_heads % 4 == 0 && layers * a.view.kv_heads * batch >= kManyKeeps ? 4 : 1;
+    const dim3 grid(layers * (a.view.kv_heads / heads), batch);
     auto go = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        if (a.m <= 8) paged_keep_kernel<HD, 8><<<grid, kRowThreads, 0, s>>>(a);
-        else paged_keep_kernel<HD, kTreeTokens><<<grid, kRowThreads, 0, s>>>(a);
+        if (a.m <= 8) paged_keep_kernel<HD, 8><<<grid, kRowThreads, 0, s>>>(a, heads);
+        else paged_keep_kernel<HD, kTreeTokens><<<grid, kRowThreads, 0, s>>>(a, heads);
     };
     if (a.view.head_dim == 64) go(std::integral_constant<int, 64>{});
     else go(std::integral_constant<int, 128>{});

@@ -53,11 +53,25 @@ struct PagedRotation {
     int32_t halves;
 };
 
-// Parents of a launch's tokens, [sequence][n].
+// A byte for each of a launch's tokens, [sequence][padded(n)].  They are read as words at
+// uniform addresses, 64 bytes a sequence whatever its number (hence the bytes behind the
+// last): the argument block lies far from the GPU, and only scalar loads of it are quick.
+struct TreeBytes {
+    uint32_t words[kTreeBytes / 4 + kTreeTokens / 4];
+};
+constexpr int tree_pitch(int n) { return (n + 3) & ~3; }
+
+// Parents of a launch's tokens.
 struct PagedTree {
-    uint8_t parents[kTreeBytes];
+    TreeBytes parents;
 };
 struct PagedChain {};
+
+// A grid row's sequence, counted from slot0 and its tensors' first, and its cached tokens.
+struct PagedRow {
+    int32_t position;
+    int32_t sequence;
+};
 
 // Rows appended to one layer, or values read from several.
 struct PagedRowsArgs {
@@ -99,8 +113,7 @@ struct PagedAttendArgs {
     int32_t split_steps;  // steps per split at most, a multiple of kSplitQuantumSteps
     float* partials;      // [pair][split]: stats [rows of a chunk][2], then sums [rows][head_dim]
     uint32_t* counters;   // [pair] arrived splits, kCounterStride apart, zero between launches
-    int32_t positions[kPagedBatch];
-    uint8_t order[kPagedBatch];       // the sequence of each grid row, longest first
+    PagedRow order[kPagedBatch];      // of each grid row, longest first
 };
 
 struct PagedKeepArgs {
@@ -109,7 +122,7 @@ struct PagedKeepArgs {
     int32_t slot0;
     int32_t m;
     int32_t positions[kPagedBatch];
-    uint8_t accepted[kTreeBytes];     // [sequence][m], 255 past the path's end
+    TreeBytes accepted;               // 255 past the path's end
 };
 
 constexpr int kMapEntries = 512;

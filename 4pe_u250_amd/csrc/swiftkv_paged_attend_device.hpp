@@ -256,18 +256,19 @@ struct Share {
     // `id`: the workgroup's (split, chunk, head), heads fastest, so that a head's workgroups
     // share an XCD's L2.
     __device__ __forceinline__ void start(const PagedAttendArgs& a, const Tree& tree, int id, int lane) {
-        b = a.order[blockIdx.y];
+        const PagedRow of_grid = a.order[blockIdx.y];
+        b = of_grid.sequence;
+        p = of_grid.position;
         kh = id % a.view.kv_heads;
         id /= a.view.kv_heads;
         split = id % a.splits;
         chunk = a.chunks - 1 - id / a.splits;    // the longest first
         row_first = chunk * ROWS;
         rows = min(ROWS, a.group * a.n - row_first);
-        p = a.positions[b];
         count = a.n;
         live = 0;
         if constexpr (kTree) {
-            place = tree_place(tree.parents + b * a.n, a.n, lane);
+            place = tree_place(tree.parents, b, a.n, lane);
             live = __ballot(place.live);
             count = __popcll(live);
         }

@@ -103,13 +103,22 @@ PagedRotation rotation_of(const swiftkv_rotary_table* table, int32_t halves) {
 }
 
 // Sequences of one launch of n tokens each.
-int32_t launch_batch(bool tree, int32_t n) { return tree ? std::min<int32_t>(kPagedBatch, kTreeBytes / n) : kPagedBatch; }
+int32_t launch_batch(bool tree, int32_t n) { return tree ? std::min<int32_t>(kPagedBatch, kTreeBytes / tree_pitch(n)) : kPagedBatch; }
+
+// Rows b0 .. b0 + nb - 1 of [batch][n] numbers below 64 as bytes, -1 and -2 as these.
+void set_bytes(TreeBytes& t, const int32_t* numbers, int32_t b0, int32_t nb, int32_t n, uint8_t minus_one, uint8_t minus_two) {
+    uint8_t* dst = reinterpret_cast<uint8_t*>(t.words);
+    const int32_t pitch = tree_pitch(n);
+    for (int32_t b = 0; b < nb; ++b, dst += pitch) {
+        const int32_t* src = numbers + static_cast<int64_t>(b0 + b) * n;
+        for (int32_t i = 0; i < n; ++i) dst[i] = src[i] == -1 ? minus_one : src[i] == -2 ? minus_two : static_cast<uint8_t>(src[i]);
+        for (int32_t i = n; i < pitch; ++i) dst[i] = minus_two;
+    }
+}
 
 const PagedTree* tree_of(PagedTree& t, const int32_t* parents, int32_t b0, int32_t nb, int32_t n) {
     if (!parents) return nullptr;
-    const int32_t* src = parents + static_cast<int64_t>(b0) * n;
-    for (int32_t i = 0; i < nb * n; ++i)
-        t.parents[i] = src[i] == -1 ? kTreeRoot : src[i] == -2 ? kTreeNone : static_cast<uint8_t>(src[i]);
+    set_bytes(t.parents, parents, b0, nb, n, kTreeRoot, kTreeNone);
     return &t;
 }
 
@@ -408,11 +417,10 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
         a.chunks = plan.chunks;
         a.splits = plan.splits;
         a.split_steps = plan.split_steps;
-        std::memcpy(a.positions, positions + b0, sizeof(int32_t) * static_cast<size_t>(nb));
-        for (int32_t b = 0; b < nb; ++b) a.order[b] = static_cast<uint8_t>(b);
+        for (int32_t b = 0; b < nb; ++b) a.order[b] = {positions[b0 + b], b};
         if (nb > 1)
-            std::sort(a.order, a.order + nb, [&](uint8_t x, uint8_t y) {
-                return a.positions[x] != a.positions[y] ? a.positions[x] > a.positions[y] : x < y;
+            std::sort(a.order, a.order + nb, [](const PagedRow& x, const PagedRow& y) {
+                return x.position != y.position ? x.position > y.position : x.sequence < y.sequence;
             });
         PagedTree tree;
         const PagedTree* const trees = tree_of(tree, parents, b0, nb, n);
@@ -455,7 +463,7 @@ int swiftkv_paged_keep(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t
             const int32_t nb = std::min(most, batch - b0);
             a.slot0 = seq0 + b0;
             std::memcpy(a.positions, positions + b0, sizeof(int32_t) * static_cast<size_t>(nb));
-            for (int32_t i = 0; i < nb * m; ++i) a.accepted[i] = static_cast<uint8_t>(accepted[static_cast<int64_t>(b0) * m + i]);
+            set_bytes(a.accepted, accepted, b0, nb, m, 255, 255);
             SKV_HIP(launch_paged_keep(a, layers, nb, ctx->stream));
         }
     }

@@ -30,10 +30,21 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t x, int lane) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(x), lane))) |
            static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(x >> 32), lane))) << 32;
 }
-__device__ __forceinline__ TreePlace tree_place(const uint8_t* parents, int n, int lane) {
-    const uint8_t parent = lane < n ? parents[lane] : kTreeNone;
+// Byte i (below 64) of a sequence's; `sequence` and n are uniform.
+__device__ __forceinline__ uint32_t tree_byte(const TreeBytes& bytes, int sequence, int n, int i) {
+    typedef uint32_t Words __attribute__((ext_vector_type(kTreeTokens / 4), aligned(4)));
+    Words words = *reinterpret_cast<const Words*>(bytes.words + sequence * (tree_pitch(n) / 4));
+    asm("" : "+s"(words));               // one load of all, not each under the condition below
+    uint32_t mine = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeTokens / 4; ++w)
+        if (i >> 2 == w) mine = words[w];
+    return mine >> (8 * (i & 3)) & 0xffu;
+}
+__device__ __forceinline__ TreePlace tree_place(const TreeBytes& parents, int sequence, int n, int lane) {
+    const uint32_t parent = lane < n ? tree_byte(parents, sequence, n, lane) : kTreeNone;
     TreePlace t{uint64_t(1) << lane, parent != kTreeNone};
-    int up = parent < kTreeTokens ? parent : lane;
+    int up = parent < kTreeTokens ? static_cast<int>(parent) : lane;
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
         t.mask |= from_lane(t.mask, up);
