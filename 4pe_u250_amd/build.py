@@ -45,7 +45,8 @@ HIP_FLAGS = [
 ]
 SOURCES = ["swiftkv_kernels.hip", "swiftkv_synth.hip", "swiftkv_exact.hip", "swiftkv_exact_short.hip",
            "swiftkv_block.hip", "swiftkv_block_prompt.hip", "swiftkv_rotary.hip", "swiftkv_paged.hip",
-           "swiftkv_paged_attend.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp", "swiftkv_paged_capi.cpp"]
+           "swiftkv_paged_attend.hip", "swiftkv_paged_many.hip", "swiftkv_capi.cpp", "swiftkv_block_capi.cpp",
+           "swiftkv_paged_capi.cpp"]
 HOST_SRC = os.path.join(PKG_DIR, "host", "swiftkv_host.cpp")
 HOST_BIN = os.path.join(PKG_DIR, "swiftkv_host")
 
@@ -74,7 +75,7 @@ def _compile(sources, extra, folder):
 
 def _link(objects, lib):
     tmp = lib + ".tmp"
-    out = _run([HIPCC, f"--offload-arch={ARCH}", "-shared", *objects, "-o", tmp])
+    out = _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-Wl,-z,defs", *objects, "-o", tmp])
     os.replace(tmp, lib)
     return out
 
