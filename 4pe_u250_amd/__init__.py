@@ -130,6 +130,7 @@ _SIGNATURES = {
     "swiftkv_paged_attention": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp,
                                           _i32, _i32, C.c_float, _vp, _i64]),
     "swiftkv_paged_keep": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp]),
+    "swiftkv_debug_set_paged_rows": (C.c_int, [_vp, _i32]),
     "swiftkv_debug_paged_plan": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "swiftkv_device_alloc": (C.c_int, [_vp, _sz, C.POINTER(_vp)]),
     "swiftkv_device_free": (C.c_int, [_vp, _vp]),
@@ -283,6 +284,10 @@ class Context:
 
     def synchronize(self) -> None:
         _check(lib().swiftkv_synchronize(self.handle))
+
+    def set_paged_rows(self, rows: int) -> None:
+        """Testing aid: the rows of a paged attention workgroup for calls with more than 16; 0: the plan's."""
+        _check(lib().swiftkv_debug_set_paged_rows(self.handle, rows))
 
     def set_split_tokens(self, n: int) -> None:
         _check(lib().swiftkv_set_split_tokens(self.handle, int(n)))

@@ -119,6 +119,7 @@ struct swiftkv_context {
     uint32_t* block_workspace = nullptr;
     // The same of the paged cache's attention, allocated with the first paged cache.
     uint32_t* paged_workspace = nullptr;
+    int32_t paged_rows = 0;     // testing aid: rows of a paged attention workgroup, 0 = the plan's
 };
 
 struct swiftkv_graph {

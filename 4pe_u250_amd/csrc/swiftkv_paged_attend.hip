@@ -33,10 +33,10 @@ __device__ __forceinline__ v2f fetch2(const float* p) {
 // count themselves; the last to arrive joins all in split order, so the result does not
 // depend on who that is.  32 rows are too many for one workgroup to join in good time:
 // a launch of paged_join_kernel does it.
-template <typename T, int HD, int R, int RW, typename Tree>
-__global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_attend_kernel(const PagedAttendArgs a, const Tree tree) {
-    using Tile = RowTile<T, HD, R>;
-    constexpr int ROWS = R * RW, THREADS = kAttendThreads * RW;
+template <typename T, int HD, int R, int RT, typename Tree>
+__global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const PagedAttendArgs a, const Tree tree) {
+    using Tile = RowTile<T, HD, R, R * RT == 16>;
+    constexpr int ROWS = R * RT, THREADS = kAttendThreads;
     using S = Share<ROWS, Tree>;
     constexpr int NL = Tile::NL, CG = HD / 4, kPitch = HD + 8;
     constexpr int kPolicy = 2;                   // nontemporal: a page is read once
@@ -44,8 +44,8 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
     __shared__ __align__(16) v4f lds[kWaves * CG * (ROWS + 1)];     // queries, then the waves' sums
     __shared__ float stats[kWaves][ROWS][2];
     __shared__ uint32_t arrived;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / RW;
-    const int g = lane / R, place = lane % R, my_row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW * R + place;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane / R, place = lane % R;
     S share;
     share.start(a, tree, blockIdx.x, lane);
     if (share.split >= share.my_splits) return;
@@ -68,11 +68,15 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
     T* const staged = reinterpret_cast<T*>(lds);
     share.template stage_queries<T, HD, THREADS>(a, staged);
     __syncthreads();
-    Tile tile;
-    tile.clear();
-    share.sees(a, tile, my_row);
+    Tile tiles[RT];
 #pragma unroll
-    for (int s = 0; s < Tile::NS; ++s) tile.q[s] = *reinterpret_cast<const Half8<T>*>(staged + my_row * kPitch + (s * Tile::G + g) * 8);
+    for (int rt = 0; rt < RT; ++rt) {
+        tiles[rt].clear();
+        share.sees(a, tiles[rt], rt * R + place);
+#pragma unroll
+        for (int s = 0; s < Tile::NS; ++s)
+            tiles[rt].q[s] = *reinterpret_cast<const Half8<T>*>(staged + (rt * R + place) * kPitch + (s * Tile::G + g) * 8);
+    }
 
     const int k_lane = R == 16 ? lane * 16 : (((place >> 3) & 1) * 64 + g * 16 + (place >> 4) * 8 + ((place >> 2) & 1) * 4 + (place & 3)) * 16;
     const int v_lane = R == 16 ? lane * 16 : ((place >> 4) * 64 + g * 16 + (place & 15)) * 16;
@@ -95,9 +99,9 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
     };
     // The scores of a step are formed while the weights of the one before are.
     int step = step_begin + wave, at = 0;
-    float s[Tile::NV];
+    float s[RT][Tile::NV];
     __amdgpu_buffer_rsrc_t next = cells_of(step, 0);
-    auto seen = [&](int st) { return st < step_end ? tile.seen(st, g) : 0u; };
+    auto seen = [&](const Tile& tile, int st) { return st < step_end ? tile.seen(st, g) : 0u; };
     auto turn_pages = [&]() {
         if (__builtin_expect(++at == 64, 0)) {
             load_pages(step + 2 * kWaves);
@@ -107,43 +111,66 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
     if (step < step_end) {
         load_k(next);
         load_v(next);
-        tile.scores(kb, s);
-        tile.hide(seen(step), s);
-        tile.rise(s, a.scale);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const uint32_t bits = seen(tiles[rt], step);
+            tiles[rt].scores(kb, s[rt]);
+            tiles[rt].hide(bits, s[rt]);
+            tiles[rt].rise(s[rt], a.scale);
+        }
         next = cells_of(step + kWaves, ++at);
         load_k(next);
     }
-    auto run = [&](auto masked, int end) {
+    auto run = [&](auto masked, int end) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         for (; step < end; step += kWaves) {
             turn_pages();
             const __amdgpu_buffer_rsrc_t after = cells_of(step + 2 * kWaves, at);
-            float sn[Tile::NV];
-            Half8<T> w[Tile::TERMS][Tile::NP];
-            tile.scores(kb, sn);
-            load_k(after);
-            tile.weights(s, a.scale, w);
+            float sn[RT][Tile::NV];
+            Half8<T> w[RT][Tile::TERMS][Tile::NP];
+            uint32_t bits[RT];
             if constexpr (kMasked)
-                if (__builtin_expect(tile.no_numbers(vb), 0)) tile.part_with_no_numbers(vb, seen(step));
-            tile.add(vb, w);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) bits[rt] = seen(tiles[rt], step + kWaves);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) tiles[rt].scores(kb, sn[rt]);
+            load_k(after);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) tiles[rt].weights(s[rt], a.scale, w[rt]);
+            if constexpr (kMasked)
+                if (__builtin_expect(tiles[0].no_numbers(vb), 0)) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) tiles[rt].part_with_no_numbers(vb, seen(tiles[rt], step));
+                    Tile::clean(vb);
+                }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) tiles[rt].add(vb, w[rt]);
             load_v(next);
-            if constexpr (kMasked) tile.hide(seen(step + kWaves), sn);
-            tile.rise(sn, a.scale);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if constexpr (kMasked) tiles[rt].hide(bits[rt], sn[rt]);
+                tiles[rt].rise(sn[rt], a.scale);
+            }
             next = after;
 #pragma unroll
-            for (int i = 0; i < Tile::NV; ++i) s[i] = sn[i];
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < Tile::NV; ++i) s[rt][i] = sn[rt][i];
         }
     };
     run(std::false_type{}, share.plain_end - kWaves);
     run(std::true_type{}, step_end);
 
     __syncthreads();                             // everyone has its queries
-    const float sum = Tile::groups_sum(tile.l);
-    if (g == 0) {
-        stats[wave][my_row][0] = tile.m;
-        stats[wave][my_row][1] = sum;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float sum = Tile::groups_sum(tiles[rt].l);
+        if (g == 0) {
+            stats[wave][rt * R + place][0] = tiles[rt].m;
+            stats[wave][rt * R + place][1] = sum;
+        }
+        tiles[rt].leave(lds + wave * CG * (ROWS + 1), ROWS + 1, rt * R + place, g);
     }
-    tile.leave(lds + wave * CG * (ROWS + 1), ROWS + 1, my_row, g);
     __syncthreads();
     constexpr int kItems = ROWS * CG / THREADS;
 #pragma unroll
@@ -161,7 +188,7 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
         float* const dst = share.template partial<HD>(a, share.split);
         if (share.my_splits == 1) {
             share.template finish<T, HD>(a, row, quad, all.l, all.o);
-        } else if (R == 16) {
+        } else if (ROWS == 16) {
             if (quad == 0) publish2(dst + row * 2, all.m, all.l);
             publish2(dst + ROWS * 2 + row * HD + quad * 4, all.o[0], all.o[1]);
             publish2(dst + ROWS * 2 + row * HD + quad * 4 + 2, all.o[2], all.o[3]);
@@ -170,7 +197,7 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
             *reinterpret_cast<v4f*>(dst + ROWS * 2 + row * HD + quad * 4) = all.o;
         }
     }
-    if constexpr (R == 16) {
+    if constexpr (ROWS == 16) {
         if (share.my_splits == 1) return;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // what was published has arrived
         __syncthreads();
@@ -193,7 +220,7 @@ __global__ __launch_bounds__(kAttendThreads * RW, R == 16 ? 3 : 2) void paged_at
                 for (int j = 0; j < kAtOnce; ++j) {
                     const float* src = share.template partial<HD>(a, min(j0 + j, share.my_splits - 1));
                     ml[k][j] = fetch2(src + row * 2);
-                    const v2f low = fetch2(src + R * 2 + row * HD + quad * 4), high = fetch2(src + R * 2 + row * HD + quad * 4 + 2);
+                    const v2f low = fetch2(src + ROWS * 2 + row * HD + quad * 4), high = fetch2(src + ROWS * 2 + row * HD + quad * 4 + 2);
                     sums[k][j] = v4f{low[0], low[1], high[0], high[1]};
                 }
             }
@@ -260,15 +287,15 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, const PagedTree* tree, 
     with_shape(a, t, [&](auto tag, auto hd) {
         using T = decltype(tag);
         constexpr int HD = decltype(hd)::value;
-        auto go = [&](auto r, auto rw) {
-            constexpr int R = decltype(r)::value, RW = decltype(rw)::value;
-            if (tree) paged_attend_kernel<T, HD, R, RW><<<grid, kAttendThreads * RW, 0, s>>>(a, *tree);
-            else paged_attend_kernel<T, HD, R, RW><<<grid, kAttendThreads * RW, 0, s>>>(a, PagedChain{});
+        auto go = [&](auto r, auto rt) {
+            constexpr int R = decltype(r)::value, RT = decltype(rt)::value;
+            if (tree) paged_attend_kernel<T, HD, R, RT><<<grid, kAttendThreads, 0, s>>>(a, *tree);
+            else paged_attend_kernel<T, HD, R, RT><<<grid, kAttendThreads, 0, s>>>(a, PagedChain{});
         };
         using std::integral_constant;
         if (rows == 16) go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
         else if (rows == 32) go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-        else go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+        else go(integral_constant<int, 16>{}, integral_constant<int, 3>{});
     });
     return hipGetLastError();
 }
@@ -284,6 +311,7 @@ hipError_t launch_paged_join(const PagedAttendArgs& a, const PagedTree* tree, in
             else paged_join_kernel<T, HD, ROWS><<<grid, kAttendThreads, 0, s>>>(a, PagedChain{});
         };
         if (rows == 32) go(std::integral_constant<int, 32>{});
+        else if (rows == 48) go(std::integral_constant<int, 48>{});
         else if (rows == 64) go(std::integral_constant<int, 64>{});
         else if (rows == 128) go(std::integral_constant<int, 128>{});
         else go(std::integral_constant<int, 256>{});

@@ -41,12 +41,13 @@ __device__ __forceinline__ int row_token(uint32_t group_magic, int r) {
 }
 
 // The bits of tokens tok0 .. tok0 + 31 that a row sees: all before `first`, and
-// those of `mask` from there on.
+// those of `mask` from there on.  Without a branch, and the kernels ask for them before
+// they form the scores: where a branch lay between matrix products and the reading of
+// their results, hipcc 7.2 left the waits for them out on one of its paths.
 __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask) {
-    const int d = tok0 - first;
-    if (d >= 0) return d < 64 ? static_cast<uint32_t>(mask >> d) : 0u;
-    if (d <= -kStepTokens) return ~0u;
-    return ((1u << -d) - 1u) | static_cast<uint32_t>(mask << -d);
+    const int d = tok0 - first, below = min(max(-d, 0), 63), past = min(max(d, 0), 63);
+    const uint32_t bits = static_cast<uint32_t>(((mask << below) | ((1ull << below) - 1ull)) >> past);
+    return d < 64 ? bits : 0u;
 }
 
 // R rows of a wave: their queries as B operands, and softmax(scale q k^T) v over the
@@ -66,7 +67,7 @@ __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask
 // 16 rows leave the matrix instructions idle, so a bfloat16 weight is two terms there
 // (2^-16 of it); with more rows it is one, 2^-8.  A float16 weight is 2^(kShift +
 // kSlack) at most and is good to 2^-11, or to 2^-36 of the row's largest.
-template <typename T, int HD, int R>
+template <typename T, int HD, int R, bool FINE = false>
 struct RowTile {
     using P = Product<T, R>;
     using Sum = typename P::Sum;
@@ -78,7 +79,7 @@ struct RowTile {
     static constexpr int NS = HD / (8 * G);      // products of a score
     static constexpr int ND = HD / R;            // output tiles
     static constexpr int NE = R * R / 64;        // sums of a lane in one
-    static constexpr int TERMS = R == 16 && !kHalf ? 2 : 1;
+    static constexpr int TERMS = FINE && !kHalf ? 2 : 1;
     static constexpr float kSlack = 4.0f, kShift = kHalf ? 11.0f : 0.0f;
     typedef uint32_t Pairs __attribute__((ext_vector_type(4)));
 
@@ -184,7 +185,7 @@ struct RowTile {
     // 0 times an infinity or a NaN is a NaN, so where rows see different tokens, what is
     // no number leaves V and reaches the rows that see it by itself: products of ones
     // count such values.
-    __device__ __forceinline__ void part_with_no_numbers(Half8<T> (&vb)[NL], uint32_t bits) {
+    __device__ __forceinline__ void part_with_no_numbers(const Half8<T> (&vb)[NL], uint32_t bits) {
 #pragma unroll 1
         for (int kind = 0; kind < 3; ++kind) {   // NaN, inf, -inf: from `low` on, `span` patterns
             const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
@@ -210,6 +211,8 @@ struct RowTile {
                 for (int e = 0; e < NE; ++e) acc[d][e] += n[e] > 0.0f ? value : 0.0f;
             }
         }
+    }
+    static __device__ __forceinline__ void clean(Half8<T> (&vb)[NL]) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             Pairs u = __builtin_bit_cast(Pairs, vb[i]);
@@ -302,7 +305,7 @@ struct Share {
     // All rows' queries, turned, to LDS with a pitch of HD + 8.
     template <typename T, int HD, int THREADS>
     __device__ __forceinline__ void stage_queries(const PagedAttendArgs& a, T* staged) const {
-        constexpr int kChunks = HD / 8, kItems = (ROWS * kChunks + THREADS - 1) / THREADS, kAtOnce = kItems < 8 ? kItems : 8;
+        constexpr int kChunks = HD / 8, kItems = (ROWS * kChunks + THREADS - 1) / THREADS, kAtOnce = kItems < 4 ? kItems : 4;
         static_assert(kItems % kAtOnce == 0 && THREADS % kChunks == 0, "whole batches");
         const int c = threadIdx.x % kChunks;
         // (threads past the last row take that one again)
@@ -336,12 +339,15 @@ struct Share {
         }
     }
     // The call's rows that fall into steps [begin, end) of the split -- with WAVES, a step of
-    // each WAVES-th from the wave-th -- to the cache, by THREADS threads, two chunks' loads of
-    // each at a time; whether there were any.
+    // each WAVES-th from the wave-th -- to the cache, by THREADS threads, N chunks' loads of
+    // each at a time (two are quicker where a wave has several, and slower code where it has
+    // one: 26 tokens 16.6 us a call against 17.7, one token 10.6 against 10.8); whether
+    // there were any.
     template <typename T, int HD, int THREADS, int WAVES>
     __device__ __forceinline__ bool append(const PagedAttendArgs& a, const int32_t* table, uint8_t* layer_head, int64_t page_bytes, int thread,
                                            int wave) const {
         constexpr int kChunks = HD / 8;
+        constexpr int N = ROWS == 32 || ROWS == 48 ? 2 : 1;
         const bool fast = aligned_rotation(a.rotation);
         bool any = false;
         if (p < 0) return false;
@@ -353,15 +359,15 @@ struct Share {
         const int items = (t1 - t0) * kChunks;
         any = true;
 #pragma unroll 1
-        for (int base = 0; base < items; base += 2 * THREADS) {
-            Chunk<T> k[2];
-            Half8<T> v[2];
-            int page[2];
+        for (int base = 0; base < items; base += N * THREADS) {
+            Chunk<T> k[N];
+            Half8<T> v[N];
+            int page[N];
             auto token_of = [&](int x) { return t0 + min(base + x * THREADS + thread, items - 1) / kChunks; };
             const int c = thread % kChunks;
             static_assert(THREADS % kChunks == 0, "a thread's chunk stays");
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < N; ++x) {
                 const int tok = token_of(x), i = tok - p;
                 const int64_t at = static_cast<int64_t>(b) * a.n + i;
                 const T* const row = static_cast<const T*>(a.k) + at * a.k_stride + kh * HD;
@@ -372,7 +378,7 @@ struct Share {
                 else k[x].own = turned(row, c, a.rotation, cs);
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < N; ++x) {
                 const int tok = token_of(x), step = tok / kStepTokens, t = tok % kStepTokens;
                 if (base + x * THREADS + thread >= items || page[x] < 0) continue;
                 uint8_t* const cells = layer_head + page[x] * page_bytes + (step % kPageSteps) * paged_step_bytes(HD);

@@ -6,7 +6,6 @@
 
 #include <algorithm>
 #include <cstring>
-#include <cstdlib>
 #include <new>
 
 #include "swiftkv_paged.hpp"
@@ -38,6 +37,9 @@ constexpr int64_t kMaxGroups = int64_t(1) << 23;
 constexpr int64_t kMaxSplitGroups = 2048;
 constexpr int64_t kMaxPartialRows = int64_t(1) << 16;
 constexpr size_t kPartialFloats = static_cast<size_t>(kMaxPartialRows) * (2 + 128);
+
+// Turns (below) from which workgroups of more than 32 rows pay; for one sequence.
+constexpr int64_t kManyTurns = 2048, kManyTurnsAlone = 16384;
 
 // What every call on a range of sequences of a paged cache checks.
 int check_call(const swiftkv_context* ctx, const swiftkv_paged_cache* c, int32_t layer, int32_t layers, int32_t seq0,
@@ -146,30 +148,61 @@ int append_rows(const swiftkv_context* ctx, const PagedRotation& rotation, const
     return SWIFTKV_OK;
 }
 
-PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t group, int32_t kv_heads, int32_t n,
+// The kernel of a call goes by its rows (query tokens times grouped heads) and by turns,
+// steps times chunks of 256 rows times key/value heads.  Up to 16 and 32 rows a workgroup
+// holds them all.  More go, where turns are few, by 32 to workgroups of their own, whose
+// repeated reads the L2s serve; where they are many, to workgroups of 48 (three tiles of 16
+// rows a wave: loads bound these), 64, 128 or 256 (cells shared in LDS).  us of a call onto
+// 4031 tokens, 32 heads over 8, the kernel taken against the next: 8 sequences x 16 tokens
+// (64 rows) 64 34.9, 32 37.0; x 24 (96 rows) 128 42.1, 32 49.8, 64 44.4; x 64 (256 rows) 256
+// 68, 32 99, 64 72; 64 x 12 (48 rows) 48 192, 64 203; 64 x 16 64 204, 32 290; one sequence x 26
+// 32 16.6, 64 25.8, 128 27; x 64 32 26.1, 64 26.5, 256 37.  Long chunks of one sequence read few
+// cells for many rows: 512 tokens onto 4095 32 59.9, 64 72, 256 68; 4096 onto none 256 176, 32 258.
+//
+// Splits make a workgroup for each CU and not more, of at most 32 a sequence and at most the
+// square root of its 64-token tiles, since they are joined: us of a step, tokens of this
+// rule's splits against others: one sequence at 4096 512 11.1; 256 11.7, 1024 12.7; 4 at 4096
+// 512 16.9; 1024 19.5; 8 at 4096 1024 26.5; 512 30.3, 2048 30.3; 32 at 4096 none 86.7; 2048
+// 92.5; 64 none 172; 2048 189; one at 32000 1408; 1024 29.6, 2048 31.2, 4096 45.7.
+PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t forced_rows, int32_t group, int32_t kv_heads, int32_t n,
                          const int32_t* positions, int32_t batch) {
     PagedPlan p{};
     const int64_t rows = static_cast<int64_t>(group) * n;
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    if (getenv("PROWS") && p.rows > 32) p.rows = atoi(getenv("PROWS"));
+    auto steps_of = [&](int32_t b) {
+        return positions[b] < 0 ? 0 : (static_cast<int64_t>(positions[b]) + n + kStepTokens - 1) / kStepTokens;
+    };
+    int64_t turns = 0, longest = 1;
+    for (int32_t b = 0; b < batch; ++b) {
+        turns += steps_of(b);
+        longest = std::max(longest, steps_of(b));
+    }
+    turns *= (rows + 255) / 256 * kv_heads;
+    if (rows <= 16) p.rows = 16;
+    else if (forced_rows > 0) p.rows = forced_rows;
+    else if (rows <= 32 || turns < kManyTurns || (batch == 1 && turns < kManyTurnsAlone)) p.rows = 32;
+    else p.rows = rows <= 48 ? 48 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     p.chunks = static_cast<int32_t>((rows + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.chunks;
-    int64_t longest = 0, total = 0;
-    for (int32_t b = 0; b < batch; ++b) {
-        const int64_t len = positions[b] < 0 ? 0 : static_cast<int64_t>(positions[b]) + n;
-        const int64_t steps = (len + kStepTokens - 1) / kStepTokens;
-        longest = std::max(longest, steps);
-        total += steps;
-    }
-    longest = std::max<int64_t>(longest, 1);
-    total *= static_cast<int64_t>(kv_heads) * p.chunks;
-    int64_t per = std::max<int64_t>((total + cus - 1) / cus, (longest + 15) / 16);
+    auto whole = [](int64_t steps) { return (steps + kSplitQuantumSteps - 1) / kSplitQuantumSteps * kSplitQuantumSteps; };
+    auto groups = [&](int64_t per) {
+        int64_t sum = 0;
+        for (int32_t b = 0; b < batch; ++b) sum += std::max<int64_t>(1, (steps_of(b) + per - 1) / per);
+        return sum * kv_heads * p.chunks;
+    };
+    const int64_t most_splits = std::min<int64_t>(32, std::ceil(std::sqrt(longest / 2.0)));
+    int64_t low = whole((longest + most_splits - 1) / most_splits), per = whole(longest);
+    if (pairs < cus)
+        while (low < per) {              // the fewest steps with which the workgroups find a CU each
+            const int64_t middle = whole((low + per - kSplitQuantumSteps) / 2);
+            if (groups(middle) <= cus) per = middle;
+            else low = middle + kSplitQuantumSteps;
+        }
     if (split_tokens > 0) per = split_tokens / kStepTokens;
     // what the workspace holds
     const int64_t most = std::min(kMaxSplitGroups, kMaxPartialRows / p.rows) / pairs;
     if (most <= 1) per = longest;
     else per = std::max(per, (longest + most - 1) / most);
-    per = (per + kSplitQuantumSteps - 1) / kSplitQuantumSteps * kSplitQuantumSteps;
+    per = whole(per);
     p.split_steps = static_cast<int32_t>(per);
     p.splits = static_cast<int32_t>((longest + per - 1) / per);
     p.appends = n <= kTreeTokens;
@@ -400,7 +433,7 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
     const int32_t most = launch_batch(parents != nullptr, n);
     for (int32_t b0 = 0; b0 < batch; b0 += most) {
         const int32_t nb = std::min(most, batch - b0);
-        const PagedPlan plan = plan_attention(ctx->cus, ctx->split_tokens, group, view.kv_heads, n, positions + b0, nb);
+        const PagedPlan plan = plan_attention(ctx->cus, ctx->split_tokens, ctx->paged_rows, group, view.kv_heads, n, positions + b0, nb);
         const int64_t first = static_cast<int64_t>(b0) * n;
         a.q = static_cast<const char*>(q) + first * q_stride * 2;
         a.out = static_cast<char*>(out) + first * out_stride * 2;
@@ -424,7 +457,7 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
             });
         PagedTree tree;
         const PagedTree* const trees = tree_of(tree, parents, b0, nb, n);
-        SKV_HIP(plan.rows <= (getenv("PD64") ? 64 : 32) ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)
+        SKV_HIP(plan.rows <= 48 ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)
                                 : launch_paged_many(a, trees, nb, plan.rows, cache->type, ctx->stream));
         if (plan.splits > 1 && plan.rows > 16)
             SKV_HIP(launch_paged_join(a, trees, nb, plan.rows, cache->type, ctx->stream));
@@ -474,6 +507,14 @@ int swiftkv_paged_keep(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t
     return ok();
 }
 
+int swiftkv_debug_set_paged_rows(swiftkv_context* ctx, int32_t rows) {
+    if (!ctx) return fail(SWIFTKV_EINVAL, "null context");
+    if (rows != 0 && rows != 32 && rows != 48 && rows != 64 && rows != 128 && rows != 256)
+        return fail(SWIFTKV_EINVAL, "rows %d: must be 0, 32, 48, 64, 128 or 256", rows);
+    ctx->paged_rows = rows;
+    return ok();
+}
+
 int swiftkv_debug_paged_plan(int32_t cus, int32_t split_tokens, int32_t heads, int32_t kv_heads, int32_t n,
                              const int32_t* positions, int32_t batch, int32_t* out_rows, int32_t* out_chunks,
                              int32_t* out_splits, int32_t* out_split_tokens) {
@@ -481,7 +522,7 @@ int swiftkv_debug_paged_plan(int32_t cus, int32_t split_tokens, int32_t heads, i
     if (cus < 1 || split_tokens < 0 || kv_heads < 1 || kv_heads > 256 || heads < kv_heads || heads % kv_heads != 0 ||
         heads / kv_heads > 64 || n < 1 || n > kPagedMaxSeq || batch < 1 || batch > kPagedBatch)
         return fail(SWIFTKV_EINVAL, "cus %d, heads %d over %d, n %d, batch %d", cus, heads, kv_heads, n, batch);
-    const PagedPlan p = plan_attention(cus, split_tokens, heads / kv_heads, kv_heads, n, positions, batch);
+    const PagedPlan p = plan_attention(cus, split_tokens, 0, heads / kv_heads, kv_heads, n, positions, batch);
     *out_rows = p.rows;
     *out_chunks = p.chunks;
     *out_splits = p.splits;

@@ -113,10 +113,11 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     float s[Tile::NV], s1[Tile::NV];
     arrive(integral_constant<int, SLOTS - 1>{});
     {
+        const uint32_t bits = seen(step_begin + team);
         Half8<T> kb[NL];
         operands(kb, k_cells(0));
         tile.scores(kb, s);
-        tile.hide(seen(step_begin + team), s);
+        tile.hide(bits, s);
         tile.rise(s, a.scale);
     }
     arrive(integral_constant<int, SLOTS - 2>{});
@@ -130,15 +131,19 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
         const int k_free = k_slot == 0 ? SLOTS - 1 : k_slot - 1, v_free = v_slot == 0 ? SLOTS - 1 : v_slot - 1;
         load_turn(step0 + SLOTS * TEAMS, step0 + (SLOTS - 1) * TEAMS, k_free, v_free);
         if (!kMasked || step < step_end) {
+            const uint32_t bits = kMasked ? seen(step + TEAMS) : 0u;
             Half8<T> kb[NL], vb[NL], w[Tile::TERMS][Tile::NP];
             operands(kb, k_cells(k_slot));
             operands(vb, v_cells(v_slot));
             tile.scores(kb, then);
             tile.weights(now, a.scale, w);
             if constexpr (kMasked)
-                if (step >= share.plain_end && __builtin_expect(tile.no_numbers(vb), 0)) tile.part_with_no_numbers(vb, seen(step));
+                if (step >= share.plain_end && __builtin_expect(tile.no_numbers(vb), 0)) {
+                    tile.part_with_no_numbers(vb, seen(step));
+                    Tile::clean(vb);
+                }
             tile.add(vb, w);
-            if constexpr (kMasked) tile.hide(seen(step + TEAMS), then);
+            if constexpr (kMasked) tile.hide(bits, then);
             tile.rise(then, a.scale);
         }
         if (__builtin_expect(step0 + (SLOTS + 2) * TEAMS > window + 128, 0)) {

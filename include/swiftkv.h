@@ -609,6 +609,11 @@ int swiftkv_paged_keep(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t
                        const int32_t* positions, const int32_t* accepted, int32_t batch, int32_t m,
                        int32_t* out_positions);
 
+/* Testing aid with no counterpart in the reference: every later swiftkv_paged_attention of the
+ * context with more than 16 rows (n times the query heads that share a key/value head) takes the
+ * kernel for workgroups of `rows` rows -- 32, 48, 64, 128 or 256 -- instead of the plan's; 0
+ * returns to that.  All compute the same function. */
+int swiftkv_debug_set_paged_rows(swiftkv_context* ctx, int32_t rows);
 /* Testing aid with no counterpart in the reference, host-only: the plan of one attention
  * launch of batch <= 64 sequences on a device of `cus` compute units: rows of a
  * workgroup's chunk, chunks of a (sequence, key/value head), splits of the longest

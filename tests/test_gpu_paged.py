@@ -99,6 +99,87 @@ def test_trees(skv, ctx, t, dim, heads, kv):
     rig.check_values()
 
 
+@pytest.fixture
+def forced(ctx, request):
+    ctx.set_paged_rows(request.param)
+    yield request.param
+    ctx.set_paged_rows(0)
+
+
+every_shape = pytest.mark.parametrize("forced", [32, 48, 64, 128, 256], indirect=True)
+
+
+@every_shape
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_every_shape(skv, ctx, t, dim, forced):
+    """Each kernel for more than 16 rows on trees and chains of few and many rows, short and long sequences, rows that
+    fill no chunk, splits of one step and of many; repeated calls give the same bits."""
+    rig = P.Rig(skv, ctx, t, 10, 2, dim, batch=3, capacity=1600, rotation=P.Rotation(dim, halves=dim == 64), seed=forced)
+    rig.map_all()
+    rig.append([0, 0, 0], 1500)
+    rng = np.random.default_rng(forced)
+    try:
+        for n, at in ((4, [0, 31, 1500]), (13, [700, -1, 64]), (64, [1500, 0, 333]), (27, [90, 1023, 5])):
+            for split in (0, 256):
+                ctx.set_split_tokens(split)
+                trees = [P.random_tree(rng, n, c, deep) for c, deep in ((n, 0.5), ((n + 1) // 2, 0.0), (n, 0.9))]
+                q, k, v = (rig.random(3, n, h, dim)[1] for h in (10, 2, 2))
+                first, out = rig.attend(at, n, trees, q=q, k=k, v=v)
+                rig.compare(first, out, at, trees)
+                rig.check_values()
+                np.testing.assert_array_equal(rig.attend(at, n, trees, q=q, k=k, v=v)[1], out)
+                rig.check_attention(at, n)
+        ctx.set_split_tokens(0)
+        rig.check_attention([3, 0, 900], 150)
+        rig.check_attention([1000, 64, -1], 150, scale=-0.2)
+        rig.check_values()
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@every_shape
+def test_long_scans_of_every_shape(skv, ctx, forced):
+    """More steps than a window of the table holds, in one split and in several."""
+    rig = P.Rig(skv, ctx, "bf16", 4, 1, 64, batch=1, capacity=17000, rotation=P.Rotation(64, 17000), seed=forced)
+    rig.map_all()
+    rig.append([0], 16900)
+    try:
+        for split in (32768, 8192, 0):
+            ctx.set_split_tokens(split)
+            rig.check_attention([16900], 9)
+            rig.check_attention([16389], 70)
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@every_shape
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_no_numbers_in_every_shape(skv, ctx, t, forced, what):
+    """A value that is no number reaches the tokens that see it, wherever in a step or a turn it stands."""
+    dim, n = 64, 40
+    rig = P.Rig(skv, ctx, t, 2, 1, dim, capacity=512, seed=1)
+    rig.map_all()
+    junk = np.full((1, 512, 1, dim), what)
+    for p in (0, 77, 380):
+        rig.append([0], 512, k=junk, v=junk)
+        rig.append([0], p) if p else None
+        tree = [[-1] + [(i - 1) // 2 for i in range(1, n)]]
+        own, _, _ = P.places(tree[0])
+        q, k, v = (rig.random(1, n, h, dim)[1] for h in (2, 1, 1))
+        first, good = rig.attend([p], n, tree, q=q, k=k, v=v)
+        rig.compare(first, good, [p], tree)
+        for node in (0, 3, 17, 39):
+            bad = v.copy()
+            bad[0, node, 0, [1, 40]] = what
+            _, out = rig.attend([p], n, tree, q=q, k=k, v=bad)
+            sees = own[:, node]
+            np.testing.assert_array_equal(out[0, ~sees], good[0, ~sees])
+            np.testing.assert_array_equal(out[0][:, :, 2:40], good[0][:, :, 2:40])
+            assert (np.isnan(out[0, sees][:, :, [1, 40]]) if np.isnan(what) else out[0, sees][:, :, [1, 40]] == what).all()
+
+
 def test_a_chain_as_a_tree(skv, ctx):
     """The same tokens with parents written out and without give the same outputs, bit for bit."""
     rig = P.Rig(skv, ctx, "bf16", 8, 2, 128, batch=2, capacity=640, rotation=P.Rotation(128), seed=1)
@@ -489,7 +570,7 @@ def test_refusals(skv, ctx):
         (lambda: rig.cache.map(0, [8]), E), (lambda: rig.cache.map(0, [-2]), E), (lambda: rig.cache.map(2, [0]), E),
         (lambda: rig.cache.map(0, [0], first=4), E), (lambda: rig.cache.map(0, [0, 1, 2, 3, 4]), E), (lambda: rig.cache.map(0, [0], first=-1), E),
         (lambda: rig.cache.copy(0, 8), E), (lambda: rig.cache.copy(-1, 0), E),
-        (create(layers=0), A), (create(pages=0), A), (create(batch=0), A), (create(heads=3, kv=2), A), (create(heads=65), A),
+        (lambda: ctx.set_paged_rows(16), A), (create(layers=0), A), (create(pages=0), A), (create(batch=0), A), (create(heads=3, kv=2), A), (create(heads=65), A),
         (create(dim=96), A), (create(length=0), A), (create(length=131073), A), (create(dtype=skv.F32), A), (create(dtype=7), A),
         (create(layers=256, pages=1 << 24, heads=256, kv=256, dim=128), skv.ENOMEM),
     ]

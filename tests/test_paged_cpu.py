@@ -68,6 +68,7 @@ def test_null_checks_without_device(skv):
                                      0) == skv.EINVAL
     assert b"null" in L.swiftkv_last_error()
     assert L.swiftkv_paged_keep(None, None, 0, 1, 0, pos, pos, 1, 1, None) == skv.EINVAL
+    assert L.swiftkv_debug_set_paged_rows(None, 0) == skv.EINVAL
     assert L.swiftkv_paged_cache_bytes(None) == 0 and L.swiftkv_paged_cache_destroy(None) == skv.OK
 
 
@@ -81,6 +82,7 @@ def test_plan_stays_within_the_workspace(skv, heads, kv, n, batch, split):
     for longest in (0, 1, 200, 4095, 120000):
         at = [longest] + [int(x) for x in rng.integers(-1, longest + 1, batch - 1)]
         rows, chunks, splits, tokens = skv.paged_plan(heads, kv, n, at, split_tokens=split)
+        assert rows in (16, 32, 48, 64, 128, 256) and (rows > 16 or chunks == 1)
         assert rows * chunks >= n * (heads // kv) > rows * (chunks - 1)
         assert tokens % 128 == 0 and splits * tokens >= longest + n > (splits - 1) * tokens
         if splits > 1:
