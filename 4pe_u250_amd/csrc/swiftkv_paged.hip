@@ -79,40 +79,61 @@ __global__ __launch_bounds__(kRowThreads) void paged_append_kernel(const PagedRo
     }
 }
 
-// The reverse, with the same lanes (16-bit patterns of either type): workgroup
-// (key/value head, step, layer and sequence).
-template <int HD>
+// The reverse (16-bit patterns of either type): workgroup (HEADS key/value heads of a
+// layer, window of OCTETS octets of tokens, sequence).  All loads of a thread go out
+// before the first is waited for, and of few tokens a workgroup takes four heads' where
+// that leaves enough of them: 8 tokens of 64 sequences, 32 layers and 8 heads 37 us a
+// launch (49 with one head and step a workgroup and K's loads behind V's transposition),
+// for which the cells' lines bound it: a token's K is 16 bytes of 16 lines, an octet's V
+// 2 KiB.  A prompt of 4095 tokens and 32 heads 21 us, 6.3 TB/s read and written.
+template <int HD, int OCTETS, int HEADS>
 __global__ __launch_bounds__(kRowThreads) void paged_values_kernel(const PagedRowsArgs a, int batch) {
     using T = uint16_t;
-    constexpr int kChunks = HD / 8, kItems = kStepTokens * kChunks / kRowThreads;
+    typedef T Eight __attribute__((ext_vector_type(8)));
+    constexpr int kChunks = HD / 8, kTokens = 8 * OCTETS, kItems = HEADS * OCTETS * HD / kRowThreads;
     constexpr int kPitch = HD + 8;
-    __shared__ __align__(16) T rows[kStepTokens * kPitch];
-    const int kh = blockIdx.x, b = blockIdx.z % batch, layer = blockIdx.z / batch;
+    static_assert(HEADS * OCTETS * HD % kRowThreads == 0 && HD % 64 == 0 && 8 % (64 / kChunks) == 0, "a wave's items are of one octet");
+    __shared__ __align__(16) T rows[HEADS * kTokens * kPitch];
+    const int kh0 = blockIdx.x * HEADS, b = blockIdx.z % static_cast<uint32_t>(batch), layer = blockIdx.z / static_cast<uint32_t>(batch);
     const int p = a.positions[b], end = p + a.n;
     if (p < 0) return;
-    const int step = p / kStepTokens + static_cast<int>(blockIdx.y), tok0 = step * kStepTokens;
-    if (tok0 >= end) return;
-    const uint8_t* const cells = step_cells(a.view, a.slot0 + b, a.layer + layer, kh, step);
-    if (cells == nullptr) return;
+    const int octet0 = p / 8 + static_cast<int>(blockIdx.y) * OCTETS;
+    if (octet0 * 8 >= end) return;
+    // Item it * kRowThreads + thread: head, octet, and a channel of V or a token and chunk of
+    // K.  (What lies behind the last token takes that one's place, and is not written.)
+    const uint32_t wave0 = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u), lane = threadIdx.x & 63, chunk = lane % kChunks;
+    const int32_t* const table = a.view.table + static_cast<int64_t>(a.slot0 + b) * a.view.entries;
+    const int64_t page_bytes = a.view.kv_heads * paged_record_bytes(HD);
+    const uint8_t* const head0 = a.view.base + paged_record(a.view, a.layer + layer, 0, kh0);
+    auto token_of = [&](int it) { return octet0 * 8 + static_cast<int>((it * kRowThreads + wave0 + lane) / kChunks % kTokens); };
+    Eight kk[kItems], vv[kItems];
+    int page[kItems];
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, octet = item / HD, channel = item % HD;
-        if (tok0 + octet * 8 >= end || tok0 + octet * 8 + 8 <= p) continue;
-        const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(cells + v_cell(octet, channel, HD));
+        const uint32_t first = it * kRowThreads + wave0, head = first / (OCTETS * HD);
+        const int octet = min(octet0 + static_cast<int>(first / HD % OCTETS), (end - 1) / 8);
+        page[it] = table[octet * 8 / kPageTokens];
+        const uint8_t* const cells = head0 + head * paged_record_bytes(HD) + max(page[it], 0) * page_bytes + octet * 8 / kStepTokens % kPageSteps * paged_step_bytes(HD);
+        kk[it] = *reinterpret_cast<const Eight*>(cells + k_cell(min(max(token_of(it), p), end - 1) % kStepTokens, chunk));
+        vv[it] = *reinterpret_cast<const Eight*>(cells + v_cell(octet % 4, first % HD + lane, HD));
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) rows[(octet * 8 + j) * kPitch + channel] = w.v[j];
+    for (int it = 0; it < kItems; ++it) {
+        const uint32_t item = it * kRowThreads + threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rows[(item / HD * 8 + j) * kPitch + item % HD] = vv[it][j];
     }
     __syncthreads();
     const int64_t stride = static_cast<int64_t>(a.view.kv_heads) * HD;
     const int64_t row0 = layer * a.layer_rows + static_cast<int64_t>(b) * a.n - p;
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
-        const int item = it * kRowThreads + threadIdx.x, t = item / kChunks, chunk = item % kChunks;
-        const int tok = tok0 + t;
-        if (tok < p || tok >= end) continue;
-        const int64_t at = (row0 + tok) * stride + kh * HD + 8 * chunk;
-        *reinterpret_cast<Vec8<T>*>(static_cast<T*>(a.k_out) + at) = *reinterpret_cast<const Vec8<T>*>(cells + k_cell(t, chunk));
-        *reinterpret_cast<Vec8<T>*>(static_cast<T*>(a.v_out) + at) = *reinterpret_cast<const Vec8<T>*>(rows + t * kPitch + 8 * chunk);
+        const int tok = token_of(it), head = (it * kRowThreads + wave0) / (OCTETS * HD);
+        if (page[it] < 0 || tok < p || tok >= end) continue;
+        const int64_t at = (row0 + tok) * stride + (kh0 + head) * HD + 8 * chunk;
+        *reinterpret_cast<Eight*>(static_cast<T*>(a.k_out) + at) = kk[it];
+        *reinterpret_cast<Eight*>(static_cast<T*>(a.v_out) + at) =
+            *reinterpret_cast<const Eight*>(rows + (head * kTokens + tok - octet0 * 8) * kPitch + 8 * chunk);
     }
 }
 
@@ -202,8 +223,11 @@ void with_half(ElementType t, F&& f) {
     else f(_Float16{});
 }
 
-// (layer, key/value head, sequence) triples from which a workgroup keeps four heads' rows.
-constexpr int kManyKeeps = 4096;
+// (layer, key/value head, sequence) triples from which a workgroup takes four heads' few rows.
+constexpr int kManyHeads = 4096;
+int heads_of(const PagedView& v, int layers, int batch) {
+    return v.kv_heads % 4 == 0 && layers * v.kv_heads * batch >= kManyHeads ? 4 : 1;
+}
 
 int touched_steps(int n) { return (n + 2 * kStepTokens - 2) / kStepTokens; }
 
@@ -227,14 +251,20 @@ hipError_t launch_paged_append(const PagedRowsArgs& a, const PagedTree* tree, in
 }
 
 hipError_t launch_paged_values(const PagedRowsArgs& a, int layers, int batch, hipStream_t s) {
-    const dim3 grid(a.view.kv_heads, touched_steps(a.n), layers * batch);
-    if (a.view.head_dim == 64) paged_values_kernel<64><<<grid, kRowThreads, 0, s>>>(a, batch);
-    else paged_values_kernel<128><<<grid, kRowThreads, 0, s>>>(a, batch);
+    auto go = [&](auto octets, auto heads) {
+        constexpr int OCTETS = decltype(octets)::value, HEADS = decltype(heads)::value;
+        const dim3 grid(a.view.kv_heads / HEADS, (a.n + 6 + 8 * OCTETS) / (8 * OCTETS), layers * batch);
+        if (a.view.head_dim == 64) paged_values_kernel<64, OCTETS, HEADS><<<grid, kRowThreads, 0, s>>>(a, batch);
+        else paged_values_kernel<128, OCTETS, HEADS><<<grid, kRowThreads, 0, s>>>(a, batch);
+    };
+    using std::integral_constant;
+    if (a.n <= 9 && heads_of(a.view, layers, batch) == 4) go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    else go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     return hipGetLastError();
 }
 
 hipError_t launch_paged_keep(const PagedKeepArgs& a, int layers, int batch, hipStream_t s) {
-    const int heads = a.m <= 8 && a.view.kv_heads % 4 == 0 && layers * a.view.kv_heads * batch >= kManyKeeps ? 4 : 1;
+    const int heads = a.m <= 8 ? heads_of(a.view, layers, batch) : 1;
     const dim3 grid(layers * (a.view.kv_heads / heads), batch);
     auto go = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
