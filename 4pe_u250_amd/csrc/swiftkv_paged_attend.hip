@@ -33,13 +33,13 @@ __device__ __forceinline__ v2f fetch2(const float* p) {
 // count themselves; the last to arrive joins all in split order, so the result does not
 // depend on who that is.  32 rows are too many for one workgroup to join in good time:
 // a launch of paged_join_kernel does it.
-template <typename T, int HD, int R, int RT, typename Tree>
+template <typename T, int HD, int R, int RT, bool ONCE, typename Tree>
 __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const PagedAttendArgs a, const Tree tree) {
     using Tile = RowTile<T, HD, R, R * RT == 16>;
     constexpr int ROWS = R * RT, THREADS = kAttendThreads;
     using S = Share<ROWS, Tree>;
     constexpr int NL = Tile::NL, CG = HD / 4, kPitch = HD + 8;
-    constexpr int kPolicy = 2;                   // nontemporal: a page is read once
+    constexpr int kPolicy = ONCE ? 2 : 0;        // 2: nontemporal
     constexpr int kStepBytes = 2 * kStepTokens * HD * 2;
     __shared__ __align__(16) v4f lds[kWaves * CG * (ROWS + 1)];     // queries, then the waves' sums
     __shared__ float stats[kWaves][ROWS][2];
@@ -287,15 +287,26 @@ hipError_t launch_paged_attend(const PagedAttendArgs& a, const PagedTree* tree, 
     with_shape(a, t, [&](auto tag, auto hd) {
         using T = decltype(tag);
         constexpr int HD = decltype(hd)::value;
-        auto go = [&](auto r, auto rt) {
+        auto go = [&](auto r, auto rt, auto once) {
             constexpr int R = decltype(r)::value, RT = decltype(rt)::value;
-            if (tree) paged_attend_kernel<T, HD, R, RT><<<grid, kAttendThreads, 0, s>>>(a, *tree);
-            else paged_attend_kernel<T, HD, R, RT><<<grid, kAttendThreads, 0, s>>>(a, PagedChain{});
+            constexpr bool ONCE = decltype(once)::value;
+            if (tree) paged_attend_kernel<T, HD, R, RT, ONCE><<<grid, kAttendThreads, 0, s>>>(a, *tree);
+            else paged_attend_kernel<T, HD, R, RT, ONCE><<<grid, kAttendThreads, 0, s>>>(a, PagedChain{});
         };
         using std::integral_constant;
-        if (rows == 16) go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-        else if (rows == 32) go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-        else go(integral_constant<int, 16>{}, integral_constant<int, 3>{});
+        using std::true_type;
+        using std::false_type;
+        constexpr integral_constant<int, 1> one{};
+        constexpr integral_constant<int, 2> two{};
+        constexpr integral_constant<int, 3> three{};
+        constexpr integral_constant<int, 16> narrow{};
+        constexpr integral_constant<int, 32> wide{};
+        if (rows == 16) go(narrow, one, true_type{});
+        else if (rows == 48) go(narrow, three, true_type{});
+        else if (rows == 32 && a.chunks == 1) go(wide, one, true_type{});
+        else if (rows == 32) go(wide, one, false_type{});
+        else if (a.chunks == 1) go(wide, two, true_type{});
+        else go(wide, two, false_type{});
     });
     return hipGetLastError();
 }

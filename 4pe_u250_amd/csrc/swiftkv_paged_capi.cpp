@@ -39,7 +39,7 @@ constexpr int64_t kMaxPartialRows = int64_t(1) << 16;
 constexpr size_t kPartialFloats = static_cast<size_t>(kMaxPartialRows) * (2 + 128);
 
 // Turns (below) from which workgroups of more than 32 rows pay; for one sequence.
-constexpr int64_t kManyTurns = 2048, kManyTurnsAlone = 16384;
+constexpr int64_t kManyTurns = 32768;
 
 // What every call on a range of sequences of a paged cache checks.
 int check_call(const swiftkv_context* ctx, const swiftkv_paged_cache* c, int32_t layer, int32_t layers, int32_t seq0,
@@ -150,14 +150,15 @@ int append_rows(const swiftkv_context* ctx, const PagedRotation& rotation, const
 
 // The kernel of a call goes by its rows (query tokens times grouped heads) and by turns,
 // steps times chunks of 256 rows times key/value heads.  Up to 16 and 32 rows a workgroup
-// holds them all.  More go, where turns are few, by 32 to workgroups of their own, whose
-// repeated reads the L2s serve; where they are many, to workgroups of 48 (three tiles of 16
-// rows a wave: loads bound these), 64, 128 or 256 (cells shared in LDS).  us of a call onto
-// 4031 tokens, 32 heads over 8, the kernel taken against the next: 8 sequences x 16 tokens
-// (64 rows) 64 34.9, 32 37.0; x 24 (96 rows) 128 42.1, 32 49.8, 64 44.4; x 64 (256 rows) 256
-// 68, 32 99, 64 72; 64 x 12 (48 rows) 48 192, 64 203; 64 x 16 64 204, 32 290; one sequence x 26
-// 32 16.6, 64 25.8, 128 27; x 64 32 26.1, 64 26.5, 256 37.  Long chunks of one sequence read few
-// cells for many rows: 512 tokens onto 4095 32 59.9, 64 72, 256 68; 4096 onto none 256 176, 32 258.
+// holds them all.  Where turns are many, its cells shall be read by few workgroups: 48 rows
+// (three tiles of 16 a wave: loads bound these), 64 (two of 32), 128 or 256 (cells shared in
+// LDS).  Where they are few, workgroups shall be many: 32 rows, or 64 where 32 would leave a
+// CU more than one.  us of a call onto 4031 tokens, 32 heads over 8, the kernel taken against
+// others: 64 sequences x 12 tokens (48 rows) 48 190, 64 192, 32 209; x 16 64 196, 128 217; x 24
+// 128 230, 32 265; x 64 256 353, 128 413, 64 502; 8 x 16 32 31.6, 64 34.4; x 24 32 38.5, 64
+// 40.0, 128 42.7; x 32 64 42.0, 32 43.1; x 64 64 59.4, 32 69.2, 256 65.5; one sequence x 26 32
+// 16.9, 64 21.7; x 512 64 53.1, 32 61.8, 256 66.9; x 1024 64 102, 256 112; 4 x 512 256 168, 64
+// 200; a prompt of 2048 tokens 64 79.4, 32 75.1, 128 73.0; of 4096 256 176, 64 209.
 //
 // Splits make a workgroup for each CU and not more, of at most 32 a sequence and at most the
 // square root of its 64-token tiles, since they are joined: us of a step, tokens of this
@@ -171,27 +172,29 @@ PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t forced_rows,
     auto steps_of = [&](int32_t b) {
         return positions[b] < 0 ? 0 : (static_cast<int64_t>(positions[b]) + n + kStepTokens - 1) / kStepTokens;
     };
-    int64_t turns = 0, longest = 1;
+    int64_t turns = 0, longest = 1, live = 0;
     for (int32_t b = 0; b < batch; ++b) {
+        live += positions[b] >= 0;
         turns += steps_of(b);
         longest = std::max(longest, steps_of(b));
     }
     turns *= (rows + 255) / 256 * kv_heads;
     if (rows <= 16) p.rows = 16;
     else if (forced_rows > 0) p.rows = forced_rows;
-    else if (rows <= 32 || turns < kManyTurns || (batch == 1 && turns < kManyTurnsAlone)) p.rows = 32;
+    else if (rows <= 32 || (turns < kManyTurns && rows * kv_heads * live < 32 * cus)) p.rows = 32;
+    else if (turns < kManyTurns) p.rows = 64;
     else p.rows = rows <= 48 ? 48 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     p.chunks = static_cast<int32_t>((rows + p.rows - 1) / p.rows);
     const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.chunks;
     auto whole = [](int64_t steps) { return (steps + kSplitQuantumSteps - 1) / kSplitQuantumSteps * kSplitQuantumSteps; };
     auto groups = [&](int64_t per) {
         int64_t sum = 0;
-        for (int32_t b = 0; b < batch; ++b) sum += std::max<int64_t>(1, (steps_of(b) + per - 1) / per);
+        for (int32_t b = 0; b < batch; ++b) sum += (steps_of(b) + per - 1) / per;
         return sum * kv_heads * p.chunks;
     };
     const int64_t most_splits = std::min<int64_t>(32, std::ceil(std::sqrt(longest / 2.0)));
     int64_t low = whole((longest + most_splits - 1) / most_splits), per = whole(longest);
-    if (pairs < cus)
+    if (live * kv_heads * p.chunks < cus)
         while (low < per) {              // the fewest steps with which the workgroups find a CU each
             const int64_t middle = whole((low + per - kSplitQuantumSteps) / 2);
             if (groups(middle) <= cus) per = middle;
@@ -457,7 +460,7 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
             });
         PagedTree tree;
         const PagedTree* const trees = tree_of(tree, parents, b0, nb, n);
-        SKV_HIP(plan.rows <= 48 ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)
+        SKV_HIP(plan.rows <= 64 ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)
                                 : launch_paged_many(a, trees, nb, plan.rows, cache->type, ctx->stream));
         if (plan.splits > 1 && plan.rows > 16)
             SKV_HIP(launch_paged_join(a, trees, nb, plan.rows, cache->type, ctx->stream));

@@ -24,7 +24,7 @@ template <int HD, int RW>
 struct ManyShape {
     static constexpr int TEAMS = kManyWaves / RW, ROWS = 32 * RW;
     static constexpr int kHalfBytes = kStepTokens * HD * 2;  // K or V of a step
-    static constexpr int SLOTS = TEAMS < 4 || HD == 64 ? 3 : 2;
+    static constexpr int SLOTS = 3;
     static constexpr int kRing = 2 * SLOTS * TEAMS * kHalfBytes;
     static constexpr int kMerge = TEAMS * (HD / 4) * (ROWS + 1) * 16;
     static constexpr int kQueries = ROWS * (HD + 8) * 2;
@@ -220,8 +220,7 @@ hipError_t launch_paged_many(const PagedAttendArgs& a, const PagedTree* tree, in
         else paged_many_kernel<T, HD, RW><<<grid, kManyThreads, 0, s>>>(a, PagedChain{});
     };
     auto shaped = [&](auto tag, auto hd) {
-        if (rows == 64) go(tag, hd, integral_constant<int, 2>{});
-        else if (rows == 128) go(tag, hd, integral_constant<int, 4>{});
+        if (rows == 128) go(tag, hd, integral_constant<int, 4>{});
         else go(tag, hd, integral_constant<int, 8>{});
     };
     auto typed = [&](auto tag) {
