@@ -60,10 +60,9 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
     uint8_t* const layer_head = a.view.base + paged_record(a.view, a.layer, 0, kh);
     const int64_t page_bytes = a.view.kv_heads * paged_record_bytes(HD);
 
-    // A wave appends the call's rows to the steps that it will scan.  (Another wave or
-    // workgroup that reads them for other rows writes the same bytes.)
-    if (a.k != nullptr && share.template append<T, HD, 64, kWaves>(a, table, layer_head, page_bytes, lane, wave))
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the scan's loads find them
+    // The call's rows are appended by every workgroup that scans them, with the same bytes:
+    // its own writes are what it finds then.
+    if (a.k != nullptr) share.template append<T, HD, THREADS>(a, table, layer_head, page_bytes, wave, lane);
 
     T* const staged = reinterpret_cast<T*>(lds);
     share.template stage_queries<T, HD, THREADS>(a, staged);

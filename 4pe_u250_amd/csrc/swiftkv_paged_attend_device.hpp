@@ -338,34 +338,25 @@ struct Share {
             }
         }
     }
-    // The call's rows that fall into steps [begin, end) of the split -- with WAVES, a step of
-    // each WAVES-th from the wave-th -- to the cache, by THREADS threads, N chunks' loads of
-    // each at a time (two are quicker where a wave has several, and slower code where it has
-    // one: 26 tokens 16.6 us a call against 17.7, one token 10.6 against 10.8); whether
-    // there were any.
-    template <typename T, int HD, int THREADS, int WAVES>
-    __device__ __forceinline__ bool append(const PagedAttendArgs& a, const int32_t* table, uint8_t* layer_head, int64_t page_bytes, int thread,
-                                           int wave) const {
-        constexpr int kChunks = HD / 8;
-        constexpr int N = ROWS == 32 || ROWS == 48 ? 2 : 1;
+    // The call's rows that fall into the split's steps to the cache, by the whole workgroup, N
+    // chunks' loads of a thread at a time (two are quicker where it has several, and slower
+    // code where it has one: us of a step, 26 tokens 15.2 and 15.6, one token 10.8 and 10.6).
+    // What it writes has arrived when it returns; everyone's has behind the next barrier.
+    template <typename T, int HD, int THREADS>
+    __device__ __forceinline__ void append(const PagedAttendArgs& a, const int32_t* table, uint8_t* layer_head, int64_t page_bytes, int wave,
+                                           int lane) const {
+        constexpr int kChunks = HD / 8, N = ROWS == 32 || ROWS == 48 || ROWS == 64 ? 2 : 1;
+        static_assert(64 % kChunks == 0, "a thread's chunk stays");
+        const int t0 = max(p, step_begin * kStepTokens), t1 = min(p + count, step_end * kStepTokens);
+        if (p < 0 || t0 >= t1) return;
         const bool fast = aligned_rotation(a.rotation);
-        bool any = false;
-        if (p < 0) return false;
-        const int first_step = max(p / kStepTokens, step_begin), my_step = first_step + ((wave - (first_step - step_begin)) & (WAVES - 1));
+        const int items = (t1 - t0) * kChunks, c = lane % kChunks;
 #pragma unroll 1
-        for (int s = my_step; WAVES == 1 ? !any : s < step_end; s += WAVES) {
-        const int t0 = max(p, (WAVES == 1 ? step_begin : s) * kStepTokens), t1 = min(p + count, (WAVES == 1 ? step_end : s + 1) * kStepTokens);
-        if (t0 >= t1) break;
-        const int items = (t1 - t0) * kChunks;
-        any = true;
-#pragma unroll 1
-        for (int base = 0; base < items; base += N * THREADS) {
+        for (int base = wave * 64; base < items; base += N * THREADS) {
             Chunk<T> k[N];
             Half8<T> v[N];
             int page[N];
-            auto token_of = [&](int x) { return t0 + min(base + x * THREADS + thread, items - 1) / kChunks; };
-            const int c = thread % kChunks;
-            static_assert(THREADS % kChunks == 0, "a thread's chunk stays");
+            auto token_of = [&](int x) { return t0 + min(base + x * THREADS + lane, items - 1) / kChunks; };
 #pragma unroll
             for (int x = 0; x < N; ++x) {
                 const int tok = token_of(x), i = tok - p;
@@ -380,7 +371,7 @@ struct Share {
 #pragma unroll
             for (int x = 0; x < N; ++x) {
                 const int tok = token_of(x), step = tok / kStepTokens, t = tok % kStepTokens;
-                if (base + x * THREADS + thread >= items || page[x] < 0) continue;
+                if (base + x * THREADS + lane >= items || page[x] < 0) continue;
                 uint8_t* const cells = layer_head + page[x] * page_bytes + (step % kPageSteps) * paged_step_bytes(HD);
                 *reinterpret_cast<Half8<T>*>(cells + k_cell(t, c)) = fast ? k[x].turned(c, a.rotation) : k[x].own;
                 T* const dst = reinterpret_cast<T*>(cells + v_cell(t / 8, 8 * c, HD)) + t % 8;
@@ -388,8 +379,7 @@ struct Share {
                 for (int j = 0; j < 8; ++j) dst[8 * j] = v[x][j];
             }
         }
-        }
-        return any;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     // A row's values, sums over the sum of weights: zero for rows without a token.
     template <typename T, int HD>

@@ -86,8 +86,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     // same bytes: its own writes are what it finds then.
     const bool late = a.k != nullptr && share.p >= 0 && (step_begin + SLOTS * TEAMS) * kStepTokens > share.p;
     if (!late) load_first();
-    if (a.k != nullptr && share.template append<T, HD, kManyThreads, 1>(a, table, layer_head, page_bytes, threadIdx.x, 0))
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (a.k != nullptr) share.template append<T, HD, kManyThreads>(a, table, layer_head, page_bytes, wave, lane);
     T* const staged = reinterpret_cast<T*>(lds + M::kRing);
     share.template stage_queries<T, HD, kManyThreads>(a, staged);
     __syncthreads();
