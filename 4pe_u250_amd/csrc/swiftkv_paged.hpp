@@ -1,6 +1,6 @@
 // swiftkv_paged.hpp -- layout and kernel arguments of the paged cache, shared by
 // swiftkv_paged_capi.cpp and the kernels (swiftkv_paged.hip,
-// swiftkv_paged_attend.hip).
+// swiftkv_paged_attend.hip, swiftkv_paged_many.hip).
 #pragma once
 
 #include "swiftkv_block.hpp"
@@ -95,7 +95,7 @@ struct PagedAttendArgs {
     PagedRotation rotation;
     const void* q;
     void* out;
-    const void* k;        // new rows, appended by the same launch (chunks == 1 only); null: none
+    const void* k;        // new rows, appended by the same launch (n <= kTreeTokens); null: none
     const void* v;
     int64_t q_stride;
     int64_t out_stride;
@@ -132,7 +132,7 @@ struct PagedMapArgs {
     int32_t pages[kMapEntries];
 };
 
-// Rows of an attention workgroup's chunk.
+// A split is a multiple of so many steps.
 constexpr int kSplitQuantumSteps = 4;
 
 hipError_t launch_paged_map(const PagedMapArgs& a, hipStream_t s);
@@ -141,9 +141,9 @@ hipError_t launch_paged_append(const PagedRowsArgs& a, const PagedTree* tree, in
 hipError_t launch_paged_values(const PagedRowsArgs& a, int layers, int batch, hipStream_t s);
 hipError_t launch_paged_keep(const PagedKeepArgs& a, int layers, int batch, hipStream_t s);
 hipError_t launch_paged_copy(const PagedView& v, int64_t from, int64_t to, hipStream_t s);
-// rows: of a chunk, 16 or 32 (a.chunks == 1)
+// rows: of a chunk, 16 (a.chunks == 1), 32, 48 or 64
 hipError_t launch_paged_attend(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);
-// rows: 64, 128 or 256; a.k null
+// rows: 128 or 256
 hipError_t launch_paged_many(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);
 // The splits of such calls, of more than 16 rows
 hipError_t launch_paged_join(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s);

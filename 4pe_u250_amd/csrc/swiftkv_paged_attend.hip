@@ -23,15 +23,21 @@ __device__ __forceinline__ v2f fetch2(const float* p) {
     return v2f{__uint_as_float(static_cast<uint32_t>(w)), __uint_as_float(static_cast<uint32_t>(w >> 32))};
 }
 
-// All rows of a (sequence, key/value head), R at most, over the steps of one split.
-// Reading the cells bounds it: each wave takes steps w, w + 4, ... and loads their
-// cells as operands, 1 KiB of consecutive bytes an instruction and past the caches,
-// K of the next step during the softmax and V after the products, as registers fall
-// free.  The waves meet in LDS.
+// ROWS = R * RT rows of a (sequence, key/value head) over the steps of one split.  Reading
+// the cells bounds it: each wave takes steps w, w + 4, ... and loads their cells as
+// operands, 1 KiB of consecutive bytes an instruction, K of the next step during the softmax
+// and V after the products, as registers fall free; with RT > 1 each serves RT tiles of
+// rows.  The waves meet in LDS.  One token of 64 sequences at 4096 170 us, 6.3 TB/s of
+// K and V; 64 rows of each 196 us, 5.4 TB/s.  Where chunks share the cells, what a CU's loads
+// deliver bounds it: 512 tokens onto 4095 53 us and 0.68 PFLOP/s with 64 rows, 62 with 32.
+//
+// ONCE: no other workgroup reads the cells, and they pass the caches (64 sequences x 16
+// tokens 196 us, kept in the caches 210); if others do they stay (512 tokens 53 us, passing
+// the caches 54; 64 tokens of 8 sequences 59 and 70).
 //
 // 16 rows: a sequence's splits publish (m, l, sums), wait until that has arrived, and
 // count themselves; the last to arrive joins all in split order, so the result does not
-// depend on who that is.  32 rows are too many for one workgroup to join in good time:
+// depend on who that is.  More rows are too many for one workgroup to join in good time:
 // a launch of paged_join_kernel does it.
 template <typename T, int HD, int R, int RT, bool ONCE, typename Tree>
 __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const PagedAttendArgs a, const Tree tree) {

@@ -1,6 +1,6 @@
 // swiftkv_paged_capi.cpp -- host side of the paged cache (include/swiftkv.h):
 // objects, argument checks, launch plans.  Kernels: swiftkv_paged.hip,
-// swiftkv_paged_attend.hip.  As in swiftkv_capi.cpp no exception crosses the C
+// swiftkv_paged_attend.hip, swiftkv_paged_many.hip.  As in swiftkv_capi.cpp no exception crosses the C
 // boundary, and a refused call enqueues nothing.
 #include "swiftkv_block_host.hpp"
 
@@ -38,7 +38,7 @@ constexpr int64_t kMaxSplitGroups = 2048;
 constexpr int64_t kMaxPartialRows = int64_t(1) << 16;
 constexpr size_t kPartialFloats = static_cast<size_t>(kMaxPartialRows) * (2 + 128);
 
-// Turns (below) from which workgroups of more than 32 rows pay; for one sequence.
+// Turns (plan_attention) from which they are many.
 constexpr int64_t kManyTurns = 32768;
 
 // What every call on a range of sequences of a paged cache checks.
