@@ -337,6 +337,51 @@ def test_keep(skv, ctx, t, dim):
     rig.check_values()
 
 
+@pytest.mark.parametrize("t,dim,capacity", [("bf16", 64, 128), ("f16", 128, 64)])
+def test_few_rows_of_many_heads(skv, ctx, t, dim, capacity):
+    """Enough heads that a workgroup takes four: rows kept and read at every place in an octet, over pages' ends."""
+    layers, batch = 32, 16
+    rig = P.Rig(skv, ctx, t, 8, 8, dim, batch=batch, layers=layers, capacity=capacity, seed=dim)
+    rig.map_all()
+    for layer in range(layers):
+        rig.append([0] * batch, capacity, layer=layer)
+    places = [(5 * b) % (capacity - 9) for b in range(batch - 2)] + [-1, capacity - 9]
+    for n in range(1, 10):
+        got = rig.values(places, n, 0, layers)
+        for b, p in enumerate(places):
+            for layer in range(layers):
+                for g, w in zip(got, rig.rows(layer, b, np.arange(max(p, 0), max(p, 0) + n))):
+                    if p < 0:
+                        assert np.isnan(g[layer, b]).all()       # as they were, 0xff
+                    else:
+                        np.testing.assert_array_equal(g[layer, b], w)
+    room = min(capacity, 64)
+    paths = [sorted(int(a) for a in rig.rng.choice(room - 9, 8, replace=False)) for _ in range(batch)]
+    rig.keep([min(p, capacity - room + 9) if p >= 0 else p for p in places], paths)
+    rig.check_values()
+
+
+@pytest.mark.parametrize("n", [1, 5, 40, 100])
+def test_sequences_that_sit_out(skv, ctx, n):
+    """All of a call's sequences, or all but one long one."""
+    rig = P.Rig(skv, ctx, "bf16", 8, 2, 64, batch=64, pages=60, capacity=3200, rotation=P.Rotation(64), seed=n)
+    rig.map(40, list(range(50)))
+    rig.append([-1] * 40 + [0] + [-1] * 23, 3000)
+    _, out = rig.attend([-1] * 64, n)
+    assert (out == 0).all()
+    rig.check_attention([-1] * 40 + [2990] + [-7] * 23, n)
+
+
+@pytest.mark.parametrize("heads", [4, 20, 40, 64])
+def test_the_longest_sequence(skv, ctx, heads):
+    rig = P.Rig(skv, ctx, "f16", heads, 1, 64, capacity=131072, seed=heads)
+    rig.map_all()
+    rig.append([0], 131072)
+    rig.check_attention([131071], 1)
+    if heads < 40:
+        rig.check_attention([131072 - 9], 9, [[-1] + [(i - 1) // 2 for i in range(1, 9)]])
+
+
 def test_shared_prefix(skv, ctx):
     """Sequences that share their first pages, each with a copy of the one that it goes on in."""
     rig = P.Rig(skv, ctx, "bf16", 4, 2, 64, batch=3, pages=9, layers=2, capacity=256, rotation=P.Rotation(64), seed=6)
