@@ -114,6 +114,11 @@ struct PagedAttendArgs {
     float* partials;      // [pair][split]: stats [rows of a chunk][2], then sums [rows][head_dim]
     uint32_t* counters;   // [pair] arrived splits, kCounterStride apart, zero between launches
     PagedRow order[kPagedBatch];      // of each grid row, longest first
+    // Not 0: the grid is one row of so many splits, first_split[y] the sum of those before
+    // order[y]'s (two a word; all ones behind the last).
+    int32_t all_splits;
+    int32_t batch;
+    uint32_t first_split[kPagedBatch / 2];
 };
 
 struct PagedKeepArgs {

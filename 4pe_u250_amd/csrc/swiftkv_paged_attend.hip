@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane / R, place = lane % R;
     S share;
-    share.start(a, tree, blockIdx.x, lane);
+    share.start(a, tree, lane);
     if (share.split >= share.my_splits) return;
     const int b = share.b, kh = share.kh, p = share.p, step_begin = share.step_begin, step_end = share.step_end;
 
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(const PagedA
     Share<ROWS, Tree> share;
     // (heads fastest, as the workgroups that left the partial results)
     const int kh = blockIdx.x % a.view.kv_heads, id = blockIdx.x / a.view.kv_heads, part = id % (ROWS / kRows);
-    share.start(a, tree, kh + id / (ROWS / kRows) * a.view.kv_heads * a.splits, threadIdx.x & 63);
+    share.start(a, tree, blockIdx.y, kh + id / (ROWS / kRows) * a.view.kv_heads * a.splits, a.splits, threadIdx.x & 63);
     const int row = part * kRows + threadIdx.x / CG, quad = threadIdx.x % CG;
     if (share.my_splits == 1 || row >= share.rows) return;
     Joined all;
@@ -288,7 +288,7 @@ void with_shape(const PagedAttendArgs& a, ElementType t, F&& f) {
 }  // namespace
 
 hipError_t launch_paged_attend(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s) {
-    const dim3 grid(a.view.kv_heads * a.splits * a.chunks, batch);
+    const dim3 grid = a.all_splits ? dim3(a.view.kv_heads * a.chunks * a.all_splits) : dim3(a.view.kv_heads * a.chunks * a.splits, batch);
     with_shape(a, t, [&](auto tag, auto hd) {
         using T = decltype(tag);
         constexpr int HD = decltype(hd)::value;

@@ -256,16 +256,37 @@ struct Share {
     TreePlace place;
     uint64_t live;                               // tokens of the tree
 
-    // `id`: the workgroup's (split, chunk, head), heads fastest, so that a head's workgroups
-    // share an XCD's L2.
-    __device__ __forceinline__ void start(const PagedAttendArgs& a, const Tree& tree, int id, int lane) {
-        const PagedRow of_grid = a.order[blockIdx.y];
+    // The workgroup's share.  Consecutive workgroups go to XCDs in turn; if the splits that a
+    // short sequence does not have lay among them, some XCDs would get more than their CUs
+    // hold.  The grid is one row of the splits that there are then (trees of 16 sequences of up
+    // to 32511, 20 heads over 4: 99 us against 125).
+    __device__ __forceinline__ void start(const PagedAttendArgs& a, const Tree& tree, int lane) {
+        if (a.all_splits == 0) return start(a, tree, blockIdx.y, blockIdx.x, a.splits, lane);
+        typedef uint32_t Words __attribute__((ext_vector_type(kPagedBatch / 4), aligned(4)));
+        Words low = *reinterpret_cast<const Words*>(a.first_split), high = *reinterpret_cast<const Words*>(a.first_split + kPagedBatch / 4);
+        asm("" : "+s"(low), "+s"(high));
+        uint32_t mine = ~0u;
+#pragma unroll
+        for (int w = 0; w < kPagedBatch / 4; ++w) {
+            if (lane == w) mine = low[w];
+            if (lane == w + kPagedBatch / 4) mine = high[w];
+        }
+        const int unit = a.view.kv_heads * a.chunks, at = blockIdx.x / static_cast<uint32_t>(unit);
+        const int y = __popcll(__ballot(static_cast<int>(mine & 0xffffu) <= at)) + __popcll(__ballot(static_cast<int>(mine >> 16) <= at)) - 1;
+        auto first = [&](int i) { return static_cast<int>(static_cast<uint32_t>(__builtin_amdgcn_readlane(mine, i >> 1)) >> (i & 1) * 16 & 0xffffu); };
+        const int before = first(y), next = y + 1 < a.batch ? first(y + 1) : a.all_splits;
+        start(a, tree, y, blockIdx.x - before * unit, next - before, lane);
+    }
+    // `id`: the (split, chunk, head) of grid row y, heads fastest, so that a head's
+    // workgroups share an XCD's L2.
+    __device__ __forceinline__ void start(const PagedAttendArgs& a, const Tree& tree, int y, int id, int splits, int lane) {
+        const PagedRow of_grid = a.order[y];
         b = of_grid.sequence;
         p = of_grid.position;
         kh = id % a.view.kv_heads;
         id /= a.view.kv_heads;
-        split = id % a.splits;
-        chunk = a.chunks - 1 - id / a.splits;    // the longest first
+        split = id % splits;
+        chunk = a.chunks - 1 - id / splits;      // the longest first
         row_first = chunk * ROWS;
         rows = min(ROWS, a.group * a.n - row_first);
         count = a.n;

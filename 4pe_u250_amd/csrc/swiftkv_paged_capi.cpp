@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <iterator>
 #include <new>
 
 #include "swiftkv_paged.hpp"
@@ -37,6 +38,8 @@ constexpr int64_t kMaxGroups = int64_t(1) << 23;
 constexpr int64_t kMaxSplitGroups = 2048;
 constexpr int64_t kMaxPartialRows = int64_t(1) << 16;
 constexpr size_t kPartialFloats = static_cast<size_t>(kMaxPartialRows) * (2 + 128);
+
+constexpr int32_t kXcds = 8;
 
 // Turns (plan_attention) from which they are many.
 constexpr int64_t kManyTurns = 32768;
@@ -458,6 +461,21 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
             std::sort(a.order, a.order + nb, [](const PagedRow& x, const PagedRow& y) {
                 return x.position != y.position ? x.position > y.position : x.sequence < y.sequence;
             });
+        a.batch = nb;
+        a.all_splits = 0;
+        if (plan.splits > 1) {
+            std::fill(std::begin(a.first_split), std::end(a.first_split), ~0u);
+            for (int32_t y = 0; y < nb; ++y) {
+                uint32_t& word = a.first_split[y / 2];
+                const uint32_t first = static_cast<uint32_t>(a.all_splits);
+                word = y % 2 ? (word & 0xffffu) | first << 16 : (word & 0xffff0000u) | first;
+                const int32_t steps = a.order[y].position < 0 ? 0 : (a.order[y].position + n + kStepTokens - 1) / kStepTokens;
+                a.all_splits += std::max(1, (steps + plan.split_steps - 1) / plan.split_steps);
+            }
+            // Finding its split costs a workgroup 1 us, for nothing where none is missing or
+            // each is a workgroup on every XCD anyway.
+            if (a.all_splits == nb * plan.splits || view.kv_heads % kXcds == 0) a.all_splits = 0;
+        }
         PagedTree tree;
         const PagedTree* const trees = tree_of(tree, parents, b0, nb, n);
         SKV_HIP(plan.rows <= 64 ? launch_paged_attend(a, trees, nb, plan.rows, cache->type, ctx->stream)

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane / 32, place = lane % 32, row = wave % RW * 32 + place, team = wave / RW;
     Share<ROWS, Tree> share;
-    share.start(a, tree, blockIdx.x, lane);
+    share.start(a, tree, lane);
     if (share.split >= share.my_splits) return;
     const int step_begin = share.step_begin, step_end = share.step_end;
 
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
 
 hipError_t launch_paged_many(const PagedAttendArgs& a, const PagedTree* tree, int batch, int rows, ElementType t, hipStream_t s) {
     using std::integral_constant;
-    const dim3 grid(a.view.kv_heads * a.splits * a.chunks, batch);
+    const dim3 grid = a.all_splits ? dim3(a.view.kv_heads * a.chunks * a.all_splits) : dim3(a.view.kv_heads * a.chunks * a.splits, batch);
     auto go = [&](auto tag, auto hd, auto rw) {
         using T = decltype(tag);
         constexpr int HD = decltype(hd)::value, RW = decltype(rw)::value;
