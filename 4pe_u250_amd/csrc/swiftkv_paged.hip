@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append_kernel(const PagedRo
         place = tree_place(tree.parents, b, a.n, lane);
         end = p + __popcll(__ballot(place.live));
     }
-    if (tok0 >= end) return;
+    if (!step_has_new(tok0, p, end)) return;
     uint8_t* const cells = step_cells(a.view, a.slot0 + b, a.layer, kh, step);
     if (cells == nullptr) return;
     const int64_t row0 = static_cast<int64_t>(b) * a.n;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append_kernel(const PagedRo
         const int item = it * kRowThreads + threadIdx.x, t = item / kChunks, chunk = item % kChunks;
         const int tok = tok0 + t;
         const bool fresh = tok >= p && tok < end;
-        const int i = min(max(tok, p), end - 1) - p;         // (lanes without a row of their own take the nearest)
+        const int i = nearest_row(tok, p, end);
         int position = p + i;
         if constexpr (kTree) position = p + __popcll(from_lane(place.mask, i)) - 1;
         const Half8<T> kk = turned(k + (row0 + i) * a.k_stride, chunk, a.rotation, angles(a.rotation, position));

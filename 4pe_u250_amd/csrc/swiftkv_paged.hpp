@@ -4,6 +4,7 @@
 #pragma once
 
 #include "swiftkv_block.hpp"
+#include "swiftkv_paged_rows.hpp"
 
 namespace swiftkv {
 

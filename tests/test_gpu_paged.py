@@ -655,3 +655,26 @@ def test_pages_taken_and_given_back(skv, ctx):
     rig.check_attention([71], 5, [[-1, 0, 0, 1, 2]], seq0=1)
     with pytest.raises(skv.SwiftKVError):
         rig.append([0], 1)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 7, 33, 64])
+def test_trees_without_tokens_come_first(skv, ctx, t, n):
+    """Sequences that bring no tokens before and among ones that do, at every kind of place in a step, k and v in the
+    middle of larger buffers: nothing of theirs changes, and the others' rows are as ever."""
+    kv, dim = 2, 64
+    rig = P.Rig(skv, ctx, t, 4, kv, dim, batch=5, capacity=256, rotation=P.Rotation(dim), seed=n)
+    rig.map_all()
+    rig.append([0] * 5, 190)
+    rng = np.random.default_rng(n)
+    for at in ([5, 63, 100, 190, 64], [31, 32, 0, 1, 127], [190, 96, 33, 5, 95]):
+        trees = [P.random_tree(rng, n, c) for c in (0, 0, n, 0, (n + 1) // 2)]
+        (kr, k), (vr, v) = (rig.random(7, n, kv, dim) for _ in "kv")
+        row = 2 * n * kv * dim
+        dk, dv = ctx.to_device(kr), ctx.to_device(vr)
+        skv.swiftkv_paged_append(ctx, dk.ptr + row, dv.ptr + row, rig.cache, 0, at, n=n, table=rig.table, parents=sum(trees, []))
+        ctx.synchronize()
+        rig.note(at, k[1:6], v[1:6], trees)
+        rig.check_values()
+        rig.check_attention(at, n, trees)
+        rig.check_values()

@@ -55,6 +55,49 @@ def test_host_rules(tmp_path):
     subprocess.run([exe], check=True)
 
 
+def run_rules(tmp_path, text):
+    src = tmp_path / "rules.cpp"
+    src.write_text(text)
+    exe = str(tmp_path / "rules")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-D_GLIBCXX_ASSERTIONS", "-I",
+                    os.path.join(REPO, "4pe_u250_amd", "csrc"), str(src), "-o", exe], check=True)
+    subprocess.run([exe], check=True)
+
+
+APPENDED_ROWS = r"""
+#include <cassert>
+#include <initializer_list>
+#include "swiftkv_paged_rows.hpp"
+using namespace swiftkv;
+int main() {
+    for (int n : {1, 2, 7, 31, 32, 33, 64, 65, 100})
+        for (int p = 0; p < 200; ++p)
+            for (int count = 0; count <= n; ++count) {       // of a tree; n for a chain
+                int stored = 0;
+                for (int y = 0; y < (n + 62) / 32; ++y) {    // the launch's steps
+                    const int tok0 = (p / 32 + y) * 32, end = p + count;
+                    if (!step_has_new(tok0, p, end)) continue;
+                    for (int tok = tok0; tok < tok0 + 32; ++tok) {
+                        const int i = nearest_row(tok, p, end);
+                        assert(i >= 0 && i < count);         // every load is of a row that is there
+                        if (tok >= p && tok < end) {
+                            assert(i == tok - p);
+                            ++stored;
+                        }
+                    }
+                }
+                assert(stored == count);
+            }
+    return 0;
+}
+"""
+
+
+def test_rows_that_an_append_reads(tmp_path):
+    """None before a sequence's first or behind its last, for trees without tokens too."""
+    run_rules(tmp_path, APPENDED_ROWS)
+
+
 def test_null_checks_without_device(skv):
     L = skv.lib()
     pos = np.zeros(1, np.int32).ctypes.data_as(C.c_void_p)
