@@ -314,8 +314,8 @@ struct Share {
         return row_token(a.group_magic, row_first + min(row, rows - 1));
     }
     __device__ __forceinline__ int position(int i) const {
-        if constexpr (kTree) return p + __popcll(from_lane(place.mask, i)) - 1;
-        else return p + i;
+        if constexpr (kTree) return turn_position(p, __popcll(from_lane(place.mask, i)) - 1, live >> i & 1);
+        else return turn_position(p, i, true);
     }
     template <typename Tile>
     __device__ __forceinline__ void sees(const PagedAttendArgs& a, Tile& tile, int row) const {
@@ -346,7 +346,7 @@ struct Share {
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) {
                     const int row = row_of(it0 + k), i = token(a, row);
-                    x[k].load(source(i, row), c, a.rotation, angles(a.rotation, max(position(i), 0)));
+                    x[k].load(source(i, row), c, a.rotation, angles(a.rotation, position(i)));
                 }
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) leave(row_of(it0 + k), x[k].turned(c, a.rotation));
@@ -355,7 +355,7 @@ struct Share {
 #pragma unroll 1
             for (int it = 0; it < kItems; ++it) {
                 const int row = row_of(it), i = token(a, row);
-                leave(row, turned(source(i, row), c, a.rotation, angles(a.rotation, max(position(i), 0))));
+                leave(row, turned(source(i, row), c, a.rotation, angles(a.rotation, position(i))));
             }
         }
     }

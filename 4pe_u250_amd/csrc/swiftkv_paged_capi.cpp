@@ -96,7 +96,7 @@ int check_tokens(const swiftkv_paged_cache* c, const swiftkv_rotary_table* table
         }
         if (positions[b] < 0) continue;
         if (int rc = check_pages(c, seq0 + b, b, positions[b], count, writes)) return rc;
-        if (table && static_cast<int64_t>(positions[b]) + depth >= table->positions)
+        if (table && !turns_within(positions[b], depth, table->positions))
             return fail(SWIFTKV_ERANGE, "positions[%d] = %d: token positions up to %lld outside the table (%d)", b, positions[b],
                         static_cast<long long>(positions[b]) + depth, table->positions);
     }

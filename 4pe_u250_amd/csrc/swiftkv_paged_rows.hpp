@@ -18,4 +18,13 @@ SWIFTKV_RULE bool step_has_new(int tok0, int p, int end) { return p < end && tok
 // of [p, end) the nearest.
 SWIFTKV_RULE int nearest_row(int tok, int p, int end) { return (tok < p ? p : tok < end ? tok : end - 1) - p; }
 
+// The position by which a token's query and key are turned: p cached tokens and its depth
+// in the call.  Rows without a token and sequences that sit out (p < 0) are not turned by
+// positions that the call's checks have bounded, and take 0.
+SWIFTKV_RULE int turn_position(int p, int depth, bool live) { return p >= 0 && live ? p + depth : 0; }
+
+// Whether the positions of a call's tokens, the deepest at `depth` (-1: none), are within a
+// table of so many.
+SWIFTKV_RULE bool turns_within(int p, int depth, int positions) { return p < 0 || static_cast<long long>(p) + depth < positions; }
+
 }  // namespace swiftkv

@@ -129,7 +129,7 @@ class Rig:
             if p < 0:
                 continue
             _, depth, live = places(chain(n) if parents is None else parents[b])
-            kk = k[b] if self.rotation is None else self.rotation.turn(k[b], p + depth, self.t)
+            kk = k[b] if self.rotation is None else self.rotation.turn(k[b], np.where(live, p + depth, 0), self.t)
             page, place = self.slots(seq0 + b, p + np.arange(n)[live])
             self.store[0][layer, page, place] = kk[live]
             self.store[1][layer, page, place] = v[b][live]
@@ -195,7 +195,7 @@ class Rig:
             assert (out[b][~live] == 0).all(), f"rows without a token of sequence {b}"
             tokens = p + int(live.sum())
             keys, values = self.rows(layer, seq0 + b, np.arange(tokens))
-            turned = q[b] if self.rotation is None else self.rotation.turn(q[b], p + depth, self.t)
+            turned = q[b] if self.rotation is None else self.rotation.turn(q[b], np.where(live, p + depth, 0), self.t)
             seen = np.concatenate([np.ones((int(live.sum()), p), bool), own[live][:, live]], 1)
             for h in range(self.heads):
                 kh, vh = keys[:, h // group], values[:, h // group]

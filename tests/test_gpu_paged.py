@@ -678,3 +678,30 @@ def test_trees_without_tokens_come_first(skv, ctx, t, n):
         rig.check_values()
         rig.check_attention(at, n, trees)
         rig.check_values()
+
+
+@every_shape
+@pytest.mark.parametrize("halves", [True, False])
+def test_the_end_of_the_rotary_table(skv, ctx, forced, halves):
+    """Sequences as long as the table that bring no tokens, ones that sit out of calls of more tokens than the table has
+    positions, and the last position itself."""
+    dim, positions = 64, 150
+    rig = P.Rig(skv, ctx, "bf16", 8, 2, dim, batch=3, capacity=320, rotation=P.Rotation(dim, positions, halves=halves), seed=forced)
+    rig.map_all()
+    rig.append([0] * 3, positions)
+    rng = np.random.default_rng(forced)
+    for n in (1, 9, 40):
+        trees = [P.random_tree(rng, n, c) for c in (0, n, 0)]
+        at = [positions, positions - n, positions]
+        rig.append(at, n, trees)
+        rig.check_values()
+        rig.check_attention(at, n, trees)
+        rig.check_attention(at, n, trees, append=False)
+    star = [[-1] + [0] * 7, [-2] * 8, [-1] * 8]              # depths of 1, none and 0
+    rig.check_attention([positions - 2, positions, positions - 1], 8, star)
+    _, out = rig.attend([-1] * 3, 300)
+    assert (out == 0).all()
+    _, out = rig.attend([-1, -300, -7], 64, [P.chain(64)] * 3)
+    assert (out == 0).all()
+    rig.check_attention([0, -1, -1], positions)
+    rig.check_values()

@@ -98,6 +98,49 @@ def test_rows_that_an_append_reads(tmp_path):
     run_rules(tmp_path, APPENDED_ROWS)
 
 
+TURNED_POSITIONS = r"""
+#include <cassert>
+#include <initializer_list>
+#include "swiftkv_paged_host.hpp"
+#include "swiftkv_paged_rows.hpp"
+using namespace swiftkv;
+int main() {
+    for (int positions : {1, 2, 64, 100})
+        for (int n : {1, 2, 7, 64})
+            for (int p : {-2147483647 - 1, -64, -5, -1, 0, 1, 36, 63, 64, 93, 98, 99, 100, 101}) {
+                // a chain, and trees of every number of tokens: chains, and stars under one token
+                if (turns_within(p, n - 1, positions))
+                    for (int i = 0; i < n; ++i) {
+                        const int at = turn_position(p, i, true);
+                        assert(at >= 0 && at < positions && (p < 0 || at == p + i));
+                    }
+                for (int count = 0; count <= n; ++count)
+                    for (int star = 0; star < 2; ++star) {
+                        int parents[64], depth[64];
+                        for (int i = 0; i < n; ++i) {
+                            parents[i] = i >= count ? -2 : star && i > 0 ? 0 : i - 1;
+                            depth[i] = parents[i] < 0 ? 0 : depth[parents[i]] + 1;
+                        }
+                        assert(tree_tokens(parents, n) == count);
+                        if (!turns_within(p, tree_depth(parents, count), positions)) continue;
+                        for (int i = 0; i < n; ++i) {        // rows without a token too: their queries are read
+                            const int at = turn_position(p, depth[i], i < count);
+                            assert(at >= 0 && at < positions && (p < 0 || i >= count || at == p + depth[i]));
+                        }
+                    }
+            }
+    assert(!turns_within(2147483647, 63, 2147483647) && turns_within(100, -1, 100) && !turns_within(100, 0, 100));
+    return 0;
+}
+"""
+
+
+def test_positions_that_are_looked_up(tmp_path):
+    """All within the table for every call that the check lets pass: full sequences that bring no tokens, sequences that
+    sit out, rows without a token."""
+    run_rules(tmp_path, TURNED_POSITIONS)
+
+
 def test_null_checks_without_device(skv):
     L = skv.lib()
     pos = np.zeros(1, np.int32).ctypes.data_as(C.c_void_p)
