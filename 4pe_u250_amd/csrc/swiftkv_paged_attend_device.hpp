@@ -66,7 +66,10 @@ __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask
 //
 // 16 rows leave the matrix instructions idle, so a bfloat16 weight is two terms there
 // (2^-16 of it); with more rows it is one, 2^-8.  A float16 weight is 2^(kShift +
-// kSlack) at most and is good to 2^-11, or to 2^-36 of the row's largest.
+// kSlack) at most and is good to 2^-11, or to 2^-36 of the row's largest.  A bfloat16
+// weight is 2^-18 at most, so that kPagedMaxSeq of them times the largest values stay in
+// FP32's range, 2^127 together, here and where waves and splits are joined; what that takes
+// from the other end is below 2^-104 of the row's largest weight.
 template <typename T, int HD, int R, bool FINE = false>
 struct RowTile {
     using P = Product<T, R>;
@@ -80,7 +83,8 @@ struct RowTile {
     static constexpr int ND = HD / R;            // output tiles
     static constexpr int NE = R * R / 64;        // sums of a lane in one
     static constexpr int TERMS = FINE && !kHalf ? 2 : 1;
-    static constexpr float kSlack = 4.0f, kShift = kHalf ? 11.0f : 0.0f;
+    static constexpr float kSlack = 4.0f, kShift = kHalf ? 11.0f : -22.0f;
+    static_assert(kHalf || (1 << static_cast<int>(-kShift - kSlack)) > kPagedMaxSeq, "sums of weights times values");
     typedef uint32_t Pairs __attribute__((ext_vector_type(4)));
 
     Half8<T> q[NS];

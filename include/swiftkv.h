@@ -590,7 +590,8 @@ int swiftkv_paged_values(swiftkv_context* ctx, const swiftkv_paged_cache* cache,
  * softmax sums and outputs are held in FP32; a softmax weight is rounded to the element
  * type (bfloat16: 2^-8 of it, or 2^-16 with at most 16 rows, n times the query heads that
  * share a key/value head; float16: 2^-11, or 2^-36 of the row's largest where that is
- * more).  Results do not depend on which workgroup ends first.
+ * more).  Sums of any finite values stay in range; bfloat16 outputs may be off by a further
+ * 2^-127 for each token seen.  Results do not depend on which workgroup ends first.
  * swiftkv_set_split_tokens applies. */
 int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* table, int32_t halves, const void* q,
                             int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

@@ -705,3 +705,63 @@ def test_the_end_of_the_rotary_table(skv, ctx, forced, halves):
     assert (out == 0).all()
     rig.check_attention([0, -1, -1], positions)
     rig.check_values()
+
+
+@pytest.mark.parametrize("n", [1, 7, 40])
+def test_large_values(skv, ctx, n):
+    """Values near bfloat16's largest, of equal and of different weights: their sums are far beyond FP32's range, their
+    means are not."""
+    tokens = 4096
+    rig = P.Rig(skv, ctx, "bf16", 8, 2, 64, capacity=tokens, seed=n)
+    rig.map_all()
+    try:
+        for k_size, v in ((0.0, 3e38), (0.0, -1e35), (1.0, 3e38), (1.0, None)):
+            value = rig.rng.uniform(-3e38, 3e38, (1, tokens, 2, 64)) if v is None else np.full((1, tokens, 2, 64), v)
+            rig.append([0], tokens, k=rig.rng.standard_normal((1, tokens, 2, 64)) * k_size, v=value)
+            for split in (0, 256, 4096):
+                ctx.set_split_tokens(split)
+                out = rig.check_attention([tokens - n], n, append=False)
+                assert np.isfinite(out).all()
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@every_shape
+def test_large_values_in_every_shape(skv, ctx, forced):
+    rig = P.Rig(skv, ctx, "bf16", 10, 2, 128, capacity=1600, seed=forced)
+    rig.map_all()
+    rig.append([0], 1500, v=np.full((1, 1500, 2, 128), 3e38))
+    tree = [P.random_tree(np.random.default_rng(0), 20)]
+    for how in (dict(parents=tree, v=np.full((1, 20, 2, 128), 3e38)), dict(parents=tree, v=np.full((1, 20, 2, 128), -3e38)), {}):
+        rig.check_attention([1500], 20, **how)
+
+
+@pytest.mark.parametrize("n", [1, 9])
+def test_large_values_of_the_longest_sequence(skv, ctx, n):
+    """All weights just below the 2^4 by which scores may lie above the reference value that the first ones set, of as
+    many tokens as a sequence holds, in long splits and in the plan's."""
+    tokens, dim = 131072, 64
+    rig = P.Rig(skv, ctx, "bf16", 4, 1, dim, capacity=tokens, seed=0)
+    rig.map_all()
+    k = np.zeros((1, tokens, 1, dim))
+    k[0, 256:, 0, 0] = 2.6875                # times log2(e): 3.877
+    rig.append([0], tokens, k=k, v=np.full((1, tokens, 1, dim), 3e38))
+    q = np.zeros((1, n, 4, dim))
+    q[..., 0] = 1.0
+    try:
+        for split in (32768, 0):
+            ctx.set_split_tokens(split)
+            out = rig.check_attention([tokens - n], n, append=False, q=q, scale=1.0)
+            assert np.isfinite(out).all()
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_small_values(skv, ctx, n):
+    """Far below 1, where weights times values are near FP32's smallest numbers: 4096 tokens' 2^-127 each are 2^-115 together,
+    2^-20 of these, of which the bound allows a weighted value more."""
+    rig = P.Rig(skv, ctx, "bf16", 8, 2, 64, capacity=4096, seed=n)
+    rig.map_all()
+    rig.append([0], 4096, v=rig.rng.uniform(0.5, 1.0, (1, 4096, 2, 64)) * 2.0 ** -95)
+    rig.check_attention([4096 - n], n, append=False)
