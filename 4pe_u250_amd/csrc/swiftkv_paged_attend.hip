@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
         for (int i = 0; i < NL; ++i) vb[i] = load(cells, v_lane, kStepBytes / 2 + cell_at(i));
     };
     // The scores of a step are formed while the weights of the one before are.
-    int step = step_begin + wave, at = 0;
+    int step = step_begin + wave, at = 0, again = step_end;     // the step from which V has to be looked at again
     float s[RT][Tile::NV];
     __amdgpu_buffer_rsrc_t next = cells_of(step, 0);
     auto seen = [&](const Tile& tile, int st) { return st < step_end ? tile.seen(st, g) : 0u; };
@@ -143,9 +143,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) tiles[rt].weights(s[rt], a.scale, w[rt]);
             if constexpr (kMasked)
-                if (__builtin_expect(tiles[0].no_numbers(vb), 0)) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) tiles[rt].part_with_no_numbers(vb, seen(tiles[rt], step));
+                if (__builtin_expect(Tile::no_numbers(vb), 0)) {
+                    again = min(again, step);
                     Tile::clean(vb);
                 }
 #pragma unroll
@@ -165,6 +164,16 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
     };
     run(std::false_type{}, share.plain_end - kWaves);
     run(std::true_type{}, step_end);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+        if (tiles[rt].no_number_sums()) again = step_begin + wave;
+    if (__builtin_expect(again < step_end, 0))
+        look_again<kWaves>(tiles, vb, again, step_end, g, [&](int st, Half8<T> (&x)[NL]) __attribute__((always_inline)) {
+            const int page = __builtin_amdgcn_readfirstlane(table[st / kPageSteps]);
+            const __amdgpu_buffer_rsrc_t cells = step_resource(layer_head, page_bytes, page, st, step_end, kStepBytes);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) x[i] = load(cells, v_lane, kStepBytes / 2 + cell_at(i));
+        });
 
     __syncthreads();                             // everyone has its queries
 #pragma unroll

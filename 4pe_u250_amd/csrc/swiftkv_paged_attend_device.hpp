@@ -186,9 +186,27 @@ struct RowTile {
         return __any(bad != 0);
     }
 
-    // 0 times an infinity or a NaN is a NaN, so where rows see different tokens, what is
-    // no number leaves V and reaches the rows that see it by itself: products of ones
-    // count such values.
+    // A weight that rounds to 0 times an infinity is a NaN, a second term may have the other
+    // sign, and rows of a masked step do not all see its values.  So what is no number takes
+    // no part in sums: where it made them none, they start again from 0 (drop), where rows
+    // see different tokens it leaves V first (clean), and the steps are gone through once
+    // more for it alone (look_again).  It then reaches the rows that see it, whatever their
+    // weights: products of ones count such values.
+    __device__ __forceinline__ bool no_number_sums() const {
+        float x[4] = {};                         // (a sum that leaves the range is looked at for nothing)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < NE; ++e) x[e & 3] += acc[d][e];
+        const float sum = (x[0] + x[1]) + (x[2] + x[3]);
+        return __any(!(fabsf(sum) < INFINITY));
+    }
+    __device__ __forceinline__ void drop() {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < NE; ++e) acc[d][e] = fabsf(acc[d][e]) < INFINITY ? acc[d][e] : 0.0f;
+    }
     __device__ __forceinline__ void part_with_no_numbers(const Half8<T> (&vb)[NL], uint32_t bits) {
 #pragma unroll 1
         for (int kind = 0; kind < 3; ++kind) {   // NaN, inf, -inf: from `low` on, `span` patterns
@@ -247,6 +265,21 @@ struct RowTile {
                 quads[(d * (R / 4) + e * G + g) * pitch + row] = v4f{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
     }
 };
+
+// What is no number to the sums of a wave's rows: its steps first, first + STRIDE, ... below
+// `end` again.  load(step, vb): V of a step as operands.
+template <int STRIDE, typename Tile, int RT, typename Operands, typename Load>
+__device__ __forceinline__ void look_again(Tile (&tiles)[RT], Operands& vb, int first, int end, int g, Load&& load) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) tiles[rt].drop();
+#pragma unroll 1
+    for (int step = first; step < end; step += STRIDE) {
+        load(step, vb);
+        if (!Tile::no_numbers(vb)) continue;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) tiles[rt].part_with_no_numbers(vb, tiles[rt].seen(step, g));
+    }
+}
 
 // A workgroup's share of a call: ROWS rows of a chunk, the steps of a split.
 template <int ROWS, typename Tree>
@@ -437,13 +470,27 @@ struct Joined {
 #pragma unroll
         for (int j = 0; j < N; ++j) top = fmaxf(top, ml[j][0]);
         const float safe = top == -INFINITY ? 0.0f : top, f0 = fast_exp2(m - safe);
+        const v4f before = o;
         l *= f0;
         o *= f0;
+        float f[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float f = fast_exp2(ml[j][0] - safe);
-            l += ml[j][1] * f;
-            o += sums[j] * f;
+            f[j] = fast_exp2(ml[j][0] - safe);
+            l += ml[j][1] * f[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[j][e], f[j], o[e]);
+        }
+        // An infinity stays one where its factor is 0.
+        const float all = (o[0] + o[1]) + (o[2] + o[3]);
+        if (__builtin_expect(__any(all != all), 0)) {
+            auto finite = [](float x) { return fabsf(x) < INFINITY; };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] = finite(before[e]) ? before[e] * f0 : before[e];
+#pragma unroll
+                for (int j = 0; j < N; ++j) o[e] = finite(sums[j][e]) ? __builtin_fmaf(sums[j][e], f[j], o[e]) : o[e] + sums[j][e];
+            }
         }
         m = top;
     }

@@ -90,7 +90,8 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     T* const staged = reinterpret_cast<T*>(lds + M::kRing);
     share.template stage_queries<T, HD, kManyThreads>(a, staged);
     __syncthreads();
-    Tile tile;
+    Tile tiles[1];
+    Tile& tile = tiles[0];
     tile.clear();
     share.sees(a, tile, row);
 #pragma unroll
@@ -123,6 +124,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
 
     // Slots of this turn's V and the next turn's K, and of what this turn asks for.
     int step0 = step_begin, v_slot = 0, k_slot = 1;
+    int again = step_end;                        // the step from which V has to be looked at again
     // One turn: weights and sums of the scores `now`, scores `then` of the next.
     auto turn = [&](auto masked, const float (&now)[Tile::NV], float (&then)[Tile::NV]) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
@@ -137,8 +139,8 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
             tile.scores(kb, then);
             tile.weights(now, a.scale, w);
             if constexpr (kMasked)
-                if (step >= share.plain_end && __builtin_expect(tile.no_numbers(vb), 0)) {
-                    tile.part_with_no_numbers(vb, seen(step));
+                if (step >= share.plain_end && __builtin_expect(Tile::no_numbers(vb), 0)) {
+                    again = min(again, step);
                     Tile::clean(vb);
                 }
             tile.add(vb, w);
@@ -164,6 +166,19 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     run(std::false_type{}, share.plain_end - 3 * TEAMS + 1);
     run(std::true_type{}, step_end);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // nothing is on its way to LDS any more
+    if (tile.no_number_sums()) again = step_begin + team;
+    if (__builtin_expect(again < step_end, 0)) {
+        Half8<T> vb[NL];
+        look_again<TEAMS>(tiles, vb, again, step_end, g, [&](int st, Half8<T> (&x)[NL]) __attribute__((always_inline)) {
+            const int page = __builtin_amdgcn_readfirstlane(table[st / kPageSteps]);
+            const __amdgpu_buffer_rsrc_t cells = step_resource(layer_head, page_bytes, page, st, step_end, kStepBytes);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int at = kHalfBytes + (i >> 1) * 2048 + (i & 1) * 512;
+                x[i] = __builtin_bit_cast(Half8<T>, __builtin_amdgcn_raw_buffer_load_b128(cells, v_lane + (at & 4095), at & ~4095, 0));
+            }
+        });
+    }
     __syncthreads();
 
     // The teams' sums meet in LDS, quads of channels of a row together.

@@ -586,7 +586,8 @@ int swiftkv_paged_values(swiftkv_context* ctx, const swiftkv_paged_cache* cache,
  *             position, are zero
  *   scale     multiplies q.k; 0 stands for 1 / sqrt(head_dim); its magnitude within
  *             [2^-100, 2^100]
- * What a row does not see does not reach it, infinities and NaN included.  Scores,
+ * What a row does not see does not reach it, infinities and NaN included; an infinity or a
+ * NaN of V that it sees makes its output channel one, however small its weight.  Scores,
  * softmax sums and outputs are held in FP32; a softmax weight is rounded to the element
  * type (bfloat16: 2^-8 of it, or 2^-16 with at most 16 rows, n times the query heads that
  * share a key/value head; float16: 2^-11, or 2^-36 of the row's largest where that is

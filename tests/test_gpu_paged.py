@@ -765,3 +765,58 @@ def test_small_values(skv, ctx, n):
     rig.map_all()
     rig.append([0], 4096, v=rig.rng.uniform(0.5, 1.0, (1, 4096, 2, 64)) * 2.0 ** -95)
     rig.check_attention([4096 - n], n, append=False)
+
+
+def seen_no_numbers(skv, ctx, rig, p, n, heads, parents=None):
+    """Values that are no numbers among the cached tokens, where they are far from the sequence's end and near it: they make
+    their channels what a sum of weights above zero times values is, whatever the weights and splits; all else stays."""
+    dim, kv = rig.dim, rig.kv
+    at = [2, 700, p - 1]
+    q = rig.random(1, n, heads, dim)[1]
+    q[..., 0] = 4.0
+    k, v = (rig.random(1, p, kv, dim)[1] for _ in "kv")
+    try:
+        for lift in (0.0, -70.0, 20.0):                      # scores of these tokens: with the others, far below, above
+            kk = k.copy()
+            kk[..., 0] = 0.0
+            kk[0, at, :, 0] = lift
+            for split in (0, 256, 4096):
+                ctx.set_split_tokens(split)
+                rig.append([0], p, k=kk, v=v)
+                first, good = rig.attend([p], n, parents, q=q, append=False, scale=0.5) if parents is None else \
+                    rig.attend([p], n, parents, q=q, k=np.zeros((1, n, kv, dim)), v=np.ones((1, n, kv, dim)), scale=0.5)
+                assert np.isfinite(good).all()
+                bad = v.copy()
+                bad[0, at[0], :, 1], bad[0, at[1], :, 5], bad[0, at[2], :, 40] = np.inf, -np.inf, np.nan
+                bad[0, at[0], :, 9], bad[0, at[1], :, 9] = np.inf, -np.inf
+                bad[0, at[1:], :, 63] = np.inf
+                rig.append([0], p, k=kk, v=bad)
+                _, out = rig.attend([p], n, parents, q=q, append=False, scale=0.5) if parents is None else \
+                    rig.attend([p], n, parents, q=q, k=np.zeros((1, n, kv, dim)), v=np.ones((1, n, kv, dim)), scale=0.5)
+                for c, want in ((1, np.inf), (5, -np.inf), (40, np.nan), (9, np.nan), (63, np.inf)):
+                    np.testing.assert_array_equal(out[..., c], np.full(out.shape[:-1], want), err_msg=f"channel {c}, lift {lift}, split {split}")
+                rest = [c for c in range(dim) if c not in (1, 5, 9, 40, 63)]
+                np.testing.assert_array_equal(out[..., rest], good[..., rest], err_msg=f"lift {lift}, split {split}")
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 7])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_seen_no_numbers(skv, ctx, t, n, dim):
+    rig = P.Rig(skv, ctx, t, 2, 1, dim, capacity=1600, seed=n)
+    rig.map_all()
+    rig.append([0], 1600)
+    seen_no_numbers(skv, ctx, rig, 1500, n, 2, [P.chain(n)])
+    seen_no_numbers(skv, ctx, rig, 1500, n, 2)
+
+
+@every_shape
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_seen_no_numbers_in_every_shape(skv, ctx, t, dim, forced):
+    rig = P.Rig(skv, ctx, t, 4, 1, dim, capacity=1600, seed=forced)
+    rig.map_all()
+    rig.append([0], 1600)
+    seen_no_numbers(skv, ctx, rig, 1500, 20, 4, [P.random_tree(np.random.default_rng(1), 20)])
