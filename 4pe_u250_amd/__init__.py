@@ -919,7 +919,9 @@ def swiftkv_paged_keep(ctx: Context, cache: PagedCache, layer0: int, layers: int
                        seq0: int = 0) -> list:
     """Move the rows of each sequence's accepted drafted tokens (accepted [batch * m],
     rising, then -1) to cached tokens position[b], position[b] + 1, ... of `layers`
-    layers.  Returns the numbers of tokens then cached."""
+    layers: a path of the tree from its root on, each token a child of the one before, so
+    that keys are turned by the positions that they get.  Returns the numbers of tokens
+    then cached."""
     pos, batch, _keep = _positions(ctx, position)
     at, count, _owner = _int32s(accepted)
     if count != batch * m:

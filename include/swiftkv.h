@@ -603,9 +603,10 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
 /* Keep the accepted path of each sequence's tree: the row of drafted token accepted[b * m +
  * j] (cached token positions[b] + accepted) moves to cached token positions[b] + j, in
  * layers layer0 .. layer0 + layers - 1.  accepted: host [batch * m], rising within
- * [0, SWIFTKV_TREE_TOKENS), each a descendant of the one before (so that its key has been
- * turned by the position that it gets), then -1; m <= SWIFTKV_TREE_TOKENS.  A negative
- * position skips its sequence.
+ * [0, SWIFTKV_TREE_TOKENS), then -1; m <= SWIFTKV_TREE_TOKENS.  The first has to be one that
+ * continued the cached tokens, and each other one a child of the one before: the keys that
+ * move have then been turned by the positions that they get.  (The call does not know the
+ * trees, and moves the rows of any rising path.)  A negative position skips its sequence.
  *   out_positions   NULL, or host [batch]: the number of tokens then cached */
 int swiftkv_paged_keep(swiftkv_context* ctx, swiftkv_paged_cache* cache, int32_t layer0, int32_t layers, int32_t seq0,
                        const int32_t* positions, const int32_t* accepted, int32_t batch, int32_t m,

@@ -820,3 +820,22 @@ def test_seen_no_numbers_in_every_shape(skv, ctx, t, dim, forced):
     rig.map_all()
     rig.append([0], 1600)
     seen_no_numbers(skv, ctx, rig, 1500, 20, 4, [P.random_tree(np.random.default_rng(1), 20)])
+
+
+def test_keys_of_kept_paths(skv, ctx):
+    """A path of children from the root on leaves keys that are turned by the positions that they then have; one that
+    leaves a generation out leaves them as the call turned them."""
+    dim, p, n = 64, 90, 12
+    rig = P.Rig(skv, ctx, "bf16", 2, 2, dim, batch=2, capacity=192, rotation=P.Rotation(dim), seed=3)
+    rig.map_all()
+    rig.append([0, 0], p)
+    tree = [-1, 0, 0, 2, 2, 4, 1, 5, 5, 7, 8, -1]            # 0 - 2 - 4 - 5 - 8 - 10 is a path
+    k = rig.random(2, n, 2, dim)[1]
+    rig.append([p, p], n, [tree, tree], k=k)
+    paths = [[0, 2, 4, 5, 8, 10], [0, 4, 5, 8, 10, -1]]
+    assert rig.keep([p, p], paths) == [p + 6, p + 5]
+    rig.check_values()
+    for b, off in ((0, [0] * 6), (1, [0, 1, 1, 1, 1])):
+        path = [a for a in paths[b] if a >= 0]
+        want = rig.rotation.turn(k[b, path], p + np.arange(len(path)) + off, "bf16")
+        np.testing.assert_array_equal(rig.rows(0, b, p + np.arange(len(path)))[0], want)
