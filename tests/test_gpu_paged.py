@@ -839,3 +839,33 @@ def test_keys_of_kept_paths(skv, ctx):
         path = [a for a in paths[b] if a >= 0]
         want = rig.rotation.turn(k[b, path], p + np.arange(len(path)) + off, "bf16")
         np.testing.assert_array_equal(rig.rows(0, b, p + np.arange(len(path)))[0], want)
+
+
+@pytest.mark.parametrize("cached", [0, 62, 64, 100])
+def test_a_serving_program(skv, ctx, cached):
+    """Steps of a drafted tree over pages' ends: pages are given to a sequence as its tokens need them, entries that have one
+    keep it, and no cached token is lost."""
+    layers, n, dim = 2, 4, 64
+    rig = P.Rig(skv, ctx, "bf16", 8, 2, dim, batch=2, pages=12, layers=layers, capacity=384, rotation=P.Rotation(dim), seed=cached)
+    free, pages, seq = list(range(12)), [], 1
+
+    def give(tokens):
+        more = [free.pop() for _ in range(-(-tokens // 64) - len(pages))]
+        rig.map(seq, more, first=len(pages))
+        pages.extend(more)
+        return len(more)
+
+    rig.map(0, [free.pop(3)])                                # another sequence's
+    rig.append([0], 64)
+    give(cached)
+    for layer in range(layers if cached else 0):
+        rig.append([0], cached, layer=layer, seq0=seq)
+    tree, given = [skv.TREE_ROOT, 0, 0, 1], 0
+    for turn in range(60):
+        given += give(cached + n)
+        for layer in range(layers):
+            rig.check_attention([cached], n, [tree], layer=layer, seq0=seq)
+        path = [[0, 1, 3], [0, 2, -1], [0, -1, -1], [-1, -1, -1]][turn % 4]
+        cached = rig.keep([cached], [path], seq0=seq)[0]
+        rig.check_values()
+    assert given >= 1 and 64 * len(pages) >= cached
