@@ -589,11 +589,11 @@ int swiftkv_paged_values(swiftkv_context* ctx, const swiftkv_paged_cache* cache,
  * What a row does not see does not reach it, infinities and NaN included; an infinity or a
  * NaN of V that it sees makes its output channel one, however small its weight.  Scores,
  * softmax sums and outputs are held in FP32; a softmax weight is rounded to the element
- * type (bfloat16: 2^-8 of it, or 2^-16 with at most 16 rows, n times the query heads that
- * share a key/value head; float16: 2^-11, or 2^-36 of the row's largest where that is
- * more).  Sums of any finite values stay in range; bfloat16 outputs may be off by a further
- * 2^-127 for each token seen.  Results do not depend on which workgroup ends first.
- * swiftkv_set_split_tokens applies. */
+ * type: bfloat16 2^-8 of it, or 2^-16 with at most 16 rows, n times the query heads that
+ * share a key/value head; float16 2^-11; or, where that is more, 2^-104 (bfloat16) and 2^-36
+ * (float16) of the row's largest.  Sums of any finite values stay in range; bfloat16 outputs
+ * may be off by a further 2^-127 for each token seen.  Results do not depend on which
+ * workgroup ends first.  swiftkv_set_split_tokens applies. */
 int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* table, int32_t halves, const void* q,
                             int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                             swiftkv_paged_cache* cache, int32_t layer_index, int32_t seq0, const int32_t* positions,
