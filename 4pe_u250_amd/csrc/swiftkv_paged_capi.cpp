@@ -156,18 +156,25 @@ int append_rows(const swiftkv_context* ctx, const PagedRotation& rotation, const
 // holds them all.  Where turns are many, its cells shall be read by few workgroups: 48 rows
 // (three tiles of 16 a wave: loads bound these), 64 (two of 32), 128 or 256 (cells shared in
 // LDS).  Where they are few, workgroups shall be many: 32 rows, or 64 where 32 would leave a
-// CU more than one.  us of a call onto 4031 tokens, 32 heads over 8, the kernel taken against
-// others: 64 sequences x 12 tokens (48 rows) 48 190, 64 192, 32 209; x 16 64 196, 128 217; x 24
-// 128 230, 32 265; x 64 256 353, 128 413, 64 502; 8 x 16 32 31.6, 64 34.4; x 24 32 38.5, 64
-// 40.0, 128 42.7; x 32 64 42.0, 32 43.1; x 64 64 59.4, 32 69.2, 256 65.5; one sequence x 26 32
-// 16.9, 64 21.7; x 512 64 53.1, 32 61.8, 256 66.9; x 1024 64 102, 256 112; 4 x 512 256 168, 64
-// 200; a prompt of 2048 tokens 64 79.4, 32 75.1, 128 73.0; of 4096 256 176, 64 209.
+// CU more than one.  us of a call onto 4031 tokens, 32 heads of 128 over 8, the kernel taken
+// against others: 64 sequences x 12 tokens (48 rows) 48 188, 64 192, 32 204; x 16 64 195, 32 210,
+// 128 219; x 24 128 228, 64 255, 32 257; x 64 256 357, 128 424, 64 468; 8 x 16 32 31.2, 64 35.1; x
+// 24 32 34.8, 64 39.3, 128 43.0; x 64 64 57.2, 32 67.2, 128 67.9; one sequence x 26 32 16.0, 64
+// 20.2; x 512 64 54.9, 32 61.1, 256 67.4; x 1024 64 105, 256 114; 4 x 512 256 174, 64 190; a prompt
+// of 4096 tokens onto none 256 179, 128 209.
+//
+// What the rule does not see: a chunk of a prompt scans what it sees and turns count as if
+// each saw all, so prompts onto none get more rows than is best (512 tokens 64 19.0, 32 15.8;
+// 1024 64 35.1, 32 30.5; 2048 64 81.5, 128 74.7), and 8 x 32 tokens are where the two meet (64
+// 39.2, 32 37.7).
 //
 // Splits make a workgroup for each CU and not more, of at most 32 a sequence and at most the
 // square root of its 64-token tiles, since they are joined: us of a step, tokens of this
-// rule's splits against others: one sequence at 4096 512 11.1; 256 11.7, 1024 12.7; 4 at 4096
-// 512 16.9; 1024 19.5; 8 at 4096 1024 26.5; 512 30.3, 2048 30.3; 32 at 4096 none 86.7; 2048
-// 92.5; 64 none 172; 2048 189; one at 32000 1408; 1024 29.6, 2048 31.2, 4096 45.7.
+// rule's splits against others: one sequence at 4096 512 10.7; 256 11.8, 1024 12.4; 4 at 4096
+// 512 16.6; 1024 19.6; 8 at 4096 1024 26.1; 512 29.4, 2048 30.3; 32 at 4096 none 85.8; 2048
+// 90.9; 64 none 170; 2048 180; one at 32000 1408 29.6; 1024 30.0, 2048 31.4, 4096 45.7.  It goes by
+// how many workgroups there are, not by what each scans: one sequence of 32000 among 63 of 100
+// is not split (282; in 4 splits 83).
 PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t forced_rows, int32_t group, int32_t kv_heads, int32_t n,
                          const int32_t* positions, int32_t batch) {
     PagedPlan p{};
