@@ -47,6 +47,9 @@ __host__ __device__ inline int64_t paged_record(const PagedView& v, int layer, i
     return ((static_cast<int64_t>(layer) * v.pages + page) * v.kv_heads + kv_head) * paged_record_bytes(v.head_dim);
 }
 
+// Exponents by which a weight may lie above those of a row's reference score.
+constexpr float kScoreSlack = 4.0f;
+
 // The rotation of a call's queries and keys; table null: none.
 struct PagedRotation {
     const float2* table;  // [positions][rotary_dim / 2] (cos, sin)
@@ -103,6 +106,7 @@ struct PagedAttendArgs {
     int64_t k_stride;
     int64_t v_stride;
     float scale;          // log2(e) times the caller's magnitude
+    float slack;          // kScoreSlack over it
     int32_t negative;     // the caller's scale is: queries change their sign
     int32_t group;        // query heads per key/value head
     uint32_t group_magic; // ceil(2^32 / group), 0 for 1

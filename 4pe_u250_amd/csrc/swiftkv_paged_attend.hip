@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
             const uint32_t bits = seen(tiles[rt], step);
             tiles[rt].scores(kb, s[rt]);
             tiles[rt].hide(bits, s[rt]);
-            tiles[rt].rise(s[rt], a.scale);
+            tiles[rt].rise(s[rt], a);
         }
         next = cells_of(step + kWaves, ++at);
         load_k(next);
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if constexpr (kMasked) tiles[rt].hide(bits[rt], sn[rt]);
-                tiles[rt].rise(sn[rt], a.scale);
+                tiles[rt].rise(sn[rt], a);
             }
             next = after;
 #pragma unroll
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
     for (int rt = 0; rt < RT; ++rt) {
         const float sum = Tile::groups_sum(tiles[rt].l);
         if (g == 0) {
-            stats[wave][rt * R + place][0] = tiles[rt].m;
+            stats[wave][rt * R + place][0] = tiles[rt].reference();
             stats[wave][rt * R + place][1] = sum;
         }
         tiles[rt].leave(lds + wave * CG * (ROWS + 1), ROWS + 1, rt * R + place, g);
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
             sums[w] = lds[(w * CG + quad) * (ROWS + 1) + row];
         }
         Joined all;
-        all.add(ml, sums);
+        all.add(ml, sums, a.scale);
         float* const dst = share.template partial<HD>(a, share.split);
         if (share.my_splits == 1) {
             share.template finish<T, HD>(a, row, quad, all.l, all.o);
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const P
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j)
                     if (j0 + j >= share.my_splits) ml[k][j] = v2f{-INFINITY, 0.0f}, sums[k][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-                all[k].add(ml[k], sums[k]);
+                all[k].add(ml[k], sums[k], a.scale);
             }
         }
 #pragma unroll
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(const PagedA
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j)
             if (j0 + j >= share.my_splits) ml[j] = v2f{-INFINITY, 0.0f}, sums[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        all.add(ml, sums);
+        all.add(ml, sums, a.scale);
     }
     share.template finish<T, HD>(a, row, quad, all.l, all.o);
 }

@@ -59,19 +59,23 @@ __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask
 //           rounded to the cache's type.
 //
 // Both A operands are the cache's cells as they lie (swiftkv_paged.hpp).  Nothing
-// moves between lanes but, now and then, a row's maximum: the reference value that
-// weights are taken over follows it only when a score is more than 2^kSlack above,
-// with p <= 2^kSlack until then.  (That branch is marked unlikely, which also keeps
-// the sums' registers where the products want them.)
+// moves between lanes but, now and then, a row's maximum: the reference score that
+// weights are taken over follows it only when a score is above its limit, with p <=
+// 2^kScoreSlack until then.  (That branch is marked unlikely, which also keeps the sums'
+// registers where the products want them.)  A score's difference to the reference is
+// formed before it is scaled, and is 0 for equal scores.  (A multiply-add with the scaled
+// reference is an instruction less, 420 us against 429 for 4096 tokens onto 4095, and leaves
+// the product's rounding, more than all of a weight where scaled scores reach 2^24.  Loops of
+// both kinds: 64 tokens of 8 sequences 56 us against 57, 26 tokens 15.4 against 15.3.)
 //
 // 16 rows leave the matrix instructions idle, so a bfloat16 weight is two terms there
 // (2^-16 of it); with more rows it is one, 2^-8, as much as the output's own rounding (two
 // terms: 64 tokens of 8 sequences 69.5 us against 56.5, 512 onto 4095 68 against 54, 4096 onto
-// 4095 572 against 419).  A float16 weight is 2^(kShift +
-// kSlack) at most and is good to 2^-11, or to 2^-36 of the row's largest.  A bfloat16
-// weight is 2^-18 at most, so that kPagedMaxSeq of them times the largest values stay in
-// FP32's range, 2^127 together, here and where waves and splits are joined; what that takes
-// from the other end is below 2^-104 of the row's largest weight.
+// 4095 572 against 419).  A float16 weight is 2^(kShift + kScoreSlack) at most and is good to
+// 2^-11, or to 2^-36 of the row's largest.  A bfloat16 weight is 2^-18 at most, so that
+// kPagedMaxSeq of them times the largest values stay in FP32's range, 2^127 together, here
+// and where waves and splits are joined; what that takes from the other end is below 2^-104
+// of the row's largest weight.  (Up to 2^0.5 more where the limit was rounded up.)
 template <typename T, int HD, int R, bool FINE = false>
 struct RowTile {
     using P = Product<T, R>;
@@ -85,22 +89,24 @@ struct RowTile {
     static constexpr int ND = HD / R;            // output tiles
     static constexpr int NE = R * R / 64;        // sums of a lane in one
     static constexpr int TERMS = FINE && !kHalf ? 2 : 1;
-    static constexpr float kSlack = 4.0f, kShift = kHalf ? 11.0f : -22.0f;
-    static_assert(kHalf || (1 << static_cast<int>(-kShift - kSlack)) > kPagedMaxSeq, "sums of weights times values");
+    static constexpr float kShift = kHalf ? 11.0f : -22.0f;
+    static_assert(kHalf || (1 << static_cast<int>(-kShift - kScoreSlack)) > kPagedMaxSeq, "sums of weights times values");
     typedef uint32_t Pairs __attribute__((ext_vector_type(4)));
 
     Half8<T> q[NS];
     Sum acc[ND];
-    float m, l;
+    float t, limit, l;                           // reference score (0 before the first), where it follows, sum of weights
     uint64_t mask;
     int first;                                   // what the row sees: seen_bits' arguments
 
     __device__ __forceinline__ void clear() {
-        m = -INFINITY;
-        l = 0.0f;
+        t = l = 0.0f;
+        limit = -INFINITY;
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[i] = Sum{};
     }
+    // The reference score as others see it: -inf without one.
+    __device__ __forceinline__ float reference() const { return limit == -INFINITY ? -INFINITY : t; }
 
     __device__ __forceinline__ void scores(const Half8<T> (&kb)[NL], float (&s)[NV]) const {
         if constexpr (R == 16) {
@@ -137,17 +143,20 @@ struct RowTile {
         return x + __shfl_xor(x, 32);
     }
 
-    // The reference value follows scores that are far above it.
-    __device__ __forceinline__ void rise(const float (&s)[NV], float scale) {
+    // The reference score follows scores above its limit: `slack` above it, or at it where
+    // FP32 has none within an eighth of that.
+    __device__ __forceinline__ void rise(const float (&s)[NV], const PagedAttendArgs& a) {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < NV; ++i) top = fmaxf(top, s[i]);
-        top *= scale;
-        if (__builtin_expect(__any(top > m + kSlack), 0)) {
+        if (__builtin_expect(__any(top > limit), 0)) {
             top = groups_max(top);
-            const float next = top > m + kSlack ? top : m;
-            const float fall = next == -INFINITY ? 1.0f : fast_exp2(m - next);
-            m = next;
+            const bool follows = top > limit;
+            const float fall = follows && limit != -INFINITY ? fast_exp2((t - top) * a.scale) : 1.0f;
+            float above = top + a.slack;
+            if (above - top > 1.125f * a.slack) above = top;
+            t = follows ? top : t;
+            limit = follows ? above : limit;
             l *= fall;
 #pragma unroll
             for (int i = 0; i < ND; ++i) acc[i] *= fall;
@@ -155,13 +164,12 @@ struct RowTile {
     }
     // Scores to weights, as B operands.
     __device__ __forceinline__ void weights(const float (&s)[NV], float scale, Half8<T> (&w)[TERMS][NP]) {
-        const float c = kShift - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
         for (int o = 0; o < NP; ++o) {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = fast_exp2(__builtin_fmaf(s[8 * o + j], scale, c));
+                x[j] = fast_exp2(__builtin_fmaf(s[8 * o + j] - t, scale, kShift));
                 w[0][o][j] = static_cast<T>(x[j]);
                 if constexpr (TERMS == 2) w[TERMS - 1][o][j] = static_cast<T>(x[j] - static_cast<float>(w[0][o][j]));
             }
@@ -461,24 +469,24 @@ struct Share {
     }
 };
 
-// Partial results (m, l, sums) joined one after another.
+// Partial results (reference score, sum of weights, sums) joined one after another.
 struct Joined {
     float m = -INFINITY, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     // N of them at once.
     template <int N>
-    __device__ __forceinline__ void add(const v2f (&ml)[N], const v4f (&sums)[N]) {
+    __device__ __forceinline__ void add(const v2f (&ml)[N], const v4f (&sums)[N], float scale) {
         float top = m;
 #pragma unroll
         for (int j = 0; j < N; ++j) top = fmaxf(top, ml[j][0]);
-        const float safe = top == -INFINITY ? 0.0f : top, f0 = fast_exp2(m - safe);
+        const float safe = top == -INFINITY ? 0.0f : top, f0 = fast_exp2((m - safe) * scale);
         const v4f before = o;
         l *= f0;
         o *= f0;
         float f[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            f[j] = fast_exp2(ml[j][0] - safe);
+            f[j] = fast_exp2((ml[j][0] - safe) * scale);
             l += ml[j][1] * f[j];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[j][e], f[j], o[e]);

@@ -436,6 +436,7 @@ int swiftkv_paged_attention(swiftkv_context* ctx, const swiftkv_rotary_table* ta
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     a.scale = (scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(view.head_dim)) : magnitude) * kLog2E;
+    a.slack = kScoreSlack / a.scale;
     a.negative = scale < 0.0f;
     a.group = group;
     a.group_magic = group == 1 ? 0u : static_cast<uint32_t>(((uint64_t(1) << 32) + group - 1) / group);

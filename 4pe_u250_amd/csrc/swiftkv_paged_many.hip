@@ -118,7 +118,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
         operands(kb, k_cells(0));
         tile.scores(kb, s);
         tile.hide(bits, s);
-        tile.rise(s, a.scale);
+        tile.rise(s, a);
     }
     arrive(integral_constant<int, SLOTS - 2>{});
 
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
                 }
             tile.add(vb, w);
             if constexpr (kMasked) tile.hide(bits, then);
-            tile.rise(then, a.scale);
+            tile.rise(then, a);
         }
         if (__builtin_expect(step0 + (SLOTS + 2) * TEAMS > window + 128, 0)) {
             window += 64;
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
     v4f* const quads = reinterpret_cast<v4f*>(lds);
     const float sum = Tile::groups_sum(tile.l);
     if (g == 0) {
-        stats[team][row][0] = tile.m;
+        stats[team][row][0] = tile.reference();
         stats[team][row][1] = sum;
     }
     tile.leave(quads + team * CG * (ROWS + 1), ROWS + 1, row, g);
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(const Paged
             all.l = ml[0][1];
             all.o = sums[0];
         } else {
-            all.add(ml, sums);
+            all.add(ml, sums, a.scale);
         }
         if (share.my_splits == 1) {
             share.template finish<T, HD>(a, r, quad, all.l, all.o);

@@ -869,3 +869,55 @@ def test_a_serving_program(skv, ctx, cached):
         cached = rig.keep([cached], [path], seq0=seq)[0]
         rig.check_values()
     assert given >= 1 and 64 * len(pages) >= cached
+
+
+def large_scores(skv, ctx, rig, t, n, heads, tokens):
+    """Scores so large that FP32 holds them in steps of 2^-5 to 2^9: equal ones weigh the same, and where half of the tokens
+    are above the others by far more than a step, they alone count.  A weight is a rounding of the type off, the output
+    another, and sums one of FP32 a token."""
+    dim, kv = rig.dim, rig.kv
+    half = tokens // 2
+    k = np.zeros((1, tokens, kv, dim))
+    v = rig.random(1, tokens, kv, dim)[1] + 2.0
+    v = R.typed(v, t)[1]
+    q = np.zeros((1, n, heads, dim))
+    q[..., 0] = 1.0
+    for exponent in (18, 21, 22, 23, 24, 25, 26, 27, 28, 29, 30, 32):
+        for sign in (1.0, -1.0):
+            for high in (0, 1):
+                k[0, :, :, 0] = 1.0
+                k[0, high * half:high * half + half, :, 0] += 2.0 ** -7
+                rig.append([0], tokens, k=k, v=v)
+                _, out = rig.attend([tokens - n], n, q=q, append=False, scale=sign * 1.37 * 2.0 ** exponent)
+                assert np.isfinite(out).all(), (exponent, sign, high)
+                best = high if sign > 0 else 1 - high
+                for i in range(n):
+                    at = np.arange(tokens - n + i + 1)
+                    at = at[at >= half] if best else at[at < half]
+                    for h in range(heads):
+                        x = v[0, at, h // (heads // kv)]
+                        want = x.mean(0)
+                        off = (2 * R.HALF_STEP[t] + tokens * 2.0 ** -24 + 2.0 ** -18) * np.abs(x).mean(0)
+                        err = np.abs(out[0, i, h] - want)
+                        assert (err <= off).all(), (exponent, sign, high, i, h, (err / off).max())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 7])
+def test_large_scores(skv, ctx, t, n):
+    rig = P.Rig(skv, ctx, t, 2, 1, 64, capacity=1024, seed=n)
+    rig.map_all()
+    try:
+        for split in (0, 256, 4096):
+            ctx.set_split_tokens(split)
+            large_scores(skv, ctx, rig, t, n, 2, 1000)
+    finally:
+        ctx.set_split_tokens(0)
+
+
+@every_shape
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_large_scores_in_every_shape(skv, ctx, t, forced):
+    rig = P.Rig(skv, ctx, t, 4, 1, 128, capacity=1024, seed=forced)
+    rig.map_all()
+    large_scores(skv, ctx, rig, t, 20, 4, 1000)
