@@ -28,8 +28,8 @@ __device__ __forceinline__ v2f fetch2(const float* p) {
 // operands, 1 KiB of consecutive bytes an instruction, K of the next step during the softmax
 // and V after the products, as registers fall free; with RT > 1 each serves RT tiles of
 // rows.  The waves meet in LDS.  One token of 64 sequences at 4096 170 us, 6.3 TB/s of
-// K and V; 64 rows of each 194 us, 5.5 TB/s.  Where chunks share the cells, what a CU's loads
-// deliver bounds it: 512 tokens onto 4095 54 us and 0.68 PFLOP/s with 64 rows, 61 with 32.
+// K and V; 64 rows of each 195 us, 5.5 TB/s.  Where chunks share the cells, what a CU's loads
+// deliver bounds it: 512 tokens onto 4095 54 us and 0.68 PFLOP/s with 64 rows, 59 with 32.
 //
 // ONCE: no other workgroup reads the cells, and they pass the caches (one token of 64
 // sequences 170 us, 16 tokens 194; kept in the caches 185 and 204); if others do they stay (512
@@ -38,7 +38,7 @@ __device__ __forceinline__ v2f fetch2(const float* p) {
 // 16 rows: a sequence's splits publish (m, l, sums), wait until that has arrived, and
 // count themselves; the last to arrive joins all in split order, so the result does not
 // depend on who that is.  The partial results of more rows are joined by a launch of
-// paged_join_kernel, whose workgroups share the rows out (26 tokens onto 4095: 4.0 us of 15.2).
+// paged_join_kernel, whose workgroups share the rows out (26 tokens onto 4095: 4.0 us of 15.8).
 template <typename T, int HD, int R, int RT, bool ONCE, typename Tree>
 __global__ __launch_bounds__(kAttendThreads, 2) void paged_attend_kernel(const PagedAttendArgs a, const Tree tree) {
     using Tile = RowTile<T, HD, R, R * RT == 16>;

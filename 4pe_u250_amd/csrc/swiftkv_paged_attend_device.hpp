@@ -70,8 +70,8 @@ __device__ __forceinline__ uint32_t seen_bits(int tok0, int first, uint64_t mask
 //
 // 16 rows leave the matrix instructions idle, so a bfloat16 weight is two terms there
 // (2^-16 of it); with more rows it is one, 2^-8, as much as the output's own rounding (two
-// terms: 64 tokens of 8 sequences 69.5 us against 56.5, 512 onto 4095 68 against 54, 4096 onto
-// 4095 572 against 419).  A float16 weight is 2^(kShift + kScoreSlack) at most and is good to
+// terms: 64 tokens of 8 sequences 69 us against 60, 512 onto 4095 70 against 55, 4096 onto 4095
+// 606 against 441).  A float16 weight is 2^(kShift + kScoreSlack) at most and is good to
 // 2^-11, or to 2^-36 of the row's largest.  A bfloat16 weight is 2^-18 at most, so that
 // kPagedMaxSeq of them times the largest values stay in FP32's range, 2^127 together, here
 // and where waves and splits are joined; what that takes from the other end is below 2^-104

@@ -157,24 +157,24 @@ int append_rows(const swiftkv_context* ctx, const PagedRotation& rotation, const
 // (three tiles of 16 a wave: loads bound these), 64 (two of 32), 128 or 256 (cells shared in
 // LDS).  Where they are few, workgroups shall be many: 32 rows, or 64 where 32 would leave a
 // CU more than one.  us of a call onto 4031 tokens, 32 heads of 128 over 8, the kernel taken
-// against others: 64 sequences x 12 tokens (48 rows) 48 188, 64 192, 32 204; x 16 64 195, 32 210,
-// 128 219; x 24 128 228, 64 255, 32 257; x 64 256 357, 128 424, 64 468; 8 x 16 32 31.2, 64 35.1; x
-// 24 32 34.8, 64 39.3, 128 43.0; x 64 64 57.2, 32 67.2, 128 67.9; one sequence x 26 32 16.0, 64
-// 20.2; x 512 64 54.9, 32 61.1, 256 67.4; x 1024 64 105, 256 114; 4 x 512 256 174, 64 190; a prompt
-// of 4096 tokens onto none 256 179, 128 209.
+// against others: 64 sequences x 12 tokens (48 rows) 48 190, 64 192, 32 207; x 16 64 195, 32 210,
+// 128 216; x 24 128 225, 64 255, 32 261; x 64 256 351, 128 407, 64 467; 8 x 16 32 31.4, 64 35.2; x
+// 24 32 35.0, 64 38.5, 128 43.3; x 64 64 56.6, 32 65.4, 256 66.5; one sequence x 26 32 16.1, 64
+// 20.3; x 512 64 53.5, 32 58.8, 256 67.6; x 1024 64 102, 32 111, 256 114; 4 x 512 256 171, 64 185; a
+// prompt of 4096 tokens onto none 256 178, 128 207.
 //
 // What the rule does not see: a chunk of a prompt scans what it sees and turns count as if
-// each saw all, so prompts onto none get more rows than is best (512 tokens 64 19.0, 32 15.8;
-// 1024 64 35.1, 32 30.5; 2048 64 81.5, 128 74.7), and 8 x 32 tokens are where the two meet (64
-// 39.2, 32 37.7).
+// each saw all, so prompts onto none get more rows than is best (512 tokens 64 19.4, 32 16.0;
+// 1024 64 35.8, 32 31.0; 2048 64 81.7, 32 74.4), and 8 x 32 tokens are where the two meet (64
+// 40.0, 32 36.8).
 //
 // Splits make a workgroup for each CU and not more, of at most 32 a sequence and at most the
 // square root of its 64-token tiles, since they are joined: us of a step, tokens of this
-// rule's splits against others: one sequence at 4096 512 10.7; 256 11.8, 1024 12.4; 4 at 4096
-// 512 16.6; 1024 19.6; 8 at 4096 1024 26.1; 512 29.4, 2048 30.3; 32 at 4096 none 85.8; 2048
-// 90.9; 64 none 170; 2048 180; one at 32000 1408 29.6; 1024 30.0, 2048 31.4, 4096 45.7.  It goes by
+// rule's splits against others: one sequence at 4096 512 10.9; 256 12.0, 1024 12.6; 4 at 4096
+// 512 16.5; 1024 19.6; 8 at 4096 1024 26.3; 512 29.3, 2048 30.5; 32 at 4096 none 85.6; 2048
+// 90.7; 64 none 169; 2048 180; one at 32000 1408 29.6; 1024 30.1, 2048 31.4, 4096 46.0.  It goes by
 // how many workgroups there are, not by what each scans: one sequence of 32000 among 63 of 100
-// is not split (282; in 4 splits 83).
+// is not split (280; in 4 splits 84).
 PagedPlan plan_attention(int32_t cus, int32_t split_tokens, int32_t forced_rows, int32_t group, int32_t kv_heads, int32_t n,
                          const int32_t* positions, int32_t batch) {
     PagedPlan p{};

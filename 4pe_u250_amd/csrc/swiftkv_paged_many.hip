@@ -19,7 +19,7 @@ constexpr int kManyWaves = 8;
 // step while it forms the weights of this one, so K lies one turn ahead of V.  Each has
 // SLOTS slots: a turn asks for cells SLOTS - 1 turns ahead, into the slots that nobody
 // reads in it, waits for those that it asked for SLOTS - 2 turns before, and ends with a
-// barrier.  4096 tokens onto 4095 419 us, 0.98 PFLOP/s with 256 rows.
+// barrier.  4096 tokens onto 4095 434 us, 0.95 PFLOP/s with 256 rows.
 template <int HD, int RW>
 struct ManyShape {
     static constexpr int TEAMS = kManyWaves / RW, ROWS = 32 * RW;

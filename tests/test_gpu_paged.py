@@ -921,3 +921,31 @@ def test_large_scores_in_every_shape(skv, ctx, t, forced):
     rig = P.Rig(skv, ctx, t, 4, 1, 128, capacity=1024, seed=forced)
     rig.map_all()
     large_scores(skv, ctx, rig, t, 20, 4, 1000)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 20])
+def test_the_largest_and_smallest_scales(skv, ctx, t, n):
+    """2^-100 weighs all tokens alike, 2^100 leaves the token with the largest score, or with a negative scale the
+    smallest."""
+    tokens, dim = 700, 64
+    rig = P.Rig(skv, ctx, t, 4, 2, dim, capacity=tokens, seed=n)
+    rig.map_all()
+    k = rig.random(1, tokens, 2, dim)[1] * 0.25
+    k[..., 0] = np.arange(tokens)[None, :, None] % 89        # several tokens share a score
+    k[..., 1:] = 0.0
+    v = rig.random(1, tokens, 2, dim)[1]
+    rig.append([0], tokens, k=k, v=v)
+    q = np.zeros((1, n, 4, dim))
+    q[..., 0] = 1.0
+    for scale in (2.0 ** -100, -2.0 ** -100, 2.0 ** 100, -2.0 ** 100):
+        _, out = rig.attend([tokens - n], n, q=q, append=False, scale=scale)
+        for i in range(n):
+            at = np.arange(tokens - n + i + 1)
+            if abs(scale) > 1:
+                score = np.sign(scale) * (at % 89)
+                at = at[score == score.max()]
+            for h in range(4):
+                x = v[0, at, h // 2]
+                off = (2 * R.HALF_STEP[t] + tokens * 2.0 ** -24 + 2.0 ** -18) * np.abs(x).mean(0) + 2.0 ** -25
+                assert (np.abs(out[0, i, h] - x.mean(0)) <= off).all(), (scale, i, h)
